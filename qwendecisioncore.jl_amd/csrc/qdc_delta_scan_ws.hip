@@ -31,6 +31,7 @@
 // the operands' refills (timing only) the scan of the first took 227 us, so what its
 // loads cost beside the products is the next thing to gain.
 #include "qdc_common.hpp"
+#include "qdc_hip_cache.h"
 #include "qdc_hip_workspace.h"
 
 namespace qdc {
@@ -59,6 +60,7 @@ struct ChunkArgs {
     void *out;
     const float *q, *k, *v, *beta, *decay;
     float *ws;
+    float *state;  // [batch, H, vd, kd] after the last token, where it is kept
     int64_t ld_qk, ld_v;  // elements between the token rows of q and k, and of v
     int S, H, vd, groups, chunks, slices;  // slices = vd / 16
     int64_t units;        // batch * heads * chunks (prepare)
@@ -218,7 +220,9 @@ template <int V> __device__ __forceinline__ void load_vec(const float *p, float 
 // chunk's k and q rows once between them, two chunks ahead, into one of two LDS
 // tiles, and refill their operands from the tile of the next chunk: the same loads
 // from memory by every wavefront took a third of the kernel's time to issue.
-template <int KB, int KSPLIT, typename TO>
+//
+// KEEP: the state after the last token goes to a.state.
+template <int KB, int KSPLIT, typename TO, bool KEEP>
 __global__ __launch_bounds__(KSPLIT > 1 ? KSPLIT * kWave : kBlock, 2) void delta_chunk_scan(
     ChunkArgs a) {
     constexpr int KBW = KB / KSPLIT;
@@ -521,6 +525,16 @@ __global__ __launch_bounds__(KSPLIT > 1 ? KSPLIT * kWave : kBlock, 2) void delta
         read_output(chunks - 1, due);
         store(chunks - 1, due);
     }
+    if constexpr (KEEP) {  // S^T's block t, row 4 lg + j, column lr: a lane's own column
+        if (live) {
+            float *dst = a.state + ((int64_t)bh * a.vd + col) * (16 * KB) + ks * (16 * KBW);
+#pragma unroll
+            for (int t = 0; t < KBW; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    dst[16 * V * (t / V) + V * (4 * lg + j) + t % V] = st[t][j];
+        }
+    }
 }
 
 }  // namespace
@@ -542,12 +556,11 @@ extern "C" int64_t qdc_delta_scan_workspace(int64_t batch, int64_t seq, int64_t 
     return batch * heads * chunks * kRecord * 4;
 }
 
-extern "C" int32_t qdc_delta_scan_ws(void *out, int32_t out_dtype, const float *q, const float *k,
-                                     const float *v, const float *beta, const float *decay,
-                                     int64_t batch, int64_t seq, int64_t heads, int64_t key_heads,
-                                     int64_t key_dim, int64_t value_dim, int64_t ld_qk,
-                                     int64_t ld_v, void *workspace, int64_t workspace_bytes,
-                                     hipStream_t stream) {
+static int32_t scan_ws(void *out, int32_t out_dtype, float *state, bool keep, const float *q,
+                       const float *k, const float *v, const float *beta, const float *decay,
+                       int64_t batch, int64_t seq, int64_t heads, int64_t key_heads,
+                       int64_t key_dim, int64_t value_dim, int64_t ld_qk, int64_t ld_v,
+                       void *workspace, int64_t workspace_bytes, hipStream_t stream) {
     if (!valid_dtype(out_dtype)) return QDC_ERR_DTYPE;
     if (batch < 0 || seq < 0 || heads <= 0 || key_heads <= 0 || value_dim <= 0 ||
         heads % key_heads)
@@ -558,8 +571,10 @@ extern "C" int32_t qdc_delta_scan_ws(void *out, int32_t out_dtype, const float *
     if (need == 0 || workspace_bytes < need || ld_qk % 4 || ld_v % 4 ||
         ld_qk >= ((int64_t)1 << 25) || ld_v >= ((int64_t)1 << 25))  // 32-bit chunk offsets
         return QDC_ERR_SHAPE;
-    if (!out || !q || !k || !v || !beta || !decay || !workspace) return QDC_ERR_NULL;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(workspace))
+    if (!out || !q || !k || !v || !beta || !decay || !workspace || (keep && !state))
+        return QDC_ERR_NULL;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(workspace) ||
+        !aligned16(state))
         return QDC_ERR_SHAPE;
     const int64_t tokens = batch * seq;
     const int64_t out_bytes = tokens * heads * value_dim * elem_size(out_dtype);
@@ -570,7 +585,14 @@ extern "C" int32_t qdc_delta_scan_ws(void *out, int32_t out_dtype, const float *
         overlaps(workspace, need, beta, tokens * heads * 4) ||
         overlaps(workspace, need, decay, tokens * heads * 4))
         return QDC_ERR_ALIAS;
+    const int64_t kept = keep ? batch * heads * value_dim * key_dim * 4 : 0;
+    if (overlaps(state, kept, out, out_bytes) || overlaps(state, kept, q, qk_bytes) ||
+        overlaps(state, kept, k, qk_bytes) || overlaps(state, kept, v, v_bytes) ||
+        overlaps(state, kept, beta, tokens * heads * 4) ||
+        overlaps(state, kept, decay, tokens * heads * 4) || overlaps(state, kept, workspace, need))
+        return QDC_ERR_ALIAS;
     ChunkArgs a{};
+    a.state = state;
     a.out = out;
     a.q = q;
     a.k = k;
@@ -598,18 +620,23 @@ extern "C" int32_t qdc_delta_scan_ws(void *out, int32_t out_dtype, const float *
     // 1501 tokens 214 / 167; 640 slices, 1501 tokens 222 / 242; 1024 slices, 2048
     // tokens 350 / 474.  (Two wavefronts a slice lost to one of these everywhere.)
     const bool whole = slices > 512;
+#define QDC_CHUNK_LAUNCH(KB, KSPLIT, TO)                                                        \
+    if (keep)                                                                                   \
+        hipLaunchKernelGGL((delta_chunk_scan<KB, KSPLIT, TO, true>), grid, block, 0, stream,    \
+                           a);                                                                  \
+    else                                                                                        \
+        hipLaunchKernelGGL((delta_chunk_scan<KB, KSPLIT, TO, false>), grid, block, 0, stream, a);
 #define QDC_CHUNK_SCAN(KB, KSPLIT)                                                              \
     {                                                                                           \
         const int64_t groups = KSPLIT > 1 ? a.slices : ceil_div(a.slices, (int64_t)4);          \
         a.by_groups = make_fastdiv((uint32_t)groups);                                           \
         const dim3 grid((uint32_t)(batch * heads * groups));                                    \
         const dim3 block(KSPLIT > 1 ? KSPLIT * kWave : kBlock);                                 \
-        if (out_dtype == QDC_BF16)                                                              \
-            hipLaunchKernelGGL((delta_chunk_scan<KB, KSPLIT, bf16_t>), grid, block, 0, stream,  \
-                               a);                                                              \
-        else                                                                                    \
-            hipLaunchKernelGGL((delta_chunk_scan<KB, KSPLIT, float>), grid, block, 0, stream,   \
-                               a);                                                              \
+        if (out_dtype == QDC_BF16) {                                                            \
+            QDC_CHUNK_LAUNCH(KB, KSPLIT, bf16_t)                                                \
+        } else {                                                                                \
+            QDC_CHUNK_LAUNCH(KB, KSPLIT, float)                                                 \
+        }                                                                                       \
         return launch_status();                                                                 \
     }
 #define QDC_CHUNKED(KB, PARTS)                                                                  \
@@ -625,5 +652,27 @@ extern "C" int32_t qdc_delta_scan_ws(void *out, int32_t out_dtype, const float *
     QDC_CHUNKED(2, 2)
 #undef QDC_CHUNKED
 #undef QDC_CHUNK_SCAN
+#undef QDC_CHUNK_LAUNCH
     return QDC_ERR_SHAPE;
+}
+
+extern "C" int32_t qdc_delta_scan_ws(void *out, int32_t out_dtype, const float *q, const float *k,
+                                     const float *v, const float *beta, const float *decay,
+                                     int64_t batch, int64_t seq, int64_t heads, int64_t key_heads,
+                                     int64_t key_dim, int64_t value_dim, int64_t ld_qk,
+                                     int64_t ld_v, void *workspace, int64_t workspace_bytes,
+                                     hipStream_t stream) {
+    return scan_ws(out, out_dtype, nullptr, false, q, k, v, beta, decay, batch, seq, heads,
+                   key_heads, key_dim, value_dim, ld_qk, ld_v, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t qdc_delta_scan_state(void *out, int32_t out_dtype, float *state, const float *q,
+                                        const float *k, const float *v, const float *beta,
+                                        const float *decay, int64_t batch, int64_t seq,
+                                        int64_t heads, int64_t key_heads, int64_t key_dim,
+                                        int64_t value_dim, int64_t ld_qk, int64_t ld_v,
+                                        void *workspace, int64_t workspace_bytes,
+                                        hipStream_t stream) {
+    return scan_ws(out, out_dtype, state, true, q, k, v, beta, decay, batch, seq, heads, key_heads,
+                   key_dim, value_dim, ld_qk, ld_v, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,649 @@
+// qdc_paged_attention.hip -- attention of one token's queries over the pages of its
+// cache row, with the output gate:
+//     out_h = sigmoid(gate_h) * sum_j softmax_j(scale q_h . k_j) v_j,  j <= position.
+//
+// Every key and value is read once for the (up to 16) query heads that share it, so
+// the reads of the pages are all that it has to cost.  The work is cut by what is
+// there, not by what could be: the keys of all entries, head after head, are one row
+// of tiles (32 keys bf16, 16 fp32) that the workgroups share out evenly, whatever the
+// lengths are.  Each workgroup finds its tiles from the positions by itself; a piece
+// that begins and ends within a head's keys leaves its maximum, sum and unnormalised
+// output in the workspace, and a second launch joins the pieces of a head in order.
+//
+// Scores are formed transposed, S^T = K Q^T on the matrix cores: a lane then holds
+// the scores of one head for some keys, the operand layout of O^T = V^T P^T, and the
+// running maximum, sum and rescaling are in-lane but for two lane swaps a tile.  Which
+// keys and which values sit in a matrix operand's slots is free as long as both
+// operands agree, so K, V and the pages' rows go from memory to operands in 16-byte
+// pieces with no stop in LDS: V's 8 keys x 8 values of a lane are paired into operands
+// with one byte permute each.  For bf16 pages the weights enter the product as two bf16
+// terms: rounded to one they would add as much error as the output's own rounding, and
+// the matrix cores have time for both.
+#include <cfloat>
+
+#include "qdc_cache.hpp"
+
+namespace qdc {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = kBlock / kWave;
+constexpr int kHeads = 16;          // query heads of a unit: a matrix operand's columns
+constexpr int kLogWgs = 9;          // workgroups that share the tiles: two a compute unit
+constexpr uint32_t kMinTiles = 4;   // fewer a workgroup leave wavefronts without a tile
+
+struct PagedAttention {
+    void *out;
+    const void *q, *k, *v, *gate;
+    const int32_t *table, *index, *positions;
+    int32_t *error_flag;
+    float *pieces, *stats;  // [2 workgroups][heads of a unit][head_dim], [..][2]
+    int64_t q_tok, q_head, gate_tok, gate_head, out_tok, width;
+    int n, heads, kv, group, unit_heads, head_groups, rows, pages, shift, log_wgs;
+    int out_dtype;
+    float scale_log2;       // scale * log2(e)
+};
+
+template <typename T> constexpr int tile_keys() { return sizeof(T) == 2 ? 32 : 16; }
+
+// Keys of entry i: 0 for one that is no token.
+__device__ __forceinline__ int entry_keys(const PagedAttention &a, int i, bool &bad) {
+    const int row = a.index[i], pos = a.positions[i];
+    bad = row >= a.rows && pos >= 0;
+    if (row < 0 || pos < 0 || bad) return 0;
+    const int64_t reach = a.width << a.shift;
+    bad = pos >= reach;
+    return bad ? (int)reach : pos + 1;
+}
+
+// Inclusive prefix sum over a wavefront.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    const int l = threadIdx.x % kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const uint32_t o = (uint32_t)__shfl_up((int)v, d, kWave);
+        if (l >= d) v += o;
+    }
+    return v;
+}
+
+// The entries as rows of tiles, seen 64 at a time by a wavefront: lane l holds entry
+// first + l's tiles and where they end.
+template <int TILE> struct Entries {
+    const PagedAttention &a;
+    int first;
+    uint32_t tiles, end, before, all;  // before: tiles of earlier chunks; all: this one's
+
+    __device__ __forceinline__ void load(int at) {
+        first = at;
+        const int i = at + (int)(threadIdx.x % kWave);
+        bool bad;
+        tiles = i < a.n ? (uint32_t)(entry_keys(a, i, bad) + TILE - 1) / TILE : 0u;
+        end = wave_scan(tiles);
+        all = __builtin_amdgcn_readlane(end, kWave - 1);
+    }
+    // all entries' tiles; leaves the first chunk in place
+    __device__ __forceinline__ uint32_t total() {
+        before = 0;
+        uint32_t sum = 0;
+        for (int at = (a.n - 1) / kWave * kWave; at >= 0; at -= kWave) {
+            load(at);
+            sum += all;
+        }
+        return sum;
+    }
+    __device__ __forceinline__ void next() {
+        before += all;
+        load(first + kWave);
+    }
+};
+
+// Workgroups that work, as a power of two: fewer where there are few tiles.
+__device__ __forceinline__ int log_workers(int log_wgs, uint32_t tiles) {
+    while (log_wgs > 0 && (tiles >> log_wgs) < kMinTiles) --log_wgs;
+    return log_wgs;
+}
+
+__device__ __forceinline__ float swap_max(float v) {  // over lanes l, l^16, l^32, l^48
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// What is left of a weight after its leading bf16 term, cut off and not rounded: never
+// negative, and for a weight above 0 never 0, so that a value of infinity stays one
+// (2^-126 is below half a step of any sum that shows).  The two terms together are
+// within 2^-16 of the weight.
+__device__ __forceinline__ float rest(float p) {
+    return p > 0.0f ? fmaxf(p - __uint_as_float(__float_as_uint(p) & 0xffff0000u), 0x1p-126f)
+                    : p;
+}
+
+// N consecutive outputs of head h of entry i, values dim .., with the gate.
+template <typename T, int HD, int N>
+__device__ __forceinline__ void store_out(const PagedAttention &a, int i, int h, int dim,
+                                          float (&o)[N]) {
+    if (a.gate) {
+        const T *g = (const T *)a.gate + (int64_t)i * a.gate_tok + (int64_t)h * a.gate_head + dim;
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] *= sigmoid(to_f32(g[j]));
+    }
+    const int64_t at = (int64_t)i * a.out_tok + (int64_t)h * HD + dim;
+    if constexpr (N == 4) {
+        if (a.out_dtype == QDC_BF16) store_frag((bf16_t *)a.out + at, o);
+        else if (a.out_dtype == QDC_F32) store_frag((float *)a.out + at, o);
+        else store_frag((split_t *)a.out + at, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (a.out_dtype == QDC_BF16) put_elem((bf16_t *)a.out, at + j, o[j]);
+            else if (a.out_dtype == QDC_F32) put_elem((float *)a.out, at + j, o[j]);
+            else put_elem((split_t *)a.out, at + j, o[j]);
+        }
+    }
+}
+
+// One wavefront's operands and sums over its tiles of one head group.
+//   K: lane (lr, lg) holds values DS s + V lg .. of key 16 sub + lr.
+//   V: values 16 VD c + VD lr .. of keys 16 sub + 4 lg + r.
+//   S^T, P: head lr, keys 16 sub + 4 lg + r.   O^T[c][j]: head lr, values
+//   16 VD c + VD (4 lg + r) + j.
+template <typename T, int HD> struct Lanes {
+    static constexpr bool BF = sizeof(T) == 2;
+    static constexpr int V = Elem<T>::kVec, SUBS = BF ? 2 : 1, DS = 4 * V, STEPS = HD / DS;
+    static constexpr int VD = BF && HD > 64 ? 8 : 4, VC = HD / (16 * VD);
+    static constexpr int VW = VD * (int)sizeof(T) / 4;  // registers of a V piece
+    typedef uint32_t piece __attribute__((ext_vector_type(VW)));
+    u32x4 k[SUBS][STEPS];
+    piece v[SUBS][4][VC];
+    f32x4 o[VC][VD];
+    float base, sum;
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int j = 0; j < VD; ++j) o[c][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        base = -FLT_MAX;  // finite: a masked score is -inf
+        sum = 0.0f;
+    }
+};
+
+template <typename T, int HD>
+__global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
+    typedef Lanes<T, HD> L;
+    constexpr int TILE = tile_keys<T>(), KT = kWave / L::SUBS;
+    constexpr int VEC = HD / kWave;  // outputs of a thread per pass of 4 heads
+    __shared__ __align__(16) u32x4 sq[L::STEPS][kWave];
+    __shared__ __align__(16) float so[kWaves][4][HD + 4];
+    __shared__ float sm[kWaves][kHeads], sl[kWaves][kHeads];
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
+    const int lr = l % 16, lg = l / 16;
+    const uint32_t units = (uint32_t)(a.kv * a.head_groups);
+    Entries<TILE> es{a};
+    const uint32_t all = es.total() * units;
+    const int lw = log_workers(a.log_wgs, all);
+    if (blockIdx.x >> lw) return;
+    uint32_t t = (uint32_t)(((uint64_t)all * blockIdx.x) >> lw);
+    const uint32_t t_end = (uint32_t)(((uint64_t)all * (blockIdx.x + 1)) >> lw);
+    const int mask = (1 << a.shift) - 1;
+    L x;
+    while (t < t_end) {
+        while (units * (es.before + es.all) <= t) es.next();
+        // the entry that holds tile t, and the part of it up to t_end
+        const uint64_t past = __ballot(units * (es.before + es.end) > t);
+        const int el = __builtin_ctzll(past), entry = es.first + el;
+        const uint32_t tiles = __builtin_amdgcn_readlane(es.tiles, el);
+        const uint32_t rel = t - units * (es.before + __builtin_amdgcn_readlane(es.end, el) - tiles);
+        const uint32_t unit = rel / tiles, j0 = rel - unit * tiles;
+        const uint32_t j1 = min(tiles, j0 + (t_end - t));
+        t += j1 - j0;
+        const int kvh = (int)unit / a.head_groups, hg = (int)unit - kvh * a.head_groups;
+        const int head0 = kvh * a.group + hg * kHeads;
+        const int gu = min(kHeads, a.group - hg * kHeads);
+        bool bad;
+        const int keys = __builtin_amdgcn_readfirstlane(entry_keys(a, entry, bad));
+        const int row = __builtin_amdgcn_readfirstlane(a.index[entry]);
+        const int32_t *pages = a.table + (int64_t)row * a.width;
+
+        // this wavefront's tiles: every fourth
+        const int jw = (int)j0 + wv, cnt = (int)j1 > jw ? ((int)j1 - jw + kWaves - 1) / kWaves : 0;
+        int32_t ids = -1;  // lane l: the page of tile k0 + l / SUBS, sub l % SUBS
+        auto fetch_ids = [&](int k0) {
+            const int k = k0 + l / L::SUBS;
+            const int key = (jw + kWaves * k) * TILE + 16 * (l % L::SUBS);
+            if (k < cnt) ids = pages[min(key, keys - 1) >> a.shift];
+        };
+        fetch_ids(0);
+        int limit[L::SUBS];  // keys of the tile's halves that count
+        int64_t from[L::SUBS];
+        auto locate = [&](int k) {  // where tile k lies
+            if (k && k % KT == 0) fetch_ids(k);
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s) {
+                const int key0 = (jw + kWaves * k) * TILE + 16 * s;
+                const int id = __builtin_amdgcn_readlane(ids, k % KT * L::SUBS + s);
+                const bool ok = (uint32_t)id < (uint32_t)a.pages;
+                from[s] = (((int64_t)(ok ? id : 0) * a.kv + kvh) << a.shift) * HD;
+                const int left = min(max(keys - key0, 0), 16);
+                limit[s] = ok ? left : 0;
+                if (!ok && left && l == 0) raise_flag(a.error_flag);
+            }
+        };
+        // keys past the end read the last one
+        auto place = [&](int key) { return (min(key, keys - 1) & mask) * HD; };
+        auto load_k = [&](int k) {
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s) {
+                const T *p = (const T *)a.k + from[s] +
+                             (place((jw + kWaves * k) * TILE + 16 * s + lr) + L::V * lg);
+#pragma unroll
+                for (int i = 0; i < L::STEPS; ++i) x.k[s][i] = load_raw(p + L::DS * i);
+            }
+        };
+        auto load_v = [&](int k) {
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const T *p = (const T *)a.v + from[s] +
+                                 (place((jw + kWaves * k) * TILE + 16 * s + 4 * lg + r) + L::VD * lr);
+#pragma unroll
+                    for (int c = 0; c < L::VC; ++c)
+                        x.v[s][r][c] = *reinterpret_cast<const typename L::piece *>(
+                            p + 16 * L::VD * c);
+                }
+        };
+        if (cnt) {
+            locate(0);
+            load_k(0);
+            load_v(0);
+        }
+        // q as the other operand of the scores, heads past the group's repeat its last
+        for (int i = threadIdx.x; i < L::STEPS * kWave; i += kBlock) {
+            const int s = i / kWave, ln = i % kWave;
+            sq[s][ln] = load_raw((const T *)a.q + (int64_t)entry * a.q_tok +
+                                 (int64_t)(head0 + min(ln % 16, gu - 1)) * a.q_head + L::DS * s +
+                                 L::V * (ln / 16));
+        }
+        __syncthreads();
+        x.clear();
+        for (int k = 0; k < cnt; ++k) {
+            f32x4 sc[L::SUBS];
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < L::STEPS; ++i) {
+                const u32x4 qf = sq[i][l];
+#pragma unroll
+                for (int s = 0; s < L::SUBS; ++s) {
+                    if constexpr (L::BF) {
+                        sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8, x.k[s][i]), __builtin_bit_cast(bf16x8, qf),
+                            sc[s], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(x.k[s][i][e]), __uint_as_float(qf[e]), sc[s], 0, 0,
+                                0);
+                    }
+                }
+            }
+            int now[L::SUBS];
+            bool cut = false;
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s) now[s] = limit[s], cut = cut || limit[s] < 16;
+            const bool more = k + 1 < cnt;
+            if (more) {
+                locate(k + 1);
+                load_k(k + 1);
+            }
+            if (cut) {
+#pragma unroll
+                for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (4 * lg + r < now[s]) continue;
+                        sc[s][r] = -__builtin_inff();
+#pragma unroll
+                        for (int c = 0; c < L::VC; ++c)  // 0 times what lies there may be NaN
+                            x.v[s][r][c] = typename L::piece(0u);
+                    }
+            }
+            float top = sc[0][0];
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[s][r]);
+            top = fmaxf(swap_max(top) * a.scale_log2, x.base);
+            if (__any(top > x.base)) {
+                const float f = __builtin_amdgcn_exp2f(x.base - top);
+                x.sum *= f;
+#pragma unroll
+                for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < L::VD; ++j) x.o[c][j] *= f;
+                x.base = top;
+            }
+            float p[L::SUBS][4];
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[s][r] = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(sc[s][r], a.scale_log2, -x.base));
+                    x.sum += p[s][r];
+                }
+            if constexpr (L::BF) {
+                u32x4 hi, lo;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p0 = p[i / 2][2 * (i % 2)], p1 = p[i / 2][2 * (i % 2) + 1];
+                    hi[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0),
+                                                  0x07060302u);
+                    lo[i] = pack_bf16x2(rest(p0), rest(p1));
+                }
+#pragma unroll
+                for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < L::VD; ++j) {
+                        u32x4 vf;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            vf[i] = __builtin_amdgcn_perm(
+                                x.v[i / 2][2 * (i % 2) + 1][c][j / 2],
+                                x.v[i / 2][2 * (i % 2)][c][j / 2],
+                                j % 2 ? 0x07060302u : 0x05040100u);
+                        const bf16x8 vb = __builtin_bit_cast(bf16x8, vf);
+                        x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            vb, __builtin_bit_cast(bf16x8, hi), x.o[c][j], 0, 0, 0);
+                        x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            vb, __builtin_bit_cast(bf16x8, lo), x.o[c][j], 0, 0, 0);
+                    }
+            } else {
+#pragma unroll
+                for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < L::VD; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(x.v[0][r][c][j]), p[0][r], x.o[c][j], 0, 0, 0);
+            }
+            if (more) load_v(k + 1);
+        }
+        // the wavefronts' sums together, four heads at a time
+        x.sum = swap_sum32(swap_sum16(x.sum));
+        if (lg == 0) {
+            sm[wv][lr] = x.base;
+            sl[wv][lr] = x.sum;
+        }
+        const bool whole = j0 == 0 && j1 == tiles;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (j0 == 0);
+        for (int h0 = 0; h0 < gu; h0 += 4) {
+            const int hh = lr - h0;
+            if (hh >= 0 && hh < 4)
+#pragma unroll
+                for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < L::VD; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            so[wv][hh][16 * L::VD * c + L::VD * (4 * lg + r) + j] = x.o[c][j][r];
+            __syncthreads();
+            const int h = h0 + threadIdx.x / kWave, dim = VEC * l;
+            if (h < gu) {
+                float top = sm[0][h], acc[VEC] = {}, total = 0.0f;
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][h]);
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(sm[w][h] - top);
+                    total = __builtin_fmaf(f, sl[w][h], total);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        acc[e] = __builtin_fmaf(f, so[w][h - h0][dim + e], acc[e]);
+                }
+                if (whole) {
+                    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) acc[e] *= inv;
+                    store_out<T, HD, VEC>(a, entry, head0 + h, dim, acc);
+                } else {
+                    float *dst = a.pieces + (slot * a.unit_heads + h) * HD + dim;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) dst[e] = acc[e];
+                    if (l == 0) {
+                        float *st = a.stats + (slot * a.unit_heads + h) * 2;
+                        st[0] = top;
+                        st[1] = total;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// A workgroup per (entry, head): the pieces of its keys, in order; zeros for an entry
+// without keys; nothing where one workgroup had them all.
+template <typename T, int HD>
+__global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a) {
+    constexpr int TILE = tile_keys<T>();
+    constexpr int LPP = HD / 4, PARTS = kBlock / LPP;  // lanes of a piece's row, rows at a time
+    __shared__ float weight[1 << kLogWgs], top_of[kWaves], sum_of[kWaves];
+    __shared__ __align__(16) float so[PARTS][HD];
+    const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
+    const int entry = blockIdx.x / a.heads, h = blockIdx.x - entry * a.heads;
+    const int kvh = h / a.group, in_group = h - kvh * a.group;
+    const int hg = in_group / kHeads, hu = in_group - hg * kHeads;
+    const uint32_t units = (uint32_t)(a.kv * a.head_groups);
+    Entries<TILE> es{a};
+    const uint32_t all = es.total() * units;
+    while (es.first + kWave <= entry) es.next();
+    const uint32_t tiles = __builtin_amdgcn_readlane(es.tiles, entry - es.first);
+    if (h == 0 && threadIdx.x == 0) {
+        bool bad;
+        entry_keys(a, entry, bad);
+        if (bad) raise_flag(a.error_flag);
+    }
+    const int dim = HD / kWave * l;
+    if (tiles == 0) {
+        float zero[HD / kWave] = {};
+        // 0 whatever the gate holds
+        PagedAttention b = a;
+        b.gate = nullptr;
+        if (wv == 0) store_out<T, HD, HD / kWave>(b, entry, h, dim, zero);
+        return;
+    }
+    const int lw = log_workers(a.log_wgs, all);
+    const uint32_t first = units * (es.before + __builtin_amdgcn_readlane(es.end, entry - es.first) -
+                                    tiles) + (uint32_t)(kvh * a.head_groups + hg) * tiles;
+    // the workgroups that hold its first and its last tile: w of tile t is the last with
+    // all * w / 2^lw <= t
+    const uint32_t w0 = (uint32_t)((((uint64_t)(first + 1) << lw) - 1) / all);
+    const uint32_t w1 = (uint32_t)((((uint64_t)(first + tiles) << lw) - 1) / all);
+    if (w0 == w1) return;
+    const int parts = (int)(w1 - w0) + 1;
+    auto slot = [&](int p) {
+        return ((2 * (int64_t)(w0 + p) + (p == 0)) * a.unit_heads + hu);
+    };
+    float top = -FLT_MAX;
+    for (int p = threadIdx.x; p < parts; p += kBlock) top = fmaxf(top, a.stats[2 * slot(p)]);
+    top = swap_max(top);
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d, kWave));
+    if (l == 0) top_of[wv] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, top_of[w]);
+    float sum = 0.0f;
+    for (int p = threadIdx.x; p < parts; p += kBlock) {
+        const float f = __builtin_amdgcn_exp2f(a.stats[2 * slot(p)] - top);
+        weight[p] = f;
+        sum = __builtin_fmaf(f, a.stats[2 * slot(p) + 1], sum);
+    }
+    sum = group_sum<kWave>(sum);
+    if (l == 0) sum_of[wv] = sum;
+    __syncthreads();
+    const int part = threadIdx.x / LPP, d4 = 4 * (threadIdx.x % LPP);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = part; p < parts; p += PARTS) {
+        const f32x4 o = *reinterpret_cast<const f32x4 *>(a.pieces + slot(p) * HD + d4);
+        const float f = weight[p];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(f, o[e], acc[e]);
+    }
+    *reinterpret_cast<f32x4 *>(&so[part][d4]) = acc;
+    __syncthreads();
+    if (wv) return;
+    float total = 0.0f, o[HD / kWave] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) total += sum_of[w];
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
+#pragma unroll
+    for (int e = 0; e < HD / kWave; ++e) {
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) o[e] += so[p][dim + e];
+        o[e] *= inv;
+    }
+    store_out<T, HD, HD / kWave>(a, entry, h, dim, o);
+}
+
+// The most tiles that a call of these sizes can have, 0 when there are too many or the
+// sizes are not taken.
+int64_t most_tiles(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t width,
+                   int64_t page_size, int32_t dtype) {
+    if (!valid_dtype(dtype) || n <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256) || width <= 0 ||
+        page_shift(page_size) < 0)
+        return 0;
+    const int64_t lim = (int64_t)1 << 31;
+    // the join has a workgroup per head of an entry
+    if (heads >= ((int64_t)1 << 20) || n >= ((int64_t)1 << 24) / heads || width >= lim / page_size)
+        return 0;
+    const int64_t units = kv_heads * ceil_div(heads / kv_heads, (int64_t)kHeads);
+    const int64_t tile = dtype == QDC_BF16 ? tile_keys<bf16_t>() : tile_keys<float>();
+    const int64_t tiles = ceil_div(width * page_size, tile);
+    return tiles >= lim / units / n ? 0 : tiles * units * n;
+}
+
+int log_workgroups(int64_t tiles) {
+    int lw = 0;
+    while (lw < kLogWgs && ((int64_t)kMinTiles << lw) < tiles) ++lw;
+    return lw;
+}
+
+int64_t unit_heads(int64_t heads, int64_t kv_heads) {
+    const int64_t g = heads / kv_heads;
+    return g < kHeads ? g : kHeads;
+}
+
+}  // namespace
+}  // namespace qdc
+
+using namespace qdc;
+
+extern "C" int64_t qdc_paged_attention_workspace(int64_t n, int64_t heads, int64_t kv_heads,
+                                                 int64_t head_dim, int64_t width,
+                                                 int64_t page_size, int32_t dtype) {
+    const int64_t tiles = most_tiles(n, heads, kv_heads, head_dim, width, page_size, dtype);
+    if (tiles == 0) return 0;
+    // two pieces a workgroup, each with its maximum and sum
+    return ((int64_t)2 << log_workgroups(tiles)) * unit_heads(heads, kv_heads) * (head_dim + 2) * 4;
+}
+
+extern "C" int32_t qdc_paged_attention(
+    void *out, int32_t out_dtype, const void *q, const void *k_pages, const void *v_pages,
+    const void *gate, const int32_t *table, const int32_t *index, const int32_t *positions,
+    int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rows, int64_t width,
+    int64_t pages, int64_t page_size, int64_t q_tok, int64_t q_head, int64_t gate_tok,
+    int64_t gate_head, int64_t out_tok, float scale, int32_t dtype, void *workspace,
+    int64_t workspace_bytes, int32_t *error_flag, hipStream_t stream) {
+    if (!valid_dtype(dtype) || (!valid_dtype(out_dtype) && out_dtype != QDC_BF16X2))
+        return QDC_ERR_DTYPE;
+    if (n < 0 || rows <= 0 || pages <= 0) return QDC_ERR_SHAPE;
+    const int64_t tiles =
+        most_tiles(n ? n : 1, heads, kv_heads, head_dim, width, page_size, dtype);
+    const int64_t lim = (int64_t)1 << 31;
+    if (tiles == 0 || rows >= lim || pages >= lim) return QDC_ERR_SHAPE;
+    const int64_t es = elem_size(dtype), per = 16 / es, oes = elem_size(out_dtype);
+    if (q_head < head_dim || q_tok < 0 || (q_tok | q_head) % per || out_tok < heads * head_dim ||
+        out_tok % (16 / oes))
+        return QDC_ERR_SHAPE;
+    if (gate && (gate_head < head_dim || gate_tok < 0 || (gate_tok | gate_head) % per))
+        return QDC_ERR_SHAPE;
+    if (!(scale > 0.0f) || !(scale * 1.4426950408889634f < __builtin_inff())) return QDC_ERR_RANGE;
+    if (n == 0) return QDC_OK;
+    if (!out || !q || !k_pages || !v_pages || !table || !index || !positions || !workspace)
+        return QDC_ERR_NULL;
+    if (!aligned16(out) || !aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) ||
+        !aligned16(gate) || !aligned16(workspace))
+        return QDC_ERR_SHAPE;
+    const int64_t need = qdc_paged_attention_workspace(n, heads, kv_heads, head_dim, width,
+                                                       page_size, dtype);
+    if (workspace_bytes < need) return QDC_ERR_SHAPE;
+    const int64_t store = pages * kv_heads * page_size * head_dim * es;
+    const Range outs[3] = {{out, ((n - 1) * out_tok + heads * head_dim) * oes},
+                           {workspace, need},
+                           {error_flag, error_flag ? 4 : 0}};
+    const Range ins[7] = {
+        {q, grid_span(n, heads, q_tok, q_head, head_dim, es)},
+        {gate, gate ? grid_span(n, heads, gate_tok, gate_head, head_dim, es) : 0},
+        {k_pages, store}, {v_pages, store}, {table, rows * width * 4},
+        {index, n * 4}, {positions, n * 4}};
+    if (any_alias(outs, 3, ins, 7)) return QDC_ERR_ALIAS;
+    PagedAttention a{};
+    a.out = out;
+    a.q = q;
+    a.k = k_pages;
+    a.v = v_pages;
+    a.gate = gate;
+    a.table = table;
+    a.index = index;
+    a.positions = positions;
+    a.error_flag = error_flag;
+    a.q_tok = q_tok;
+    a.q_head = q_head;
+    a.gate_tok = gate_tok;
+    a.gate_head = gate_head;
+    a.out_tok = out_tok;
+    a.width = width;
+    a.n = (int)n;
+    a.heads = (int)heads;
+    a.kv = (int)kv_heads;
+    a.group = (int)(heads / kv_heads);
+    a.unit_heads = (int)unit_heads(heads, kv_heads);
+    a.head_groups = (int)ceil_div(heads / kv_heads, (int64_t)kHeads);
+    a.rows = (int)rows;
+    a.pages = (int)pages;
+    a.shift = page_shift(page_size);
+    a.log_wgs = log_workgroups(tiles);
+    a.out_dtype = out_dtype;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const dim3 grid(1u << a.log_wgs), join((uint32_t)(n * heads)), block(kBlock);
+    a.pieces = reinterpret_cast<float *>(workspace);
+    a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;
+#define QDC_PAGED(T, HD)                                                                       \
+    if (head_dim == HD) {                                                                      \
+        hipLaunchKernelGGL((paged_attention<T, HD>), grid, block, 0, stream, a);               \
+        const int32_t status = launch_status();                                                \
+        if (status != QDC_OK) return status;                                                   \
+        hipLaunchKernelGGL((paged_attention_join<T, HD>), join, block, 0, stream, a);          \
+        return launch_status();                                                                \
+    }
+    if (dtype == QDC_BF16) {
+        QDC_PAGED(bf16_t, 64)
+        QDC_PAGED(bf16_t, 128)
+        QDC_PAGED(bf16_t, 256)
+    }
+    QDC_PAGED(float, 64)
+    QDC_PAGED(float, 128)
+    QDC_PAGED(float, 256)
+#undef QDC_PAGED
+    return QDC_ERR_SHAPE;
+}

@@ -78,6 +78,26 @@ WORKSPACE_SIGNATURES = {
     "qdc_linear_f32": (_i32, [_vp] * 7 + [_i64] * 8 + [_f32, _i32, _i32, _vp]),
 }
 
+# the entry points of include/qdc_hip_cache.h, likewise
+CACHE_SIGNATURES = {
+    "qdc_cache_version": (ctypes.c_char_p, []),
+    "qdc_prepare_paged": (_i32, [_vp] * 14 + [_i64] * 16 + [_f32, _i32, _vp, _vp]),
+    "qdc_paged_attention_workspace": (_i64, [_i64] * 6 + [_i32]),
+    "qdc_paged_attention": (_i32, [_vp, _i32] + [_vp] * 7 + [_i64] * 13
+                            + [_f32, _i32, _vp, _i64, _vp, _vp]),
+    "qdc_pages_extend": (_i32, [_vp] * 7 + [_i64] * 5 + [_vp, _vp]),
+    "qdc_pages_free": (_i32, [_vp] * 5 + [_i64] * 5 + [_vp, _vp]),
+    "qdc_pages_fork": (_i32, [_vp] * 6 + [_i64] * 5 + [_vp] + [_i64] * 3
+                       + [_vp, _i64, _vp, _vp]),
+    "qdc_pages_compact_workspace": (_i64, [_i64]),
+    "qdc_pages_compact": (_i32, [_vp] * 3 + [_i64] * 3 + [_vp] + [_i64] * 2
+                          + [_vp, _i64, _vp]),
+    "qdc_copy_pages": (_i32, [_vp] * 3 + [_i64] * 4 + [_vp, _vp]),
+    "qdc_delta_step": (_i32, [_vp, _i32, _vp, _i32, _i64, _vp, _i64] + [_vp] * 7 + [_i64] * 6
+                       + [_f32, _vp, _vp]),
+    "qdc_delta_scan_state": (_i32, [_vp, _i32] + [_vp] * 6 + [_i64] * 8 + [_vp, _i64, _vp]),
+}
+
 _lib = None
 
 
@@ -94,7 +114,8 @@ def lib():
                 f"{LIB_PATH} is not built; run `make -C qwendecisioncore.jl_amd/csrc` "
                 "or __graft_entry__.build()")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in (SIGNATURES | WORKSPACE_SIGNATURES).items():
+        for name, (res, args) in (SIGNATURES | WORKSPACE_SIGNATURES
+                                  | CACHE_SIGNATURES).items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args

@@ -711,13 +711,17 @@ def _token_rows(t: torch.Tensor) -> int | None:
 
 def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Tensor,
                decay: torch.Tensor, out_dtype: torch.dtype = torch.float32,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None,
+               state: torch.Tensor | None = None) -> torch.Tensor:
     """Gated delta rule recurrence (the DeltaNet "existing path", not a fused
     row op): fp32 q, k ``[B, S, KH, kd]``, v ``[B, S, H, vd]`` whose tokens are
     rows of contiguous heads (contiguous tensors, or the column blocks of one
     ``[T, q|k|v]`` buffer that ``delta_prologue(..., interleaved=True)``
     returns; q and k with the same row stride), contiguous beta and decay
-    ``[B, S, H]`` -> ``[B, S, H, vd]`` in ``out_dtype`` (or into ``out``)."""
+    ``[B, S, H]`` -> ``[B, S, H, vd]`` in ``out_dtype`` (or into ``out``).  ``state``
+    (contiguous float32 ``[B, H, vd, kd]``) takes the state after the last token, from
+    which ``cache_ops.delta_step`` goes on; only for key sizes of 32, 64 or 128, value
+    sizes of a multiple of 16 and rows of 16 bytes."""
     _device(q, k, v, beta, decay)
     for t in (beta, decay):
         if t.dtype != torch.float32 or not t.is_contiguous():
@@ -749,8 +753,22 @@ def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, beta: torch.Te
     long = S > (48 if B * H * (vd // 16) > 512 else 32)
     rows16 = (ld_k % 4 == 0 and ld_v % 4 == 0 and max(ld_k, ld_v) < 1 << 25
               and not any(t.data_ptr() % 16 for t in (q, k, v)))
-    need = lib().qdc_delta_scan_workspace(B, S, H, kd, vd) if long and rows16 else 0
-    if need:
+    need = lib().qdc_delta_scan_workspace(B, S, H, kd, vd) \
+        if rows16 and (long or state is not None) else 0
+    if state is not None:
+        _device(q, state)
+        if state.shape != (B, H, vd, kd) or state.dtype != torch.float32 \
+                or not state.is_contiguous():
+            raise ValueError("state must be a contiguous float32 [B, H, vd, kd] tensor")
+        if B == 0 or S == 0:
+            state.zero_()   # no token: empty
+            return out
+        if not need:
+            raise ValueError("no state is kept for these sizes, strides or alignments")
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(lib().qdc_delta_scan_state(args[0], args[1], state.data_ptr(), *args[2:],
+                                         work.data_ptr(), need, _stream(q)), "delta_scan")
+    elif need:
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
         check(lib().qdc_delta_scan_ws(*args, work.data_ptr(), need, _stream(q)), "delta_scan")
     else:

@@ -1,0 +1,1001 @@
+"""The operators of a cache that the backbone decodes from (include/qdc_hip_cache.h,
+qdc_amd.cache_ops): their argument checks, which need no GPU, and each against a plain
+form in 64 bits, at the lengths, pages, masks and rows where they can go wrong."""
+import math
+import os
+import re
+
+import numpy as np
+import pytest
+import torch
+
+from conftest import ROOT, normwise
+from qdc_amd import _lib, cache_ops, ops
+
+F32, BF16, X2 = _lib.QDC_F32, _lib.QDC_BF16, _lib.QDC_BF16X2
+FAKE, FAR = 0x10000, 1 << 56  # aligned addresses never dereferenced by validation
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.bfloat16]
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}  # half a step, relative
+
+
+# ---------------------------------------------------------- argument checks --
+def test_exports_match_header():
+    text = open(os.path.join(ROOT, "include", "qdc_hip_cache.h")).read()
+    names = set(re.findall(r"^\s*(?:const\s+)?\w+\s*\*?\s*(qdc_\w+)\s*\(", text, re.M))
+    assert names == set(_lib.CACHE_SIGNATURES)
+    for name in names:
+        assert hasattr(_lib.lib(), name), name
+    version = re.search(r'#define\s+QDC_HIP_CACHE_VERSION\s+"([^"]+)"', text).group(1)
+    assert _lib.lib().qdc_cache_version().decode() == version
+
+
+def test_prepare_paged_validation():
+    names = ("q_out", "k_out", "k_pages", "v_pages", "q", "k", "v", "q_norm", "k_norm", "cos",
+             "sin", "index", "positions", "table")
+
+    def f(dtype=BF16, tokens=4, heads=4, kv=2, hd=64, rd=16, tlen=100, rows=3, width=5, pages=7,
+          page=16, q_tok=256, q_head=64, k_tok=128, k_head=64, v_tok=128, v_head=64, flag=None,
+          **at):
+        ptr = [at.get(n, FAR + (i << 40)) for i, n in enumerate(names)]
+        return _lib.lib().qdc_prepare_paged(*ptr, tokens, heads, kv, hd, rd, tlen, rows, width,
+                                            pages, page, q_tok, q_head, k_tok, k_head, v_tok,
+                                            v_head, 1e-6, dtype, flag, None)
+
+    assert f(dtype=X2) == -3
+    assert f(hd=96) == -2 and f(page=8) == -2 and f(page=24) == -2 and f(page=512) == -2
+    assert f(rd=15) == -2 and f(rd=66) == -2 and f(heads=0) == -2 and f(kv=0) == -2
+    assert f(rows=0) == -2 and f(width=0) == -2 and f(pages=0) == -2 and f(tokens=-1) == -2
+    assert f(q_head=32) == -2 and f(k_tok=132) == -2 and f(v_head=68) == -2 and f(q_tok=-8) == -2
+    assert f(tokens=1 << 24) == -2                  # grid
+    for n in names:
+        if n != "k_out":
+            assert f(**{n: 0}) == -1, n
+    for n in ("q", "k_out", "v_pages", "cos"):
+        assert f(**{n: FAR + 8}) == -2, n
+    assert f(q=FAR + 64) == -5 and f(k_out=FAR + 64) == -5       # over q_out
+    assert f(flag=FAR + (2 << 40)) == -5                         # the flag in a page
+    assert f(tokens=0, q=0) == 0
+
+
+def test_paged_attention_validation():
+    names = ("q", "k", "v", "gate", "table", "index", "positions")
+    size = _lib.lib().qdc_paged_attention_workspace
+    need = size(3, 8, 2, 128, 5, 16, BF16)
+    assert need > 0
+    assert size(3, 8, 3, 128, 5, 16, BF16) == 0 and size(3, 8, 2, 96, 5, 16, BF16) == 0
+    assert size(3, 8, 2, 128, 5, 20, BF16) == 0 and size(3, 8, 2, 128, 5, 16, X2) == 0
+    assert size(1 << 24, 8, 2, 128, 5, 16, BF16) == 0            # the join's grid
+    assert size(1 << 15, 8, 2, 128, 1 << 20, 256, BF16) == 0     # tiles past 31 bits
+
+    def f(dtype=BF16, odt=BF16, n=3, heads=8, kv=2, hd=128, rows=4, width=5, pages=7, page=16,
+          q_tok=1024, q_head=128, g_tok=1024, g_head=128, o_tok=1024, scale=0.1, ws=FAR + (9 << 40),
+          nbytes=need, out=FAR + (8 << 40), flag=None, **at):
+        ptr = [at.get(x, FAR + (i << 40)) for i, x in enumerate(names)]
+        return _lib.lib().qdc_paged_attention(out, odt, *ptr, n, heads, kv, hd, rows, width, pages,
+                                              page, q_tok, q_head, g_tok, g_head, o_tok, scale,
+                                              dtype, ws, nbytes, flag, None)
+
+    assert f(dtype=X2) == -3 and f(odt=9) == -3
+    assert f(heads=7) == -2 and f(hd=96) == -2 and f(page=12) == -2 and f(rows=0) == -2
+    assert f(pages=0) == -2 and f(width=0) == -2 and f(n=-1) == -2
+    assert f(q_head=64) == -2 and f(q_tok=1028) == -2 and f(g_head=120) == -2
+    assert f(o_tok=1016) == -2 and f(o_tok=1028) == -2
+    assert f(scale=0.0) == -4 and f(scale=-1.0) == -4 and f(scale=float("inf")) == -4
+    assert f(scale=float("nan")) == -4 and f(scale=3e38) == -4
+    for x in ("q", "k", "v", "table", "index", "positions"):
+        assert f(**{x: 0}) == -1, x
+    assert f(out=0) == -1 and f(ws=0) == -1
+    assert f(q=FAR + 8) == -2 and f(gate=FAR + 4) == -2 and f(ws=FAR + (9 << 40) + 8) == -2
+    assert f(nbytes=need - 1) == -2
+    assert f(out=FAR + (1 << 40)) == -5 and f(ws=FAR + (8 << 40)) == -5
+    assert f(n=0, q=0) == 0
+
+
+def test_pages_validation():
+    lib = _lib.lib()
+    T, L, R, S = (FAR + (i << 40) for i in range(4))
+    I, P, W, POOL = (FAR + (i << 40) for i in range(4, 8))
+
+    def ext(pos=P, table=T, n=4, rows=5, width=6, pages=7, page=16, index=I, counts=None):
+        return lib.qdc_pages_extend(pos, table, L, R, S, index, counts, n, rows, width, pages, page,
+                                    None, None)
+
+    for bad in (dict(n=-1), dict(rows=0), dict(rows=1 << 18), dict(width=0), dict(pages=0),
+                dict(page=17), dict(n=1 << 24), dict(width=1 << 28, page=256)):
+        assert ext(**bad) == -2, bad
+    assert ext(pos=None) == -1 and ext(table=None) == -1 and ext(index=None) == -1
+    assert ext(pos=T + 4) == -5 and ext(index=L) == -5 and ext(counts=P + 8) == -5
+    assert ext(n=0, table=None, index=None, pos=None) == 0
+    free = lambda index=I, n=4, page=16: lib.qdc_pages_free(T, L, R, S, index, n, 5, 6, 7, page,  # noqa: E731
+                                                            None, None)
+    assert free(index=None) == -1 and free(index=R) == -5 and free(page=1) == -2
+    assert free(n=0, index=None) == 0
+
+    def fork(par=I, ch=P, n=4, pool=POOL, planes=2, heads=2, token=128, ws=W, nbytes=64):
+        return lib.qdc_pages_fork(T, L, R, S, par, ch, n, 5, 6, 7, 16, pool, planes, heads, token,
+                                  ws, nbytes, None, None)
+
+    assert fork(token=120) == -2 and fork(token=0) == -2 and fork(heads=0) == -2
+    assert fork(planes=-1) == -2 and fork(planes=1 << 16) == -2 and fork(nbytes=63) == -2
+    assert fork(ws=W + 4) == -2 and fork(pool=POOL + 4) == -2 and fork(planes=1 << 14, heads=4) == -2
+    assert fork(par=None) == -1 and fork(pool=None) == -1 and fork(ws=None) == -1
+    assert fork(ws=POOL) == -5 and fork(ch=T) == -5 and fork(n=0, par=None) == 0
+
+    def compact(table=T, pool=POOL, planes=2, nbytes=4096, pages=7, ws=W, have=100):
+        return lib.qdc_pages_compact(table, R, S, 5, 6, pages, pool, planes, nbytes, ws, have, None)
+
+    assert lib.qdc_pages_compact_workspace(7) == 100 and lib.qdc_pages_compact_workspace(0) == 0
+    assert compact(pages=0) == -2 and compact(nbytes=4100) == -2 and compact(have=99) == -2
+    assert compact(planes=1 << 16) == -2 and compact(ws=W + 8) == -2
+    assert compact(table=None) == -1 and compact(pool=None) == -1 and compact(ws=None) == -1
+    assert compact(ws=POOL + 16) == -5 and compact(pool=T) == -5
+
+    def copy(pool=POOL, src=I, dst=P, n=4, planes=2, items=7, nbytes=64):
+        return lib.qdc_copy_pages(pool, src, dst, n, planes, items, nbytes, None, None)
+
+    assert copy(n=-1) == -2 and copy(n=1 << 16) == -2 and copy(nbytes=8) == -2
+    assert copy(items=0) == -2 and copy(pool=POOL + 4) == -2
+    assert copy(planes=1 << 30, items=1 << 30, nbytes=1 << 30) == -2
+    assert copy(pool=None) == -1 and copy(src=None) == -1 and copy(src=POOL + 16) == -5
+    assert copy(n=0, pool=None) == 0 and copy(planes=0, pool=None) == 0
+
+
+def test_delta_step_validation():
+    names = ("proj", "conv", "a_decay", "dt_bias", "norm", "ring", "state", "index", "positions")
+
+    def f(odt=BF16, dt=BF16, ld=1024, taps=4, n=3, rows=5, kh=2, kd=64, vh=4, vd=32,
+          out=FAR + (12 << 40), flag=None, **at):
+        p = {x: at.get(x, FAR + (i << 40)) for i, x in enumerate(names)}
+        return _lib.lib().qdc_delta_step(out, odt, p["proj"], dt, ld, p["conv"], taps, p["a_decay"],
+                                         p["dt_bias"], p["norm"], p["ring"], p["state"],
+                                         p["index"], p["positions"], n, rows, kh, kd, vh, vd, 1e-6,
+                                         flag, None)
+
+    assert f(dt=X2) == -3 and f(odt=F32) == -3 and f(odt=X2, dt=F32) == -3
+    assert f(kd=96) == -2 and f(vd=24) == -2 and f(vd=272) == -2 and f(vh=3) == -2
+    assert f(taps=0) == -2 and f(taps=9) == -2 and f(rows=0) == -2 and f(n=-1) == -2
+    assert f(ld=2 * 128 + 128 + 128 + 7) == -2 and f(n=1 << 22) == -2
+    for x in names:
+        assert f(**{x: 0}) == -1, x
+    assert f(out=0) == -1 and f(state=FAR + 4) == -2
+    assert f(out=FAR + 16) == -5 and f(ring=FAR + (6 << 40)) == -5
+    assert f(flag=FAR + (6 << 40)) == -5 and f(n=0, proj=0) == 0
+
+
+def test_delta_scan_state_validation():
+    need = _lib.lib().qdc_delta_scan_workspace(2, 33, 4, 64, 32)
+
+    def f(state=FAR + (3 << 40), ws=FAR + (2 << 40), out=FAR + (1 << 40)):
+        return _lib.lib().qdc_delta_scan_state(out, F32, state, FAR, FAR, FAR, FAR, FAR, 2, 33, 4, 2,
+                                               64, 32, 128, 128, ws, need, None)
+
+    assert f(state=None) == -1 and f(state=FAR + 8) == -2 and f(state=FAR + 16) == -5
+    assert f(state=FAR + (2 << 40)) == -5 and f(state=FAR + (1 << 40) - 16) == -5
+
+
+def test_host_tensors_are_refused():
+    """Every operator needs device tensors, and a page table's are checked together."""
+    z = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt)  # noqa: E731
+    i = z(2, dt=torch.int32)
+    book = cache_ops.page_table(2, 3, 4, 16, "cpu")
+    assert book.free.tolist() == [4, 3, 2, 1, 0]
+    calls = [lambda: cache_ops.prepare_paged(z(2, 4, 64), z(2, 2, 64), z(2, 2, 64), z(64), z(64),
+                                             None, 0, 1e-6, i, i, book.table, z(4, 2, 16, 64),
+                                             z(4, 2, 16, 64)),
+             lambda: cache_ops.paged_attention(z(2, 4, 64), z(4, 2, 16, 64), z(4, 2, 16, 64),
+                                               book.table, i, i, 0.1),
+             lambda: cache_ops.extend_pages(book, i), lambda: cache_ops.free_pages(book, i),
+             lambda: cache_ops.fork_pages(book, i, i), lambda: cache_ops.compact_pages(book),
+             lambda: cache_ops.copy_pages(z(1, 4, 16), i, i),
+             lambda: cache_ops.delta_step(z(2, 600), z(384, 4), z(4), z(4), z(32), 1e-6,
+                                          z(2, 4, 384), z(2, 4, 32, 64), i, i, 2, 64, 4, 32)]
+    for call in calls:
+        with pytest.raises(ValueError, match="device tensors required"):
+            call()
+    for bad in ((0, 1, 1, 16), (1, 0, 1, 16), (1, 1, 0, 16), (1, 1, 1, 24)):
+        with pytest.raises(ValueError):
+            cache_ops.page_table(*bad, "cpu")
+
+
+# ------------------------------------------------------------------ helpers --
+def ints(values):
+    return torch.tensor(np.asarray(values, np.int32).reshape(-1), device=DEV)
+
+
+def flag():
+    return torch.zeros(1, dtype=torch.int32, device=DEV)
+
+
+def scattered(rng, lengths, page, spare=2, width=None):
+    """A table whose rows' pages lie anywhere among ``pages``."""
+    blocks = [-(-n // page) for n in lengths]
+    pages = sum(blocks) + spare
+    table = np.full((len(lengths), width or max(1, *blocks)), -1, np.int32)
+    order = iter(rng.permutation(pages))
+    for row, b in zip(table, blocks):
+        row[:b] = [next(order) for _ in range(b)]
+    return table, pages
+
+
+# ------------------------------------------------------------ prepare_paged --
+# heads, KV heads, head size, rotated values (none, all, halves that are no whole
+# 16-byte piece), page size
+PREPARE = [(4, 2, 64, 16, 16), (1, 1, 64, 0, 32), (3, 1, 64, 6, 16), (8, 2, 256, 64, 64),
+           (6, 6, 128, 128, 16), (2, 1, 256, 20, 256), (5, 5, 128, 24, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,rd,page", PREPARE)
+@pytest.mark.parametrize("T", [1, 37])
+def test_prepare_paged(T, H, KV, hd, rd, page, dtype):
+    """Against 64 bits.  fp32: the sum of squares is off by at most head_dim half
+    steps, its root and the products by a few, and a rotated value is a sum of two
+    such: (head_dim + 16) 2^-24 of the row's largest value.  bf16 adds its own half
+    step.  What is not stored is left as it was, bit for bit."""
+    rng = np.random.default_rng(T * 1000 + H * 100 + hd + rd)
+    rows, reach = 3, 150
+    table, pages = scattered(rng, [reach] * rows, page)
+    # distinct places; some entries no token, in each of the ways
+    places = rng.permutation(rows * reach)[:T]
+    index, pos = places // reach, places % reach
+    if T > 9:
+        pos[3], index[5] = -1, -1
+        index[6] = rows                               # no row of the cache
+        pos[7] = table.shape[1] * page                # behind the table
+        gone = (int(index[8]), int(pos[8]) // page)
+        table[gone] = pages                           # no page
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32)).to(dtype)  # noqa: E731
+    qg, kv = t(T, H, 2, hd), t(T, 2, KV + 1, hd)      # q beside a gate, k and v in wider rows
+    qn, kn = t(hd) * 0.1, t(hd) * 0.1
+    old = torch.full((2, pages, KV, page, hd), float("nan"), dtype=dtype)
+    tables = ops.rope_tables(max(1, table.shape[1] * page), rd, 1e4, DEV) if rd else None
+    d = lambda x: x.to(DEV)  # noqa: E731
+    qd, kvd, store, f = d(qg), d(kv), d(old), flag()
+    k_out = torch.empty((T, KV, hd), dtype=dtype, device=DEV) if T > 1 else None
+    got_q = cache_ops.prepare_paged(qd[:, :, 0], kvd[:, 0, :KV], kvd[:, 1, 1:], d(qn), d(kn), tables,
+                                    rd, 1e-6, ints(index), ints(pos), d(torch.from_numpy(table)),
+                                    store[0], store[1], k_out=k_out, error_flag=f)
+
+    live = [index[i] >= 0 and 0 <= pos[i] < table.shape[1] * page and index[i] < rows
+            and table[index[i], pos[i] // page] < pages for i in range(T)]
+    at = np.where(live, pos, 0)
+
+    def expect(x, w):
+        x, w = x.double(), w.double()
+        x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * (1 + w)
+        top = x.abs().amax(-1, keepdim=True)
+        if rd:
+            cos, sin = (c.double().cpu()[at][:, None] for c in tables)
+            keep = torch.tensor(live)[:, None, None]
+            cos, sin = torch.where(keep, cos, 1.0), torch.where(keep, sin, 0.0)
+            a, b = x[..., :rd // 2], x[..., rd // 2:rd]
+            x = torch.cat([a * cos - b * sin, b * cos + a * sin, x[..., rd:]], -1)
+        tol = (hd + 16) * 2.0 ** -24 * top
+        return x, tol if dtype == torch.float32 else tol + HALF[dtype] * x.abs()
+
+    def near(got, pair):
+        exp, tol = pair
+        assert ((got.double().cpu() - exp).abs() <= tol).all()
+
+    near(got_q, expect(qg[:, :, 0], qn))
+    k = expect(kv[:, 0, :KV], kn)
+    if k_out is not None:
+        near(k_out, k)
+    got = store.cpu()
+    touched = torch.zeros(pages, page, dtype=torch.bool)
+    for i in range(T):
+        if live[i]:
+            p, o = int(table[index[i], pos[i] // page]), int(pos[i]) % page
+            touched[p, o] = True
+            near(got[0, p, :, o], (k[0][i], k[1][i]))
+            assert torch.equal(got[1, p, :, o], kv[i, 1, 1:])
+    assert torch.isnan(got.float()[:, ~touched.unsqueeze(1).expand(pages, KV, page)]).all()
+    bad = T > 9
+    assert f.item() == int(bad)
+
+
+@pytest.mark.gpu
+def test_prepare_paged_refusals():
+    z = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt, device=DEV)  # noqa: E731
+    i, q, k, n, pg = ints([0, 1]), z(2, 4, 64), z(2, 2, 64), z(64), z(4, 2, 16, 64)
+    table = z(2, 3, dt=torch.int32)
+    ok = dict(q=q, k=k, v=k.clone(), q_norm=n, k_norm=n, tables=None, rotary_dim=0, eps=1e-6,
+              rows=i, positions=i, table=table, k_pages=pg, v_pages=pg.clone())
+    cache_ops.prepare_paged(**ok)
+    empty = dict(ok, q=q[:0], k=k[:0], v=k[:0], rows=i[:0], positions=i[:0])
+    assert cache_ops.prepare_paged(**empty).shape == (0, 4, 64)
+    for bad in (dict(q=q[:1]), dict(v=z(2, 1, 64)), dict(q=q.bfloat16()), dict(q_norm=z(32)),
+                dict(rows=i.long()), dict(positions=ints([0])), dict(table=table.float()),
+                dict(k_pages=z(4, 1, 16, 64)), dict(v_pages=pg.bfloat16()),
+                dict(k_pages=pg.transpose(0, 1)), dict(rotary_dim=16),
+                dict(q=z(2, 4, 96), k=z(2, 2, 96), v=z(2, 2, 96), q_norm=z(96), k_norm=z(96),
+                     k_pages=z(4, 2, 16, 96), v_pages=z(4, 2, 16, 96)),
+                dict(k_pages=z(4, 2, 24, 64), v_pages=z(4, 2, 24, 64)),
+                dict(q_out=q), dict(k_out=z(2, 2, 64, dt=torch.bfloat16)), dict(v_pages=pg),
+                dict(error_flag=z(1)), dict(error_flag=torch.zeros(1, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            cache_ops.prepare_paged(**dict(ok, **bad))
+
+
+# ---------------------------------------------------------- paged_attention --
+def attend_exact(q, k, v, table, index, pos, scale, gate, page):
+    """64 bits, and per element what the result may differ by before its own rounding.
+
+    A score is a sum of head_dim fp32 products and a multiply: off by at most
+    (head_dim + 2) 2^-24 of scale sum |q k|, and the exponent taken from it by 2 steps
+    of its own size; a weight exp() of that by as much relatively, with 4 half steps of
+    the exponential; sums of n weights and products by 2 n half steps at worst, in
+    chains of a tile's and of the tiles' lengths, n <= 2 (32 + tiles); the two terms of
+    a weight are 2^-16 off (the first is cut to 8 bits, the rest below 2^-7 of it rounded to
+    8 bits).  All of it times the weighted mean of |v|."""
+    n, H, hd = q.shape
+    KV = k.shape[1]
+    out, tol = torch.zeros(n, H, hd, dtype=torch.float64), torch.zeros(n, H, hd, dtype=torch.float64)
+    for i in range(n):
+        if index[i] < 0 or pos[i] < 0 or index[i] >= len(table):
+            continue
+        places = [(int(table[index[i], j // page]), j % page)
+                  for j in range(min(int(pos[i]) + 1, table.shape[1] * page))]
+        places = [x for x in places if 0 <= x[0] < k.shape[0]]
+        if not places:
+            continue
+        p, o = (torch.tensor(x) for x in zip(*places))
+        for g in range(KV):
+            kk, vv = k[p, g, o].double(), v[p, g, o].double()
+            for h in range(g * (H // KV), (g + 1) * (H // KV)):
+                qq = q[i, h].double()
+                s = (kk * qq).sum(-1) * scale
+                w = torch.softmax(s, 0)
+                out[i, h] = (w[:, None] * vv).sum(0)
+                size = float((kk.abs() * qq.abs()).sum(-1).max()) * scale
+                top = float(s.abs().max())
+                rel = 2 * ((hd + 2) * size + 4 * top + 4 + 2 * (32 + len(places) / 16)) * 2.0 ** -24
+                tol[i, h] = (rel + 2.0 ** -16) * (w[:, None] * vv.abs()).sum(0)
+    if gate is not None:
+        s = torch.sigmoid(gate.double())
+        out, tol = out * s, tol * s + out.abs() * s * 2.0 ** -21
+    return out.reshape(n, H * hd), tol.reshape(n, H * hd)
+
+
+def attend_case(seed, H, KV, hd, page, lengths, dtype, order=None, spread=1.5):
+    """q, gate, pages that hold NaN wherever no token is, table, lengths."""
+    rng = np.random.default_rng(seed)
+    table, pages = scattered(rng, lengths, page)
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32)).to(dtype)  # noqa: E731
+    kv = t(2, pages, KV, page, hd)
+    held = np.zeros((pages, page), bool)
+    for row, n in zip(table, lengths):
+        for j in range(n):
+            held[row[j // page], j % page] = True
+    kv[:, ~torch.from_numpy(held).unsqueeze(1).expand(pages, KV, page)] = float("nan")
+    index = np.arange(len(lengths)) if order is None else np.asarray(order)
+    return t(len(index), H, hd) * spread, t(len(index), H, 2, hd)[:, :, 0], kv[0], kv[1], table, index
+
+
+def attend_check(case, pos, page, dtype, out_dtype, gated=True, table=None):
+    q, gate, k, v, real, index = case
+    table = real if table is None else table
+    scale = q.shape[2] ** -0.5
+    f = flag()
+    got = cache_ops.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), torch.from_numpy(table).to(DEV),
+                                    ints(index), ints(pos), scale,
+                                    gate=gate.to(DEV) if gated else None, out_dtype=out_dtype,
+                                    error_flag=f)
+    exp, tol = attend_exact(q, k, v, table, index, pos, scale, gate if gated else None, page)
+    if out_dtype == ops.BF16X2:
+        got, tol = ops.join_split(got), tol + 2.0 ** -17 * exp.abs()
+    elif out_dtype == torch.bfloat16 or (out_dtype is None and dtype == torch.bfloat16):
+        tol = tol + HALF[torch.bfloat16] * (exp.abs() + tol)
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    assert ((got - exp).abs() <= tol).all(), float(((got - exp).abs() / tol.clamp(min=1e-30)).max())
+    return f.item()
+
+
+# query heads of a KV head on both sides of 4 (a pass of the join) and 16 (a group);
+# lengths around the tiles (16, 32), the pages and the four wavefronts' share
+LENGTHS = [1, 0, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 200, 300]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,page", [(4, 2, 64, 16), (8, 2, 256, 64), (5, 1, 128, 32),
+                                          (16, 1, 64, 16), (20, 1, 128, 16), (3, 3, 256, 128),
+                                          (34, 2, 64, 256)])
+def test_paged_attention(H, KV, hd, page, dtype):
+    case = attend_case(H * hd + page, H, KV, hd, page, LENGTHS, dtype,
+                       order=np.random.default_rng(H).permutation(len(LENGTHS)))
+    pos = np.array(LENGTHS)[case[-1]] - 1
+    for out, gated in ((None, True), (torch.float32, False), (ops.BF16X2, True)):
+        if out == ops.BF16X2 and dtype == torch.float32 and hd == 64:
+            out = torch.bfloat16
+        assert attend_check(case, pos, page, dtype, out, gated) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_attention_many_entries(dtype):
+    """More entries than a wavefront sees at once, several of one row at positions of
+    their own, and entries that are no token among them."""
+    rng = np.random.default_rng(5)
+    lengths = [int(x) for x in rng.integers(0, 90, 40)]
+    order = rng.integers(0, 40, 151)
+    case = attend_case(6, 4, 2, 64, 16, lengths, dtype, order=order)
+    pos = np.array([rng.integers(-1, lengths[r]) if lengths[r] else -1 for r in order])
+    index = case[-1]
+    index[[3, 70, 150]] = -1
+    assert attend_check(case, pos, 16, dtype, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,lengths", [(4, 1, 64, [9000]), (8, 2, 256, [3001, 2, 777]),
+                                             (12, 4, 128, [0, 1, 5000, 0, 33])])
+def test_paged_attention_long(H, KV, hd, lengths, dtype):
+    """One row's keys over many workgroups, and very different rows beside each other."""
+    case = attend_case(hd, H, KV, hd, 64, lengths, dtype, spread=3.0)
+    assert attend_check(case, np.array(lengths) - 1, 64, dtype, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_attention_rising_scores(dtype):
+    """Scores that rise along the keys by hundreds, so that begun sums are rescaled,
+    and a last key far below: its weight is nothing."""
+    q, gate, k, v, table, index = case = attend_case(9, 4, 1, 64, 16, [400], dtype)
+    for j in range(400):
+        k[table[0, j // 16], 0, j % 16] = torch.where(q[0, 0] > 0, 1.0, -1.0) * (j / 40.0)
+    k[table[0, 399 // 16], 0, 399 % 16] = -k[table[0, 398 // 16], 0, 398 % 16]
+    assert attend_check(case, np.array([399]), 16, dtype, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_attention_bad_tables(dtype):
+    """Pages that are none, positions behind the table and rows that are none: left out
+    and flagged, the other entries as they should be."""
+    lengths = [100, 130, 64, 40]
+    case = attend_case(11, 4, 2, 64, 16, lengths, dtype, order=[0, 1, 2, 3, 9])
+    table = case[4].copy()
+    table[0, 2], table[0, 6], table[2, :] = -1, case[2].shape[0], 1 << 30
+    pos = np.array([99, 129, 63, 39, 10])
+    assert attend_check(case, pos, 16, dtype, None, table=table) == 1
+    full = table.shape[1] * 16                       # 144: row 1 holds 130, the rest NaN
+    short = [144, 144]
+    case = attend_case(12, 4, 2, 64, 16, short, dtype)
+    assert attend_check(case, np.array([full + 50, 2 ** 31 - 1]), 16, dtype, None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_attention_nan_and_inf(dtype):
+    """A NaN or infinity that a row really holds shows in that row alone; a score of
+    minus infinity is a weight of nothing."""
+    q, gate, k, v, table, index = attend_case(13, 4, 2, 64, 16, [50, 60, 70, 80], dtype)
+    k[table[0, 1], 0, 3, 5] = float("nan")
+    v[table[1, 2], 1, 4, 7] = float("inf")
+    q[2, 0, 0] = 1.0
+    k[table[2, 0], 0, 2, 0] = -float("inf")          # head 0 of entry 2: key 2 masked
+    d = lambda x: x.to(DEV)  # noqa: E731
+    got = cache_ops.paged_attention(d(q), d(k), d(v), d(torch.from_numpy(table)), ints(index),
+                                    ints([49, 59, 69, 79]), 0.125).float().cpu().view(4, 4, 64)
+    assert torch.isnan(got[0, :2]).all() and torch.isfinite(got[0, 2:]).all()
+    assert torch.isfinite(got[1, :2]).all() and (got[1, 2:, 7] == float("inf")).all()
+    assert torch.isfinite(got[1, 2:, :7]).all() and torch.isfinite(got[3]).all()
+    exp, _ = attend_exact(q, k, v, table, index, [49, 59, 69, 79], 0.125, None, 16)
+    assert normwise(got[2, 0], exp.view(4, 4, 64)[2, 0]) <= 2 * HALF[dtype] + 1e-5
+
+
+@pytest.mark.gpu
+def test_paged_attention_refusals():
+    z = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt, device=DEV)  # noqa: E731
+    i, q, pg, table = ints([0, 1]), z(2, 4, 64), z(4, 2, 16, 64), z(2, 3, dt=torch.int32)
+    ok = dict(q=q, k_pages=pg, v_pages=pg, table=table, rows=i, positions=i, scale=0.1)
+    cache_ops.paged_attention(**ok)
+    assert cache_ops.paged_attention(**dict(ok, q=q[:0], rows=i[:0], positions=i[:0])).shape == (0, 256)
+    for bad in (dict(q=q[0]), dict(q=q.half()), dict(q=z(2, 3, 64)), dict(v_pages=pg[:2]),
+                dict(k_pages=pg.bfloat16(), v_pages=pg.bfloat16()), dict(table=table.long()),
+                dict(rows=ints([0])), dict(positions=i.long()), dict(scale=0.0),
+                dict(scale=float("nan")), dict(gate=q[:1]), dict(gate=q.bfloat16()),
+                dict(out_dtype=torch.float16), dict(out_dtype="f8"),
+                dict(q=z(2, 4, 32), k_pages=z(4, 2, 16, 32), v_pages=z(4, 2, 16, 32)),
+                dict(k_pages=z(4, 2, 10, 64), v_pages=z(4, 2, 10, 64)),
+                dict(table=z(2, 3, dt=torch.int32).cpu()), dict(error_flag=i.long())):
+        with pytest.raises(ValueError):
+            cache_ops.paged_attention(**dict(ok, **bad))
+
+
+# -------------------------------------------------------------------- pages --
+class Model:
+    """The page table in plain Python, as the operators' documentation has it."""
+
+    def __init__(self, rows, width, pages, page):
+        self.rows, self.width, self.pages, self.page = rows, width, pages, page
+        self.table = [[] for _ in range(rows)]
+        self.lengths, self.refs = [0] * rows, [0] * pages
+        self.stack = list(range(pages - 1, -1, -1))
+
+    def good(self, rows):
+        rows = [r for r in rows if r >= 0]
+        return len(set(rows)) == len(rows) and all(r < self.rows for r in rows)
+
+    def extend(self, rows, counts):
+        live = [(r, c) for r, c in zip(rows, counts) if r >= 0]
+        if not self.good(rows) or any(c < 0 or self.lengths[r] + c > self.width * self.page
+                                      for r, c in live):
+            return [-1] * len(rows), True
+        need = [-(-(self.lengths[r] + c) // self.page) - len(self.table[r]) for r, c in live]
+        if sum(need) > len(self.stack):
+            return [-1] * len(rows), True
+        out = []
+        need = iter(need)
+        for r, c in zip(rows, counts):
+            out.append(-1 if r < 0 else self.lengths[r])
+            if r >= 0:
+                for _ in range(next(need)):
+                    self.table[r].append(self.stack.pop())
+                    self.refs[self.table[r][-1]] = 1
+                self.lengths[r] += c
+        return out, False
+
+    def free(self, rows):
+        if not self.good(rows):
+            return True
+        listed = [p for r in rows if r >= 0 for p in self.table[r]]
+        for p in listed:
+            self.refs[p] -= 1
+        last = {p: i for i, p in enumerate(listed)}
+        left = [p for i, p in enumerate(listed) if self.refs[p] == 0 and last[p] == i]
+        self.stack += left[::-1]
+        for r in rows:
+            if r >= 0:
+                self.table[r], self.lengths[r] = [], 0
+        return False
+
+    def fork(self, parents, children, data=None):
+        live = [(p, c) for p, c in zip(parents, children) if p >= 0 and c >= 0]
+        kids = [c for _, c in live]
+        if not self.good(kids) or any(p >= self.rows or p in kids for p, _ in live) or \
+                any(self.lengths[c] for c in kids):
+            return True
+        if sum(self.lengths[p] % self.page > 0 for p, _ in live) > len(self.stack):
+            return True
+        for p, c in live:
+            full, part = divmod(self.lengths[p], self.page)
+            self.table[c], self.lengths[c] = self.table[p][:full], self.lengths[p]
+            for x in self.table[c]:
+                self.refs[x] += 1
+            if part:
+                new = self.stack.pop()
+                self.refs[new] = 1
+                self.table[c].append(new)
+                if data is not None:
+                    data[:, new, :, :part] = data[:, self.table[p][full], :, :part]
+        return False
+
+    def compact(self, data=None):
+        live = [p for p in range(self.pages) if self.refs[p] > 0]
+        m = len(live)
+        holes = [p for p in range(m) if self.refs[p] <= 0]
+        to = dict(zip([p for p in live if p >= m], holes))
+        for src, dst in to.items():
+            self.refs[dst], self.refs[src] = self.refs[src], 0
+            if data is not None:
+                data[:, dst] = data[:, src]
+        self.table = [[to.get(p, p) for p in row] for row in self.table]
+        self.stack = list(range(self.pages - 1, m - 1, -1))
+
+    def check(self, book):
+        table = [row + [-1] * (self.width - len(row)) for row in self.table]
+        assert book.table.tolist() == table
+        assert book.lengths.tolist() == self.lengths and book.refs.tolist() == self.refs
+        free = book.free.tolist()
+        assert free[0] == len(self.stack) and free[1:1 + free[0]] == self.stack
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,pages,page,dtype,dim", [(12, 6, 40, 16, torch.float32, 4),
+                                                             (7, 3, 11, 64, torch.bfloat16, 64),
+                                                             (30, 9, 300, 32, torch.bfloat16, 8)])
+def test_pages_life(rows, width, pages, page, dtype, dim):
+    """Rows that grow, fork, end and move together in any order, whole numbers and
+    copies exact after every call; calls that cannot be done whole among them."""
+    rng = np.random.default_rng(rows * page)
+    book, ref = cache_ops.page_table(rows, width, pages, page, DEV), Model(rows, width, pages, page)
+    data = torch.from_numpy(rng.standard_normal((3, pages, 2, page, dim), dtype=np.float32)).to(dtype)
+    pool = data.to(DEV)
+    refused = {"extend": 0, "fork": 0, "free": 0}
+    for step in range(60):
+        f = flag()
+        what = rng.choice(["extend", "extend", "extend", "fork", "fork", "free", "compact"])
+        n = int(rng.integers(1, rows // 2 + 2))
+        some = rng.permutation(rows)[:n].tolist()
+        if rng.random() < 0.15:
+            some[rng.integers(n)] = int(rng.choice([-1, rows, some[0]]))
+        if what == "extend":
+            counts = [int(c) for c in rng.choice([0, 1, 1, page - 1, page, 2 * page + 3], len(some))]
+            if rng.random() < 0.1:
+                counts[-1] = -1
+            got = cache_ops.extend_pages(book, ints(some), ints(counts), error_flag=f)
+            exp, bad = ref.extend(some, counts)
+            assert got.tolist() == exp
+        elif what == "fork":
+            empty = [r for r in range(rows) if not ref.lengths[r]]
+            rng.shuffle(empty)
+            kids = (empty + some)[:n]
+            parents = [int(x) for x in rng.integers(-1, rows, len(kids))]
+            cache_ops.fork_pages(book, ints(parents), ints(kids), pool, error_flag=f)
+            bad = ref.fork(parents, kids, data)
+        elif what == "free":
+            cache_ops.free_pages(book, ints(some), error_flag=f)
+            bad = ref.free(some)
+        else:
+            cache_ops.compact_pages(book, pool)
+            ref.compact(data)
+            bad = False
+        refused[what] = refused.get(what, 0) + bool(bad)
+        assert f.item() == int(bad), (step, what)
+        ref.check(book)
+        assert torch.equal(pool.cpu(), data), (step, what)
+    assert refused["extend"] and refused["fork"]
+
+
+@pytest.mark.gpu
+def test_pages_many_rows():
+    """More rows in a call than the bookkeeping takes at once, pages that hundreds of
+    rows share, and rows that free them in one call."""
+    rows, width, pages, page = 2600, 4, 6000, 16
+    book, ref = cache_ops.page_table(rows, width, pages, page, DEV), Model(rows, width, pages, page)
+    rng = np.random.default_rng(3)
+    some = rng.permutation(rows)[:1300].tolist()
+    counts = [int(c) for c in rng.integers(1, width * page + 1, 1300)]
+    got, (exp, bad) = cache_ops.extend_pages(book, ints(some), ints(counts)), ref.extend(some, counts)
+    assert got.tolist() == exp and not bad
+    ref.check(book)
+    kids = [r for r in range(rows) if not ref.lengths[r]][:1200]
+    parents = [some[i % 3] for i in range(len(kids))]
+    cache_ops.fork_pages(book, ints(parents), ints(kids))
+    assert not ref.fork(parents, kids)
+    ref.check(book)
+    gone = rng.permutation(some[:900] + kids[:1100]).tolist()
+    cache_ops.free_pages(book, ints(gone))
+    assert not ref.free(gone)
+    ref.check(book)
+    cache_ops.compact_pages(book)
+    ref.compact()
+    ref.check(book)
+
+
+@pytest.mark.gpu
+def test_fork_and_free_give_the_stack_back():
+    book = cache_ops.page_table(9, 8, 50, 16, DEV)
+    cache_ops.extend_pages(book, ints([4, 2]), ints([50, 17]))
+    before = [t.clone() for t in book[:4]]
+    for _ in range(3):
+        cache_ops.fork_pages(book, ints([4, 2, 4, 4]), ints([0, 8, 1, 3]))
+        cache_ops.free_pages(book, ints([0, 8, 1, 3]))
+        for a, b in zip(before, book[:4]):
+            assert torch.equal(a, b)
+    # a parent that ends before its children: they keep its pages
+    cache_ops.fork_pages(book, ints([4]), ints([0]))
+    cache_ops.free_pages(book, ints([4]))
+    assert book.lengths.tolist() == [50, 0, 17, 0, 0, 0, 0, 0, 0]
+    assert sorted(book.refs.tolist())[-6:] == [1] * 6 and book.free[0].item() == 50 - 6
+
+
+@pytest.mark.gpu
+def test_copy_pages():
+    rng = np.random.default_rng(1)
+    for shape, dtype in (((2, 9, 4), torch.float32), ((1, 300, 3, 40), torch.bfloat16),
+                         ((5, 20, 1025, 4), torch.float32)):
+        data = torch.from_numpy(rng.standard_normal(shape, dtype=np.float32)).to(dtype)
+        pool, f = data.to(DEV), flag()
+        order = rng.permutation(shape[1])
+        src, dst = order[:3].tolist() * 2, order[3:9].tolist()
+        cache_ops.copy_pages(pool, ints(src), ints(dst), error_flag=f)
+        data[:, dst] = data[:, src]
+        assert torch.equal(pool.cpu(), data) and f.item() == 0
+        # dst twice: the first; dst that is a src, src and dst out of range: not at all;
+        # a negative index: left out
+        a, b, c, d, e = order[:5].tolist()
+        n = shape[1]
+        cache_ops.copy_pages(pool, ints([a, b, c, n, a, -1]), ints([d, d, a, e, n, e]), error_flag=f)
+        data[:, d] = data[:, a]
+        assert torch.equal(pool.cpu(), data) and f.item() == 1
+    cache_ops.copy_pages(pool, ints([]), ints([]))
+
+
+@pytest.mark.gpu
+def test_pages_refusals():
+    book = cache_ops.page_table(3, 4, 5, 16, DEV)
+    i, pool = ints([0, 1]), torch.zeros(2, 5, 2, 16, 8, device=DEV)
+    for bad in (lambda: cache_ops.extend_pages(book, i.long()),
+                lambda: cache_ops.extend_pages(book, i, ints([1])),
+                lambda: cache_ops.extend_pages(book, i, positions=ints([1])),
+                lambda: cache_ops.extend_pages(book._replace(page_size=20), i),
+                lambda: cache_ops.extend_pages(book._replace(free=book.free[1:]), i),
+                lambda: cache_ops.extend_pages(book._replace(lengths=book.refs), i),
+                lambda: cache_ops.free_pages(book, i.cpu()),
+                lambda: cache_ops.fork_pages(book, i, ints([2])),
+                lambda: cache_ops.fork_pages(book, i, i, pool[:, :4]),
+                lambda: cache_ops.fork_pages(book, i, i, pool.transpose(2, 3)),
+                lambda: cache_ops.fork_pages(book, i, i, torch.zeros(2, 5, 2, 16, 6, device=DEV,
+                                                                     dtype=torch.bfloat16)),
+                lambda: cache_ops.compact_pages(book, pool[:, :4]),
+                lambda: cache_ops.copy_pages(pool[:, :, 0], i, i),
+                lambda: cache_ops.copy_pages(torch.zeros(2, 5, 3, device=DEV), i, i),
+                lambda: cache_ops.copy_pages(pool, i, ints([2]))):
+        with pytest.raises(ValueError):
+            bad()
+    assert book.lengths.tolist() == [0, 0, 0]
+
+
+# --------------------------------------------------------------- delta_step --
+# key heads, value heads, key size, value size, taps
+STEP = [(2, 4, 128, 128, 4), (1, 1, 32, 16, 1), (2, 2, 64, 48, 2), (1, 4, 128, 256, 4),
+        (4, 8, 32, 80, 8), (3, 3, 64, 144, 3)]
+
+
+def step_exact(s, KH, kd, H, vd, taps):
+    """64 bits on the CPU; rows are updated in place."""
+    kw, vw = KH * kd, H * vd
+    cq = 2 * kw + vw
+    out = torch.zeros(len(s["rows"]), H, vd, dtype=torch.float64)
+    proj, ring, state = s["proj"].double(), s["ring"].double(), s["state"].double()
+    done = set()
+    for i, (row, p) in enumerate(zip(s["rows"], s["pos"])):
+        if row < 0 or p < 0 or row >= len(ring) or row in done:
+            continue
+        done.add(row)
+        ring[row, p % taps] = proj[i, :cq]
+        x = torch.zeros(cq, dtype=torch.float64)
+        for lag in range(min(taps, p + 1)):
+            x += ring[row, (p - lag) % taps] * s["conv"][:, taps - 1 - lag].double()
+        x = x * torch.sigmoid(x)
+        q, k, v = x[:kw].view(KH, kd), x[kw:2 * kw].view(KH, kd), x[2 * kw:].view(H, vd)
+        q = q / torch.sqrt((q * q).sum(-1, keepdim=True) + 1e-6) / math.sqrt(kd)
+        k = k / torch.sqrt((k * k).sum(-1, keepdim=True) + 1e-6)
+        q, k = (t.repeat_interleave(H // KH, 0) for t in (q, k))
+        tail = proj[i, cq:]
+        z, a, b = tail[:vw].view(H, vd), tail[vw:vw + H], tail[vw + H:vw + 2 * H]
+        f = torch.exp(s["a_decay"].double() *
+                      torch.nn.functional.softplus(a + s["dt_bias"].double(), threshold=200.0))
+        S = state[row] * f[:, None, None] if p else torch.zeros_like(state[row])
+        u = torch.sigmoid(b)[:, None] * (v - (S * k[:, None]).sum(-1))
+        S = S + u[..., None] * k[:, None]
+        state[row] = S
+        o = (S * q[:, None]).sum(-1)
+        o = o / torch.sqrt((o * o).mean(-1, keepdim=True) + 1e-6) * s["norm"].double()
+        out[i] = o * z * torch.sigmoid(z)
+    return out.view(-1, vw), ring, state
+
+
+def step_case(seed, KH, H, kd, vd, taps, n, rows, dtype):
+    rng = np.random.default_rng(seed)
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32))  # noqa: E731
+    cq = 2 * KH * kd + H * vd
+    return {"proj": t(n, cq + H * vd + 2 * H + 5).to(dtype), "conv": t(cq, taps) * 0.5,
+            "a_decay": -torch.exp(t(H)), "dt_bias": t(H), "norm": (1 + 0.1 * t(vd)).to(dtype),
+            "ring": t(rows, taps, cq).to(dtype), "state": t(rows, H, vd, kd) * 0.3,
+            "rows": [int(r) for r in rng.permutation(rows)[:n]],
+            "pos": [int(p) for p in rng.integers(0, 2 * taps + 3, n)]}
+
+
+def step_run(s, KH, H, kd, vd, out_dtype=None, error_flag=None):
+    d = {k: v.to(DEV) for k, v in s.items() if isinstance(v, torch.Tensor)}
+    out = cache_ops.delta_step(d["proj"], d["conv"], d["a_decay"], d["dt_bias"], d["norm"], 1e-6,
+                               d["ring"], d["state"], ints(s["rows"]), ints(s["pos"]), KH, kd, H, vd,
+                               out_dtype=out_dtype, error_flag=error_flag)
+    return out, d["ring"], d["state"]
+
+
+def step_near(got, exp, KH, kd, vd, dtype, split=False):
+    """fp32 throughout: a state is one product and sum after dot products of kd terms,
+    off by at most (kd + 40) half steps of the largest value in its head (u and the
+    gates take some tens of operations); an output row is normalised, so its values
+    are off by as much of the row's largest, then rounded to its type."""
+    (out, ring, state), (eo, er, es) = got, exp
+    assert torch.equal(ring.double().cpu(), er)
+    top = es.abs().amax((-1, -2), keepdim=True).clamp(min=1.0)
+    assert ((state.double().cpu() - es).abs() <= (kd + 40) * 2.0 ** -24 * top).all()
+    out = (ops.join_split(out) if split else out).double().cpu()
+    rows = eo.view(len(eo), -1, vd)
+    size = rows.abs().amax(-1, keepdim=True).expand_as(rows).reshape_as(eo)
+    half = 2.0 ** -17 if split else HALF[dtype]
+    # the norm divides by the row's size: relative errors of its values come out alike
+    tol = 4 * (kd + vd + 40) * 2.0 ** -24 * size + half * eo.abs()
+    assert ((out - eo).abs() <= tol).all(), float(((out - eo).abs() / tol.clamp(min=1e-30)).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("KH,H,kd,vd,taps", STEP)
+def test_delta_step(KH, H, kd, vd, taps, dtype):
+    s = step_case(kd + vd, KH, H, kd, vd, taps, 7, 9, dtype)
+    f = flag()
+    got = step_run(s, KH, H, kd, vd, error_flag=f)
+    step_near(got, step_exact(s, KH, kd, H, vd, taps), KH, kd, vd, dtype)
+    assert f.item() == 0
+    if dtype == torch.bfloat16:
+        got = step_run(s, KH, H, kd, vd, out_dtype=ops.BF16X2)
+        step_near(got, step_exact(s, KH, kd, H, vd, taps), KH, kd, vd, dtype, split=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_delta_step_rows(dtype):
+    """Rows at position 0 start empty whatever they held, NaN too; entries that are no
+    token, a row named twice and one that is none: zeros, and the cache as it was."""
+    KH, H, kd, vd, taps = 2, 4, 64, 32, 4
+    s = step_case(3, KH, H, kd, vd, taps, 9, 12, dtype)
+    s["pos"] = [0, 2, -1, 9, 5, 6, 7, 1, 3]
+    r0, r1 = s["rows"][0], s["rows"][1]
+    s["ring"][r0], s["state"][r0] = float("nan"), float("nan")
+    s["ring"][r1, 3] = float("nan")             # position -1 of a row at position 2
+    s["rows"][4], s["rows"][5], s["rows"][6] = -1, s["rows"][3], 12
+    f = flag()
+    got = step_run(s, KH, H, kd, vd, error_flag=f)
+    exp = step_exact(s, KH, kd, H, vd, taps)
+    assert f.item() == 1 and (got[0][[2, 4, 5, 6]] == 0).all()
+    assert torch.isnan(got[1].float().cpu()[r0, 1:]).all()
+    assert torch.isfinite(got[2][r0]).all()
+    exp = (exp[0], torch.nan_to_num(exp[1]), exp[2])
+    step_near((got[0], torch.nan_to_num(got[1].double()), got[2]), exp, KH, kd, vd, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,KH,H,kd,vd", [(5, 2, 4, 128, 128), (40, 1, 2, 64, 48), (70, 16, 64, 32, 32)])
+def test_steps_continue_a_scan(S, KH, H, kd, vd):
+    """A prompt through the prologue, the scan (with its last state) and the gated norm,
+    and then tokens one by one: the same as the whole sequence at once, to the fp32 bar
+    of 1e-5 that both forms hold."""
+    taps, more, dtype = 4, 6, torch.float32
+    rng = np.random.default_rng(S)
+    kw, vw = KH * kd, H * vd
+    cq = 2 * kw + vw
+    width = -(-(cq + vw + 2 * H) // 4) * 4
+    B = 9 if H == 64 else 2                # both forms of the scan
+    d = lambda x: torch.from_numpy(np.asarray(x, np.float32)).to(DEV)  # noqa: E731
+    proj = d(rng.standard_normal((B, S + more, width)))
+    conv, norm = d(rng.standard_normal((cq, taps)) * 0.5), d(1 + 0.1 * rng.standard_normal(vd))
+    decay, bias = d(-np.exp(rng.standard_normal(H))), d(rng.standard_normal(H) - 2)
+
+    def whole(n):
+        p = proj[:, :n].reshape(B * n, width).contiguous()
+        q, k, v, beta, dec = ops.delta_prologue(p, conv, decay, bias, n, KH, kd, H, vd,
+                                                interleaved=True)
+        shape = lambda t: t.view(B, n, *t.shape[1:])  # noqa: E731
+        return [shape(t) for t in (q, k, v, beta, dec)]
+
+    state = torch.empty(B, H, vd, kd, device=DEV)
+    out = ops.delta_scan(*whole(S), state=state)
+    assert normwise(out.cpu(), ops.delta_scan(*whole(S)).cpu()) <= 1e-6
+    ring = torch.full((B, taps, cq), float("nan"), device=DEV)
+    for p in range(max(0, S - taps), S):
+        ring[:, p % taps] = proj[:, p, :cq]
+    steps = []
+    for p in range(S, S + more):
+        steps.append(cache_ops.delta_step(proj[:, p], conv, decay, bias, norm, 1e-6, ring, state,
+                                          ints(range(B)), ints([p] * B), KH, kd, H, vd))
+    full = ops.delta_scan(*whole(S + more)).view(-1, H, vd)
+    z = proj[..., cq:cq + vw].reshape(-1, H, vd).contiguous()
+    exp = ops.native_gated_rms(full, z, norm, 1e-6).view(B, S + more, vw)[:, S:]
+    assert normwise(torch.stack(steps, 1).cpu(), exp.cpu()) <= 1e-5
+    last = torch.empty_like(state)
+    ops.delta_scan(*whole(S + more), state=last)
+    assert normwise(state.cpu(), last.cpu()) <= 1e-5
+
+
+@pytest.mark.gpu
+def test_delta_step_refusals():
+    KH, H, kd, vd = 2, 4, 64, 32
+    s = step_case(1, KH, H, kd, vd, 4, 2, 3, torch.float32)
+    d = {k: v.to(DEV) for k, v in s.items() if isinstance(v, torch.Tensor)}
+    ok = dict(d, eps=1e-6, rows=ints([0, 1]), positions=ints([0, 1]), key_heads=KH, key_dim=kd,
+              value_heads=H, value_dim=vd)
+    cache_ops.delta_step(**ok)
+    for bad in (dict(proj=d["proj"][:, :519]), dict(proj=d["proj"].bfloat16()),
+                dict(conv=d["conv"][:5]), dict(conv=d["conv"].t()), dict(state=d["state"].bfloat16()),
+                dict(state=d["state"][:2]), dict(ring=d["ring"][:, :3]), dict(norm=d["norm"][:8]),
+                dict(a_decay=d["a_decay"][:2]), dict(rows=ints([0])),
+                dict(positions=ints([0, 1]).long()), dict(out_dtype=torch.bfloat16),
+                dict(out_dtype=ops.BF16X2), dict(key_heads=3), dict(state=d["ring"])):
+        with pytest.raises(ValueError):
+            cache_ops.delta_step(**dict(ok, **bad))
+    with pytest.raises(ValueError):       # a state where the scan keeps none
+        q = torch.zeros(1, 4, 1, 96, device=DEV)
+        g = torch.zeros(1, 4, 1, device=DEV)
+        ops.delta_scan(q, q, q, g, g, state=torch.zeros(1, 1, 96, 96, device=DEV))
+
+
+# ---------------------------------------------------------- how they are run --
+def decode_inputs(seed=0, n=6, dtype=torch.bfloat16):
+    rng = np.random.default_rng(seed)
+    H, KV, hd, page, pages, width = 4, 2, 64, 16, 60, 8
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32)).to(dtype).to(DEV)  # noqa: E731
+    book = cache_ops.page_table(n + 2, width, pages, page, DEV)
+    rows = ints(rng.permutation(n + 2)[:n])
+    cache_ops.extend_pages(book, rows, ints(rng.integers(1, 60, n)))
+    return dict(q=t(n, H, hd), k=t(n, KV, hd), v=t(n, KV, hd), gate=t(n, H, hd), norm=t(hd) * 0.1,
+                pool=t(2, pages, KV, page, hd), book=book, rows=rows,
+                tables=ops.rope_tables(width * page, 16, 1e4, DEV))
+
+
+def decode_step(s, positions=None):
+    """The attention layer's part of a step: a place for the token, q and k prepared
+    and stored, attention over the row."""
+    pos = cache_ops.extend_pages(s["book"], s["rows"], positions=positions)
+    q = cache_ops.prepare_paged(s["q"], s["k"], s["v"], s["norm"], s["norm"], s["tables"], 16, 1e-6,
+                                s["rows"], pos, s["book"].table, s["pool"][0], s["pool"][1])
+    return cache_ops.paged_attention(q, s["pool"][0], s["pool"][1], s["book"].table, s["rows"], pos,
+                                     0.125, gate=s["gate"])
+
+
+@pytest.mark.gpu
+def test_captured_step():
+    """A step recorded into a graph and replayed, with eager work between, gives what
+    the eager steps give: the positions move on the device."""
+    a, b = decode_inputs(), decode_inputs()
+    pos = torch.empty(6, dtype=torch.int32, device=DEV)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        decode_step(b)                          # lazy initialisation outside the capture
+        eager = [decode_step(a)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = decode_step(b, pos)
+    for _ in range(5):
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        eager.append(decode_step(a))
+        assert torch.equal(got, eager[-1])
+        assert torch.equal(a["book"].table, b["book"].table)
+        assert torch.equal(a["pool"], b["pool"])
+    assert not torch.equal(eager[1], eager[2])
+
+
+@pytest.mark.gpu
+def test_other_stream_and_same_results():
+    """On a side stream the kernels wait for that stream's work alone, and two runs give
+    the same bits."""
+    want = decode_step(decode_inputs(7))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        s = decode_inputs(7)
+        big = torch.randn(4096, 4096, device=DEV)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        s["q"] = s["q"] + 0.0 * big[0, 0].bfloat16()     # behind the products
+        got = decode_step(s)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(want, got)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Pages whose byte offsets, and element offsets, pass 2^32."""
+    hd, page, KV = 256, 256, 2
+    pages = (1 << 32) // (KV * page * hd) + 3             # 4.3e9 elements of bf16 a tensor
+    free = torch.cuda.mem_get_info()[0]
+    if free < 5 * pages * KV * page * hd:
+        pytest.skip("needs 22 GB of device memory")
+    k = torch.zeros((pages, KV, page, hd), dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    rng = np.random.default_rng(0)
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32)).bfloat16().to(DEV)  # noqa: E731
+    table = ints([pages - 1, 0, pages - 2]).view(1, 3)
+    T = 600
+    q, kn, vn, norm = t(T, 4, hd), t(T, KV, hd), t(T, KV, hd), t(hd) * 0.1
+    rows, pos = ints([0] * T), ints(range(T))
+    qp = cache_ops.prepare_paged(q, kn, vn, norm, norm, None, 0, 1e-6, rows, pos, table, k, v)
+    got = cache_ops.paged_attention(qp[-3:], k, v, table, rows[-3:], pos[-3:], 0.0625)
+    small = torch.stack([x[[pages - 1, 0, pages - 2]] for x in (k, v)])
+    want = cache_ops.paged_attention(qp[-3:], small[0], small[1], ints([0, 1, 2]).view(1, 3),
+                                     rows[-3:], pos[-3:], 0.0625)
+    assert torch.equal(got, want) and torch.isfinite(want).all() and want.abs().max() > 0
+    assert torch.equal(small[1].transpose(1, 2).reshape(-1, KV, hd)[:T], vn)
