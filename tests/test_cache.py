@@ -1,0 +1,202 @@
+"""Sequences continued token by token (qdc_amd.cache.BackboneCache): prompts, steps,
+forks, ends and moves together, as a server uses them, against the forward of the
+whole sequence."""
+import numpy as np
+import pytest
+import torch
+
+from conftest import normwise
+
+MODES = {"f32": (torch.float32, False), "bf16": (torch.bfloat16, False),
+         "mlp": (torch.bfloat16, "mlp"), "all": (torch.bfloat16, "all")}
+# fp32: both paths hold 1e-5 of the exact forward.  bf16 with split GEMM inputs: 1e-2,
+# the bar that both paths hold; stored in bf16 throughout: each within it, so twice that
+# between the two.
+BARS = {"f32": 2e-5, "bf16": 2e-2, "mlp": 1e-2, "all": 1e-2}
+
+
+def model_of(mode, config="synthetic", seed=21):
+    from qdc_amd import backbone
+    from qdc_amd import config as C
+    from qdc_amd.weights import random_weights
+    cfg = {"synthetic": C.synthetic_inference_config, "plumbing": C.plumbing_config}[config]()
+    weights = random_weights(cfg, seed=seed)
+    dtype, split = MODES[mode]
+    if dtype == torch.bfloat16:
+        from oracle import qdc_oracle as O
+        weights = {k: O.round_bf16(v) for k, v in weights.items()}
+    return backbone.QwenBackbone.from_weights(weights, cfg, "cuda:0", dtype, split_gemm_inputs=split)
+
+
+def whole(model, ids):
+    from qdc_amd import backbone
+    return backbone.backbone_last_hidden(model, np.asarray(ids), np.ones(len(ids), np.int64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("config", ["synthetic", "plumbing"])
+@pytest.mark.parametrize("mode", list(MODES))
+def test_sequences(mode, config):
+    """Padded prompts of several lengths, steps, forks that part, a parent that ends
+    before its children, a move of all pages and steps after it."""
+    from qdc_amd.cache import BackboneCache
+    model = model_of(mode, config)
+    cache = BackboneCache(model, rows=10, pages=40, page_size=16, max_tokens=120)
+    rng = np.random.default_rng(1)
+    vocab = model.vocab
+    held = {}
+
+    def check(rows, got):
+        for r, g in zip(rows, got):
+            exp = whole(model, held[r])
+            assert normwise(g, exp) <= BARS[mode], (r, len(held[r]), normwise(g, exp))
+
+    lengths = [50, 33, 3, 64]
+    ids = rng.integers(0, vocab, (4, 70))
+    mask = np.zeros((4, 70), np.int64)
+    for i, n in enumerate(lengths):
+        mask[i, 70 - n:] = 1
+    rows, got = cache.prefill(ids, mask)
+    held.update({r: ids[i, 70 - n:].tolist() for i, (r, n) in enumerate(zip(rows, lengths))})
+    check(rows, got)
+    one, got = cache.prefill(rng.integers(0, vocab, 1))   # a prompt of one token
+    free_before = cache.free_page_count()
+    cache.free(one)
+    assert cache.free_page_count() == free_before + 1
+
+    def step(which):
+        new = rng.integers(0, vocab, len(which))
+        got = cache.step(which, new)
+        for r, t in zip(which, new):
+            held[r].append(int(t))
+        check(which, got)
+
+    for _ in range(3):
+        step(rows)
+    step([rows[2], rows[0]])
+    kids = cache.fork([rows[0], rows[3], rows[0], rows[2]])
+    for k, p in zip(kids, (rows[0], rows[3], rows[0], rows[2])):
+        held[k] = list(held[p])
+    for _ in range(2):
+        step(kids + rows)
+    cache.free([rows[0], kids[1]])
+    del held[rows[0]], held[kids[1]]
+    left = [kids[2], rows[1], kids[0], rows[3], rows[2], kids[3]]
+    step(left)
+    cache.compact()
+    used = 40 - cache.free_page_count()
+    assert cache.book.table.max().item() == used - 1
+    for _ in range(18):                                   # over page borders
+        step(left)
+    assert cache.lengths() == {r: len(t) for r, t in held.items()}
+    cache.free(left)
+    assert cache.free_page_count() == 40 and not cache.lengths()
+
+
+@pytest.mark.gpu
+def test_too_few_pages_leaves_everything():
+    """A prompt, a step or a fork that does not fit raises, and what was there goes on."""
+    from qdc_amd.cache import BackboneCache
+    model = model_of("f32")
+    cache = BackboneCache(model, rows=5, pages=6, page_size=16, max_tokens=64)
+    rng = np.random.default_rng(2)
+    tokens = rng.integers(0, model.vocab, (2, 47)).tolist()
+    (a, b), _ = cache.prefill(tokens)
+    held = {a: list(tokens[0]), b: list(tokens[1])}
+    for call in (lambda: cache.prefill(rng.integers(0, model.vocab, 5)), lambda: cache.fork([a]),
+                 lambda: cache.fork([a, b, a, b])):
+        with pytest.raises(RuntimeError):
+            call()
+        assert cache.lengths() == {a: 47, b: 47}
+
+    def step(rows):
+        new = rng.integers(0, model.vocab, len(rows))
+        for r, t, g in zip(rows, new, cache.step(rows, new)):
+            held[r].append(int(t))
+            assert normwise(g, whole(model, held[r])) <= BARS["f32"]
+
+    step([a, b])                                          # 48: the pages are full
+    with pytest.raises(RuntimeError):
+        cache.step([b, a], [1, 2])
+    assert cache.lengths() == {a: 48, b: 48}
+    kid, = cache.fork([a])                                # full pages are shared
+    held[kid] = list(held[a])
+    cache.free([b])
+    for _ in range(3):
+        step([a, kid])
+
+
+@pytest.mark.gpu
+def test_refusals():
+    import dataclasses
+
+    from qdc_amd import backbone
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.config import synthetic_inference_config
+    from qdc_amd.weights import random_weights
+    model = model_of("f32")
+    for bad in (dict(rows=0, pages=4), dict(rows=2, pages=0), dict(rows=2, pages=4, page_size=20),
+                dict(rows=2, pages=4, max_tokens=0)):
+        with pytest.raises(ValueError):
+            BackboneCache(model, **bad)
+    for change in (dict(head_dim=32), dict(key_dim=48), dict(value_dim=40), dict(conv_kernel=9)):
+        cfg = dataclasses.replace(synthetic_inference_config(), **change)
+        other = backbone.QwenBackbone.from_weights(random_weights(cfg, seed=1), cfg)
+        with pytest.raises(ValueError):
+            BackboneCache(other, rows=2, pages=4)
+    cache = BackboneCache(model, rows=3, pages=8, page_size=16, max_tokens=40)
+    (row,), _ = cache.prefill([1, 2, 3])
+    mask = lambda *m: np.array([m])  # noqa: E731
+    for bad in (lambda: cache.prefill([]), lambda: cache.prefill([model.vocab]),
+                lambda: cache.prefill([[1, 2]], mask(1, 0)), lambda: cache.prefill([[1, 2]], mask(0, 0)),
+                lambda: cache.prefill([[1, 2, 3]], mask(1, 0, 1)), lambda: cache.prefill([[1, 2]], mask(0, 2)),
+                lambda: cache.prefill([[1, 2]], mask(1)), lambda: cache.prefill(np.ones((1, 1, 2))),
+                lambda: cache.prefill(np.ones(41)), lambda: cache.step([row], [-1]),
+                lambda: cache.step([row], [1, 2]), lambda: cache.step([], []),
+                lambda: cache.step([row, row], [1, 2]), lambda: cache.step([row + 1], [1]),
+                lambda: cache.fork([row, 99]), lambda: cache.free([row, row]), lambda: cache.free([9])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        cache.fork([row, row, row])                       # rows
+    assert cache.fork([]) == [] and cache.lengths() == {row: 3}
+    long, _ = cache.prefill(np.ones(40))
+    with pytest.raises(ValueError):
+        cache.step(long, [1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kinds", [("full_attention",), ("linear_attention", "linear_attention")])
+def test_one_kind_of_layer(kinds):
+    """Models with no state to keep, or with no pages."""
+    import dataclasses
+
+    from qdc_amd import backbone
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.config import synthetic_inference_config
+    from qdc_amd.weights import random_weights
+    cfg = dataclasses.replace(synthetic_inference_config(), layer_types=kinds)
+    model = backbone.QwenBackbone.from_weights(random_weights(cfg, seed=2), cfg)
+    cache = BackboneCache(model, rows=4, pages=16, page_size=16)
+    rng = np.random.default_rng(4)
+    ids = rng.integers(0, cfg.vocab, 21).tolist()
+    (row,), got = cache.prefill(ids)
+    assert normwise(got[0], whole(model, ids)) <= BARS["f32"]
+    kid, = cache.fork([row])
+    cache.compact()
+    for t in rng.integers(0, cfg.vocab, 4).tolist():
+        ids.append(t)
+        got = cache.step([kid, row], [t, t])
+        assert np.array_equal(got[0], got[1])
+        assert normwise(got[0], whole(model, ids)) <= BARS["f32"]
+
+
+def test_packed_integers():
+    """Host vectors to the device in one copy, each starting on 16 bytes."""
+    from types import SimpleNamespace
+
+    from qdc_amd.cache import BackboneCache
+    self = SimpleNamespace(model=SimpleNamespace(device="cpu"))
+    a, b, c = BackboneCache._ints(self, np.arange(5), np.array([[7, 8], [9, -1]]), np.array([3]))
+    assert a.tolist() == [0, 1, 2, 3, 4] and b.tolist() == [7, 8, 9, -1] and c.tolist() == [3]
+    assert b.data_ptr() - a.data_ptr() == 32 and c.data_ptr() - b.data_ptr() == 16
