@@ -20,6 +20,7 @@
 // terms: rounded to one they would add as much error as the output's own rounding, and
 // the matrix cores have time for both.
 #include <cfloat>
+#include <type_traits>
 
 #include "qdc_cache.hpp"
 
@@ -30,8 +31,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kWaves = kBlock / kWave;
 constexpr int kHeads = 16;          // query heads of a unit: a matrix operand's columns
-constexpr int kLogWgs = 9;          // workgroups that share the tiles: two a compute unit
-constexpr uint32_t kMinTiles = 4;   // fewer a workgroup leave wavefronts without a tile
+constexpr uint32_t kMinTiles = 4;  // fewer a workgroup leave wavefronts without a tile
+constexpr int kMaxLogWgs = 9;
 
 struct PagedAttention {
     void *out;
@@ -47,9 +48,8 @@ struct PagedAttention {
 
 template <typename T> constexpr int tile_keys() { return sizeof(T) == 2 ? 32 : 16; }
 
-// Keys of entry i: 0 for one that is no token.
-__device__ __forceinline__ int entry_keys(const PagedAttention &a, int i, bool &bad) {
-    const int row = a.index[i], pos = a.positions[i];
+// Keys of an entry: 0 for one that is no token.
+__device__ __forceinline__ int entry_keys(const PagedAttention &a, int row, int pos, bool &bad) {
     bad = row >= a.rows && pos >= 0;
     if (row < 0 || pos < 0 || bad) return 0;
     const int64_t reach = a.width << a.shift;
@@ -68,22 +68,32 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
-// The entries as rows of tiles, seen 64 at a time by a wavefront: lane l holds entry
-// first + l's tiles and where they end.
-template <int TILE> struct Entries {
+// The work of the call is a line: entry by entry, unit by unit (KV head and group of its
+// query heads), kBegin tiles' worth for beginning a unit and then its tiles.  A
+// wavefront sees 64 entries at a time: lane l holds entry first + l.
+template <typename T, int HD> struct Line {
+    static constexpr int TILE = tile_keys<T>();
+    // What beginning a unit costs beside a tile: the chain to its page numbers, the
+    // join of its wavefronts, about as long as 64 KB of pages take.
+    static constexpr uint32_t kBegin = 65536 / (TILE * HD * 2 * (int)sizeof(T));
     const PagedAttention &a;
-    int first;
-    uint32_t tiles, end, before, all;  // before: tiles of earlier chunks; all: this one's
+    const uint32_t units;
+    int first, row, keys;
+    uint32_t end, before, all;  // this entry's end within the chunk; earlier chunks; this one
 
+    __device__ __forceinline__ uint32_t length(int keys) const {
+        return keys ? ((uint32_t)(keys + TILE - 1) / TILE + kBegin) * units : 0u;
+    }
     __device__ __forceinline__ void load(int at) {
         first = at;
         const int i = at + (int)(threadIdx.x % kWave);
         bool bad;
-        tiles = i < a.n ? (uint32_t)(entry_keys(a, i, bad) + TILE - 1) / TILE : 0u;
-        end = wave_scan(tiles);
+        row = i < a.n ? a.index[i] : -1;
+        keys = entry_keys(a, row, i < a.n ? a.positions[i] : -1, bad);
+        end = wave_scan(length(keys));
         all = __builtin_amdgcn_readlane(end, kWave - 1);
     }
-    // all entries' tiles; leaves the first chunk in place
+    // the whole line; leaves the first chunk in place
     __device__ __forceinline__ uint32_t total() {
         before = 0;
         uint32_t sum = 0;
@@ -100,8 +110,8 @@ template <int TILE> struct Entries {
 };
 
 // Workgroups that work, as a power of two: fewer where there are few tiles.
-__device__ __forceinline__ int log_workers(int log_wgs, uint32_t tiles) {
-    while (log_wgs > 0 && (tiles >> log_wgs) < kMinTiles) --log_wgs;
+__device__ __forceinline__ int log_workers(int log_wgs, uint32_t line) {
+    while (log_wgs > 0 && (line >> log_wgs) < kMinTiles) --log_wgs;
     return log_wgs;
 }
 
@@ -145,6 +155,14 @@ __device__ __forceinline__ void store_out(const PagedAttention &a, int i, int h,
     }
 }
 
+// Pages stream by: read as such they come at up to 6.7 TB/s, with plain loads at 5.6.
+// (Rows that share pages read them again from a cache, which this makes the most of in
+// neither way: 40 rows over 8 prompts of 2000 tokens 34 us, 36 with plain loads; 64 rows
+// over 4 prompts of 8000, 2.1 GB of reads of 131 MB, 215 and 157 us.)
+template <typename P> __device__ __forceinline__ P load_page(const char *p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const P *>(p));
+}
+
 // One wavefront's operands and sums over its tiles of one head group.
 //   K: lane (lr, lg) holds values DS s + V lg .. of key 16 sub + lr.
 //   V: values 16 VD c + VD lr .. of keys 16 sub + 4 lg + r.
@@ -172,7 +190,7 @@ template <typename T, int HD> struct Lanes {
 };
 
 template <typename T, int HD>
-__global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
+__global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(PagedAttention a) {
     typedef Lanes<T, HD> L;
     constexpr int TILE = tile_keys<T>(), KT = kWave / L::SUBS;
     constexpr int VEC = HD / kWave;  // outputs of a thread per pass of 4 heads
@@ -181,31 +199,32 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
     __shared__ float sm[kWaves][kHeads], sl[kWaves][kHeads];
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
     const int lr = l % 16, lg = l / 16;
-    const uint32_t units = (uint32_t)(a.kv * a.head_groups);
-    Entries<TILE> es{a};
-    const uint32_t all = es.total() * units;
+    Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
+    const uint32_t all = line.total();
     const int lw = log_workers(a.log_wgs, all);
     if (blockIdx.x >> lw) return;
     uint32_t t = (uint32_t)(((uint64_t)all * blockIdx.x) >> lw);
     const uint32_t t_end = (uint32_t)(((uint64_t)all * (blockIdx.x + 1)) >> lw);
     const int mask = (1 << a.shift) - 1;
+    const uint32_t off_k = (uint32_t)(lr * HD + L::V * lg) * (uint32_t)sizeof(T);
+    const uint32_t off_v = (uint32_t)(4 * lg * HD + L::VD * lr) * (uint32_t)sizeof(T);
     L x;
     while (t < t_end) {
-        while (units * (es.before + es.all) <= t) es.next();
-        // the entry that holds tile t, and the part of it up to t_end
-        const uint64_t past = __ballot(units * (es.before + es.end) > t);
-        const int el = __builtin_ctzll(past), entry = es.first + el;
-        const uint32_t tiles = __builtin_amdgcn_readlane(es.tiles, el);
-        const uint32_t rel = t - units * (es.before + __builtin_amdgcn_readlane(es.end, el) - tiles);
-        const uint32_t unit = rel / tiles, j0 = rel - unit * tiles;
-        const uint32_t j1 = min(tiles, j0 + (t_end - t));
-        t += j1 - j0;
+        while (line.before + line.all <= t) line.next();
+        // the entry and unit that hold place t, and the tiles of it up to t_end
+        const int el = __builtin_ctzll(__ballot(line.before + line.end > t)), entry = line.first + el;
+        const int keys = __builtin_amdgcn_readlane(line.keys, el);
+        const int row = __builtin_amdgcn_readlane(line.row, el);
+        const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE, span = tiles + line.kBegin;
+        const uint32_t rel = t - (line.before + __builtin_amdgcn_readlane(line.end, el) -
+                                  line.length(keys));
+        const uint32_t unit = rel / span, p0 = rel - unit * span, p1 = min(span, p0 + (t_end - t));
+        t += p1 - p0;
+        if (p1 <= line.kBegin) continue;
+        const uint32_t j0 = p0 > line.kBegin ? p0 - line.kBegin : 0, j1 = p1 - line.kBegin;
         const int kvh = (int)unit / a.head_groups, hg = (int)unit - kvh * a.head_groups;
         const int head0 = kvh * a.group + hg * kHeads;
         const int gu = min(kHeads, a.group - hg * kHeads);
-        bool bad;
-        const int keys = __builtin_amdgcn_readfirstlane(entry_keys(a, entry, bad));
-        const int row = __builtin_amdgcn_readfirstlane(a.index[entry]);
         const int32_t *pages = a.table + (int64_t)row * a.width;
 
         // this wavefront's tiles: every fourth
@@ -218,6 +237,7 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
         };
         fetch_ids(0);
         int limit[L::SUBS];  // keys of the tile's halves that count
+        // bytes to the half's first key: its 16 lie in one page, those past the end too
         int64_t from[L::SUBS];
         auto locate = [&](int k) {  // where tile k lies
             if (k && k % KT == 0) fetch_ids(k);
@@ -226,40 +246,36 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
                 const int key0 = (jw + kWaves * k) * TILE + 16 * s;
                 const int id = __builtin_amdgcn_readlane(ids, k % KT * L::SUBS + s);
                 const bool ok = (uint32_t)id < (uint32_t)a.pages;
-                from[s] = (((int64_t)(ok ? id : 0) * a.kv + kvh) << a.shift) * HD;
+                from[s] = ((((int64_t)(ok ? id : 0) * a.kv + kvh) << a.shift) + (key0 & mask)) *
+                          (HD * (int)sizeof(T));
                 const int left = min(max(keys - key0, 0), 16);
                 limit[s] = ok ? left : 0;
                 if (!ok && left && l == 0) raise_flag(a.error_flag);
             }
         };
-        // keys past the end read the last one
-        auto place = [&](int key) { return (min(key, keys - 1) & mask) * HD; };
-        auto load_k = [&](int k) {
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s) {
-                const T *p = (const T *)a.k + from[s] +
-                             (place((jw + kWaves * k) * TILE + 16 * s + lr) + L::V * lg);
-#pragma unroll
-                for (int i = 0; i < L::STEPS; ++i) x.k[s][i] = load_raw(p + L::DS * i);
-            }
-        };
-        auto load_v = [&](int k) {
+        auto load_k = [&] {
 #pragma unroll
             for (int s = 0; s < L::SUBS; ++s)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const T *p = (const T *)a.v + from[s] +
-                                 (place((jw + kWaves * k) * TILE + 16 * s + 4 * lg + r) + L::VD * lr);
+                for (int i = 0; i < L::STEPS; ++i)
+                    x.k[s][i] = load_page<u32x4>((const char *)a.k + from[s] + off_k +
+                                                 L::DS * (int)sizeof(T) * i);
+        };
+        auto load_v = [&] {
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int c = 0; c < L::VC; ++c)
-                        x.v[s][r][c] = *reinterpret_cast<const typename L::piece *>(
-                            p + 16 * L::VD * c);
-                }
+                        x.v[s][r][c] = load_page<typename L::piece>(
+                            (const char *)a.v + from[s] + off_v +
+                            (r * HD + 16 * L::VD * c) * (int)sizeof(T));
         };
         if (cnt) {
             locate(0);
-            load_k(0);
-            load_v(0);
+            load_k();
+            load_v();
         }
         // q as the other operand of the scores, heads past the group's repeat its last
         for (int i = threadIdx.x; i < L::STEPS * kWave; i += kBlock) {
@@ -270,7 +286,9 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
         }
         __syncthreads();
         x.clear();
-        for (int k = 0; k < cnt; ++k) {
+        // tile k; with another after it the loads of that one follow the last use of the
+        // registers they fill (in a branch of their own they would be waited for there)
+        auto step = [&](int k, auto more) {
             f32x4 sc[L::SUBS];
 #pragma unroll
             for (int s = 0; s < L::SUBS; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -296,10 +314,11 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
             bool cut = false;
 #pragma unroll
             for (int s = 0; s < L::SUBS; ++s) now[s] = limit[s], cut = cut || limit[s] < 16;
-            const bool more = k + 1 < cnt;
-            if (more) {
+            if constexpr (decltype(more)::value) {
+                __builtin_amdgcn_sched_barrier(0);
                 locate(k + 1);
-                load_k(k + 1);
+                load_k();
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (cut) {
 #pragma unroll
@@ -373,8 +392,13 @@ __global__ __launch_bounds__(kBlock, 2) void paged_attention(PagedAttention a) {
                             x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
                                 __uint_as_float(x.v[0][r][c][j]), p[0][r], x.o[c][j], 0, 0, 0);
             }
-            if (more) load_v(k + 1);
-        }
+            if constexpr (decltype(more)::value) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_v();
+            }
+        };
+        for (int k = 0; k + 1 < cnt; ++k) step(k, std::true_type{});
+        if (cnt) step(cnt - 1, std::false_type{});
         // the wavefronts' sums together, four heads at a time
         x.sum = swap_sum32(swap_sum16(x.sum));
         if (lg == 0) {
@@ -434,20 +458,20 @@ template <typename T, int HD>
 __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a) {
     constexpr int TILE = tile_keys<T>();
     constexpr int LPP = HD / 4, PARTS = kBlock / LPP;  // lanes of a piece's row, rows at a time
-    __shared__ float weight[1 << kLogWgs], top_of[kWaves], sum_of[kWaves];
+    __shared__ float weight[1 << kMaxLogWgs], top_of[kWaves], sum_of[kWaves];
     __shared__ __align__(16) float so[PARTS][HD];
     const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
     const int entry = blockIdx.x / a.heads, h = blockIdx.x - entry * a.heads;
     const int kvh = h / a.group, in_group = h - kvh * a.group;
     const int hg = in_group / kHeads, hu = in_group - hg * kHeads;
-    const uint32_t units = (uint32_t)(a.kv * a.head_groups);
-    Entries<TILE> es{a};
-    const uint32_t all = es.total() * units;
-    while (es.first + kWave <= entry) es.next();
-    const uint32_t tiles = __builtin_amdgcn_readlane(es.tiles, entry - es.first);
+    Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
+    const uint32_t all = line.total();
+    while (line.first + kWave <= entry) line.next();
+    const int keys = __builtin_amdgcn_readlane(line.keys, entry - line.first);
+    const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE;
     if (h == 0 && threadIdx.x == 0) {
         bool bad;
-        entry_keys(a, entry, bad);
+        entry_keys(a, a.index[entry], a.positions[entry], bad);
         if (bad) raise_flag(a.error_flag);
     }
     const int dim = HD / kWave * l;
@@ -460,10 +484,11 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
         return;
     }
     const int lw = log_workers(a.log_wgs, all);
-    const uint32_t first = units * (es.before + __builtin_amdgcn_readlane(es.end, entry - es.first) -
-                                    tiles) + (uint32_t)(kvh * a.head_groups + hg) * tiles;
-    // the workgroups that hold its first and its last tile: w of tile t is the last with
-    // all * w / 2^lw <= t
+    const uint32_t first = line.before + __builtin_amdgcn_readlane(line.end, entry - line.first) -
+                           line.length(keys) + line.kBegin +
+                           (uint32_t)(kvh * a.head_groups + hg) * (tiles + line.kBegin);
+    // the workgroups that hold its first and its last tile: that of place t is the last
+    // with all * w / 2^lw <= t
     const uint32_t w0 = (uint32_t)((((uint64_t)(first + 1) << lw) - 1) / all);
     const uint32_t w1 = (uint32_t)((((uint64_t)(first + tiles) << lw) - 1) / all);
     if (w0 == w1) return;
@@ -514,10 +539,10 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
     store_out<T, HD, HD / kWave>(a, entry, h, dim, o);
 }
 
-// The most tiles that a call of these sizes can have, 0 when there are too many or the
+// The longest line that a call of these sizes can have, 0 when it is too long or the
 // sizes are not taken.
-int64_t most_tiles(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t width,
-                   int64_t page_size, int32_t dtype) {
+int64_t longest_line(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t width,
+                     int64_t page_size, int32_t dtype) {
     if (!valid_dtype(dtype) || n <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
         (head_dim != 64 && head_dim != 128 && head_dim != 256) || width <= 0 ||
         page_shift(page_size) < 0)
@@ -528,13 +553,19 @@ int64_t most_tiles(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim,
         return 0;
     const int64_t units = kv_heads * ceil_div(heads / kv_heads, (int64_t)kHeads);
     const int64_t tile = dtype == QDC_BF16 ? tile_keys<bf16_t>() : tile_keys<float>();
-    const int64_t tiles = ceil_div(width * page_size, tile);
-    return tiles >= lim / units / n ? 0 : tiles * units * n;
+    const int64_t span = ceil_div(width * page_size, tile) +
+                         65536 / (tile * head_dim * 2 * elem_size(dtype));
+    return span >= lim / units / n ? 0 : span * units * n;
 }
 
-int log_workgroups(int64_t tiles) {
+// Workgroups for a line: one a compute unit for heads of 256, whose operands take half
+// the registers of a SIMD for a wavefront, two for smaller ones (us, 256 / 512: bf16 2 x
+// 100003 keys of 256 123 / 128, 8 x 2048 12 / 13; of 64, 410 MB 73 / 66; fp32 of 256, 819
+// MB 128 / 135, of 64 136 / 124).
+int log_workgroups(int64_t line, int64_t head_dim) {
+    const int most = head_dim > 128 ? 8 : kMaxLogWgs;
     int lw = 0;
-    while (lw < kLogWgs && ((int64_t)kMinTiles << lw) < tiles) ++lw;
+    while (lw < most && ((int64_t)kMinTiles << lw) < line) ++lw;
     return lw;
 }
 
@@ -551,10 +582,10 @@ using namespace qdc;
 extern "C" int64_t qdc_paged_attention_workspace(int64_t n, int64_t heads, int64_t kv_heads,
                                                  int64_t head_dim, int64_t width,
                                                  int64_t page_size, int32_t dtype) {
-    const int64_t tiles = most_tiles(n, heads, kv_heads, head_dim, width, page_size, dtype);
-    if (tiles == 0) return 0;
+    const int64_t line = longest_line(n, heads, kv_heads, head_dim, width, page_size, dtype);
+    if (line == 0) return 0;
     // two pieces a workgroup, each with its maximum and sum
-    return ((int64_t)2 << log_workgroups(tiles)) * unit_heads(heads, kv_heads) * (head_dim + 2) * 4;
+    return ((int64_t)2 << log_workgroups(line, head_dim)) * unit_heads(heads, kv_heads) * (head_dim + 2) * 4;
 }
 
 extern "C" int32_t qdc_paged_attention(
@@ -567,10 +598,10 @@ extern "C" int32_t qdc_paged_attention(
     if (!valid_dtype(dtype) || (!valid_dtype(out_dtype) && out_dtype != QDC_BF16X2))
         return QDC_ERR_DTYPE;
     if (n < 0 || rows <= 0 || pages <= 0) return QDC_ERR_SHAPE;
-    const int64_t tiles =
-        most_tiles(n ? n : 1, heads, kv_heads, head_dim, width, page_size, dtype);
+    const int64_t line =
+        longest_line(n ? n : 1, heads, kv_heads, head_dim, width, page_size, dtype);
     const int64_t lim = (int64_t)1 << 31;
-    if (tiles == 0 || rows >= lim || pages >= lim) return QDC_ERR_SHAPE;
+    if (line == 0 || rows >= lim || pages >= lim) return QDC_ERR_SHAPE;
     const int64_t es = elem_size(dtype), per = 16 / es, oes = elem_size(out_dtype);
     if (q_head < head_dim || q_tok < 0 || (q_tok | q_head) % per || out_tok < heads * head_dim ||
         out_tok % (16 / oes))
@@ -622,7 +653,7 @@ extern "C" int32_t qdc_paged_attention(
     a.rows = (int)rows;
     a.pages = (int)pages;
     a.shift = page_shift(page_size);
-    a.log_wgs = log_workgroups(tiles);
+    a.log_wgs = log_workgroups(line, head_dim);
     a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
     const dim3 grid(1u << a.log_wgs), join((uint32_t)(n * heads)), block(kBlock);
