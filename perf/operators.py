@@ -33,20 +33,16 @@ DELTA = {"decision": (2, 4, 128, 128), "0.8b": (16, 16, 128, 128), "wide": (16, 
 TAPS = 4
 
 
-_ops = None
-
-
 def _framework():
     """The framework's operators, imported at the first call and not at each."""
-    global _ops
-    if _ops is None:
+    ops = sys.modules.get("qdc_amd.cache_ops")
+    if ops is None:
         package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                                "qwendecisioncore.jl_amd")
         if package not in sys.path:
             sys.path.insert(0, package)
-        from qdc_amd import cache_ops
-        _ops = cache_ops
-    return _ops
+        from qdc_amd import cache_ops as ops
+    return ops
 
 
 # -------------------------------------------------------------------- cases --
