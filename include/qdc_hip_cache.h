@@ -63,8 +63,8 @@ int32_t qdc_prepare_paged(void *q_out, void *k_out, void *k_pages, void *v_pages
                           int64_t k_head, int64_t v_tok, int64_t v_head, float eps, int32_t dtype,
                           int32_t *error_flag, hipStream_t stream);
 
-/* Bytes of 16-byte aligned device scratch that qdc_paged_attention needs, 0 when it
- * does not take the sizes. */
+/* Bytes of 16-byte aligned device scratch that qdc_paged_attention needs (0: none, for
+ * short rows), -1 when it does not take the sizes. */
 int64_t qdc_paged_attention_workspace(int64_t n, int64_t heads, int64_t kv_heads,
                                       int64_t head_dim, int64_t width, int64_t page_size,
                                       int32_t dtype);

@@ -34,6 +34,11 @@ constexpr int kHeads = 16;          // query heads of a unit: a matrix operand's
 constexpr uint32_t kMinTiles = 4;  // fewer a workgroup leave wavefronts without a tile
 constexpr int kMaxLogWgs = 9;
 
+// Wavefronts of a workgroup that has a unit to itself, as many as the registers let in,
+// and the tiles that it may have.
+constexpr int short_waves(int head_dim) { return head_dim == 64 ? 16 : head_dim == 128 ? 8 : 4; }
+constexpr int kShortTiles = 2;  // a wavefront's
+
 struct PagedAttention {
     void *out;
     const void *q, *k, *v, *gate;
@@ -155,6 +160,15 @@ __device__ __forceinline__ void store_out(const PagedAttention &a, int i, int h,
     }
 }
 
+// Of an entry without keys: 0 whatever the gate holds.
+template <typename T, int HD, int N>
+__device__ __forceinline__ void store_zero(const PagedAttention &a, int i, int h, int dim) {
+    PagedAttention b = a;
+    b.gate = nullptr;
+    float zero[N] = {};
+    store_out<T, HD, N>(b, i, h, dim, zero);
+}
+
 // Pages stream by: read as such they come at up to 6.7 TB/s, with plain loads at 5.6.
 // (Rows that share pages read them again from a cache, which this makes the most of in
 // neither way: 40 rows over 8 prompts of 2000 tokens 34 us, 36 with plain loads; 64 rows
@@ -189,30 +203,263 @@ template <typename T, int HD> struct Lanes {
     }
 };
 
-template <typename T, int HD>
-__global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(PagedAttention a) {
+// Tiles j0 .. j1 - 1 of a unit (KV head and group of its query heads) of an entry, by
+// WAVES wavefronts: its outputs, when `whole`, or a piece in slot `slot`.
+template <typename T, int HD, int WAVES>
+__device__ __forceinline__ void attend(const PagedAttention &a, int entry, int row, int keys,
+                                       int unit, int j0, int j1, bool whole, int64_t slot) {
     typedef Lanes<T, HD> L;
     constexpr int TILE = tile_keys<T>(), KT = kWave / L::SUBS;
     constexpr int VEC = HD / kWave;  // outputs of a thread per pass of 4 heads
     __shared__ __align__(16) u32x4 sq[L::STEPS][kWave];
-    __shared__ __align__(16) float so[kWaves][4][HD + 4];
-    __shared__ float sm[kWaves][kHeads], sl[kWaves][kHeads];
+    __shared__ __align__(16) float so[WAVES][4][HD + 4];
+    __shared__ float sm[WAVES][kHeads], sl[WAVES][kHeads];
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
     const int lr = l % 16, lg = l / 16;
+    const int mask = (1 << a.shift) - 1;
+    const uint32_t off_k = (uint32_t)(lr * HD + L::V * lg) * (uint32_t)sizeof(T);
+    const uint32_t off_v = (uint32_t)(4 * lg * HD + L::VD * lr) * (uint32_t)sizeof(T);
+    L x;
+    const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
+    const int head0 = kvh * a.group + hg * kHeads;
+    const int gu = min(kHeads, a.group - hg * kHeads);
+    const int32_t *pages = a.table + (int64_t)row * a.width;
+
+    // this wavefront's tiles: one of every WAVES
+    const int jw = j0 + wv, cnt = j1 > jw ? (j1 - jw + WAVES - 1) / WAVES : 0;
+    int32_t ids = -1;  // lane l: the page of tile k0 + l / SUBS, sub l % SUBS
+    auto fetch_ids = [&](int k0) {
+        const int k = k0 + l / L::SUBS;
+        const int key = (jw + WAVES * k) * TILE + 16 * (l % L::SUBS);
+        if (k < cnt) ids = pages[min(key, keys - 1) >> a.shift];
+    };
+    fetch_ids(0);
+    int limit[L::SUBS];  // keys of the tile's halves that count
+    // bytes to the half's first key: its 16 lie in one page, those past the end too
+    int64_t from[L::SUBS];
+    auto locate = [&](int k) {  // where tile k lies
+        if (k && k % KT == 0) fetch_ids(k);
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s) {
+            const int key0 = (jw + WAVES * k) * TILE + 16 * s;
+            const int id = __builtin_amdgcn_readlane(ids, k % KT * L::SUBS + s);
+            const bool ok = (uint32_t)id < (uint32_t)a.pages;
+            from[s] = ((((int64_t)(ok ? id : 0) * a.kv + kvh) << a.shift) + (key0 & mask)) *
+                      (HD * (int)sizeof(T));
+            const int left = min(max(keys - key0, 0), 16);
+            limit[s] = ok ? left : 0;
+            if (!ok && left && l == 0) raise_flag(a.error_flag);
+        }
+    };
+    auto load_k = [&] {
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+            for (int i = 0; i < L::STEPS; ++i)
+                x.k[s][i] = load_page<u32x4>((const char *)a.k + from[s] + off_k +
+                                             L::DS * (int)sizeof(T) * i);
+    };
+    auto load_v = [&] {
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int c = 0; c < L::VC; ++c)
+                    x.v[s][r][c] = load_page<typename L::piece>(
+                        (const char *)a.v + from[s] + off_v +
+                        (r * HD + 16 * L::VD * c) * (int)sizeof(T));
+    };
+    if (cnt) {
+        locate(0);
+        load_k();
+        load_v();
+    }
+    // q as the other operand of the scores, heads past the group's repeat its last
+    for (int i = threadIdx.x; i < L::STEPS * kWave; i += WAVES * kWave) {
+        const int s = i / kWave, ln = i % kWave;
+        sq[s][ln] = load_raw((const T *)a.q + (int64_t)entry * a.q_tok +
+                             (int64_t)(head0 + min(ln % 16, gu - 1)) * a.q_head + L::DS * s +
+                             L::V * (ln / 16));
+    }
+    __syncthreads();
+    x.clear();
+    // tile k; with another after it the loads of that one follow the last use of the
+    // registers they fill (in a branch of their own they would be waited for there)
+    auto step = [&](int k, auto more) {
+        f32x4 sc[L::SUBS];
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < L::STEPS; ++i) {
+            const u32x4 qf = sq[i][l];
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s) {
+                if constexpr (L::BF) {
+                    sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, x.k[s][i]), __builtin_bit_cast(bf16x8, qf),
+                        sc[s], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            __uint_as_float(x.k[s][i][e]), __uint_as_float(qf[e]), sc[s], 0, 0,
+                            0);
+                }
+            }
+        }
+        int now[L::SUBS];
+        bool cut = false;
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s) now[s] = limit[s], cut = cut || limit[s] < 16;
+        if constexpr (decltype(more)::value) {
+            __builtin_amdgcn_sched_barrier(0);
+            locate(k + 1);
+            load_k();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (cut) {
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (4 * lg + r < now[s]) continue;
+                    sc[s][r] = -__builtin_inff();
+#pragma unroll
+                    for (int c = 0; c < L::VC; ++c)  // 0 times what lies there may be NaN
+                        x.v[s][r][c] = typename L::piece(0u);
+                }
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[s][r]);
+        top = fmaxf(swap_max(top) * a.scale_log2, x.base);
+        if (__any(top > x.base)) {
+            const float f = __builtin_amdgcn_exp2f(x.base - top);
+            x.sum *= f;
+#pragma unroll
+            for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < L::VD; ++j) x.o[c][j] *= f;
+            x.base = top;
+        }
+        float p[L::SUBS][4];
+#pragma unroll
+        for (int s = 0; s < L::SUBS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[s][r] = __builtin_amdgcn_exp2f(
+                    __builtin_fmaf(sc[s][r], a.scale_log2, -x.base));
+                x.sum += p[s][r];
+            }
+        if constexpr (L::BF) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p0 = p[i / 2][2 * (i % 2)], p1 = p[i / 2][2 * (i % 2) + 1];
+                hi[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0),
+                                              0x07060302u);
+                lo[i] = pack_bf16x2(rest(p0), rest(p1));
+            }
+#pragma unroll
+            for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < L::VD; ++j) {
+                    u32x4 vf;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        vf[i] = __builtin_amdgcn_perm(
+                            x.v[i / 2][2 * (i % 2) + 1][c][j / 2],
+                            x.v[i / 2][2 * (i % 2)][c][j / 2],
+                            j % 2 ? 0x07060302u : 0x05040100u);
+                    const bf16x8 vb = __builtin_bit_cast(bf16x8, vf);
+                    x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        vb, __builtin_bit_cast(bf16x8, hi), x.o[c][j], 0, 0, 0);
+                    x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        vb, __builtin_bit_cast(bf16x8, lo), x.o[c][j], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < L::VD; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            __uint_as_float(x.v[0][r][c][j]), p[0][r], x.o[c][j], 0, 0, 0);
+        }
+        if constexpr (decltype(more)::value) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_v();
+        }
+    };
+    for (int k = 0; k + 1 < cnt; ++k) step(k, std::true_type{});
+    if (cnt) step(cnt - 1, std::false_type{});
+    // the wavefronts' sums together, four heads at a time
+    x.sum = swap_sum32(swap_sum16(x.sum));
+    if (lg == 0) {
+        sm[wv][lr] = x.base;
+        sl[wv][lr] = x.sum;
+    }
+    for (int h0 = 0; h0 < gu; h0 += 4) {
+        const int hh = lr - h0;
+        if (hh >= 0 && hh < 4)
+#pragma unroll
+            for (int c = 0; c < L::VC; ++c)
+#pragma unroll
+                for (int j = 0; j < L::VD; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        so[wv][hh][16 * L::VD * c + L::VD * (4 * lg + r) + j] = x.o[c][j][r];
+        __syncthreads();
+        const int h = h0 + threadIdx.x / kWave, dim = VEC * l;
+        if (h < gu && h < h0 + 4) {
+            float top = sm[0][h], acc[VEC] = {}, total = 0.0f;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sm[w][h]);
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(sm[w][h] - top);
+                total = __builtin_fmaf(f, sl[w][h], total);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    acc[e] = __builtin_fmaf(f, so[w][h - h0][dim + e], acc[e]);
+            }
+            if (whole) {
+                const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) acc[e] *= inv;
+                store_out<T, HD, VEC>(a, entry, head0 + h, dim, acc);
+            } else {
+                float *dst = a.pieces + (slot * a.unit_heads + h) * HD + dim;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) dst[e] = acc[e];
+                if (l == 0) {
+                    float *st = a.stats + (slot * a.unit_heads + h) * 2;
+                    st[0] = top;
+                    st[1] = total;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(PagedAttention a) {
+    constexpr int TILE = tile_keys<T>();
     Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
     const int lw = log_workers(a.log_wgs, all);
     if (blockIdx.x >> lw) return;
     uint32_t t = (uint32_t)(((uint64_t)all * blockIdx.x) >> lw);
     const uint32_t t_end = (uint32_t)(((uint64_t)all * (blockIdx.x + 1)) >> lw);
-    const int mask = (1 << a.shift) - 1;
-    const uint32_t off_k = (uint32_t)(lr * HD + L::V * lg) * (uint32_t)sizeof(T);
-    const uint32_t off_v = (uint32_t)(4 * lg * HD + L::VD * lr) * (uint32_t)sizeof(T);
-    L x;
     while (t < t_end) {
         while (line.before + line.all <= t) line.next();
         // the entry and unit that hold place t, and the tiles of it up to t_end
-        const int el = __builtin_ctzll(__ballot(line.before + line.end > t)), entry = line.first + el;
+        const int el = __builtin_ctzll(__ballot(line.before + line.end > t));
         const int keys = __builtin_amdgcn_readlane(line.keys, el);
         const int row = __builtin_amdgcn_readlane(line.row, el);
         const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE, span = tiles + line.kBegin;
@@ -222,234 +469,29 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
         t += p1 - p0;
         if (p1 <= line.kBegin) continue;
         const uint32_t j0 = p0 > line.kBegin ? p0 - line.kBegin : 0, j1 = p1 - line.kBegin;
-        const int kvh = (int)unit / a.head_groups, hg = (int)unit - kvh * a.head_groups;
-        const int head0 = kvh * a.group + hg * kHeads;
-        const int gu = min(kHeads, a.group - hg * kHeads);
-        const int32_t *pages = a.table + (int64_t)row * a.width;
-
-        // this wavefront's tiles: every fourth
-        const int jw = (int)j0 + wv, cnt = (int)j1 > jw ? ((int)j1 - jw + kWaves - 1) / kWaves : 0;
-        int32_t ids = -1;  // lane l: the page of tile k0 + l / SUBS, sub l % SUBS
-        auto fetch_ids = [&](int k0) {
-            const int k = k0 + l / L::SUBS;
-            const int key = (jw + kWaves * k) * TILE + 16 * (l % L::SUBS);
-            if (k < cnt) ids = pages[min(key, keys - 1) >> a.shift];
-        };
-        fetch_ids(0);
-        int limit[L::SUBS];  // keys of the tile's halves that count
-        // bytes to the half's first key: its 16 lie in one page, those past the end too
-        int64_t from[L::SUBS];
-        auto locate = [&](int k) {  // where tile k lies
-            if (k && k % KT == 0) fetch_ids(k);
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s) {
-                const int key0 = (jw + kWaves * k) * TILE + 16 * s;
-                const int id = __builtin_amdgcn_readlane(ids, k % KT * L::SUBS + s);
-                const bool ok = (uint32_t)id < (uint32_t)a.pages;
-                from[s] = ((((int64_t)(ok ? id : 0) * a.kv + kvh) << a.shift) + (key0 & mask)) *
-                          (HD * (int)sizeof(T));
-                const int left = min(max(keys - key0, 0), 16);
-                limit[s] = ok ? left : 0;
-                if (!ok && left && l == 0) raise_flag(a.error_flag);
-            }
-        };
-        auto load_k = [&] {
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s)
-#pragma unroll
-                for (int i = 0; i < L::STEPS; ++i)
-                    x.k[s][i] = load_page<u32x4>((const char *)a.k + from[s] + off_k +
-                                                 L::DS * (int)sizeof(T) * i);
-        };
-        auto load_v = [&] {
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int c = 0; c < L::VC; ++c)
-                        x.v[s][r][c] = load_page<typename L::piece>(
-                            (const char *)a.v + from[s] + off_v +
-                            (r * HD + 16 * L::VD * c) * (int)sizeof(T));
-        };
-        if (cnt) {
-            locate(0);
-            load_k();
-            load_v();
-        }
-        // q as the other operand of the scores, heads past the group's repeat its last
-        for (int i = threadIdx.x; i < L::STEPS * kWave; i += kBlock) {
-            const int s = i / kWave, ln = i % kWave;
-            sq[s][ln] = load_raw((const T *)a.q + (int64_t)entry * a.q_tok +
-                                 (int64_t)(head0 + min(ln % 16, gu - 1)) * a.q_head + L::DS * s +
-                                 L::V * (ln / 16));
-        }
-        __syncthreads();
-        x.clear();
-        // tile k; with another after it the loads of that one follow the last use of the
-        // registers they fill (in a branch of their own they would be waited for there)
-        auto step = [&](int k, auto more) {
-            f32x4 sc[L::SUBS];
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < L::STEPS; ++i) {
-                const u32x4 qf = sq[i][l];
-#pragma unroll
-                for (int s = 0; s < L::SUBS; ++s) {
-                    if constexpr (L::BF) {
-                        sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8, x.k[s][i]), __builtin_bit_cast(bf16x8, qf),
-                            sc[s], 0, 0, 0);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                __uint_as_float(x.k[s][i][e]), __uint_as_float(qf[e]), sc[s], 0, 0,
-                                0);
-                    }
-                }
-            }
-            int now[L::SUBS];
-            bool cut = false;
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s) now[s] = limit[s], cut = cut || limit[s] < 16;
-            if constexpr (decltype(more)::value) {
-                __builtin_amdgcn_sched_barrier(0);
-                locate(k + 1);
-                load_k();
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (cut) {
-#pragma unroll
-                for (int s = 0; s < L::SUBS; ++s)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (4 * lg + r < now[s]) continue;
-                        sc[s][r] = -__builtin_inff();
-#pragma unroll
-                        for (int c = 0; c < L::VC; ++c)  // 0 times what lies there may be NaN
-                            x.v[s][r][c] = typename L::piece(0u);
-                    }
-            }
-            float top = sc[0][0];
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[s][r]);
-            top = fmaxf(swap_max(top) * a.scale_log2, x.base);
-            if (__any(top > x.base)) {
-                const float f = __builtin_amdgcn_exp2f(x.base - top);
-                x.sum *= f;
-#pragma unroll
-                for (int c = 0; c < L::VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < L::VD; ++j) x.o[c][j] *= f;
-                x.base = top;
-            }
-            float p[L::SUBS][4];
-#pragma unroll
-            for (int s = 0; s < L::SUBS; ++s)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[s][r] = __builtin_amdgcn_exp2f(
-                        __builtin_fmaf(sc[s][r], a.scale_log2, -x.base));
-                    x.sum += p[s][r];
-                }
-            if constexpr (L::BF) {
-                u32x4 hi, lo;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p0 = p[i / 2][2 * (i % 2)], p1 = p[i / 2][2 * (i % 2) + 1];
-                    hi[i] = __builtin_amdgcn_perm(__float_as_uint(p1), __float_as_uint(p0),
-                                                  0x07060302u);
-                    lo[i] = pack_bf16x2(rest(p0), rest(p1));
-                }
-#pragma unroll
-                for (int c = 0; c < L::VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < L::VD; ++j) {
-                        u32x4 vf;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            vf[i] = __builtin_amdgcn_perm(
-                                x.v[i / 2][2 * (i % 2) + 1][c][j / 2],
-                                x.v[i / 2][2 * (i % 2)][c][j / 2],
-                                j % 2 ? 0x07060302u : 0x05040100u);
-                        const bf16x8 vb = __builtin_bit_cast(bf16x8, vf);
-                        x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            vb, __builtin_bit_cast(bf16x8, hi), x.o[c][j], 0, 0, 0);
-                        x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            vb, __builtin_bit_cast(bf16x8, lo), x.o[c][j], 0, 0, 0);
-                    }
-            } else {
-#pragma unroll
-                for (int c = 0; c < L::VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < L::VD; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                __uint_as_float(x.v[0][r][c][j]), p[0][r], x.o[c][j], 0, 0, 0);
-            }
-            if constexpr (decltype(more)::value) {
-                __builtin_amdgcn_sched_barrier(0);
-                load_v();
-            }
-        };
-        for (int k = 0; k + 1 < cnt; ++k) step(k, std::true_type{});
-        if (cnt) step(cnt - 1, std::false_type{});
-        // the wavefronts' sums together, four heads at a time
-        x.sum = swap_sum32(swap_sum16(x.sum));
-        if (lg == 0) {
-            sm[wv][lr] = x.base;
-            sl[wv][lr] = x.sum;
-        }
-        const bool whole = j0 == 0 && j1 == tiles;
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (j0 == 0);
-        for (int h0 = 0; h0 < gu; h0 += 4) {
-            const int hh = lr - h0;
-            if (hh >= 0 && hh < 4)
-#pragma unroll
-                for (int c = 0; c < L::VC; ++c)
-#pragma unroll
-                    for (int j = 0; j < L::VD; ++j)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            so[wv][hh][16 * L::VD * c + L::VD * (4 * lg + r) + j] = x.o[c][j][r];
-            __syncthreads();
-            const int h = h0 + threadIdx.x / kWave, dim = VEC * l;
-            if (h < gu) {
-                float top = sm[0][h], acc[VEC] = {}, total = 0.0f;
-#pragma unroll
-                for (int w = 1; w < kWaves; ++w) top = fmaxf(top, sm[w][h]);
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(sm[w][h] - top);
-                    total = __builtin_fmaf(f, sl[w][h], total);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        acc[e] = __builtin_fmaf(f, so[w][h - h0][dim + e], acc[e]);
-                }
-                if (whole) {
-                    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) acc[e] *= inv;
-                    store_out<T, HD, VEC>(a, entry, head0 + h, dim, acc);
-                } else {
-                    float *dst = a.pieces + (slot * a.unit_heads + h) * HD + dim;
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) dst[e] = acc[e];
-                    if (l == 0) {
-                        float *st = a.stats + (slot * a.unit_heads + h) * 2;
-                        st[0] = top;
-                        st[1] = total;
-                    }
-                }
-            }
-            __syncthreads();
-        }
+        attend<T, HD, kWaves>(a, line.first + el, row, keys, (int)unit, (int)j0, (int)j1,
+                              j0 == 0 && j1 == tiles, 2 * (int64_t)blockIdx.x + (j0 == 0));
     }
+}
+
+// The same where every row is short: a workgroup for a unit, whole, and no join.
+template <typename T, int HD>
+__global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short(PagedAttention a) {
+    constexpr int TILE = tile_keys<T>(), WAVES = short_waves(HD), VEC = HD / kWave;
+    const int units = a.kv * a.head_groups;
+    const int entry = blockIdx.x / units, unit = blockIdx.x - entry * units;
+    const int row = a.index[entry];
+    bool bad;
+    const int keys = entry_keys(a, row, a.positions[entry], bad);
+    if (bad && unit == 0 && threadIdx.x == 0) raise_flag(a.error_flag);
+    if (keys) {
+        attend<T, HD, WAVES>(a, entry, row, keys, unit, 0, (keys + TILE - 1) / TILE, true, 0);
+        return;
+    }
+    const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
+    for (int h = threadIdx.x / kWave; h < min(kHeads, a.group - hg * kHeads); h += WAVES)
+        store_zero<T, HD, VEC>(a, entry, kvh * a.group + hg * kHeads + h,
+                               VEC * (threadIdx.x % kWave));
 }
 
 // A workgroup per (entry, head): the pieces of its keys, in order; zeros for an entry
@@ -458,7 +500,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a) {
     constexpr int TILE = tile_keys<T>();
     constexpr int LPP = HD / 4, PARTS = kBlock / LPP;  // lanes of a piece's row, rows at a time
-    __shared__ float weight[1 << kMaxLogWgs], top_of[kWaves], sum_of[kWaves];
+    __shared__ float top_of[PARTS], sum_of[PARTS];
     __shared__ __align__(16) float so[PARTS][HD];
     const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
     const int entry = blockIdx.x / a.heads, h = blockIdx.x - entry * a.heads;
@@ -476,11 +518,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
     }
     const int dim = HD / kWave * l;
     if (tiles == 0) {
-        float zero[HD / kWave] = {};
-        // 0 whatever the gate holds
-        PagedAttention b = a;
-        b.gate = nullptr;
-        if (wv == 0) store_out<T, HD, HD / kWave>(b, entry, h, dim, zero);
+        if (wv == 0) store_zero<T, HD, HD / kWave>(a, entry, h, dim);
         return;
     }
     const int lw = log_workers(a.log_wgs, all);
@@ -496,46 +534,42 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
     auto slot = [&](int p) {
         return ((2 * (int64_t)(w0 + p) + (p == 0)) * a.unit_heads + hu);
     };
-    float top = -FLT_MAX;
-    for (int p = threadIdx.x; p < parts; p += kBlock) top = fmaxf(top, a.stats[2 * slot(p)]);
-    top = swap_max(top);
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d, kWave));
-    if (l == 0) top_of[wv] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, top_of[w]);
-    float sum = 0.0f;
-    for (int p = threadIdx.x; p < parts; p += kBlock) {
-        const float f = __builtin_amdgcn_exp2f(a.stats[2 * slot(p)] - top);
-        weight[p] = f;
-        sum = __builtin_fmaf(f, a.stats[2 * slot(p) + 1], sum);
-    }
-    sum = group_sum<kWave>(sum);
-    if (l == 0) sum_of[wv] = sum;
-    __syncthreads();
+    // Each group of LPP lanes runs over every PARTS-th piece, its maximum and sum beside
+    // the rows, so that nothing waits for a first pass over the maxima.
     const int part = threadIdx.x / LPP, d4 = 4 * (threadIdx.x % LPP);
+    float top = -FLT_MAX, sum = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = part; p < parts; p += PARTS) {
         const f32x4 o = *reinterpret_cast<const f32x4 *>(a.pieces + slot(p) * HD + d4);
-        const float f = weight[p];
+        const f32x2 s = *reinterpret_cast<const f32x2 *>(a.stats + 2 * slot(p));
+        const float m = fmaxf(top, s[0]);
+        const float f = __builtin_amdgcn_exp2f(top - m), g = __builtin_amdgcn_exp2f(s[0] - m);
+        top = m;
+        sum = __builtin_fmaf(g, s[1], f * sum);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(f, o[e], acc[e]);
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(g, o[e], f * acc[e]);
     }
     *reinterpret_cast<f32x4 *>(&so[part][d4]) = acc;
+    if (d4 == 0) {
+        top_of[part] = top;
+        sum_of[part] = sum;
+    }
     __syncthreads();
     if (wv) return;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) top = fmaxf(top, top_of[p]);
     float total = 0.0f, o[HD / kWave] = {};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += sum_of[w];
+    for (int p = 0; p < PARTS; ++p) {
+        const float f = __builtin_amdgcn_exp2f(top_of[p] - top);
+        total = __builtin_fmaf(f, sum_of[p], total);
+#pragma unroll
+        for (int e = 0; e < HD / kWave; ++e) o[e] = __builtin_fmaf(f, so[p][dim + e], o[e]);
+    }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
 #pragma unroll
-    for (int e = 0; e < HD / kWave; ++e) {
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) o[e] += so[p][dim + e];
-        o[e] *= inv;
-    }
+    for (int e = 0; e < HD / kWave; ++e) o[e] *= inv;
     store_out<T, HD, HD / kWave>(a, entry, h, dim, o);
 }
 
@@ -556,6 +590,16 @@ int64_t longest_line(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_di
     const int64_t span = ceil_div(width * page_size, tile) +
                          65536 / (tile * head_dim * 2 * elem_size(dtype));
     return span >= lim / units / n ? 0 : span * units * n;
+}
+
+// Whether rows of `width` pages are short: at most kShortTiles tiles a wavefront.  (The
+// grid of a workgroup for each unit stays below 2^32 work-items.)
+bool short_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t width,
+                int64_t page_size, int32_t dtype) {
+    const int64_t tile = dtype == QDC_BF16 ? tile_keys<bf16_t>() : tile_keys<float>();
+    const int64_t units = kv_heads * ceil_div(heads / kv_heads, (int64_t)kHeads);
+    return width * page_size <= tile * kShortTiles * short_waves((int)head_dim) &&
+           n * units < ((int64_t)1 << 22);
 }
 
 // Workgroups for a line: one a compute unit for heads of 256, whose operands take half
@@ -583,7 +627,8 @@ extern "C" int64_t qdc_paged_attention_workspace(int64_t n, int64_t heads, int64
                                                  int64_t head_dim, int64_t width,
                                                  int64_t page_size, int32_t dtype) {
     const int64_t line = longest_line(n, heads, kv_heads, head_dim, width, page_size, dtype);
-    if (line == 0) return 0;
+    if (line == 0) return -1;
+    if (short_rows(n, heads, kv_heads, head_dim, width, page_size, dtype)) return 0;
     // two pieces a workgroup, each with its maximum and sum
     return ((int64_t)2 << log_workgroups(line, head_dim)) * unit_heads(heads, kv_heads) * (head_dim + 2) * 4;
 }
@@ -610,13 +655,14 @@ extern "C" int32_t qdc_paged_attention(
         return QDC_ERR_SHAPE;
     if (!(scale > 0.0f) || !(scale * 1.4426950408889634f < __builtin_inff())) return QDC_ERR_RANGE;
     if (n == 0) return QDC_OK;
-    if (!out || !q || !k_pages || !v_pages || !table || !index || !positions || !workspace)
+    const int64_t need = qdc_paged_attention_workspace(n, heads, kv_heads, head_dim, width,
+                                                       page_size, dtype);
+    if (!out || !q || !k_pages || !v_pages || !table || !index || !positions ||
+        (need && !workspace))
         return QDC_ERR_NULL;
     if (!aligned16(out) || !aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) ||
         !aligned16(gate) || !aligned16(workspace))
         return QDC_ERR_SHAPE;
-    const int64_t need = qdc_paged_attention_workspace(n, heads, kv_heads, head_dim, width,
-                                                       page_size, dtype);
     if (workspace_bytes < need) return QDC_ERR_SHAPE;
     const int64_t store = pages * kv_heads * page_size * head_dim * es;
     const Range outs[3] = {{out, ((n - 1) * out_tok + heads * head_dim) * oes},
@@ -656,11 +702,18 @@ extern "C" int32_t qdc_paged_attention(
     a.log_wgs = log_workgroups(line, head_dim);
     a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const dim3 grid(1u << a.log_wgs), join((uint32_t)(n * heads)), block(kBlock);
+    const bool brief = need == 0;
+    const dim3 grid(brief ? (uint32_t)(n * kv_heads * a.head_groups) : 1u << a.log_wgs);
+    const dim3 join((uint32_t)(n * heads)), block(kBlock);
     a.pieces = reinterpret_cast<float *>(workspace);
     a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;
 #define QDC_PAGED(T, HD)                                                                       \
     if (head_dim == HD) {                                                                      \
+        if (brief) {                                                                           \
+            hipLaunchKernelGGL((paged_attention_short<T, HD>), grid,                           \
+                               dim3(short_waves(HD) * kWave), 0, stream, a);                   \
+            return launch_status();                                                            \
+        }                                                                                      \
         hipLaunchKernelGGL((paged_attention<T, HD>), grid, block, 0, stream, a);               \
         const int32_t status = launch_status();                                                \
         if (status != QDC_OK) return status;                                                   \

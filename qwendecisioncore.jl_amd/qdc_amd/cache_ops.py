@@ -27,9 +27,12 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .ops import (_DTYPES, _device, _dtype_code, _is_split, _rope_tables, _stream, _vector)
+from .ops import _DTYPES, _device, _is_split, _rope_tables
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
+_I32, _F32 = torch.int32, torch.float32
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class PageTable(NamedTuple):
@@ -57,49 +60,83 @@ def page_table(rows: int, width: int, pages: int, page_size: int, device) -> Pag
                      torch.zeros(pages, **i32), free, page_size)
 
 
-def _ints(t: torch.Tensor, like: torch.Tensor, name: str, n: int | None = None) -> int:
-    """Pointer of a contiguous device int32 vector (of ``n`` entries)."""
-    if t.device != like.device:
-        raise ValueError(f"tensors on different devices: {like.device} vs {t.device}")
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() \
-            or (n is not None and t.shape[0] != n):
+# The host's part of a call is the whole cost of a small one, so each check below is one
+# expression of plain attributes (a device as its index, get_device, in 0.04 us where
+# comparing device objects takes 0.12).
+def _call(dev: int, name: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on device ``dev``, made the current one for the launch if it
+    is not."""
+    if _current_device() == dev:
+        status = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _raw_stream(dev))
+    if status:
+        check(status, name)
+
+
+def _on(t: torch.Tensor) -> int:
+    """The index of a call's device, that of its first tensor."""
+    dev = t.get_device()
+    if dev < 0:
+        _device(t)
+    return dev
+
+
+def _ints(t: torch.Tensor, dev: int, name: str, n: int) -> int:
+    """Pointer of a contiguous int32 vector of ``n`` entries (-1: any number)."""
+    shape = t.shape
+    if t.dtype is not _I32 or len(shape) != 1 or (n >= 0 and shape[0] != n) \
+            or t.get_device() != dev or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 vector"
-                         + ("" if n is None else f" of {n} entries"))
+                         + (f" of {n} entries" if n >= 0 else "") + " on the call's device")
     return t.data_ptr()
 
 
-def _flag(error_flag: torch.Tensor | None, like: torch.Tensor) -> int:
+def _flag(error_flag: torch.Tensor | None, dev: int) -> int:
     if error_flag is None:
         return 0
-    if error_flag.device != like.device or error_flag.dtype != torch.int32 \
-            or error_flag.numel() < 1:
+    if error_flag.get_device() != dev or error_flag.dtype is not _I32 or error_flag.numel() < 1:
         raise ValueError("error_flag must be an int32 tensor on the call's device")
     return error_flag.data_ptr()
 
 
-def _table(table: torch.Tensor, like: torch.Tensor) -> tuple:
-    if table.device != like.device:
-        raise ValueError(f"tensors on different devices: {like.device} vs {table.device}")
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
-        raise ValueError("table must be a contiguous int32 [rows, width] tensor")
-    return table.shape
+def _table(table: torch.Tensor, dev: int) -> tuple:
+    shape = table.shape
+    if table.dtype is not _I32 or len(shape) != 2 or table.get_device() != dev \
+            or not table.is_contiguous():
+        raise ValueError("table must be a contiguous int32 [rows, width] tensor on the call's "
+                         "device")
+    return shape
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, like: torch.Tensor, kv: int, hd: int):
-    """(pages, page_size) of a layer's page tensors."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != kv \
-            or k_pages.shape[3] != hd:
-        raise ValueError("k_pages and v_pages must be [pages, kv_heads, page_size, head_dim]")
-    for t in (k_pages, v_pages):
-        if t.dtype != like.dtype or not t.is_contiguous() or t.device != like.device:
-            raise ValueError("k_pages and v_pages must be contiguous, of q's dtype and device")
-    return k_pages.shape[0], k_pages.shape[2]
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, like: torch.Tensor, dev: int):
+    """Shape of a layer's page tensors."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype is not like.dtype \
+            or v_pages.dtype is not like.dtype or k_pages.get_device() != dev \
+            or v_pages.get_device() != dev or not k_pages.is_contiguous() \
+            or not v_pages.is_contiguous():
+        raise ValueError("k_pages and v_pages must be contiguous [pages, kv_heads, page_size, "
+                         "head_dim] tensors of q's dtype and device")
+    return shape
 
 
-def _heads(t: torch.Tensor, n: int) -> tuple:
-    """(token stride, head stride) of a ``[n, heads, head_dim]`` view."""
-    return (t.stride(0) if n > 1 else t.shape[1] * t.shape[2],
-            t.stride(1) if t.shape[1] > 1 else t.shape[2])
+def _rows(t: torch.Tensor, like: torch.Tensor, dev: int, name: str):
+    """Shape and (token, head) strides of a ``[n, heads, head_dim]`` view."""
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or strides[2] != 1 or t.dtype is not like.dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous rows, of q's "
+                         "dtype and device")
+    return shape, (strides[0] if shape[0] > 1 else shape[1] * shape[2],
+                   strides[1] if shape[1] > 1 else shape[2])
+
+
+def _code(t: torch.Tensor) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"unsupported dtype {t.dtype}; expected float32 or bfloat16")
+    return code
 
 
 # --------------------------------------------------------------- attention ---
@@ -118,37 +155,39 @@ def prepare_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     and not stored; the same, with ``error_flag`` set, for one whose position is beyond
     the rotation tables or the row's pages.  Of two tokens at one position of one row,
     either may be stored, or pieces of both.  head_dim 64, 128 or 256."""
-    _device(q, k, v, q_norm, k_norm)
-    code = _dtype_code(q, k, v, q_norm, k_norm)
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] \
-            or q.shape[2] != k.shape[2]:
+    dev, code = _on(q), _code(q)
+    (T, H, hd), q_strides = _rows(q, q, dev, "q")
+    k_shape, k_strides = _rows(k, q, dev, "k")
+    v_shape, v_strides = _rows(v, q, dev, "v")
+    KV = k_shape[1]
+    if v_shape != k_shape or k_shape[0] != T or k_shape[2] != hd:
         raise ValueError("q must be [T, H, hd] and k, v [T, KV, hd]")
-    T, H, hd = q.shape
-    KV = k.shape[1]
-    for t in (q, k, v):
-        if t.stride(2) != 1:
-            raise ValueError("rows must be contiguous")
-    _vector(q_norm, hd, "q_norm")
-    _vector(k_norm, hd, "k_norm")
-    pages, page = _pages(k_pages, v_pages, q, KV, hd)
+    for w in (q_norm, k_norm):
+        if w.dtype is not q.dtype or w.numel() != hd or w.get_device() != dev \
+                or not w.is_contiguous():
+            raise ValueError(f"q_norm and k_norm must be contiguous vectors of {hd} elements, of "
+                             "q's dtype and device")
+    page_shape = _pages(k_pages, v_pages, q, dev)
+    if page_shape[1] != KV or page_shape[3] != hd:
+        raise ValueError("k_pages and v_pages must hold k's heads")
     cos, sin = _rope_tables(tables, rotary_dim, q)
-    n_rows, width = _table(table, q)
-    index, at = _ints(rows, q, "rows", T), _ints(positions, q, "positions", T)
+    n_rows, width = _table(table, dev)
+    index, at = _ints(rows, dev, "rows", T), _ints(positions, dev, "positions", T)
     if q_out is None:
         q_out = torch.empty((T, H, hd), dtype=q.dtype, device=q.device)
-    for out, shape in ((q_out, (T, H, hd)), (k_out, (T, KV, hd))):
-        if out is not None and (out.shape != shape or out.dtype != q.dtype
-                                or not out.is_contiguous() or out.device != q.device):
-            raise ValueError("q_out and k_out must be contiguous tensors of q's and k's shape, "
-                             "of q's dtype and device")
-    check(lib().qdc_prepare_paged(
-        q_out.data_ptr(), 0 if k_out is None else k_out.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(),
-        k_norm.data_ptr(), 0 if cos is None else cos.data_ptr(),
-        0 if sin is None else sin.data_ptr(), index, at, table.data_ptr(), T, H, KV, hd,
-        rotary_dim, 0 if cos is None else cos.shape[0], n_rows, width, pages, page, *_heads(q, T),
-        *_heads(k, T), *_heads(v, T), eps, code, _flag(error_flag, q), _stream(q)),
-        "prepare_paged")
+    elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.get_device() != dev \
+            or not q_out.is_contiguous():
+        raise ValueError("q_out must be a contiguous tensor of q's shape, dtype and device")
+    if k_out is not None and (k_out.shape != k_shape or k_out.dtype is not q.dtype
+                              or k_out.get_device() != dev or not k_out.is_contiguous()):
+        raise ValueError("k_out must be a contiguous tensor of k's shape, dtype and device")
+    _call(dev, "prepare_paged", lib().qdc_prepare_paged, q_out.data_ptr(),
+          0 if k_out is None else k_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+          q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+          0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), index, at,
+          table.data_ptr(), T, H, KV, hd, rotary_dim, 0 if cos is None else cos.shape[0], n_rows,
+          width, page_shape[0], page_shape[2], *q_strides, *k_strides, *v_strides, eps, code,
+          _flag(error_flag, dev))
     return q_out
 
 
@@ -164,64 +203,58 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``[n, 2*H*hd]``).  Entries that are no token give zeros; positions behind the
     table's width and pages that are none count as masked and set ``error_flag``.
     ``scale`` positive; head_dim 64, 128 or 256."""
-    _device(q)
-    code = _dtype_code(q)
-    if q.dim() != 3 or q.stride(2) != 1:
-        raise ValueError("q must be [n, H, hd] with contiguous rows")
-    n, H, hd = q.shape
-    if k_pages.dim() != 4 or k_pages.shape[1] == 0 or H % k_pages.shape[1]:
-        raise ValueError("the query heads must be a multiple of the KV heads of k_pages")
-    KV = k_pages.shape[1]
-    pages, page = _pages(k_pages, v_pages, q, KV, hd)
-    n_rows, width = _table(table, q)
-    index, at = _ints(rows, q, "rows", n), _ints(positions, q, "positions", n)
+    dev, code = _on(q), _code(q)
+    (n, H, hd), q_strides = _rows(q, q, dev, "q")
+    pages, KV, page, page_hd = _pages(k_pages, v_pages, q, dev)
+    if page_hd != hd or KV == 0 or H % KV:
+        raise ValueError("q's heads must be a multiple of those of k_pages, of one head_dim")
+    n_rows, width = _table(table, dev)
+    index, at = _ints(rows, dev, "rows", n), _ints(positions, dev, "positions", n)
     gate_at, gate_strides = 0, (0, hd)
     if gate is not None:
-        if gate.shape != q.shape or gate.dtype != q.dtype or gate.stride(2) != 1 \
-                or gate.device != q.device:
-            raise ValueError("gate must be a view like q with contiguous rows")
-        gate_at, gate_strides = gate.data_ptr(), _heads(gate, n)
-    split = _is_split(out_dtype)
-    odt = torch.bfloat16 if split else out_dtype or q.dtype
-    if odt not in _DTYPES:
-        raise ValueError("out_dtype must be float32, bfloat16 or BF16X2")
-    out = torch.empty((n, 2 * H * hd if split else H * hd), dtype=odt, device=q.device)
+        gate_shape, gate_strides = _rows(gate, q, dev, "gate")
+        if gate_shape != q.shape:
+            raise ValueError("gate must be a view like q")
+        gate_at = gate.data_ptr()
+    if out_dtype is None:
+        split, out_code, odt = False, code, q.dtype
+    else:
+        split = _is_split(out_dtype)
+        odt = torch.bfloat16 if split else out_dtype
+        out_code = _lib.QDC_BF16X2 if split else _DTYPES.get(odt)
+        if out_code is None:
+            raise ValueError("out_dtype must be float32, bfloat16 or BF16X2")
+    device = q.device
+    out = torch.empty((n, 2 * H * hd if split else H * hd), dtype=odt, device=device)
     need = lib().qdc_paged_attention_workspace(n, H, KV, hd, width, page, code)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    check(lib().qdc_paged_attention(
-        out.data_ptr(), _lib.QDC_BF16X2 if split else _DTYPES[odt], q.data_ptr(),
-        k_pages.data_ptr(), v_pages.data_ptr(), gate_at, table.data_ptr(), index, at, n, H, KV, hd,
-        n_rows, width, pages, page, *_heads(q, n), *gate_strides, H * hd, scale, code,
-        work.data_ptr(), need, _flag(error_flag, q), _stream(q)), "paged_attention")
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    _call(dev, "paged_attention", lib().qdc_paged_attention, out.data_ptr(), out_code,
+          q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), gate_at, table.data_ptr(), index,
+          at, n, H, KV, hd, n_rows, width, pages, page, *q_strides, *gate_strides, H * hd, scale,
+          code, 0 if work is None else work.data_ptr(), need, _flag(error_flag, dev))
     return out
 
 
 # ------------------------------------------------------------------- pages ---
 def _book(book: PageTable) -> tuple:
-    """The C arguments of a page table: (four pointers), (rows, width, pages, size)."""
+    """Of a page table: the device, (four pointers), (rows, width, pages, page size)."""
     table, lengths, refs, free, size = book
-    _device(table, lengths, refs, free)
-    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
-        raise ValueError("table must be a contiguous int32 [rows, width] tensor")
-    rows, width = table.shape
-    pages = refs.shape[0] if refs.dim() == 1 else -1
-    _ints(lengths, table, "lengths", rows)
-    _ints(refs, table, "refs")
-    _ints(free, table, "free", 1 + pages)
-    return ((table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), free.data_ptr()),
-            (rows, width, pages, size))
+    dev = _on(table)
+    rows, width = _table(table, dev)
+    at = (table.data_ptr(), _ints(lengths, dev, "lengths", rows), _ints(refs, dev, "refs", -1),
+          _ints(free, dev, "free", 1 + refs.shape[0]))
+    return dev, at, (rows, width, refs.shape[0], size)
 
 
-def _pool(pool: torch.Tensor | None, items: int, like: torch.Tensor, name: str):
+def _pool(pool: torch.Tensor | None, items: int, dev: int):
     """``(pointer, planes, bytes of an item)`` of a contiguous ``[planes, items, ...]``."""
     if pool is None:
         return 0, 0, 0
-    if pool.dim() < 3 or pool.shape[1] != items or not pool.is_contiguous() \
-            or pool.device != like.device:
-        raise ValueError(f"{name} must be a contiguous [planes, {items}, ...] tensor on the "
-                         "call's device")
-    return (pool.data_ptr(), pool.shape[0],
-            pool.numel() // max(1, pool.shape[0] * items) * pool.element_size())
+    shape = pool.shape
+    if len(shape) < 3 or shape[1] != items or pool.get_device() != dev or not pool.is_contiguous():
+        raise ValueError(f"pool must be a contiguous [planes, {items}, ...] tensor on the call's "
+                         "device")
+    return pool.data_ptr(), shape[0], pool.stride(1) * pool.element_size()
 
 
 def extend_pages(book: PageTable, rows: torch.Tensor, counts: torch.Tensor | None = None,
@@ -233,15 +266,14 @@ def extend_pages(book: PageTable, rows: torch.Tensor, counts: torch.Tensor | Non
     cannot be done whole -- a row out of range or named twice, a negative count, a row
     longer than its table, too few free pages -- does nothing but set every position
     to -1 and ``error_flag``."""
-    at, sizes = _book(book)
-    index = _ints(rows, book.table, "rows")
+    dev, at, sizes = _book(book)
+    index = _ints(rows, dev, "rows", -1)
     n = rows.shape[0]
-    many = 0 if counts is None else _ints(counts, book.table, "counts", n)
+    many = 0 if counts is None else _ints(counts, dev, "counts", n)
     if positions is None:
-        positions = torch.empty(n, dtype=torch.int32, device=rows.device)
-    out = _ints(positions, book.table, "positions", n)
-    check(lib().qdc_pages_extend(out, *at, index, many, n, *sizes, _flag(error_flag, book.table),
-                                 _stream(rows)), "extend_pages")
+        positions = torch.empty(n, dtype=_I32, device=rows.device)
+    _call(dev, "extend_pages", lib().qdc_pages_extend, _ints(positions, dev, "positions", n), *at,
+          index, many, n, *sizes, _flag(error_flag, dev))
     return positions
 
 
@@ -250,10 +282,9 @@ def free_pages(book: PageTable, rows: torch.Tensor,
     """Rows give up their pages and are empty; pages that no other row shares are free
     again (an empty row: nothing).  Negative rows are left out; a row out of range or
     named twice: nothing is done and ``error_flag`` is set."""
-    at, sizes = _book(book)
-    index = _ints(rows, book.table, "rows")
-    check(lib().qdc_pages_free(*at, index, rows.shape[0], *sizes, _flag(error_flag, book.table),
-                               _stream(rows)), "free_pages")
+    dev, at, sizes = _book(book)
+    _call(dev, "free_pages", lib().qdc_pages_free, *at, _ints(rows, dev, "rows", -1),
+          rows.shape[0], *sizes, _flag(error_flag, dev))
 
 
 def fork_pages(book: PageTable, parents: torch.Tensor, children: torch.Tensor,
@@ -265,30 +296,32 @@ def fork_pages(book: PageTable, parents: torch.Tensor, children: torch.Tensor,
     negative row are left out.  A child that is not empty, named twice or also a
     parent, a row out of range, too few free pages: nothing is done and ``error_flag``
     is set."""
-    at, sizes = _book(book)
-    src = _ints(parents, book.table, "parents")
+    dev, at, sizes = _book(book)
+    src = _ints(parents, dev, "parents", -1)
     n = parents.shape[0]
-    dst = _ints(children, book.table, "children", n)
-    if pool is not None and (pool.dim() != 5 or pool.shape[3] != book.page_size):
-        raise ValueError("pool must be [planes, pages, kv_heads, page_size, head_dim]")
-    pool_at, planes, _ = _pool(pool, sizes[2], book.table, "pool")
-    heads, token = (0, 0) if pool is None else (pool.shape[2], pool.shape[4] * pool.element_size())
+    dst = _ints(children, dev, "children", n)
+    pool_at, planes, _ = _pool(pool, sizes[2], dev)
+    heads = token = 0
+    if pool is not None:
+        shape = pool.shape
+        if len(shape) != 5 or shape[3] != book.page_size:
+            raise ValueError("pool must be [planes, pages, kv_heads, page_size, head_dim]")
+        heads, token = shape[2], shape[4] * pool.element_size()
     work = torch.empty(16 * n, dtype=torch.uint8, device=parents.device)
-    check(lib().qdc_pages_fork(*at, src, dst, n, *sizes, pool_at, planes, heads, token,
-                               work.data_ptr(), 16 * n, _flag(error_flag, book.table),
-                               _stream(parents)), "fork_pages")
+    _call(dev, "fork_pages", lib().qdc_pages_fork, *at, src, dst, n, *sizes, pool_at, planes,
+          heads, token, work.data_ptr(), 16 * n, _flag(error_flag, dev))
 
 
 def compact_pages(book: PageTable, pool: torch.Tensor | None = None) -> None:
     """The pages in use move to the low end, in every plane of ``pool [planes, pages,
     ...]``: with ``m`` of them, the k-th free page below ``m`` takes the k-th page in
     use from ``m`` on.  Tables and refs follow; the stack holds the rest, lowest on top."""
-    at, (rows, width, pages, _) = _book(book)
-    pool_at, planes, nbytes = _pool(pool, pages, book.table, "pool")
+    dev, at, (rows, width, pages, _) = _book(book)
+    pool_at, planes, nbytes = _pool(pool, pages, dev)
     need = lib().qdc_pages_compact_workspace(pages)
     work = torch.empty(need, dtype=torch.uint8, device=book.table.device)
-    check(lib().qdc_pages_compact(at[0], at[2], at[3], rows, width, pages, pool_at, planes, nbytes,
-                                  work.data_ptr(), need, _stream(book.table)), "compact_pages")
+    _call(dev, "compact_pages", lib().qdc_pages_compact, at[0], at[2], at[3], rows, width, pages,
+          pool_at, planes, nbytes, work.data_ptr(), need)
 
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -298,13 +331,13 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
     rows.  Pairs with a negative index are left out; a pair out of range, or whose
     ``dst`` is an earlier pair's or any pair's ``src``, is not copied and sets
     ``error_flag``."""
-    _device(pool)
-    index = _ints(src, pool, "src")
-    to = _ints(dst, pool, "dst", src.shape[0])
+    dev = _on(pool)
+    index = _ints(src, dev, "src", -1)
+    n = src.shape[0]
     items = pool.shape[1] if pool.dim() > 1 else -1
-    at, planes, nbytes = _pool(pool, items, pool, "pool")
-    check(lib().qdc_copy_pages(at, index, to, src.shape[0], planes, items, nbytes,
-                               _flag(error_flag, pool), _stream(pool)), "copy_pages")
+    at, planes, nbytes = _pool(pool, items, dev)
+    _call(dev, "copy_pages", lib().qdc_copy_pages, at, index, _ints(dst, dev, "dst", n), n, planes,
+          items, nbytes, _flag(error_flag, dev))
 
 
 # -------------------------------------------------------- linear attention ---
@@ -325,36 +358,45 @@ def delta_step(proj: torch.Tensor, conv: torch.Tensor, a_decay: torch.Tensor,
     token give zeros and leave the cache; so does a row out of range or that of an
     earlier token of the call, which sets ``error_flag``.  key_dim 32, 64 or 128,
     value_dim a multiple of 16 up to 256, up to 8 taps."""
-    _device(proj, conv, a_decay, dt_bias, norm, ring, state)
-    code = _dtype_code(proj, norm, ring)
-    channels, vw = 2 * key_heads * key_dim + value_heads * value_dim, value_heads * value_dim
-    if proj.dim() != 2 or proj.stride(1) != 1 or proj.shape[1] < channels + vw + 2 * value_heads:
+    dev, code, dtype = _on(proj), _code(proj), proj.dtype
+    vw = value_heads * value_dim
+    channels = 2 * key_heads * key_dim + vw
+    n, width = proj.shape if proj.dim() == 2 else (0, -1)
+    if width < channels + vw + 2 * value_heads or proj.stride(1) != 1:
         raise ValueError("proj must be [n, width] with contiguous rows of the q|k|v|z|a|b blocks")
-    for t in (conv, a_decay, dt_bias, state):
-        if t.dtype != torch.float32 or not t.is_contiguous():
-            raise ValueError("conv, a_decay, dt_bias and state must be contiguous float32")
-    if conv.dim() != 2 or conv.shape[0] != channels:
-        raise ValueError(f"conv must be [{channels}, taps] (the q|k|v channels)")
-    taps = conv.shape[1]
-    _vector(a_decay, value_heads, "a_decay")
-    _vector(dt_bias, value_heads, "dt_bias")
-    _vector(norm, value_dim, "norm")
-    if ring.dim() != 3 or ring.shape[1:] != (taps, channels) or not ring.is_contiguous():
-        raise ValueError(f"ring must be a contiguous [cache rows, {taps}, {channels}] tensor")
-    if state.shape != (ring.shape[0], value_heads, value_dim, key_dim):
-        raise ValueError("state must be [cache rows, value_heads, value_dim, key_dim]")
-    n = proj.shape[0]
-    index, at = _ints(rows, proj, "rows", n), _ints(positions, proj, "positions", n)
-    split = _is_split(out_dtype)
-    if split and proj.dtype != torch.bfloat16:
+    taps = conv.shape[-1]
+    if conv.shape != (channels, taps) or conv.dtype is not _F32 or conv.get_device() != dev \
+            or not conv.is_contiguous():
+        raise ValueError(f"conv must be a contiguous float32 [{channels}, taps] tensor (the q|k|v "
+                         "channels) on proj's device")
+    for t in (a_decay, dt_bias):
+        if t.dtype is not _F32 or t.numel() != value_heads or t.get_device() != dev \
+                or not t.is_contiguous():
+            raise ValueError(f"a_decay and dt_bias must be contiguous float32 vectors of "
+                             f"{value_heads} elements on proj's device")
+    if norm.dtype is not dtype or norm.numel() != value_dim or norm.get_device() != dev \
+            or not norm.is_contiguous():
+        raise ValueError(f"norm must be a contiguous vector of {value_dim} elements of proj's "
+                         "dtype and device")
+    cache_rows = state.shape[0]
+    if state.shape != (cache_rows, value_heads, value_dim, key_dim) or state.dtype is not _F32 \
+            or state.get_device() != dev or not state.is_contiguous():
+        raise ValueError("state must be a contiguous float32 [cache rows, value_heads, value_dim, "
+                         "key_dim] tensor on proj's device")
+    if ring.shape != (cache_rows, taps, channels) or ring.dtype is not dtype \
+            or ring.get_device() != dev or not ring.is_contiguous():
+        raise ValueError(f"ring must be a contiguous [cache rows, {taps}, {channels}] tensor of "
+                         "proj's dtype and device")
+    index, at = _ints(rows, dev, "rows", n), _ints(positions, dev, "positions", n)
+    split = out_dtype is not None and _is_split(out_dtype)
+    if split and dtype is not torch.bfloat16:
         raise ValueError("the split output takes a bfloat16 proj")
-    if not split and out_dtype not in (None, proj.dtype):
+    if not split and out_dtype not in (None, dtype):
         raise ValueError("out_dtype must be proj's dtype or BF16X2")
-    out = torch.empty((n, 2 * vw if split else vw), dtype=proj.dtype, device=proj.device)
-    check(lib().qdc_delta_step(
-        out.data_ptr(), _lib.QDC_BF16X2 if split else code, proj.data_ptr(), code,
-        proj.stride(0) if n > 1 else proj.shape[1], conv.data_ptr(), taps, a_decay.data_ptr(),
-        dt_bias.data_ptr(), norm.data_ptr(), ring.data_ptr(), state.data_ptr(), index, at, n,
-        ring.shape[0], key_heads, key_dim, value_heads, value_dim, eps, _flag(error_flag, proj),
-        _stream(proj)), "delta_step")
+    out = torch.empty((n, 2 * vw if split else vw), dtype=dtype, device=proj.device)
+    _call(dev, "delta_step", lib().qdc_delta_step, out.data_ptr(),
+          _lib.QDC_BF16X2 if split else code, proj.data_ptr(), code,
+          proj.stride(0) if n > 1 else width, conv.data_ptr(), taps, a_decay.data_ptr(),
+          dt_bias.data_ptr(), norm.data_ptr(), ring.data_ptr(), state.data_ptr(), index, at, n,
+          cache_rows, key_heads, key_dim, value_heads, value_dim, eps, _flag(error_flag, dev))
     return out

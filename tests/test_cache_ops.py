@@ -61,14 +61,14 @@ def test_prepare_paged_validation():
 def test_paged_attention_validation():
     names = ("q", "k", "v", "gate", "table", "index", "positions")
     size = _lib.lib().qdc_paged_attention_workspace
-    need = size(3, 8, 2, 128, 5, 16, BF16)
-    assert need > 0
-    assert size(3, 8, 3, 128, 5, 16, BF16) == 0 and size(3, 8, 2, 96, 5, 16, BF16) == 0
-    assert size(3, 8, 2, 128, 5, 20, BF16) == 0 and size(3, 8, 2, 128, 5, 16, X2) == 0
-    assert size(1 << 24, 8, 2, 128, 5, 16, BF16) == 0            # the join's grid
-    assert size(1 << 15, 8, 2, 128, 1 << 20, 256, BF16) == 0     # tiles past 31 bits
+    need = size(3, 8, 2, 128, 500, 16, BF16)
+    assert need > 0 and size(3, 8, 2, 128, 5, 16, BF16) == 0     # short rows need none
+    assert size(3, 8, 3, 128, 5, 16, BF16) == -1 and size(3, 8, 2, 96, 5, 16, BF16) == -1
+    assert size(3, 8, 2, 128, 5, 20, BF16) == -1 and size(3, 8, 2, 128, 5, 16, X2) == -1
+    assert size(1 << 24, 8, 2, 128, 5, 16, BF16) == -1           # the join's grid
+    assert size(1 << 15, 8, 2, 128, 1 << 20, 256, BF16) == -1    # tiles past 31 bits
 
-    def f(dtype=BF16, odt=BF16, n=3, heads=8, kv=2, hd=128, rows=4, width=5, pages=7, page=16,
+    def f(dtype=BF16, odt=BF16, n=3, heads=8, kv=2, hd=128, rows=4, width=500, pages=7, page=16,
           q_tok=1024, q_head=128, g_tok=1024, g_head=128, o_tok=1024, scale=0.1, ws=FAR + (9 << 40),
           nbytes=need, out=FAR + (8 << 40), flag=None, **at):
         ptr = [at.get(x, FAR + (i << 40)) for i, x in enumerate(names)]
@@ -89,7 +89,7 @@ def test_paged_attention_validation():
     assert f(q=FAR + 8) == -2 and f(gate=FAR + 4) == -2 and f(ws=FAR + (9 << 40) + 8) == -2
     assert f(nbytes=need - 1) == -2
     assert f(out=FAR + (1 << 40)) == -5 and f(ws=FAR + (8 << 40)) == -5
-    assert f(n=0, q=0) == 0
+    assert f(n=0, q=0) == 0 and f(width=5, ws=0, nbytes=0, q=0) == -1
 
 
 def test_pages_validation():
