@@ -20,7 +20,6 @@
 namespace qdc {
 namespace {
 
-constexpr int kStep = 512;  // threads
 constexpr int kMaxTaps = 8, kMaxValue = 256;
 
 struct DeltaStep {
@@ -41,72 +40,109 @@ __device__ __forceinline__ float softplus_f(float x) {
     return fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x)));
 }
 
+// A state that is larger than what the last-level cache keeps until the next call is
+// read and written as a stream.
+template <bool STREAM> __device__ __forceinline__ f32x4 load_state(const float *p) {
+    const f32x4 *q = reinterpret_cast<const f32x4 *>(p);
+    return STREAM ? __builtin_nontemporal_load(q) : *q;
+}
+template <bool STREAM> __device__ __forceinline__ void store_state(float *p, f32x4 v) {
+    f32x4 *q = reinterpret_cast<f32x4 *>(p);
+    if (STREAM) __builtin_nontemporal_store(v, q);
+    else *q = v;
+}
+
+// Threads: twice as many stream a large state 5% faster (us, 317 MB 115 / 109, 134 MB
+// 51 / 49), a small one is done sooner without (8 MB 6.5 / 6.9, 67 MB 23.7 / 24.8).
+constexpr int step_threads(bool stream) { return stream ? 1024 : 512; }
+constexpr int row_lanes(int key_dim) { return key_dim / 4 < 16 ? key_dim / 4 : 16; }
+
 // L lanes a state row, N 16-byte pieces a lane; a pass of the workgroup takes
-// kStep / L rows, PASSES passes all of them.
-template <typename T, int KD, int PASSES>
-__global__ __launch_bounds__(kStep) void delta_step(DeltaStep a) {
-    constexpr int L = KD / 4 < 16 ? KD / 4 : 16, N = KD / (4 * L), ROWS = kStep / L;
+// kStep / L rows, PASSES passes all of them.  TAPS: the convolution's taps, 0 for any.
+template <typename T, int KD, int PASSES, int TAPS, bool STREAM>
+__global__ __launch_bounds__(step_threads(STREAM)) void delta_step(DeltaStep a) {
+    constexpr int kStep = step_threads(STREAM), L = row_lanes(KD), N = KD / (4 * L);
+    constexpr int ROWS = kStep / L;
+    static_assert(2 * KD + kMaxValue <= kStep, "a thread a channel");
     __shared__ __align__(16) float qkv[2 * KD + kMaxValue], so[kMaxValue];
     __shared__ float part[kStep / kWave], gates[2];
     const int entry = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, vd = a.value_dim;
     const int row = a.index[entry], pos = a.positions[entry];
     const bool token = row >= 0 && pos >= 0;
+    // an address within the cache, whatever the entry holds; what comes from there is
+    // used only once the entry has been checked
+    const int64_t safe = min(max(row, 0), a.rows - 1);
+    const int p0 = max(pos, 0);
+
+    // everything a thread reads, the small things first: the token's channels of this
+    // head (q | k | v), their window, the gates, and then the state
+    const int g = h / a.groups, taps = TAPS ? TAPS : a.taps;
+    const int64_t kw = (int64_t)a.key_heads * KD, vw = (int64_t)a.heads * vd, cq = a.channels;
+    const T *proj = (const T *)a.proj + entry * a.ld;
+    T *ring = (T *)a.ring + safe * taps * cq;
+    const bool channel = tid < 2 * KD + vd;
+    const int64_t c = tid < KD       ? (int64_t)g * KD + tid
+                      : tid < 2 * KD ? kw + (int64_t)g * KD + (tid - KD)
+                                     : 2 * kw + (int64_t)h * vd + (tid - 2 * KD);
+    constexpr int W = TAPS ? TAPS : kMaxTaps;
+    T window[W], z = T(), norm = T();
+    float conv[W];
+    if (channel) {
+        window[0] = proj[c];
+#pragma unroll
+        for (int lag = 0; lag < W; ++lag) {  // tap taps - 1 - lag
+            if (!TAPS && lag >= taps) continue;
+            if (lag) window[lag] = ring[(int64_t)((p0 + taps - lag) % taps) * cq + c];
+            conv[lag] = a.conv[c * taps + (taps - 1 - lag)];
+        }
+    }
+    if (tid < vd) {
+        z = proj[cq + (int64_t)h * vd + tid];
+        norm = ((const T *)a.norm)[tid];
+    }
+    const float b_raw = to_f32(proj[cq + vw + a.heads + h]), a_raw = to_f32(proj[cq + vw + h]);
+    const float bias = a.dt_bias[h], decay = a.a_decay[h];
+    const int lane = tid % L, r0 = tid / L;
+    float *state = a.state + (safe * a.heads + h) * vd * KD;
+    f32x4 S[PASSES][N];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int v = min(r0 + p * ROWS, vd - 1);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            S[p][n] = load_state<STREAM>(state + (int64_t)v * KD + 4 * (lane + L * n));
+    }
+
     // a row that an earlier token of the call has: not done twice
     bool bad = token && row >= a.rows;
     if (token)
         for (int j = tid; j < entry; j += kStep)
             bad = bad || (a.index[j] == row && a.positions[j] >= 0);
-    const bool live = token && !__syncthreads_or(bad);
     const int64_t at = ((int64_t)entry * a.heads + h) * vd;
     auto put = [&](int v, float o) {
         if (a.out_dtype == QDC_BF16) put_elem((bf16_t *)a.out, at + v, o);
         else if (a.out_dtype == QDC_F32) put_elem((float *)a.out, at + v, o);
         else put_elem((split_t *)a.out, at + v, o);
     };
-    if (!live) {  // uniform
-        for (int v = tid; v < vd; v += kStep) put(v, 0.0f);
+    if (channel) {
+        float acc = 0.0f;
+#pragma unroll
+        for (int lag = W - 1; lag >= 0; --lag)  // the oldest first; before position 0 nothing
+            if ((TAPS || lag < taps) && lag <= pos) acc = acc + to_f32(window[lag]) * conv[lag];
+        qkv[tid] = silu(acc);
+    }
+    if (tid == kStep - 1) {
+        gates[0] = sigmoid(b_raw);
+        gates[1] = expf(decay * softplus_f(a_raw + bias));
+    }
+    const bool live = !__syncthreads_or(bad) && token;  // uniform
+    if (!live) {
+        if (tid < vd) put(tid, 0.0f);
         if (token && tid == 0) raise_flag(a.error_flag);
         return;
     }
-    const int lane = tid % L, r0 = tid / L;
-    float *state = a.state + ((int64_t)row * a.heads + h) * vd * KD;
-    f32x4 S[PASSES][N];
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p)
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            S[p][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (pos > 0 && r0 + p * ROWS < vd)
-                S[p][n] = *reinterpret_cast<const f32x4 *>(state + (int64_t)(r0 + p * ROWS) * KD +
-                                                           4 * (lane + L * n));
-        }
-    // the token's channels of this head: q | k | v
-    const int g = h / a.groups;
-    const int64_t kw = (int64_t)a.key_heads * KD, cq = a.channels;
-    const T *proj = (const T *)a.proj + entry * a.ld;
-    T *ring = (T *)a.ring + (int64_t)row * a.taps * cq;
-    const bool owner = h % a.groups == 0;  // of the key head's part of the ring
-    for (int i = tid; i < 2 * KD + vd; i += kStep) {
-        const int64_t c = i < KD       ? (int64_t)g * KD + i
-                          : i < 2 * KD ? kw + (int64_t)g * KD + (i - KD)
-                                       : 2 * kw + (int64_t)h * vd + (i - 2 * KD);
-        const T now = proj[c];
-        float acc = 0.0f;
-        for (int j = 0; j < a.taps; ++j) {
-            const int lag = a.taps - 1 - j;
-            if (lag > pos) continue;  // before the row's start
-            const T x = lag ? ring[(int64_t)((pos - lag) % a.taps) * cq + c] : now;
-            acc = acc + to_f32(x) * a.conv[c * a.taps + j];
-        }
-        if (owner || i >= 2 * KD) ring[(int64_t)(pos % a.taps) * cq + c] = now;
-        qkv[i] = silu(acc);
-    }
-    if (tid == 0) {
-        const int64_t vw = (int64_t)a.heads * vd;
-        gates[0] = sigmoid(to_f32(proj[cq + vw + a.heads + h]));
-        gates[1] = expf(a.a_decay[h] * softplus_f(to_f32(proj[cq + vw + h]) + a.dt_bias[h]));
-    }
-    __syncthreads();
+    if (channel && (tid >= 2 * KD || h % a.groups == 0))  // one head keeps the key head's part
+        ring[(int64_t)(pos % taps) * cq + c] = window[0];
     // the squares of q and k, each lane group alike
     float k[N][4], q[N][4], qq = 0.0f, kk = 0.0f;
 #pragma unroll
@@ -137,7 +173,7 @@ __global__ __launch_bounds__(kStep) void delta_step(DeltaStep a) {
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                S[p][n][e] *= f;
+                S[p][n][e] = pos ? S[p][n][e] * f : 0.0f;  // position 0: from an empty state
                 sk = __builtin_fmaf(S[p][n][e], k[n][e], sk);
             }
         const float u = beta * (qkv[2 * KD + v] - group_sum<L>(sk));
@@ -148,7 +184,7 @@ __global__ __launch_bounds__(kStep) void delta_step(DeltaStep a) {
                 S[p][n][e] = __builtin_fmaf(u, k[n][e], S[p][n][e]);
                 sq = __builtin_fmaf(S[p][n][e], q[n][e], sq);
             }
-            *reinterpret_cast<f32x4 *>(state + (int64_t)v * KD + 4 * (lane + L * n)) = S[p][n];
+            store_state<STREAM>(state + (int64_t)v * KD + 4 * (lane + L * n), S[p][n]);
         }
         sq = group_sum<L>(sq);
         if (lane == 0) so[v] = sq;
@@ -163,29 +199,37 @@ __global__ __launch_bounds__(kStep) void delta_step(DeltaStep a) {
 #pragma unroll
     for (int w = 0; w < kMaxValue / kWave; ++w) ss += part[w];
     const float s = rms_scale(ss, (float)vd, a.eps);
-    const float z = to_f32(proj[cq + (int64_t)h * vd + tid]);
-    put(tid, ((o * s) * to_f32(((const T *)a.norm)[tid])) * silu(z));
+    put(tid, ((o * s) * to_f32(norm)) * silu(to_f32(z)));
 }
 
 template <typename T, int KD> int32_t launch(const DeltaStep &a, int64_t n, hipStream_t stream) {
-    const dim3 grid((uint32_t)n, (uint32_t)a.heads), block(kStep);
-    constexpr int L = KD / 4 < 16 ? KD / 4 : 16;
-    switch (ceil_div((int64_t)a.value_dim, (int64_t)(kStep / L))) {
-#define QDC_STEP(P)                                                                   \
-    case P:                                                                           \
-        hipLaunchKernelGGL((delta_step<T, KD, P>), grid, block, 0, stream, a);        \
-        return launch_status();
-        QDC_STEP(1)
-        QDC_STEP(2)
-        QDC_STEP(3)
-        QDC_STEP(4)
-        QDC_STEP(5)
-        QDC_STEP(6)
-        QDC_STEP(7)
-        QDC_STEP(8)
-#undef QDC_STEP
-        default: break;
+    const dim3 grid((uint32_t)n, (uint32_t)a.heads);
+    // Bytes of state from which on it is a stream: half of the last-level cache of 256 MB.
+    // us, replayed, cached / streamed, 67 MB 23.7 / 28.2 (with 1 GB of other layers' states
+    // between two calls 33.0 / 28.9), 134 MB 55.9 / 51.1, 317 MB 130.7 / 114.8.
+    const bool stream_state =
+        a.taps == 4 && n * a.heads * a.value_dim * KD * 4 >= ((int64_t)128 << 20);
+    const dim3 block(step_threads(stream_state));
+    const int64_t passes = ceil_div((int64_t)a.value_dim, (int64_t)(block.x / row_lanes(KD)));
+#define QDC_STEP_LAUNCH(P, TAPS, STREAM)                                                 \
+    hipLaunchKernelGGL((delta_step<T, KD, P, TAPS, STREAM>), grid, block, 0, stream, a);
+#define QDC_STEP(P)                                                                      \
+    if (passes <= P) {                                                                   \
+        if (stream_state) {                                                              \
+            QDC_STEP_LAUNCH(P, 4, true)                                                  \
+        } else if (a.taps == 4) {                                                        \
+            QDC_STEP_LAUNCH(P, 4, false)                                                 \
+        } else {                                                                         \
+            QDC_STEP_LAUNCH(P, 0, false)                                                 \
+        }                                                                                \
+        return launch_status();                                                          \
     }
+    QDC_STEP(1)
+    QDC_STEP(2)
+    QDC_STEP(4)
+    QDC_STEP(8)
+#undef QDC_STEP
+#undef QDC_STEP_LAUNCH
     return QDC_ERR_SHAPE;
 }
 

@@ -846,6 +846,29 @@ def test_delta_step_rows(dtype):
 
 
 @pytest.mark.gpu
+def test_delta_step_large_state():
+    """A state of 128 MB and more is streamed: the same bits as rows a few at a time."""
+    KH, H, kd, vd, n = 16, 32, 128, 128, 70
+    g = torch.Generator(device=DEV).manual_seed(5)
+    t = lambda *s: torch.randn(s, generator=g, device=DEV)  # noqa: E731
+    cq = 2 * KH * kd + H * vd
+    assert n * H * vd * kd * 4 >= 128 << 20
+    args = [t(n, cq + H * vd + 2 * H), t(cq, 4) * 0.5, -t(H).exp(), t(H), 1 + 0.1 * t(vd), 1e-6,
+            t(n + 1, 4, cq), t(n + 1, H, vd, kd) * 0.3]
+    rows, pos = torch.randperm(n + 1, generator=g, device=DEV)[:n].int(), ints(range(n))
+    rows[7], rows[9], pos[11] = -1, rows[3], -1
+    ring, state, f = args[6].clone(), args[7].clone(), flag()
+    out = cache_ops.delta_step(*args[:6], ring, state, rows, pos, KH, kd, H, vd, error_flag=f)
+    assert f.item() == 1 and (out[[7, 9, 11]] == 0).all()
+    rows[9] = -1
+    for i in range(0, n, 10):
+        few = cache_ops.delta_step(args[0][i:i + 10], *args[1:], rows[i:i + 10].contiguous(),
+                                   pos[i:i + 10].contiguous(), KH, kd, H, vd)
+        assert torch.equal(few, out[i:i + 10])
+    assert torch.equal(ring, args[6]) and torch.equal(state, args[7])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("S,KH,H,kd,vd", [(5, 2, 4, 128, 128), (40, 1, 2, 64, 48), (70, 16, 64, 32, 32)])
 def test_steps_continue_a_scan(S, KH, H, kd, vd):
     """A prompt through the prologue, the scan (with its last state) and the gated norm,
