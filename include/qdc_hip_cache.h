@@ -143,7 +143,7 @@ int32_t qdc_pages_compact(int32_t *table, int32_t *refs, int32_t *free_pages, in
  * or whatever a row of the cache holds beside them.  A pair with a negative index is
  * left out.  A pair whose dst is an earlier pair's dst or any pair's src, or that is
  * out of range, is not copied (error_flag).  item_bytes a multiple of 16, pool 16-byte
- * aligned, n < 2^16. */
+ * aligned, n at most 4096 (every pair is held against all others). */
 int32_t qdc_copy_pages(void *pool, const int32_t *src, const int32_t *dst, int64_t n,
                        int64_t planes, int64_t items, int64_t item_bytes, int32_t *error_flag,
                        hipStream_t stream);

@@ -5,8 +5,10 @@
 // checks everything first (rows named twice by a bitmap in LDS) and then either does
 // the whole call or none of it.  It is bound by the chain of dependent loads, rows ->
 // lengths -> table -> refs, each a memory latency; the entries of a call are taken side
-// by side and their pages as one flat list, a thread a page.  The copies are launches
-// of their own that read what the first one decided.
+// by side, a thread an entry, whose values stay in registers from the checks to the
+// work (past kBook entries they are read again), and their pages as one flat list, a
+// thread a page.  The copies are launches of their own that read what the first one
+// decided.
 #include "qdc_cache.hpp"
 
 namespace qdc {
@@ -23,37 +25,40 @@ struct Book {
     int32_t *error_flag;
 };
 
-// Agent scope: atomics are done in L2, past the first-level cache.
+// refs are counted with atomics, done in L2: a load of them goes past the first-level
+// cache, and a barrier follows the atomics' returned values.
 __device__ __forceinline__ int load_past_l1(const int32_t *p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Everything this workgroup wrote or changed is seen by all of it.
-__device__ __forceinline__ void settle() {
-    __threadfence();
-    __syncthreads();
-}
-
 // Exclusive prefix sum over the workgroup and the whole; `parts` is LDS scratch.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *parts, int64_t &all) {
+__device__ __forceinline__ int block_scan(int v, int *parts, int &all) {
     const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
-    int64_t inc = v;
+    int inc = v;
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
-        const int64_t o = __shfl_up(inc, d, kWave);
+        const int o = __shfl_up(inc, d, kWave);
         if (l >= d) inc += o;
     }
     __syncthreads();  // the scratch is free
     if (l == kWave - 1) parts[wv] = inc;
     __syncthreads();
-    int64_t before = 0;
+    int before = 0;
     all = 0;
+#pragma unroll
     for (int w = 0; w < kBookWaves; ++w) {
-        const int64_t p = parts[w];
+        const int p = parts[w];
         if (w < wv) before += p;
         all += p;
     }
     return before + inc - v;
+}
+
+// Whether any thread says so, with the sum of v (below 2^31) over all of them.
+__device__ __forceinline__ bool block_sum_or(int v, bool any, int *parts, int &all) {
+    const bool some = __syncthreads_or(any);
+    block_scan(some ? 0 : v, parts, all);
+    return some;
 }
 
 __device__ __forceinline__ void clear_bits(uint32_t *bits, int n) {
@@ -67,12 +72,12 @@ __device__ __forceinline__ bool has_bit(const uint32_t *bits, int i) {
     return bits[i >> 5] >> (i & 31) & 1u;
 }
 
-__device__ __forceinline__ int64_t blocks_of(int64_t positions, int shift) {
-    return (positions + ((int64_t)1 << shift) - 1) >> shift;
+__device__ __forceinline__ int blocks_of(int64_t positions, int shift) {
+    return (int)((positions + ((int64_t)1 << shift) - 1) >> shift);
 }
 
 // The last entry whose run starts at or before `at`; starts[0] = 0, ascending.
-__device__ __forceinline__ int run_of(const int64_t *starts, int n, int64_t at) {
+__device__ __forceinline__ int run_of(const int *starts, int n, int at) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
@@ -83,56 +88,69 @@ __device__ __forceinline__ int run_of(const int64_t *starts, int n, int64_t at) 
 }
 
 // A stack that may hold anything: the number of pages that can be taken from it.
-__device__ __forceinline__ int64_t stack_count(const Book &b) {
+__device__ __forceinline__ int stack_count(const Book &b) {
     return min(max(b.free_pages[0], 0), b.pages);
+}
+
+// An entry that grows: its row, length, and the pages it has and needs.
+struct Growth {
+    int row, len, more, have, need;
+    bool bad;
+};
+__device__ __forceinline__ Growth growth_of(const Book &b, const int32_t *index,
+                                            const int32_t *counts, int i) {
+    Growth g = {-1, -1, 0, 0, 0, false};
+    if (i >= b.n) return g;
+    const int row = index[i], more = counts ? counts[i] : 1;
+    if (row < 0) return g;
+    g.bad = row >= b.rows;
+    if (g.bad) return g;
+    const int len = b.lengths[row];
+    g.bad = len < 0 || more < 0 || (int64_t)len + more > b.width << b.shift;
+    if (g.bad) return g;
+    g.row = row;
+    g.len = len;
+    g.more = more;
+    g.have = blocks_of(len, b.shift);
+    g.need = blocks_of((int64_t)len + more, b.shift) - g.have;
+    return g;
 }
 
 __global__ __launch_bounds__(kBook) void pages_extend(Book b, int32_t *positions,
                                                       const int32_t *index,
                                                       const int32_t *counts) {
     extern __shared__ uint32_t seen[];
-    __shared__ int64_t parts[kBookWaves], start[kBook];
-    __shared__ int row_of[kBook], have_of[kBook];
+    __shared__ int parts[kBookWaves], start[kBook], row_of[kBook], have_of[kBook];
+    const int count = stack_count(b);
+    const Growth mine = growth_of(b, index, counts, threadIdx.x);
     clear_bits(seen, b.rows);
-    const int64_t count = stack_count(b), reach = b.width << b.shift;
-    int64_t need = 0;
-    bool bad = false;
-    for (int i = threadIdx.x; i < b.n; i += kBook) {
-        const int row = index[i];
-        if (row < 0) continue;
-        if (row >= b.rows || set_bit(seen, row)) {
-            bad = true;
-            continue;
-        }
-        const int64_t len = b.lengths[row], more = counts ? counts[i] : 1;
-        bad = bad || len < 0 || more < 0 || len + more > reach;
-        need += blocks_of(len + more, b.shift) - blocks_of(len, b.shift);
+    int need = mine.need;
+    bool bad = mine.bad || (mine.row >= 0 && set_bit(seen, mine.row));
+    for (int i = threadIdx.x + kBook; i < b.n; i += kBook) {
+        const Growth g = growth_of(b, index, counts, i);
+        bad = bad || g.bad || (g.row >= 0 && set_bit(seen, g.row));
+        need += g.need;
     }
-    int64_t total;
-    block_scan(need, parts, total);
-    if (__syncthreads_or(bad || total > count)) {
+    int total;  // distinct rows: at most rows * width, below 2^31
+    bad = block_sum_or(need, bad, parts, total);
+    if (bad || total > count) {
         for (int i = threadIdx.x; i < b.n; i += kBook) positions[i] = -1;
         if (threadIdx.x == 0) raise_flag(b.error_flag);
         return;
     }
-    int64_t taken = 0;  // pages of earlier chunks of entries
+    int taken = 0;  // pages of earlier chunks of entries
     for (int i0 = 0; i0 < b.n; i0 += kBook) {
-        const int i = i0 + threadIdx.x, row = i < b.n ? index[i] : -1;
-        int64_t pages = 0, have = 0, len = -1, more = 0;
-        if (row >= 0) {
-            len = b.lengths[row];
-            more = counts ? counts[i] : 1;
-            have = blocks_of(len, b.shift);
-            pages = blocks_of(len + more, b.shift) - have;
-            b.lengths[row] = (int32_t)(len + more);
-        }
-        if (i < b.n) positions[i] = (int32_t)len;
-        int64_t all;
-        start[threadIdx.x] = block_scan(pages, parts, all);
-        row_of[threadIdx.x] = row;
-        have_of[threadIdx.x] = (int)have;
+        const int i = i0 + threadIdx.x;
+        const Growth g = i0 ? growth_of(b, index, counts, i) : mine;
+        if (i < b.n) positions[i] = g.len;
+        if (g.row >= 0) b.lengths[g.row] = g.len + g.more;
+        if (total == 0) continue;
+        int all;
+        start[threadIdx.x] = block_scan(g.need, parts, all);
+        row_of[threadIdx.x] = g.row;
+        have_of[threadIdx.x] = g.have;
         __syncthreads();
-        for (int64_t p = threadIdx.x; p < all; p += kBook) {
+        for (int p = threadIdx.x; p < all; p += kBook) {
             const int e = run_of(start, kBook, p);
             const int32_t page = b.free_pages[count - (taken + p)];
             b.table[row_of[e] * b.width + have_of[e] + (p - start[e])] = page;
@@ -141,96 +159,127 @@ __global__ __launch_bounds__(kBook) void pages_extend(Book b, int32_t *positions
         taken += all;
         __syncthreads();
     }
-    if (threadIdx.x == 0) b.free_pages[0] = (int32_t)(count - total);
+    if (threadIdx.x == 0) b.free_pages[0] = count - total;
 }
 
 // Pages that the rows of a call list, flat: entry by entry, block by block.  A page is
-// free when its refs, taken down once for each listing, reach nothing; the listing that
-// puts it on the stack is its last, found by writing -(place + 1) over refs with a
-// minimum.
+// free when its refs, taken down once for each listing, reach nothing.  The listing
+// that takes down the last is the only one unless another took down before it; where
+// that happened to a page that is now free, the listing that puts it on the stack is
+// its last, found by writing -(place + 1) over refs with a minimum.
 __global__ __launch_bounds__(kBook) void pages_free(Book b, const int32_t *index) {
     extern __shared__ uint32_t seen[];
-    __shared__ int64_t parts[kBookWaves], start[kBook];
-    __shared__ int row_of[kBook];
+    __shared__ int parts[kBookWaves], start[kBook], row_of[kBook];
+    int count = stack_count(b);
+    const int first = threadIdx.x < b.n ? index[threadIdx.x] : -1;
+    const int first_len = first >= 0 && first < b.rows ? b.lengths[first] : 0;
     clear_bits(seen, b.rows);
-    bool bad = false;
-    for (int i = threadIdx.x; i < b.n; i += kBook) {
+    bool bad = first >= b.rows || (first >= 0 && set_bit(seen, first));
+    for (int i = threadIdx.x + kBook; i < b.n; i += kBook) {
         const int row = index[i];
-        if (row >= 0 && (row >= b.rows || set_bit(seen, row))) bad = true;
+        bad = bad || row >= b.rows || (row >= 0 && set_bit(seen, row));
     }
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0) raise_flag(b.error_flag);
         return;
     }
-    int64_t count = stack_count(b);
-    // places of a chunk of entries in the flat list, those of its runs in LDS
-    auto chunk = [&](int i0, int64_t &all) {
-        const int i = i0 + threadIdx.x, row = i < b.n ? index[i] : -1;
-        const int64_t len = row >= 0 ? b.lengths[row] : 0;
-        const int64_t mine = min(max(blocks_of(len, b.shift), (int64_t)0), b.width);
-        start[threadIdx.x] = block_scan(mine, parts, all);
+    // a chunk of entries: the places of its runs in the flat list, and how many
+    auto chunk = [&](int i0) {
+        const int i = i0 + threadIdx.x;
+        const int row = i0 == 0 ? first : i < b.n ? index[i] : -1;
+        const int len = i0 == 0 ? first_len : row >= 0 ? b.lengths[row] : 0;
+        int all;
+        start[threadIdx.x] =
+            block_scan((int)min((int64_t)blocks_of(max(len, 0), b.shift), b.width), parts, all);
         row_of[threadIdx.x] = row;
         __syncthreads();
+        return all;
     };
-    auto entry = [&](int64_t p) {  // the table's place for place p of the chunk
+    auto entry = [&](int p) {  // the table's place for place p of the chunk
         const int e = run_of(start, kBook, p);
         return row_of[e] * b.width + (p - start[e]);
     };
-    int64_t before = 0, all = 0;
-    int last = 0;
-    for (int i0 = 0; i0 < b.n; i0 += kBook) {
-        chunk(i0, all);
-        for (int64_t p = threadIdx.x; p < all; p += kBook) {
-            const int32_t page = b.table[entry(p)];
-            if ((uint32_t)page < (uint32_t)b.pages) atomicSub(&b.refs[page], 1);
+    // one chunk whose pages are a thread's each: they stay in registers
+    int before = 0, all = chunk(0);
+    const bool small = b.n <= kBook && all <= kBook;
+    int64_t place = -1;
+    int32_t page = -1;
+    bool alone = false;  // this listing took down the last
+    bool shared = false; // a page that several listed may be free
+    for (int i0 = 0;;) {
+        for (int p = threadIdx.x; p < all; p += kBook) {
+            place = entry(p);
+            page = b.table[place];
+            if ((uint32_t)page >= (uint32_t)b.pages) continue;
+            const int old = atomicSub(&b.refs[page], 1);
+            alone = old <= 1;
+            shared = shared || old > 1;
         }
-        __syncthreads();
-        last = i0;
         before += all;
-    }
-    settle();
-    int64_t at = 0;
-    for (int i0 = 0; i0 < b.n; i0 += kBook) {
-        if (b.n > kBook) chunk(i0, all);
-        for (int64_t p = threadIdx.x; p < all; p += kBook) {
-            const int32_t page = b.table[entry(p)];
-            if ((uint32_t)page < (uint32_t)b.pages && load_past_l1(&b.refs[page]) <= 0)
-                atomicMin(&b.refs[page], -(int32_t)(at + p) - 1);
-        }
+        i0 += kBook;
+        if (i0 >= b.n) break;
         __syncthreads();
-        at += all;
+        all = chunk(i0);
     }
-    settle();
+    // (when not small, any page that others hold too asks for the second pass)
+    bool second = __syncthreads_or(shared);
+    if (second && small)
+        second = __syncthreads_or(shared && load_past_l1(&b.refs[page]) <= 0);
+    const int chunks = (b.n + kBook - 1) / kBook;
+    if (second || !small) {
+        int at = 0, seen_min = 0;
+        for (int c = 0; c < chunks; ++c) {
+            if (chunks > 1) {
+                __syncthreads();
+                all = chunk(c * kBook);
+            }
+            for (int p = threadIdx.x; p < all; p += kBook) {
+                const int32_t q = b.table[entry(p)];
+                if ((uint32_t)q < (uint32_t)b.pages && load_past_l1(&b.refs[q]) <= 0)
+                    seen_min |= atomicMin(&b.refs[q], -(at + p) - 1);
+            }
+            at += all;
+        }
+        asm volatile("" ::"v"(seen_min));  // waited for
+        __syncthreads();
+    }
     // from the back: the first of the list ends on top
-    for (int i0 = last; i0 >= 0; i0 -= kBook) {
-        if (b.n > kBook) chunk(i0, all);
+    for (int c = chunks - 1; c >= 0; --c) {
+        if (chunks > 1) {
+            __syncthreads();
+            all = chunk(c * kBook);
+        }
         before -= all;
-        for (int64_t p0 = 0; p0 < all; p0 += kBook) {
-            const int64_t p = all - 1 - (p0 + threadIdx.x);
-            int32_t page = -1;
-            int64_t place = 0;
+        for (int p0 = 0; p0 < all; p0 += kBook) {
+            const int p = all - 1 - (p0 + (int)threadIdx.x);
             bool push = false;
-            if (p >= 0) {
-                place = entry(p);
-                page = b.table[place];
-                push = (uint32_t)page < (uint32_t)b.pages &&
-                       load_past_l1(&b.refs[page]) == -(int32_t)(before + p) - 1;
+            int64_t where = -1;
+            int32_t q = -1;
+            if (small) {  // thread t holds place t: hand it to the one that counts from the back
+                where = place;
+                q = page;
+                push = (uint32_t)q < (uint32_t)b.pages &&
+                       (second ? load_past_l1(&b.refs[q]) == -(int)threadIdx.x - 1 : alone);
+            } else if (p >= 0) {
+                where = entry(p);
+                q = b.table[where];
+                push = (uint32_t)q < (uint32_t)b.pages &&
+                       load_past_l1(&b.refs[q]) == -(before + p) - 1;
             }
-            int64_t pushed;
-            const int64_t rank = block_scan(push, parts, pushed);
+            int pushed;
+            int rank = block_scan(push, parts, pushed);
+            if (small) rank = pushed - 1 - rank;
             if (push) {
-                if (count + rank < b.pages) b.free_pages[1 + count + rank] = page;
-                b.refs[page] = 0;
+                if (count + rank < b.pages) b.free_pages[1 + count + rank] = q;
+                b.refs[q] = 0;
             }
-            if (p >= 0) b.table[place] = -1;
+            if (where >= 0) b.table[where] = -1;
             count += pushed;
         }
-        __syncthreads();
-        const int i = i0 + threadIdx.x;
+        const int i = c * kBook + threadIdx.x;
         if (i < b.n && row_of[threadIdx.x] >= 0) b.lengths[row_of[threadIdx.x]] = 0;
-        __syncthreads();
     }
-    if (threadIdx.x == 0) b.free_pages[0] = (int32_t)min(count, (int64_t)b.pages);
+    if (threadIdx.x == 0) b.free_pages[0] = min(count, b.pages);
 }
 
 // What the copies of a fork read: an entry's begun page, the new one, places used.
@@ -238,91 +287,130 @@ struct Copy {
     int32_t src, dst, used, pad;
 };
 
+// A pair that forks: -1 rows when it is left out.
+struct Pair {
+    int parent, child, len;
+    bool bad;
+};
+__device__ __forceinline__ Pair pair_of(const Book &b, const int32_t *parents,
+                                        const int32_t *children, int i) {
+    Pair f = {-1, -1, 0, false};
+    if (i >= b.n) return f;
+    const int p = parents[i], c = children[i];
+    if (p < 0 || c < 0) return f;
+    f.bad = p >= b.rows || c >= b.rows;
+    if (f.bad) return f;
+    f.parent = p;
+    f.child = c;
+    f.len = b.lengths[p];
+    f.bad = b.lengths[c] != 0 || f.len < 0 || blocks_of(f.len, b.shift) > b.width;
+    return f;
+}
+
 __global__ __launch_bounds__(kBook) void pages_fork(Book b, const int32_t *parents,
                                                     const int32_t *children, Copy *copies) {
     extern __shared__ uint32_t seen[];
-    __shared__ int64_t parts[kBookWaves], start[kBook];
-    __shared__ int from[kBook], to[kBook];
+    __shared__ int parts[kBookWaves], start[kBook], from[kBook], to[kBook];
+    const int count = stack_count(b), mask = (1 << b.shift) - 1;
+    const Pair mine = pair_of(b, parents, children, threadIdx.x);
     clear_bits(seen, b.rows);
-    const int64_t count = stack_count(b);
-    const int mask = (1 << b.shift) - 1;
-    int64_t need = 0;
-    bool bad = false;
-    for (int i = threadIdx.x; i < b.n; i += kBook) {
-        const int p = parents[i], c = children[i];
-        if (p < 0 || c < 0) continue;
-        if (p >= b.rows || c >= b.rows || set_bit(seen, c) || b.lengths[c] != 0) {
-            bad = true;
-            continue;
-        }
-        const int64_t len = b.lengths[p];
-        bad = bad || len < 0 || blocks_of(len, b.shift) > b.width;
-        need += (len & mask) != 0;
+    int need = (mine.len & mask) != 0;
+    bool bad = mine.bad || (mine.child >= 0 && set_bit(seen, mine.child));
+    for (int i = threadIdx.x + kBook; i < b.n; i += kBook) {
+        const Pair f = pair_of(b, parents, children, i);
+        bad = bad || f.bad || (f.child >= 0 && set_bit(seen, f.child));
+        need += (f.len & mask) != 0;
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < b.n; i += kBook)
-        if (parents[i] >= 0 && children[i] >= 0 && parents[i] < b.rows && has_bit(seen, parents[i]))
-            bad = true;
-    int64_t total;
-    block_scan(need, parts, total);
-    const bool refused = __syncthreads_or(bad || total > count);
+    __syncthreads();  // all children are marked: no parent may be one
+    bad = bad || (mine.parent >= 0 && has_bit(seen, mine.parent));
+    for (int i = threadIdx.x + kBook; i < b.n; i += kBook) {
+        const int p = parents[i];
+        bad = bad || (children[i] >= 0 && p >= 0 && p < b.rows && has_bit(seen, p));
+    }
+    int total;
+    bad = block_sum_or(need, bad, parts, total);
+    const bool refused = bad || total > count;
     if (refused && threadIdx.x == 0) raise_flag(b.error_flag);
-    int64_t taken = 0;
+    int taken = 0;
     for (int i0 = 0; i0 < b.n; i0 += kBook) {
         const int i = i0 + threadIdx.x;
-        const int p = i < b.n ? parents[i] : -1, c = i < b.n ? children[i] : -1;
-        const bool live = p >= 0 && c >= 0 && !refused;
-        const int64_t len = live ? b.lengths[p] : 0;
-        const int used = (int)(len & mask);
-        int64_t all;
-        const int64_t rank = block_scan(used != 0, parts, all);
+        const Pair f = i0 ? pair_of(b, parents, children, i) : mine;
+        const bool live = f.parent >= 0 && !refused;
+        const int len = live ? f.len : 0, used = len & mask;
+        int all;
+        const int rank = block_scan(used != 0, parts, all);
         Copy copy = {-1, -1, 0, 0};
-        if (live) {
-            b.lengths[c] = (int32_t)len;
-            if (used) {
-                const int64_t at = len >> b.shift;
-                copy.src = b.table[p * b.width + at];
-                copy.dst = b.free_pages[count - (taken + rank)];
-                copy.used = used;
-                b.table[c * b.width + at] = copy.dst;
-                if ((uint32_t)copy.dst < (uint32_t)b.pages) b.refs[copy.dst] = 1;
-                if ((uint32_t)copy.src >= (uint32_t)b.pages ||
-                    (uint32_t)copy.dst >= (uint32_t)b.pages) {
-                    copy.used = 0;
-                    raise_flag(b.error_flag);
-                }
+        if (live) b.lengths[f.child] = len;
+        if (used) {
+            const int at = len >> b.shift;
+            copy.src = b.table[f.parent * b.width + at];
+            copy.dst = b.free_pages[count - (taken + rank)];
+            copy.used = used;
+            b.table[f.child * b.width + at] = copy.dst;
+            if ((uint32_t)copy.dst < (uint32_t)b.pages) b.refs[copy.dst] = 1;
+            if ((uint32_t)copy.src >= (uint32_t)b.pages || (uint32_t)copy.dst >= (uint32_t)b.pages) {
+                copy.used = 0;
+                raise_flag(b.error_flag);
             }
         }
         if (i < b.n) copies[i] = copy;
         taken += all;
+        if (refused) continue;
         start[threadIdx.x] = block_scan(len >> b.shift, parts, all);
-        from[threadIdx.x] = p;
-        to[threadIdx.x] = c;
+        from[threadIdx.x] = f.parent;
+        to[threadIdx.x] = f.child;
         __syncthreads();
-        for (int64_t k = threadIdx.x; k < all; k += kBook) {
-            const int e = run_of(start, kBook, k);
-            const int64_t j = k - start[e];
+        for (int k = threadIdx.x; k < all; k += kBook) {
+            const int e = run_of(start, kBook, k), j = k - start[e];
             const int32_t page = b.table[from[e] * b.width + j];
             b.table[to[e] * b.width + j] = page;
             if ((uint32_t)page < (uint32_t)b.pages) atomicAdd(&b.refs[page], 1);
         }
         __syncthreads();
     }
-    if (threadIdx.x == 0 && !refused) b.free_pages[0] = (int32_t)(count - total);
+    if (threadIdx.x == 0 && !refused) b.free_pages[0] = count - total;
 }
 
-// The used places of the begun pages: a workgroup per entry, plane and head.
+// A workgroup's copy of `chunks` 16-byte chunks to each of `n` places: four loads a thread
+// ahead of their stores, the stores as a stream.
+template <int N>
+__device__ __forceinline__ void copy_chunks(const char *src, char *const (&dst)[N], int n,
+                                            int64_t chunks) {
+    constexpr int U = 4;
+    const u32x4 *from = reinterpret_cast<const u32x4 *>(src);
+    int64_t i = threadIdx.x;
+    for (; i + (U - 1) * kBlock < chunks; i += U * kBlock) {
+        u32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = load_raw(from + i + u * kBlock);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if (k >= n) break;
+#pragma unroll
+            for (int u = 0; u < U; ++u) store_raw(dst[k] + 16 * (i + u * kBlock), v[u]);
+        }
+    }
+    for (; i < chunks; i += kBlock) {
+        const u32x4 v = load_raw(from + i);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (k < n) store_raw(dst[k] + 16 * i, v);
+    }
+}
+
+// The used places of the begun pages: a workgroup per entry, plane, head and piece.
+constexpr int64_t kBegun = 8192;
+
 __global__ __launch_bounds__(kBlock) void copy_begun(char *pool, const Copy *copies,
                                                      int64_t plane_bytes, int64_t page_bytes,
                                                      int heads, int64_t token_bytes) {
     const Copy c = copies[blockIdx.x];
-    if (c.used == 0) return;
+    const int64_t at = blockIdx.z * kBegun, bytes = c.used * token_bytes;
+    if (at >= bytes) return;
     const int plane = blockIdx.y / heads, head = blockIdx.y - plane * heads;
-    char *base = pool + plane * plane_bytes + head * (page_bytes / heads);
-    const u32x4 *src = reinterpret_cast<const u32x4 *>(base + c.src * page_bytes);
-    u32x4 *dst = reinterpret_cast<u32x4 *>(base + c.dst * page_bytes);
-    const int64_t chunks = c.used * token_bytes / 16;
-    for (int64_t i = threadIdx.x; i < chunks; i += kBlock) dst[i] = src[i];
+    char *base = pool + plane * plane_bytes + head * (page_bytes / heads) + at;
+    char *const dst[1] = {base + c.dst * page_bytes};
+    copy_chunks<1>(base + c.src * page_bytes, dst, 1, min(kBegun, bytes - at) / 16);
 }
 
 // Workspace of a move: count and pages in use, then the pages' new places, the holes
@@ -336,48 +424,55 @@ __host__ __device__ inline Moves moves_in(void *workspace, int64_t pages) {
 }
 
 __global__ __launch_bounds__(kBook) void pages_plan(int32_t *refs, int pages, Moves m) {
-    __shared__ int64_t parts[kBookWaves];
-    int64_t mine = 0, live, all;
+    __shared__ int parts[kBookWaves];
+    int mine = 0, live, all;
     for (int i = threadIdx.x; i < pages; i += kBook) mine += refs[i] > 0;
     block_scan(mine, parts, live);
-    int64_t holes = 0, movers = 0;
+    int holes = 0, movers = 0;
     for (int i0 = 0; i0 < pages; i0 += kBook) {
         const int i = i0 + threadIdx.x;
         const bool used = i < pages && refs[i] > 0;
+        // pages below `live` are holes or stay, the others move or stay free
         const bool hole = i < live && !used, mover = i >= live && used;
-        const int64_t rank = block_scan(hole, parts, all);
-        if (hole) m.hole[holes + rank] = i;
-        holes += all;
-        const int64_t rank2 = block_scan(mover, parts, all);
-        if (mover) m.page[movers + rank2] = i;
-        movers += all;
+        const int both = block_scan((int)hole | (int)mover << 16, parts, all);
+        if (hole) m.hole[holes + (both & 0xffff)] = i;
+        if (mover) m.page[movers + (both >> 16)] = i;
         if (i < pages) m.place[i] = i;
+        holes += all & 0xffff;
+        movers += all >> 16;
     }
-    settle();
-    for (int64_t k = threadIdx.x; k < movers; k += kBook) {
+    __syncthreads();
+    for (int k = threadIdx.x; k < movers; k += kBook) {
         const int page = m.page[k], hole = m.hole[k];
         m.place[page] = hole;
         refs[hole] = refs[page];
         refs[page] = 0;
     }
     if (threadIdx.x == 0) {
-        m.head[0] = (int32_t)movers;
-        m.head[1] = (int32_t)live;
+        m.head[0] = movers;
+        m.head[1] = live;
     }
 }
 
-// The moves themselves, then the tables and the stack, spread over the grid.
+// The moves themselves, a workgroup a piece of a page in a plane at a time, then the
+// tables and the stack, spread over the grid.  Small pieces side by side keep what is
+// copied at one time close together: 2 x 215 MB of pages of 64 KB a plane 77 us in pieces
+// of 4 KB, 84 of 32 KB.
+constexpr int64_t kPiece = 4096;
+constexpr uint32_t kMoveGrid = 16384;
+
 __global__ __launch_bounds__(kBlock) void pages_move(char *pool, int64_t planes,
                                                      int64_t plane_bytes, int64_t page_bytes,
                                                      Moves m, int32_t *table, int64_t entries,
                                                      int32_t *free_pages, int pages) {
     const int count = m.head[0], live = m.head[1];
-    for (int64_t u = blockIdx.x; u < count * planes; u += gridDim.x) {
-        const int64_t k = u / planes, plane = u - k * planes;
-        const u32x4 *src =
-            reinterpret_cast<const u32x4 *>(pool + plane * plane_bytes + m.page[k] * page_bytes);
-        u32x4 *dst = reinterpret_cast<u32x4 *>(pool + plane * plane_bytes + m.hole[k] * page_bytes);
-        for (int64_t i = threadIdx.x; i < page_bytes / 16; i += kBlock) dst[i] = src[i];
+    const int64_t pieces = (page_bytes + kPiece - 1) / kPiece, per_page = planes * pieces;
+    for (int64_t u = blockIdx.x; u < count * per_page; u += gridDim.x) {
+        const int64_t k = u / per_page, rest = u - k * per_page;
+        const int64_t plane = rest / pieces, at = (rest - plane * pieces) * kPiece;
+        char *base = pool + plane * plane_bytes + at;
+        char *const dst[1] = {base + m.hole[k] * page_bytes};
+        copy_chunks<1>(base + m.page[k] * page_bytes, dst, 1, min(kPiece, page_bytes - at) / 16);
     }
     const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x, step = (int64_t)gridDim.x * kBlock;
     if (count)
@@ -390,31 +485,84 @@ __global__ __launch_bounds__(kBlock) void pages_move(char *pool, int64_t planes,
         free_pages[i] = i == 0 ? free_count : i <= free_count ? pages - (int)i : 0;
 }
 
-// A workgroup per pair and part of its bytes; each checks its own pair against the call.
+// Up to kSame pairs of one src are one workgroup's for a part of a plane: read once,
+// written to each.  The first of them in the call stands for them; each checks the
+// call's pairs for itself.  (8 rows of 19 MB to 5 places each, us: pairs by themselves
+// 186, two together 175, four 181, eight 195: the writes go to as many places at once.)
+constexpr int kSame = 2;
+
 __global__ __launch_bounds__(kBlock) void copy_items(char *pool, const int32_t *src,
-                                                     const int32_t *dst, int n, int64_t planes,
+                                                     const int32_t *dst, int n,
                                                      int64_t plane_bytes, int items,
-                                                     int64_t item_bytes, int32_t *error_flag) {
-    const int i = blockIdx.x, s = src[i], d = dst[i];
-    if (s < 0 || d < 0) return;
-    bool bad = s >= items || d >= items;
+                                                     int64_t item_bytes, int64_t part_bytes,
+                                                     int parts, int32_t *error_flag) {
+    __shared__ int place[kSame], found, turned;
+    const int i = blockIdx.y, s = src[i], own = dst[i];
+    if (s < 0 || own < 0) return;
+    if (threadIdx.x < kWave) {  // which of the pairs of this src it is, and those after it
+        const int l = threadIdx.x;
+        int rank = 0, have = 0;
+        for (int j0 = 0; j0 < n; j0 += kWave) {
+            const int j = j0 + l;
+            const bool same = j < n && src[j] == s && dst[j] >= 0;
+            const uint64_t mask = __ballot(same), below = (1ull << l) - 1;
+            if (j0 <= i) {
+                const int to = i - j0 < kWave ? i - j0 : kWave;
+                rank += __popcll(to < kWave ? mask & ((1ull << to) - 1) : mask);
+            }
+            const uint64_t after = __ballot(same && j >= i);
+            const int mine = have + __popcll(after & below);
+            if (same && j >= i && mine < kSame) place[mine] = j;
+            have += __popcll(after);
+        }
+        if (l == 0) {
+            found = min(have, kSame);
+            turned = rank;
+        }
+    }
+    __syncthreads();
+    if (turned % kSame) return;
+    int to[kSame], at[kSame], k = found;
+    uint32_t bad = (uint32_t)s >= (uint32_t)items ? ~0u : 0u;
+#pragma unroll
+    for (int e = 0; e < kSame; ++e) {
+        at[e] = e < k ? place[e] : -1;
+        to[e] = e < k ? dst[at[e]] : -1;
+        if ((uint32_t)to[e] >= (uint32_t)items) bad |= 1u << e;
+    }
     for (int j = threadIdx.x; j < n; j += kBlock) {
         const int sj = src[j], dj = dst[j];
         if (sj < 0 || dj < 0) continue;
-        bad = bad || sj == d || (j < i && dj == d);
+#pragma unroll
+        for (int e = 0; e < kSame; ++e)
+            if (sj == to[e] || (j < at[e] && dj == to[e])) bad |= 1u << e;
     }
-    if (__syncthreads_or(bad)) {
-        if (threadIdx.x == 0) raise_flag(error_flag);
-        return;
+    __syncthreads();  // `found` is read
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    if (bad) atomicOr(&found, (int)bad);
+    __syncthreads();
+    bad = (uint32_t)found;
+    const int plane = blockIdx.x / parts, part = blockIdx.x - plane * parts;
+    char *base = pool + plane * plane_bytes + part * part_bytes;
+    char *out[kSame];
+    int kept = 0;
+#pragma unroll
+    for (int e = 0; e < kSame; ++e) {
+        out[e] = nullptr;
+        if (e >= k) continue;
+        if (bad >> e & 1u) {
+            if (threadIdx.x == 0) raise_flag(error_flag);
+            continue;
+        }
+#pragma unroll
+        for (int f = 0; f < kSame; ++f)
+            if (f == kept) out[f] = base + to[e] * item_bytes;
+        ++kept;
     }
-    const int64_t chunks = item_bytes / 16;
-    for (int64_t plane = 0; plane < planes; ++plane) {
-        const u32x4 *from = reinterpret_cast<const u32x4 *>(pool + plane * plane_bytes + s * item_bytes);
-        u32x4 *to = reinterpret_cast<u32x4 *>(pool + plane * plane_bytes + d * item_bytes);
-        for (int64_t c = (int64_t)blockIdx.y * kBlock + threadIdx.x; c < chunks;
-             c += (int64_t)gridDim.y * kBlock)
-            to[c] = from[c];
-    }
+    if (kept)
+        copy_chunks<kSame>(base + s * item_bytes, out, kept,
+                           min(part_bytes, item_bytes - part * part_bytes) / 16);
 }
 
 // The checks that all of these share.
@@ -499,8 +647,9 @@ extern "C" int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *ref
     // a workgroup per entry, plane and head in a grid of fewer than 2^32 work-items
     if (planes < 0 ||
         (planes > 0 && (heads <= 0 || token_bytes <= 0 || token_bytes % 16 || planes >= 65536 ||
-                        heads >= 65536 || planes * heads >= 65536 || token_bytes >= (1 << 24) ||
-                        n * planes * heads >= (1 << 24))))
+                        heads >= 65536 || planes * heads >= 65536 || token_bytes >= (1 << 20) ||
+                        n * planes * heads * ceil_div(page_size * token_bytes, kBegun) >=
+                            (1 << 24))))
         return QDC_ERR_SHAPE;
     const int64_t page_bytes = planes ? heads * page_size * token_bytes : 0;
     const int64_t bytes = pool_bytes(planes, pages, page_bytes);
@@ -517,8 +666,9 @@ extern "C" int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *ref
                                  error_flag), parents, children, copies);
     const int32_t status = launch_status();
     if (status != QDC_OK || planes == 0) return status;
-    hipLaunchKernelGGL(copy_begun, dim3((uint32_t)n, (uint32_t)(planes * heads)), dim3(kBlock), 0,
-                       stream, (char *)pool, copies, pages * page_bytes, page_bytes, (int)heads,
+    const int64_t pieces = ceil_div(page_size * token_bytes, kBegun);
+    hipLaunchKernelGGL(copy_begun, dim3((uint32_t)n, (uint32_t)(planes * heads), (uint32_t)pieces),
+                       dim3(kBlock), 0, stream, (char *)pool, copies, pages * page_bytes, page_bytes, (int)heads,
                        token_bytes);
     return launch_status();
 }
@@ -548,7 +698,11 @@ extern "C" int32_t qdc_pages_compact(int32_t *table, int32_t *refs, int32_t *fre
     hipLaunchKernelGGL(pages_plan, dim3(1), dim3(kBook), 0, stream, refs, (int)pages, m);
     const int32_t status = launch_status();
     if (status != QDC_OK) return status;
-    hipLaunchKernelGGL(pages_move, dim3(2048), dim3(kBlock), 0, stream, (char *)pool, planes,
+    const int64_t most = ceil_div(pages, (int64_t)2) * planes * ceil_div(page_bytes, kPiece);
+    const int64_t spread = ceil_div(rows * width + pages, (int64_t)kBlock);
+    const int64_t want = most > spread ? most : spread;
+    const uint32_t grid = (uint32_t)(want < kMoveGrid ? (want > 0 ? want : 1) : kMoveGrid);
+    hipLaunchKernelGGL(pages_move, dim3(grid), dim3(kBlock), 0, stream, (char *)pool, planes,
                        pages * page_bytes, page_bytes, m, table, rows * width, free_pages,
                        (int)pages);
     return launch_status();
@@ -558,8 +712,8 @@ extern "C" int32_t qdc_copy_pages(void *pool, const int32_t *src, const int32_t 
                                   int64_t planes, int64_t items, int64_t item_bytes,
                                   int32_t *error_flag, hipStream_t stream) {
     const int64_t lim = (int64_t)1 << 31;
-    if (n < 0 || n >= ((int64_t)1 << 16) || planes < 0 || planes >= lim || items <= 0 ||
-        items >= lim || item_bytes < 0 || item_bytes % 16 || item_bytes >= ((int64_t)1 << 40))
+    if (n < 0 || n > 4096 || planes < 0 || planes >= 65536 || items <= 0 || items >= lim ||
+        item_bytes < 0 || item_bytes % 16 || item_bytes >= ((int64_t)1 << 40))
         return QDC_ERR_SHAPE;
     const int64_t bytes = pool_bytes(planes, items, item_bytes);
     if (bytes < 0) return QDC_ERR_SHAPE;
@@ -569,8 +723,19 @@ extern "C" int32_t qdc_copy_pages(void *pool, const int32_t *src, const int32_t 
     const Range outs[2] = {{pool, bytes}, {error_flag, error_flag ? 4 : 0}};
     const Range ins[2] = {{src, n * 4}, {dst, n * 4}};
     if (any_alias(outs, 2, ins, 2)) return QDC_ERR_ALIAS;
-    hipLaunchKernelGGL(copy_items, dim3((uint32_t)n, 16), dim3(kBlock), 0, stream, (char *)pool,
-                       src, dst, (int)n, planes, items * item_bytes, (int)items, item_bytes,
-                       error_flag);
+    // parts of a plane's item: enough workgroups for the chip, each at least 4 KB and at
+    // most 16 KB
+    const int64_t whole = n * planes * item_bytes;
+    int64_t part = 4096;
+    while (part < (16 << 10) && whole / part > 4096) part *= 2;
+    int64_t parts = ceil_div(item_bytes, part);
+    while (n * planes * parts >= ((int64_t)1 << 24)) {
+        if (parts == 1) return QDC_ERR_SHAPE;
+        part *= 2;
+        parts = ceil_div(item_bytes, part);
+    }
+    hipLaunchKernelGGL(copy_items, dim3((uint32_t)(planes * parts), (uint32_t)n), dim3(kBlock), 0,
+                       stream, (char *)pool, src, dst, (int)n, items * item_bytes, (int)items,
+                       item_bytes, part, (int)parts, error_flag);
     return launch_status();
 }

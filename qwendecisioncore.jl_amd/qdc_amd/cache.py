@@ -149,8 +149,9 @@ class BackboneCache:
         src, dst = self._ints(np.asarray(parents), np.asarray(children))
         cache_ops.fork_pages(self.book, src, dst, self._pool(), error_flag=self._flag)
         if self.states.shape[0]:
-            cache_ops.copy_pages(self.states, src, dst)
-            cache_ops.copy_pages(self.rings, src, dst)
+            for part in zip(src.split(4096), dst.split(4096)):
+                cache_ops.copy_pages(self.states, *part)
+                cache_ops.copy_pages(self.rings, *part)
         return self._finish(None, children, children,
                             {c: self._lengths[p] for p, c in zip(parents, children)})
 

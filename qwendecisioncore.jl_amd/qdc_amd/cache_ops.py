@@ -330,7 +330,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
     items, ...]`` (items of a multiple of 16 bytes): pages, or the states and rings of
     rows.  Pairs with a negative index are left out; a pair out of range, or whose
     ``dst`` is an earlier pair's or any pair's ``src``, is not copied and sets
-    ``error_flag``."""
+    ``error_flag``.  At most 4096 pairs a call."""
     dev = _on(pool)
     index = _ints(src, dev, "src", -1)
     n = src.shape[0]

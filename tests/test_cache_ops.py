@@ -134,9 +134,9 @@ def test_pages_validation():
     def copy(pool=POOL, src=I, dst=P, n=4, planes=2, items=7, nbytes=64):
         return lib.qdc_copy_pages(pool, src, dst, n, planes, items, nbytes, None, None)
 
-    assert copy(n=-1) == -2 and copy(n=1 << 16) == -2 and copy(nbytes=8) == -2
+    assert copy(n=-1) == -2 and copy(n=4097) == -2 and copy(nbytes=8) == -2
     assert copy(items=0) == -2 and copy(pool=POOL + 4) == -2
-    assert copy(planes=1 << 30, items=1 << 30, nbytes=1 << 30) == -2
+    assert copy(planes=60000, items=1 << 30, nbytes=1 << 30) == -2 and copy(planes=1 << 16) == -2
     assert copy(pool=None) == -1 and copy(src=None) == -1 and copy(src=POOL + 16) == -5
     assert copy(n=0, pool=None) == 0 and copy(planes=0, pool=None) == 0
 
@@ -705,6 +705,21 @@ def test_copy_pages():
         data[:, d] = data[:, a]
         assert torch.equal(pool.cpu(), data) and f.item() == 1
     cache_ops.copy_pages(pool, ints([]), ints([]))
+    # more pairs of one src than a workgroup writes at once, bad ones between them
+    data = torch.from_numpy(rng.standard_normal((2, 400, 260), dtype=np.float32))
+    pool, f = data.to(DEV), flag()
+    order = rng.permutation(400).tolist()
+    src = [order[int(x)] for x in rng.integers(0, 3, 300)]
+    dst = order[3:303]
+    dst[17], dst[40], dst[41] = order[1], dst[39], 400    # a src, an earlier dst, none
+    src[100] = -1
+    cache_ops.copy_pages(pool, ints(src), ints(dst), error_flag=f)
+    for i, (a, b) in enumerate(zip(src, dst)):
+        if i not in (17, 40, 41, 100):
+            data[:, b] = data[:, a]
+    assert torch.equal(pool.cpu(), data) and f.item() == 1
+    with pytest.raises(ValueError):
+        cache_ops.copy_pages(pool, ints([0] * 4097), ints([1] * 4097))
 
 
 @pytest.mark.gpu
