@@ -73,14 +73,18 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
+// What beginning a unit costs, as bytes of pages read in that time: the chain to its page
+// numbers and the join of its wavefronts, which for heads of 256 no second workgroup of
+// the compute unit fills.  (96 rows of 0 .. 16384 keys of 256, us: 32 KB 78, 64 KB 64,
+// 128 KB 56, 256 KB 57; 200 rows of 1 .. 4000 of 64: 17.9, 17.1, 20.0, 24.6.)
+constexpr int begin_bytes(int head_dim) { return head_dim > 128 ? 131072 : 65536; }
+
 // The work of the call is a line: entry by entry, unit by unit (KV head and group of its
 // query heads), kBegin tiles' worth for beginning a unit and then its tiles.  A
 // wavefront sees 64 entries at a time: lane l holds entry first + l.
 template <typename T, int HD> struct Line {
     static constexpr int TILE = tile_keys<T>();
-    // What beginning a unit costs beside a tile: the chain to its page numbers, the
-    // join of its wavefronts, about as long as 64 KB of pages take.
-    static constexpr uint32_t kBegin = 65536 / (TILE * HD * 2 * (int)sizeof(T));
+    static constexpr uint32_t kBegin = begin_bytes(HD) / (TILE * HD * 2 * (int)sizeof(T));
     const PagedAttention &a;
     const uint32_t units;
     int first, row, keys;
@@ -588,7 +592,7 @@ int64_t longest_line(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_di
     const int64_t units = kv_heads * ceil_div(heads / kv_heads, (int64_t)kHeads);
     const int64_t tile = dtype == QDC_BF16 ? tile_keys<bf16_t>() : tile_keys<float>();
     const int64_t span = ceil_div(width * page_size, tile) +
-                         65536 / (tile * head_dim * 2 * elem_size(dtype));
+                         begin_bytes((int)head_dim) / (tile * head_dim * 2 * elem_size(dtype));
     return span >= lim / units / n ? 0 : span * units * n;
 }
 

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .ops import _DTYPES, _device, _is_split, _rope_tables
+from .ops import _DTYPES, _device, _is_split
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 _I32, _F32 = torch.int32, torch.float32
@@ -132,6 +132,22 @@ def _rows(t: torch.Tensor, like: torch.Tensor, dev: int, name: str):
                    strides[1] if shape[1] > 1 else shape[2])
 
 
+def _rope(tables, rotary_dim: int, dev: int) -> tuple:
+    """(cos pointer, sin pointer, length) of the rotation tables."""
+    if not rotary_dim:
+        return 0, 0, 0
+    if tables is None or len(tables) != 2:
+        raise ValueError("rotation needs the (cos, sin) tables of rope_tables")
+    cos, sin = tables
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] != rotary_dim // 2 or sin.shape != shape \
+            or cos.dtype is not _F32 or sin.dtype is not _F32 or cos.get_device() != dev \
+            or sin.get_device() != dev or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError("cos and sin must be contiguous float32 [n_pos, rotary_dim//2] tables of "
+                         "one shape on the call's device")
+    return cos.data_ptr(), sin.data_ptr(), shape[0]
+
+
 def _code(t: torch.Tensor) -> int:
     code = _DTYPES.get(t.dtype)
     if code is None:
@@ -170,7 +186,7 @@ def prepare_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     page_shape = _pages(k_pages, v_pages, q, dev)
     if page_shape[1] != KV or page_shape[3] != hd:
         raise ValueError("k_pages and v_pages must hold k's heads")
-    cos, sin = _rope_tables(tables, rotary_dim, q)
+    cos, sin, table_len = _rope(tables, rotary_dim, dev)
     n_rows, width = _table(table, dev)
     index, at = _ints(rows, dev, "rows", T), _ints(positions, dev, "positions", T)
     if q_out is None:
@@ -184,9 +200,8 @@ def prepare_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     _call(dev, "prepare_paged", lib().qdc_prepare_paged, q_out.data_ptr(),
           0 if k_out is None else k_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
           q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
-          0 if cos is None else cos.data_ptr(), 0 if sin is None else sin.data_ptr(), index, at,
-          table.data_ptr(), T, H, KV, hd, rotary_dim, 0 if cos is None else cos.shape[0], n_rows,
-          width, page_shape[0], page_shape[2], *q_strides, *k_strides, *v_strides, eps, code,
+          cos, sin, index, at, table.data_ptr(), T, H, KV, hd, rotary_dim, table_len, n_rows, width,
+          page_shape[0], page_shape[2], *q_strides, *k_strides, *v_strides, eps, code,
           _flag(error_flag, dev))
     return q_out
 
