@@ -461,9 +461,11 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
     uint32_t t = (uint32_t)(((uint64_t)all * blockIdx.x) >> lw);
     const uint32_t t_end = (uint32_t)(((uint64_t)all * (blockIdx.x + 1)) >> lw);
     while (t < t_end) {
-        while (line.before + line.all <= t) line.next();
+        while (line.before + line.all <= t && line.first + kWave < a.n) line.next();
         // the entry and unit that hold place t, and the tiles of it up to t_end
-        const int el = __builtin_ctzll(__ballot(line.before + line.end > t));
+        const uint64_t past = __ballot(line.before + line.end > t);
+        if (!past) return;  // the positions changed since they were added up
+        const int el = __builtin_ctzll(past);
         const int keys = __builtin_amdgcn_readlane(line.keys, el);
         const int row = __builtin_amdgcn_readlane(line.row, el);
         const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE, span = tiles + line.kBegin;

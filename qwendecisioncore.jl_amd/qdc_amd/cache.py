@@ -36,9 +36,10 @@ class BackboneCache:
     A sequence is a row number from :meth:`prefill` or :meth:`fork` until
     :meth:`free`.  Invalid ids, masks and rows raise ``ValueError`` before anything
     runs; too few free pages (or rows) raise ``RuntimeError``, and every sequence is
-    as it was before the call.  One call at a time per instance (a lock), all of them
-    on one stream, the device's current one; prefill, step and fork wait for their
-    result.  The cache takes
+    as it was before the call.  (Where torch itself raises within a call, for want of
+    memory say, the rows that the call was at are ended.)  One call at a time per
+    instance (a lock), all of them on one stream, the device's current one; prefill,
+    step and fork wait for their result.  The cache takes
     ``2 * attention layers * pages * kv_heads * page_size * head_dim`` values in the
     model's dtype, and per row and linear attention layer ``value_heads * value_dim *
     key_dim`` float32 values and ``conv_kernel`` rows of the convolution's channels."""
@@ -118,8 +119,12 @@ class BackboneCache:
         d_ids, d_mask = bb._upload(self.model, ids, mask)
         at = np.arange(S) - (S - counts[:, None])
         d_rows, d_counts, d_at = self._ints(np.asarray(rows), counts, at)
-        cache_ops.extend_pages(self.book, d_rows, d_counts, error_flag=self._flag)
-        out = self._prompt(d_ids, d_mask, d_rows, d_at.view(B, S))
+        try:
+            cache_ops.extend_pages(self.book, d_rows, d_counts, error_flag=self._flag)
+            out = self._prompt(d_ids, d_mask, d_rows, d_at.view(B, S))
+        except Exception:
+            self._end(rows, d_rows)
+            raise
         return self._finish(out, rows, rows, {r: int(c) for r, c in zip(rows, counts)})
 
     @_call
@@ -134,8 +139,12 @@ class BackboneCache:
         if any(self._lengths[r] >= self.max_tokens for r in rows):
             raise ValueError(f"A sequence holds at most {self.max_tokens} tokens.")
         d_rows, d_ids = self._ints(np.asarray(rows), ids)
-        at = cache_ops.extend_pages(self.book, d_rows, error_flag=self._flag)
-        out = self._token(d_ids, d_rows, at)
+        try:
+            at = cache_ops.extend_pages(self.book, d_rows, error_flag=self._flag)
+            out = self._token(d_ids, d_rows, at)
+        except Exception:
+            self._end(rows, d_rows)
+            raise
         return self._finish(out, [], None, {r: self._lengths[r] + 1 for r in rows})
 
     @_call
@@ -160,10 +169,7 @@ class BackboneCache:
         """Ends sequences; their rows and the pages that no other row shares are free."""
         rows = self._in_use(rows)
         if rows:
-            cache_ops.free_pages(self.book, *self._ints(np.asarray(rows)))
-        for r in rows:
-            del self._lengths[r]
-        self._unused += rows[::-1]
+            self._end(rows, *self._ints(np.asarray(rows)))
 
     @_call
     def compact(self) -> None:
@@ -189,6 +195,12 @@ class BackboneCache:
         if n > len(self._unused):
             raise RuntimeError("Too few free rows.")
         return [self._unused.pop() for _ in range(n)]
+
+    def _end(self, rows, d_rows) -> None:
+        cache_ops.free_pages(self.book, d_rows)
+        for r in rows:
+            self._lengths.pop(r, None)
+        self._unused += rows[::-1]
 
     def _ints(self, *arrays):
         """Host arrays to the device as int32 vectors, in one copy (what follows starts

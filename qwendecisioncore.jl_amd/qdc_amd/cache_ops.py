@@ -269,7 +269,9 @@ def _pool(pool: torch.Tensor | None, items: int, dev: int):
     if len(shape) < 3 or shape[1] != items or pool.get_device() != dev or not pool.is_contiguous():
         raise ValueError(f"pool must be a contiguous [planes, {items}, ...] tensor on the call's "
                          "device")
-    return pool.data_ptr(), shape[0], pool.stride(1) * pool.element_size()
+    # (strides of axes of one entry may be anything)
+    return (pool.data_ptr(), shape[0],
+            pool.numel() // max(1, shape[0] * items) * pool.element_size())
 
 
 def extend_pages(book: PageTable, rows: torch.Tensor, counts: torch.Tensor | None = None,

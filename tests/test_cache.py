@@ -127,6 +127,28 @@ def test_too_few_pages_leaves_everything():
 
 
 @pytest.mark.gpu
+def test_a_call_that_raises_ends_its_rows(monkeypatch):
+    from qdc_amd.cache import BackboneCache
+    model = model_of("f32")
+    cache = BackboneCache(model, rows=4, pages=20, page_size=16)
+    (a, b), _ = cache.prefill(np.arange(60).reshape(2, 30))
+
+    def fail(*args, **kwargs):
+        raise MemoryError("none left")
+
+    for call in (lambda: cache.prefill([1, 2, 3]), lambda: cache.step([b], [5])):
+        with monkeypatch.context() as m:
+            m.setattr(model, "_project_add_norm", fail)
+            with pytest.raises(MemoryError):
+                call()
+    assert cache.lengths() == {a: 30} and cache.free_page_count() == 18
+    got = cache.step([a], [7])
+    assert normwise(got[0], whole(model, list(range(30)) + [7])) <= BARS["f32"]
+    rows, _ = cache.prefill(np.arange(6).reshape(3, 2))
+    assert len(rows) == 3 and sorted(cache.lengths()) == [0, 1, 2, 3]
+
+
+@pytest.mark.gpu
 def test_refusals():
     import dataclasses
 

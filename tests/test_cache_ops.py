@@ -705,6 +705,13 @@ def test_copy_pages():
         data[:, d] = data[:, a]
         assert torch.equal(pool.cpu(), data) and f.item() == 1
     cache_ops.copy_pages(pool, ints([]), ints([]))
+    # one item, whose stride may be anything
+    data = torch.zeros(3, 1, 8, device=DEV).as_strided((3, 1, 8), (8, 12345, 1))
+    data += torch.arange(24, device=DEV).view(3, 1, 8)
+    assert data.is_contiguous()
+    f.zero_()
+    cache_ops.copy_pages(data, ints([0]), ints([0]), error_flag=f)
+    assert f.item() == 1 and torch.equal(data.flatten(), torch.arange(24.0, device=DEV))
     # more pairs of one src than a workgroup writes at once, bad ones between them
     data = torch.from_numpy(rng.standard_normal((2, 400, 260), dtype=np.float32))
     pool, f = data.to(DEV), flag()
