@@ -119,8 +119,11 @@ int32_t qdc_pages_free(int32_t *table, int32_t *lengths, int32_t *refs, int32_t 
  * page_size, token_bytes], NULL with planes 0: no copies) the places that hold a
  * token.  An entry with a negative parent or child is left out.  A child that is not
  * empty, named twice or a parent too, a row not below `rows`, or more pages than are
- * free: nothing is done (error_flag).  `workspace`: 16 n bytes of device scratch.
- * token_bytes a multiple of 16, pool 16-byte aligned. */
+ * free: nothing is done (error_flag).  `workspace`: qdc_pages_fork_workspace bytes of
+ * device scratch (0 where little is copied).  token_bytes a multiple of 16 below 2^20,
+ * pool 16-byte aligned. */
+int64_t qdc_pages_fork_workspace(int64_t n, int64_t page_size, int64_t planes, int64_t heads,
+                                 int64_t token_bytes);
 int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *refs, int32_t *free_pages,
                        const int32_t *parents, const int32_t *children, int64_t n, int64_t rows,
                        int64_t width, int64_t pages, int64_t page_size, void *pool,

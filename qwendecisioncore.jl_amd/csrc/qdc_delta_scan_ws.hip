@@ -60,11 +60,11 @@ struct ChunkArgs {
     void *out;
     const float *q, *k, *v, *beta, *decay;
     float *ws;
-    float *state;  // [batch, H, vd, kd] after the last token, where it is kept
     int64_t ld_qk, ld_v;  // elements between the token rows of q and k, and of v
     int S, H, vd, groups, chunks, slices;  // slices = vd / 16
     int64_t units;        // batch * heads * chunks (prepare)
     FastDiv by_chunks, by_heads, by_groups;  // by_groups: workgroups per head (scan)
+    float *state;  // [batch, H, vd, kd] after the last token, where it is kept
 };
 
 __device__ __forceinline__ f32x4 load4(const float *p) {

@@ -307,10 +307,20 @@ __device__ __forceinline__ Pair pair_of(const Book &b, const int32_t *parents,
     return f;
 }
 
+// A pool whose begun pages are copied: `planes` planes of [pages, heads, page_size] rows.
+struct Pool {
+    char *data;
+    int64_t plane_bytes, page_bytes, token_bytes;
+    int planes, heads;
+};
+
+// `copies` NULL: this workgroup copies the begun pages itself (one chunk of entries).
 __global__ __launch_bounds__(kBook) void pages_fork(Book b, const int32_t *parents,
-                                                    const int32_t *children, Copy *copies) {
+                                                    const int32_t *children, Copy *copies,
+                                                    Pool pool) {
     extern __shared__ uint32_t seen[];
     __shared__ int parts[kBookWaves], start[kBook], from[kBook], to[kBook];
+    __shared__ Copy own[kBook];
     const int count = stack_count(b), mask = (1 << b.shift) - 1;
     const Pair mine = pair_of(b, parents, children, threadIdx.x);
     clear_bits(seen, b.rows);
@@ -353,7 +363,8 @@ __global__ __launch_bounds__(kBook) void pages_fork(Book b, const int32_t *paren
                 raise_flag(b.error_flag);
             }
         }
-        if (i < b.n) copies[i] = copy;
+        if (!copies) own[threadIdx.x] = copy;
+        else if (i < b.n) copies[i] = copy;
         taken += all;
         if (refused) continue;
         start[threadIdx.x] = block_scan(len >> b.shift, parts, all);
@@ -369,6 +380,16 @@ __global__ __launch_bounds__(kBook) void pages_fork(Book b, const int32_t *paren
         __syncthreads();
     }
     if (threadIdx.x == 0 && !refused) b.free_pages[0] = count - total;
+    if (copies || refused) return;
+    const int per = pool.planes * pool.heads, l = threadIdx.x % kWave;  // a wavefront each
+    for (int u = threadIdx.x / kWave; u < b.n * per; u += kBookWaves) {
+        const Copy c = own[u / per];
+        const int plane = u % per / pool.heads, head = u % per % pool.heads;
+        char *base = pool.data + plane * pool.plane_bytes + head * (pool.page_bytes / pool.heads);
+        const u32x4 *src = reinterpret_cast<const u32x4 *>(base + c.src * pool.page_bytes);
+        u32x4 *dst = reinterpret_cast<u32x4 *>(base + c.dst * pool.page_bytes);
+        for (int k = l; k < c.used * pool.token_bytes / 16; k += kWave) dst[k] = src[k];
+    }
 }
 
 // A workgroup's copy of `chunks` 16-byte chunks to each of `n` places: four loads a thread
@@ -401,16 +422,15 @@ __device__ __forceinline__ void copy_chunks(const char *src, char *const (&dst)[
 // The used places of the begun pages: a workgroup per entry, plane, head and piece.
 constexpr int64_t kBegun = 8192;
 
-__global__ __launch_bounds__(kBlock) void copy_begun(char *pool, const Copy *copies,
-                                                     int64_t plane_bytes, int64_t page_bytes,
-                                                     int heads, int64_t token_bytes) {
+__global__ __launch_bounds__(kBlock) void copy_begun(Pool pool, const Copy *copies) {
     const Copy c = copies[blockIdx.x];
-    const int64_t at = blockIdx.z * kBegun, bytes = c.used * token_bytes;
+    const int64_t at = blockIdx.z * kBegun, bytes = c.used * pool.token_bytes;
     if (at >= bytes) return;
-    const int plane = blockIdx.y / heads, head = blockIdx.y - plane * heads;
-    char *base = pool + plane * plane_bytes + head * (page_bytes / heads) + at;
-    char *const dst[1] = {base + c.dst * page_bytes};
-    copy_chunks<1>(base + c.src * page_bytes, dst, 1, min(kBegun, bytes - at) / 16);
+    const int plane = blockIdx.y / pool.heads, head = blockIdx.y - plane * pool.heads;
+    char *base =
+        pool.data + plane * pool.plane_bytes + head * (pool.page_bytes / pool.heads) + at;
+    char *const dst[1] = {base + c.dst * pool.page_bytes};
+    copy_chunks<1>(base + c.src * pool.page_bytes, dst, 1, min(kBegun, bytes - at) / 16);
 }
 
 // Workspace of a move: count and pages in use, then the pages' new places, the holes
@@ -635,6 +655,18 @@ extern "C" int32_t qdc_pages_free(int32_t *table, int32_t *lengths, int32_t *ref
     return launch_status();
 }
 
+// Bytes that the bookkeeping workgroup copies by itself, done sooner than a second launch
+// is (5 children of a row, pages of 4 KB a head in 2 planes of 2: with the call before and
+// the one after it 27.3 us in two launches, 22.4 in one).
+constexpr int64_t kOwnCopies = 256 << 10;
+
+extern "C" int64_t qdc_pages_fork_workspace(int64_t n, int64_t page_size, int64_t planes,
+                                            int64_t heads, int64_t token_bytes) {
+    if (n <= 0 || n >= ((int64_t)1 << 24) || planes <= 0) return 0;
+    const __int128 most = (__int128)n * planes * heads * page_size * token_bytes;
+    return n <= kBook && most <= kOwnCopies ? 0 : 16 * n;
+}
+
 extern "C" int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *refs,
                                   int32_t *free_pages, const int32_t *parents,
                                   const int32_t *children, int64_t n, int64_t rows, int64_t width,
@@ -644,7 +676,7 @@ extern "C" int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *ref
                                   hipStream_t stream) {
     const int32_t st = check_book(table, lengths, refs, free_pages, n, rows, width, pages, page_size);
     if (st != QDC_OK) return st;
-    // a workgroup per entry, plane and head in a grid of fewer than 2^32 work-items
+    // a workgroup per entry, plane, head and piece in a grid of fewer than 2^32 work-items
     if (planes < 0 ||
         (planes > 0 && (heads <= 0 || token_bytes <= 0 || token_bytes % 16 || planes >= 65536 ||
                         heads >= 65536 || planes * heads >= 65536 || token_bytes >= (1 << 20) ||
@@ -655,21 +687,26 @@ extern "C" int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *ref
     const int64_t bytes = pool_bytes(planes, pages, page_bytes);
     if (bytes < 0) return QDC_ERR_SHAPE;
     if (n == 0) return QDC_OK;
-    if (!parents || !children || !workspace || (planes > 0 && !pool)) return QDC_ERR_NULL;
-    if (workspace_bytes < 16 * n || !aligned16(workspace) || !aligned16(pool)) return QDC_ERR_SHAPE;
-    const Range outs[7] = {QDC_BOOK_RANGES, {workspace, 16 * n}, {pool, bytes}};
+    const int64_t need = qdc_pages_fork_workspace(n, page_size, planes, heads, token_bytes);
+    // without copies the list of them is in LDS and unused, whatever n is
+    const bool own = need == 0;
+    if (!parents || !children || (need && !workspace) || (planes > 0 && !pool)) return QDC_ERR_NULL;
+    if (workspace_bytes < need || (need && !aligned16(workspace)) || !aligned16(pool))
+        return QDC_ERR_SHAPE;
+    const Range outs[7] = {QDC_BOOK_RANGES, {workspace, need}, {pool, bytes}};
     const Range ins[2] = {{parents, n * 4}, {children, n * 4}};
     if (any_alias(outs, 7, ins, 2)) return QDC_ERR_ALIAS;
-    Copy *copies = reinterpret_cast<Copy *>(workspace);
+    Copy *copies = own ? nullptr : reinterpret_cast<Copy *>(workspace);
+    const Pool p = {(char *)pool, pages * page_bytes, page_bytes, token_bytes, (int)planes,
+                    (int)heads};
     hipLaunchKernelGGL(pages_fork, dim3(1), dim3(kBook), bit_bytes(rows), stream,
                        make_book(table, lengths, refs, free_pages, n, rows, width, pages, page_size,
-                                 error_flag), parents, children, copies);
+                                 error_flag), parents, children, copies, p);
     const int32_t status = launch_status();
-    if (status != QDC_OK || planes == 0) return status;
+    if (status != QDC_OK || own) return status;
     const int64_t pieces = ceil_div(page_size * token_bytes, kBegun);
     hipLaunchKernelGGL(copy_begun, dim3((uint32_t)n, (uint32_t)(planes * heads), (uint32_t)pieces),
-                       dim3(kBlock), 0, stream, (char *)pool, copies, pages * page_bytes, page_bytes, (int)heads,
-                       token_bytes);
+                       dim3(kBlock), 0, stream, p, copies);
     return launch_status();
 }
 

@@ -87,6 +87,7 @@ CACHE_SIGNATURES = {
                             + [_f32, _i32, _vp, _i64, _vp, _vp]),
     "qdc_pages_extend": (_i32, [_vp] * 7 + [_i64] * 5 + [_vp, _vp]),
     "qdc_pages_free": (_i32, [_vp] * 5 + [_i64] * 5 + [_vp, _vp]),
+    "qdc_pages_fork_workspace": (_i64, [_i64] * 5),
     "qdc_pages_fork": (_i32, [_vp] * 6 + [_i64] * 5 + [_vp] + [_i64] * 3
                        + [_vp, _i64, _vp, _vp]),
     "qdc_pages_compact_workspace": (_i64, [_i64]),

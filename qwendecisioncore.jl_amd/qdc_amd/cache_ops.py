@@ -324,9 +324,10 @@ def fork_pages(book: PageTable, parents: torch.Tensor, children: torch.Tensor,
         if len(shape) != 5 or shape[3] != book.page_size:
             raise ValueError("pool must be [planes, pages, kv_heads, page_size, head_dim]")
         heads, token = shape[2], shape[4] * pool.element_size()
-    work = torch.empty(16 * n, dtype=torch.uint8, device=parents.device)
+    need = lib().qdc_pages_fork_workspace(n, sizes[3], planes, heads, token)
+    work = torch.empty(need, dtype=torch.uint8, device=parents.device) if need else None
     _call(dev, "fork_pages", lib().qdc_pages_fork, *at, src, dst, n, *sizes, pool_at, planes,
-          heads, token, work.data_ptr(), 16 * n, _flag(error_flag, dev))
+          heads, token, work.data_ptr() if need else 0, need, _flag(error_flag, dev))
 
 
 def compact_pages(book: PageTable, pool: torch.Tensor | None = None) -> None:

@@ -112,15 +112,22 @@ def test_pages_validation():
     assert free(index=None) == -1 and free(index=R) == -5 and free(page=1) == -2
     assert free(n=0, index=None) == 0
 
-    def fork(par=I, ch=P, n=4, pool=POOL, planes=2, heads=2, token=128, ws=W, nbytes=64):
+    assert lib.qdc_pages_fork_workspace(4, 16, 2, 2, 128) == 0         # little to copy
+    assert lib.qdc_pages_fork_workspace(4, 16, 2, 2, 8192) == 64
+    assert lib.qdc_pages_fork_workspace(1025, 16, 1, 1, 16) == 16400
+    assert lib.qdc_pages_fork_workspace(5000, 16, 0, 0, 0) == 0
+
+    def fork(par=I, ch=P, n=4, pool=POOL, planes=2, heads=2, token=8192, ws=W, nbytes=64):
         return lib.qdc_pages_fork(T, L, R, S, par, ch, n, 5, 6, 7, 16, pool, planes, heads, token,
                                   ws, nbytes, None, None)
 
     assert fork(token=120) == -2 and fork(token=0) == -2 and fork(heads=0) == -2
     assert fork(planes=-1) == -2 and fork(planes=1 << 16) == -2 and fork(nbytes=63) == -2
     assert fork(ws=W + 4) == -2 and fork(pool=POOL + 4) == -2 and fork(planes=1 << 14, heads=4) == -2
+    assert fork(token=1 << 20) == -2 and fork(n=4000, planes=600, nbytes=1 << 20) == -2
     assert fork(par=None) == -1 and fork(pool=None) == -1 and fork(ws=None) == -1
     assert fork(ws=POOL) == -5 and fork(ch=T) == -5 and fork(n=0, par=None) == 0
+    assert fork(token=128, ws=None, nbytes=0, ch=None) == -1
 
     def compact(table=T, pool=POOL, planes=2, nbytes=4096, pages=7, ws=W, have=100):
         return lib.qdc_pages_compact(table, R, S, 5, 6, pages, pool, planes, nbytes, ws, have, None)
@@ -598,6 +605,7 @@ class Model:
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,width,pages,page,dtype,dim", [(12, 6, 40, 16, torch.float32, 4),
                                                              (7, 3, 11, 64, torch.bfloat16, 64),
+                                                             (10, 3, 40, 64, torch.float32, 256),
                                                              (30, 9, 300, 32, torch.bfloat16, 8)])
 def test_pages_life(rows, width, pages, page, dtype, dim):
     """Rows that grow, fork, end and move together in any order, whole numbers and
