@@ -392,31 +392,21 @@ __global__ __launch_bounds__(kBook) void pages_fork(Book b, const int32_t *paren
     }
 }
 
-// A workgroup's copy of `chunks` 16-byte chunks to each of `n` places: four loads a thread
-// ahead of their stores, the stores as a stream.
-template <int N>
-__device__ __forceinline__ void copy_chunks(const char *src, char *const (&dst)[N], int n,
-                                            int64_t chunks) {
+// A workgroup's copy of `chunks` 16-byte chunks: up to four loads a thread ahead of their
+// stores, the stores as a stream.
+__device__ __forceinline__ void copy_chunks(const char *src, char *dst, int64_t chunks) {
     constexpr int U = 4;
     const u32x4 *from = reinterpret_cast<const u32x4 *>(src);
+    const int step = blockDim.x;
     int64_t i = threadIdx.x;
-    for (; i + (U - 1) * kBlock < chunks; i += U * kBlock) {
+    for (; i + (U - 1) * step < chunks; i += U * step) {
         u32x4 v[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = load_raw(from + i + u * kBlock);
+        for (int u = 0; u < U; ++u) v[u] = load_raw(from + i + u * step);
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            if (k >= n) break;
-#pragma unroll
-            for (int u = 0; u < U; ++u) store_raw(dst[k] + 16 * (i + u * kBlock), v[u]);
-        }
+        for (int u = 0; u < U; ++u) store_raw(dst + 16 * (i + u * step), v[u]);
     }
-    for (; i < chunks; i += kBlock) {
-        const u32x4 v = load_raw(from + i);
-#pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (k < n) store_raw(dst[k] + 16 * i, v);
-    }
+    for (; i < chunks; i += step) store_raw(dst + 16 * i, load_raw(from + i));
 }
 
 // The used places of the begun pages: a workgroup per entry, plane, head and piece.
@@ -429,8 +419,8 @@ __global__ __launch_bounds__(kBlock) void copy_begun(Pool pool, const Copy *copi
     const int plane = blockIdx.y / pool.heads, head = blockIdx.y - plane * pool.heads;
     char *base =
         pool.data + plane * pool.plane_bytes + head * (pool.page_bytes / pool.heads) + at;
-    char *const dst[1] = {base + c.dst * pool.page_bytes};
-    copy_chunks<1>(base + c.src * pool.page_bytes, dst, 1, min(kBegun, bytes - at) / 16);
+    copy_chunks(base + c.src * pool.page_bytes, base + c.dst * pool.page_bytes,
+                min(kBegun, bytes - at) / 16);
 }
 
 // Workspace of a move: count and pages in use, then the pages' new places, the holes
@@ -491,8 +481,8 @@ __global__ __launch_bounds__(kBlock) void pages_move(char *pool, int64_t planes,
         const int64_t k = u / per_page, rest = u - k * per_page;
         const int64_t plane = rest / pieces, at = (rest - plane * pieces) * kPiece;
         char *base = pool + plane * plane_bytes + at;
-        char *const dst[1] = {base + m.hole[k] * page_bytes};
-        copy_chunks<1>(base + m.page[k] * page_bytes, dst, 1, min(kPiece, page_bytes - at) / 16);
+        copy_chunks(base + m.page[k] * page_bytes, base + m.hole[k] * page_bytes,
+                    min(kPiece, page_bytes - at) / 16);
     }
     const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x, step = (int64_t)gridDim.x * kBlock;
     if (count)
@@ -505,84 +495,38 @@ __global__ __launch_bounds__(kBlock) void pages_move(char *pool, int64_t planes,
         free_pages[i] = i == 0 ? free_count : i <= free_count ? pages - (int)i : 0;
 }
 
-// Up to kSame pairs of one src are one workgroup's for a part of a plane: read once,
-// written to each.  The first of them in the call stands for them; each checks the
-// call's pairs for itself.  (8 rows of 19 MB to 5 places each, us: pairs by themselves
-// 186, two together 175, four 181, eight 195: the writes go to as many places at once.)
-constexpr int kSame = 2;
+// A workgroup per pair and part of a plane's item; each checks the call's pairs for itself.
+// 8 rows' states of 19 MB to 5 places each (151 MB read, 755 MB written): 150 us = 6.0 TB/s
+// in parts of 64 KB by 1024 threads; 165 in parts of 32 KB, 174 of 16 KB by 256, and 158 to
+// 172 with two to five pairs of one src in a workgroup, which reads them once: the reads of
+// the other pairs come from the caches as it is.
+constexpr int kPart = 1024;
 
-__global__ __launch_bounds__(kBlock) void copy_items(char *pool, const int32_t *src,
-                                                     const int32_t *dst, int n,
-                                                     int64_t plane_bytes, int items,
-                                                     int64_t item_bytes, int64_t part_bytes,
-                                                     int parts, int32_t *error_flag) {
-    __shared__ int place[kSame], found, turned;
-    const int i = blockIdx.y, s = src[i], own = dst[i];
-    if (s < 0 || own < 0) return;
-    if (threadIdx.x < kWave) {  // which of the pairs of this src it is, and those after it
-        const int l = threadIdx.x;
-        int rank = 0, have = 0;
-        for (int j0 = 0; j0 < n; j0 += kWave) {
-            const int j = j0 + l;
-            const bool same = j < n && src[j] == s && dst[j] >= 0;
-            const uint64_t mask = __ballot(same), below = (1ull << l) - 1;
-            if (j0 <= i) {
-                const int to = i - j0 < kWave ? i - j0 : kWave;
-                rank += __popcll(to < kWave ? mask & ((1ull << to) - 1) : mask);
-            }
-            const uint64_t after = __ballot(same && j >= i);
-            const int mine = have + __popcll(after & below);
-            if (same && j >= i && mine < kSame) place[mine] = j;
-            have += __popcll(after);
-        }
-        if (l == 0) {
-            found = min(have, kSame);
-            turned = rank;
-        }
-    }
-    __syncthreads();
-    if (turned % kSame) return;
-    int to[kSame], at[kSame], k = found;
-    uint32_t bad = (uint32_t)s >= (uint32_t)items ? ~0u : 0u;
-#pragma unroll
-    for (int e = 0; e < kSame; ++e) {
-        at[e] = e < k ? place[e] : -1;
-        to[e] = e < k ? dst[at[e]] : -1;
-        if ((uint32_t)to[e] >= (uint32_t)items) bad |= 1u << e;
-    }
-    for (int j = threadIdx.x; j < n; j += kBlock) {
-        const int sj = src[j], dj = dst[j];
-        if (sj < 0 || dj < 0) continue;
-#pragma unroll
-        for (int e = 0; e < kSame; ++e)
-            if (sj == to[e] || (j < at[e] && dj == to[e])) bad |= 1u << e;
-    }
-    __syncthreads();  // `found` is read
+__global__ __launch_bounds__(kPart) void copy_items(char *pool, const int32_t *src,
+                                                    const int32_t *dst, int n,
+                                                    int64_t plane_bytes, int items,
+                                                    int64_t item_bytes, int64_t part_bytes,
+                                                    int parts, int32_t *error_flag) {
+    __shared__ int found;
+    const int i = blockIdx.y, s = src[i], d = dst[i];
+    if (s < 0 || d < 0) return;
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
-    if (bad) atomicOr(&found, (int)bad);
+    bool bad = (uint32_t)s >= (uint32_t)items || (uint32_t)d >= (uint32_t)items;
+    for (int j = threadIdx.x; j < n; j += blockDim.x) {
+        const int sj = src[j], dj = dst[j];
+        if (sj >= 0 && dj >= 0) bad |= sj == d || (j < i && dj == d);
+    }
+    if (bad) found = 1;
     __syncthreads();
-    bad = (uint32_t)found;
+    if (found) {
+        if (threadIdx.x == 0) raise_flag(error_flag);
+        return;
+    }
     const int plane = blockIdx.x / parts, part = blockIdx.x - plane * parts;
     char *base = pool + plane * plane_bytes + part * part_bytes;
-    char *out[kSame];
-    int kept = 0;
-#pragma unroll
-    for (int e = 0; e < kSame; ++e) {
-        out[e] = nullptr;
-        if (e >= k) continue;
-        if (bad >> e & 1u) {
-            if (threadIdx.x == 0) raise_flag(error_flag);
-            continue;
-        }
-#pragma unroll
-        for (int f = 0; f < kSame; ++f)
-            if (f == kept) out[f] = base + to[e] * item_bytes;
-        ++kept;
-    }
-    if (kept)
-        copy_chunks<kSame>(base + s * item_bytes, out, kept,
-                           min(part_bytes, item_bytes - part * part_bytes) / 16);
+    copy_chunks(base + s * item_bytes, base + d * item_bytes,
+                min(part_bytes, item_bytes - part * part_bytes) / 16);
 }
 
 // The checks that all of these share.
@@ -761,18 +705,19 @@ extern "C" int32_t qdc_copy_pages(void *pool, const int32_t *src, const int32_t 
     const Range ins[2] = {{src, n * 4}, {dst, n * 4}};
     if (any_alias(outs, 2, ins, 2)) return QDC_ERR_ALIAS;
     // parts of a plane's item: enough workgroups for the chip, each at least 4 KB and at
-    // most 16 KB
+    // most 64 KB
     const int64_t whole = n * planes * item_bytes;
     int64_t part = 4096;
-    while (part < (16 << 10) && whole / part > 4096) part *= 2;
+    while (part < (64 << 10) && whole / part > 4096) part *= 2;
     int64_t parts = ceil_div(item_bytes, part);
     while (n * planes * parts >= ((int64_t)1 << 24)) {
         if (parts == 1) return QDC_ERR_SHAPE;
         part *= 2;
         parts = ceil_div(item_bytes, part);
     }
-    hipLaunchKernelGGL(copy_items, dim3((uint32_t)(planes * parts), (uint32_t)n), dim3(kBlock), 0,
-                       stream, (char *)pool, src, dst, (int)n, items * item_bytes, (int)items,
-                       item_bytes, part, (int)parts, error_flag);
+    hipLaunchKernelGGL(copy_items, dim3((uint32_t)(planes * parts), (uint32_t)n),
+                       dim3((uint32_t)(part / 16 < kPart ? part / 16 : kPart)), 0, stream,
+                       (char *)pool, src, dst, (int)n, items * item_bytes, (int)items, item_bytes,
+                       part, (int)parts, error_flag);
     return launch_status();
 }
