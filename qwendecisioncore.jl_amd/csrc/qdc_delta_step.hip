@@ -257,9 +257,9 @@ extern "C" int32_t qdc_delta_step(void *out, int32_t out_dtype, const void *proj
         return QDC_ERR_SHAPE;
     const int64_t vw = value_heads * value_dim, channels = 2 * key_heads * key_dim + vw;
     const int64_t es = elem_size(proj_dtype);
-    // a workgroup of 512 per entry and head in a grid of fewer than 2^32 work-items
+    // a workgroup of up to 1024 per entry and head in a grid of fewer than 2^32 work-items
     if (ld < channels + vw + 2 * value_heads || n >= lim || ld >= lim ||
-        n * value_heads >= ((int64_t)1 << 23))
+        n * value_heads >= ((int64_t)1 << 22))
         return QDC_ERR_SHAPE;
     if (n == 0) return QDC_OK;
     if (!out || !proj || !conv || !a_decay || !dt_bias || !norm || !ring || !state || !index ||

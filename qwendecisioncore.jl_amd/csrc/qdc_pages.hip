@@ -705,19 +705,19 @@ extern "C" int32_t qdc_copy_pages(void *pool, const int32_t *src, const int32_t 
     const Range ins[2] = {{src, n * 4}, {dst, n * 4}};
     if (any_alias(outs, 2, ins, 2)) return QDC_ERR_ALIAS;
     // parts of a plane's item: enough workgroups for the chip, each at least 4 KB and at
-    // most 64 KB
+    // most 64 KB, in a grid of fewer than 2^32 work-items
     const int64_t whole = n * planes * item_bytes;
     int64_t part = 4096;
-    while (part < (64 << 10) && whole / part > 4096) part *= 2;
-    int64_t parts = ceil_div(item_bytes, part);
-    while (n * planes * parts >= ((int64_t)1 << 24)) {
-        if (parts == 1) return QDC_ERR_SHAPE;
-        part *= 2;
+    while (part < (64 << 10) && part < item_bytes && whole / part > 4096) part *= 2;
+    int64_t parts, threads;
+    for (;; part *= 2) {
         parts = ceil_div(item_bytes, part);
+        threads = part / 16 < kPart ? part / 16 : kPart;
+        if (n * planes * parts * threads < ((int64_t)1 << 32)) break;
+        if (parts == 1) return QDC_ERR_SHAPE;
     }
     hipLaunchKernelGGL(copy_items, dim3((uint32_t)(planes * parts), (uint32_t)n),
-                       dim3((uint32_t)(part / 16 < kPart ? part / 16 : kPart)), 0, stream,
-                       (char *)pool, src, dst, (int)n, items * item_bytes, (int)items, item_bytes,
-                       part, (int)parts, error_flag);
+                       dim3((uint32_t)threads), 0, stream, (char *)pool, src, dst, (int)n,
+                       items * item_bytes, (int)items, item_bytes, part, (int)parts, error_flag);
     return launch_status();
 }

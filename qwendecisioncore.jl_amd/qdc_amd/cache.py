@@ -29,6 +29,10 @@ def _call(method):
     return call
 
 
+def _host(hidden: torch.Tensor) -> np.ndarray:
+    return hidden.float().cpu().numpy()
+
+
 class BackboneCache:
     """Up to ``rows`` sequences of one model, of up to ``max_tokens`` tokens each, whose
     attention layers share ``pages`` pages of ``page_size`` tokens.
@@ -121,9 +125,9 @@ class BackboneCache:
         d_rows, d_counts, d_at = self._ints(np.asarray(rows), counts, at)
         try:
             cache_ops.extend_pages(self.book, d_rows, d_counts, error_flag=self._flag)
-            out = self._prompt(d_ids, d_mask, d_rows, d_at.view(B, S))
+            out = _host(self._prompt(d_ids, d_mask, d_rows, d_at.view(B, S)))
         except Exception:
-            self._end(rows, d_rows)
+            self._abandon(rows, d_rows)
             raise
         return self._finish(out, rows, rows, {r: int(c) for r, c in zip(rows, counts)})
 
@@ -141,9 +145,9 @@ class BackboneCache:
         d_rows, d_ids = self._ints(np.asarray(rows), ids)
         try:
             at = cache_ops.extend_pages(self.book, d_rows, error_flag=self._flag)
-            out = self._token(d_ids, d_rows, at)
+            out = _host(self._token(d_ids, d_rows, at))
         except Exception:
-            self._end(rows, d_rows)
+            self._abandon(rows, d_rows)
             raise
         return self._finish(out, [], None, {r: self._lengths[r] + 1 for r in rows})
 
@@ -156,11 +160,15 @@ class BackboneCache:
             return []
         children = self._take(len(parents))
         src, dst = self._ints(np.asarray(parents), np.asarray(children))
-        cache_ops.fork_pages(self.book, src, dst, self._pool(), error_flag=self._flag)
-        if self.states.shape[0]:
-            for part in zip(src.split(4096), dst.split(4096)):
-                cache_ops.copy_pages(self.states, *part)
-                cache_ops.copy_pages(self.rings, *part)
+        try:
+            cache_ops.fork_pages(self.book, src, dst, self._pool(), error_flag=self._flag)
+            if self.states.shape[0]:
+                for part in zip(src.split(4096), dst.split(4096)):
+                    cache_ops.copy_pages(self.states, *part)
+                    cache_ops.copy_pages(self.rings, *part)
+        except Exception:
+            self._abandon(children, dst)
+            raise
         return self._finish(None, children, children,
                             {c: self._lengths[p] for p, c in zip(parents, children)})
 
@@ -202,6 +210,11 @@ class BackboneCache:
             self._lengths.pop(r, None)
         self._unused += rows[::-1]
 
+    def _abandon(self, rows, d_rows) -> None:
+        """Ends the rows of a call that raised; what it flagged is not the next call's."""
+        self._end(rows, d_rows)
+        self._flag.zero_()
+
     def _ints(self, *arrays):
         """Host arrays to the device as int32 vectors, in one copy (what follows starts
         on 16 bytes)."""
@@ -216,15 +229,14 @@ class BackboneCache:
 
     def _finish(self, out, taken, result, lengths):
         """Waits for the call, and takes it back if a kernel flagged it."""
-        host = None if out is None else out.float().cpu().numpy()
         if int(self._flag.item()) != 0:
             self._flag.zero_()
             self._unused += taken[::-1]
             raise RuntimeError("Too few free pages.")
         self._lengths.update(lengths)
         if result is None:
-            return host
-        return result if out is None else (result, host)
+            return out
+        return result if out is None else (result, out)
 
     # -------------------------------------------------------------- layers --
     def _split_proj(self, proj):

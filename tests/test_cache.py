@@ -149,6 +149,32 @@ def test_a_call_that_raises_ends_its_rows(monkeypatch):
 
 
 @pytest.mark.gpu
+def test_a_call_that_raises_leaves_no_flag_and_no_rows(monkeypatch):
+    """A fork whose copies raise gives its rows back, and a call that raises after its
+    kernels found too few pages does not fail the next one."""
+    from qdc_amd import cache as module
+    from qdc_amd.cache import BackboneCache
+    model = model_of("f32")
+    cache = BackboneCache(model, rows=4, pages=5, page_size=16)
+    (a,), _ = cache.prefill(np.arange(30))
+
+    def fail(*args, **kwargs):
+        raise MemoryError("none left")
+
+    for name, call in (("copy_pages", lambda: cache.fork([a, a])),
+                       ("prepare_paged", lambda: cache.prefill(np.arange(70)))):
+        with monkeypatch.context() as m:
+            m.setattr(module.cache_ops, name, fail)
+            with pytest.raises(MemoryError):
+                call()
+        assert cache.lengths() == {a: 30} and cache.free_page_count() == 3
+    kids = cache.fork([a, a, a])
+    assert len(kids) == 3 and cache.free_page_count() == 0
+    for got in cache.step([a] + kids, [7] * 4):
+        assert normwise(got, whole(model, list(range(30)) + [7])) <= BARS["f32"]
+
+
+@pytest.mark.gpu
 def test_refusals():
     import dataclasses
 

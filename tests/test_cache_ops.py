@@ -146,6 +146,9 @@ def test_pages_validation():
     assert copy(planes=60000, items=1 << 30, nbytes=1 << 30) == -2 and copy(planes=1 << 16) == -2
     assert copy(pool=None) == -1 and copy(src=None) == -1 and copy(src=POOL + 16) == -5
     assert copy(n=0, pool=None) == 0 and copy(planes=0, pool=None) == 0
+    # grids of 2^32 work-items: 4 KB a workgroup of 256, 64 KB and more one of 1024
+    assert copy(n=4096, planes=4096, nbytes=4096) == -2
+    assert copy(n=4096, planes=1024, nbytes=65536) == -2
 
 
 def test_delta_step_validation():
@@ -163,6 +166,7 @@ def test_delta_step_validation():
     assert f(kd=96) == -2 and f(vd=24) == -2 and f(vd=272) == -2 and f(vh=3) == -2
     assert f(taps=0) == -2 and f(taps=9) == -2 and f(rows=0) == -2 and f(n=-1) == -2
     assert f(ld=2 * 128 + 128 + 128 + 7) == -2 and f(n=1 << 22) == -2
+    assert f(n=1 << 20) == -2           # a workgroup of 1024 for each of its 4 heads: 2^32 threads
     for x in names:
         assert f(**{x: 0}) == -1, x
     assert f(out=0) == -1 and f(state=FAR + 4) == -2
