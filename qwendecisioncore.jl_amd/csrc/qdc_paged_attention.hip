@@ -146,15 +146,23 @@ __device__ __forceinline__ float rest(float p) {
                     : p;
 }
 
-// N consecutive outputs of head h of entry i, values dim .., with the gate.
+// The gate of N consecutive outputs of head h of entry i, values dim .., loaded ahead of
+// the work that it multiplies.
+template <typename T, int N>
+__device__ __forceinline__ void load_gate(const PagedAttention &a, int i, int h, int dim,
+                                          T (&g)[N]) {
+    if (!a.gate) return;
+    const T *p = (const T *)a.gate + (int64_t)i * a.gate_tok + (int64_t)h * a.gate_head + dim;
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] = p[j];
+}
+
 template <typename T, int HD, int N>
 __device__ __forceinline__ void store_out(const PagedAttention &a, int i, int h, int dim,
-                                          float (&o)[N]) {
-    if (a.gate) {
-        const T *g = (const T *)a.gate + (int64_t)i * a.gate_tok + (int64_t)h * a.gate_head + dim;
+                                          float (&o)[N], bool gated, const T (&g)[N]) {
+    if (gated)
 #pragma unroll
         for (int j = 0; j < N; ++j) o[j] *= sigmoid(to_f32(g[j]));
-    }
     const int64_t at = (int64_t)i * a.out_tok + (int64_t)h * HD + dim;
     if constexpr (N == 4) {
         if (a.out_dtype == QDC_BF16) store_frag((bf16_t *)a.out + at, o);
@@ -173,10 +181,9 @@ __device__ __forceinline__ void store_out(const PagedAttention &a, int i, int h,
 // Of an entry without keys: 0 whatever the gate holds.
 template <typename T, int HD, int N>
 __device__ __forceinline__ void store_zero(const PagedAttention &a, int i, int h, int dim) {
-    PagedAttention b = a;
-    b.gate = nullptr;
     float zero[N] = {};
-    store_out<T, HD, N>(b, i, h, dim, zero);
+    const T gate[N] = {};
+    store_out<T, HD, N>(a, i, h, dim, zero, false, gate);
 }
 
 // Pages stream by: read as such they come at up to 6.7 TB/s, with plain loads at 5.6.
@@ -235,6 +242,9 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     const int gu = min(kHeads, a.group - hg * kHeads);
     const int32_t *pages = a.table + (int64_t)row * a.width;
 
+    const int dim = VEC * l;
+    T gate[VEC] = {};
+    if (whole && wv < min(gu, 4)) load_gate(a, entry, head0 + wv, dim, gate);
     // this wavefront's tiles: one of every WAVES
     const int jw = j0 + wv, cnt = j1 > jw ? (j1 - jw + WAVES - 1) / WAVES : 0;
     int32_t ids = -1;  // lane l: the page of tile k0 + l / SUBS, sub l % SUBS
@@ -415,6 +425,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     }
     for (int h0 = 0; h0 < gu; h0 += 4) {
         const int hh = lr - h0;
+        if (h0 && whole && wv < min(gu - h0, 4)) load_gate(a, entry, head0 + h0 + wv, dim, gate);
         if (hh >= 0 && hh < 4)
 #pragma unroll
             for (int c = 0; c < L::VC; ++c)
@@ -424,8 +435,8 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
                     for (int r = 0; r < 4; ++r)
                         so[wv][hh][16 * L::VD * c + L::VD * (4 * lg + r) + j] = x.o[c][j][r];
         __syncthreads();
-        const int h = h0 + threadIdx.x / kWave, dim = VEC * l;
-        if (h < gu && h < h0 + 4) {
+        const int h = h0 + wv;
+        if (h < gu && wv < 4) {
             float top = sm[0][h], acc[VEC] = {}, total = 0.0f;
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) top = fmaxf(top, sm[w][h]);
@@ -441,7 +452,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
                 const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) acc[e] *= inv;
-                store_out<T, HD, VEC>(a, entry, head0 + h, dim, acc);
+                store_out<T, HD, VEC>(a, entry, head0 + h, dim, acc, a.gate, gate);
             } else {
                 float *dst = a.pieces + (slot * a.unit_heads + h) * HD + dim;
 #pragma unroll
@@ -518,6 +529,9 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
     const int entry = blockIdx.x / a.heads, h = blockIdx.x - entry * a.heads;
     const int kvh = h / a.group, in_group = h - kvh * a.group;
     const int hg = in_group / kHeads, hu = in_group - hg * kHeads;
+    const int dim = HD / kWave * l;
+    T gate[HD / kWave] = {};
+    if (wv == 0) load_gate(a, entry, h, dim, gate);
     Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
     while (line.first + kWave <= entry) line.next();
@@ -528,7 +542,6 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
         entry_keys(a, a.index[entry], a.positions[entry], bad);
         if (bad) raise_flag(a.error_flag);
     }
-    const int dim = HD / kWave * l;
     if (tiles == 0) {
         if (wv == 0) store_zero<T, HD, HD / kWave>(a, entry, h, dim);
         return;
@@ -582,7 +595,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
 #pragma unroll
     for (int e = 0; e < HD / kWave; ++e) o[e] *= inv;
-    store_out<T, HD, HD / kWave>(a, entry, h, dim, o);
+    store_out<T, HD, HD / kWave>(a, entry, h, dim, o, a.gate, gate);
 }
 
 // The longest line that a call of these sizes can have, 0 when it is too long or the

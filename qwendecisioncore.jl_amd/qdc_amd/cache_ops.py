@@ -62,7 +62,7 @@ def page_table(rows: int, width: int, pages: int, page_size: int, device) -> Pag
 
 # The host's part of a call is the whole cost of a small one, so each check below is one
 # expression of plain attributes (a device as its index, get_device, in 0.04 us where
-# comparing device objects takes 0.12).
+# comparing device objects takes 0.12; new_empty of sizes in 1.0 where empty takes 1.7).
 def _call(dev: int, name: str, fn, *args) -> None:
     """``fn(*args, stream)`` on device ``dev``, made the current one for the launch if it
     is not."""
@@ -190,7 +190,7 @@ def prepare_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     n_rows, width = _table(table, dev)
     index, at = _ints(rows, dev, "rows", T), _ints(positions, dev, "positions", T)
     if q_out is None:
-        q_out = torch.empty((T, H, hd), dtype=q.dtype, device=q.device)
+        q_out = q.new_empty(T, H, hd)
     elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.get_device() != dev \
             or not q_out.is_contiguous():
         raise ValueError("q_out must be a contiguous tensor of q's shape, dtype and device")
@@ -239,10 +239,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out_code = _lib.QDC_BF16X2 if split else _DTYPES.get(odt)
         if out_code is None:
             raise ValueError("out_dtype must be float32, bfloat16 or BF16X2")
-    device = q.device
-    out = torch.empty((n, 2 * H * hd if split else H * hd), dtype=odt, device=device)
+    out = q.new_empty(n, 2 * H * hd if split else H * hd, dtype=odt)
     need = lib().qdc_paged_attention_workspace(n, H, KV, hd, width, page, code)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
     _call(dev, "paged_attention", lib().qdc_paged_attention, out.data_ptr(), out_code,
           q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), gate_at, table.data_ptr(), index,
           at, n, H, KV, hd, n_rows, width, pages, page, *q_strides, *gate_strides, H * hd, scale,
@@ -288,7 +287,7 @@ def extend_pages(book: PageTable, rows: torch.Tensor, counts: torch.Tensor | Non
     n = rows.shape[0]
     many = 0 if counts is None else _ints(counts, dev, "counts", n)
     if positions is None:
-        positions = torch.empty(n, dtype=_I32, device=rows.device)
+        positions = rows.new_empty(n)
     _call(dev, "extend_pages", lib().qdc_pages_extend, _ints(positions, dev, "positions", n), *at,
           index, many, n, *sizes, _flag(error_flag, dev))
     return positions
@@ -325,7 +324,7 @@ def fork_pages(book: PageTable, parents: torch.Tensor, children: torch.Tensor,
             raise ValueError("pool must be [planes, pages, kv_heads, page_size, head_dim]")
         heads, token = shape[2], shape[4] * pool.element_size()
     need = lib().qdc_pages_fork_workspace(n, sizes[3], planes, heads, token)
-    work = torch.empty(need, dtype=torch.uint8, device=parents.device) if need else None
+    work = parents.new_empty(need, dtype=torch.uint8) if need else None
     _call(dev, "fork_pages", lib().qdc_pages_fork, *at, src, dst, n, *sizes, pool_at, planes,
           heads, token, work.data_ptr() if need else 0, need, _flag(error_flag, dev))
 
@@ -337,7 +336,7 @@ def compact_pages(book: PageTable, pool: torch.Tensor | None = None) -> None:
     dev, at, (rows, width, pages, _) = _book(book)
     pool_at, planes, nbytes = _pool(pool, pages, dev)
     need = lib().qdc_pages_compact_workspace(pages)
-    work = torch.empty(need, dtype=torch.uint8, device=book.table.device)
+    work = book.table.new_empty(need, dtype=torch.uint8)
     _call(dev, "compact_pages", lib().qdc_pages_compact, at[0], at[2], at[3], rows, width, pages,
           pool_at, planes, nbytes, work.data_ptr(), need)
 
@@ -411,7 +410,7 @@ def delta_step(proj: torch.Tensor, conv: torch.Tensor, a_decay: torch.Tensor,
         raise ValueError("the split output takes a bfloat16 proj")
     if not split and out_dtype not in (None, dtype):
         raise ValueError("out_dtype must be proj's dtype or BF16X2")
-    out = torch.empty((n, 2 * vw if split else vw), dtype=dtype, device=proj.device)
+    out = proj.new_empty(n, 2 * vw if split else vw)
     _call(dev, "delta_step", lib().qdc_delta_step, out.data_ptr(),
           _lib.QDC_BF16X2 if split else code, proj.data_ptr(), code,
           proj.stride(0) if n > 1 else width, conv.data_ptr(), taps, a_decay.data_ptr(),
