@@ -17,6 +17,22 @@ __device__ __forceinline__ void raise_flag(int32_t *error_flag) {
     if (error_flag) atomicOr(error_flag, 1);
 }
 
+// Inclusive prefix sum over each row of 16 lanes, and over the wavefront: lane moves of
+// the vector unit, a few cycles each where a move through LDS takes a hundred.
+__device__ __forceinline__ int row_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 below
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    return v;
+}
+__device__ __forceinline__ int wave_scan(int v) {
+    v = row_scan(v);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row 0 into 1, 2 into 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // rows 0, 1 into 2, 3
+    return v;
+}
+
 // A device range an entry point reads or writes.
 struct Range {
     const void *p;

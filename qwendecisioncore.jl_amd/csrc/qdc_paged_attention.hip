@@ -68,17 +68,6 @@ __device__ __forceinline__ int entry_keys(const PagedAttention &a, int row, int 
     return bad ? (int)reach : pos + 1;
 }
 
-// Inclusive prefix sum over a wavefront.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    const int l = threadIdx.x % kWave;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const uint32_t o = (uint32_t)__shfl_up((int)v, d, kWave);
-        if (l >= d) v += o;
-    }
-    return v;
-}
-
 // What beginning a unit costs, as bytes of pages read in that time: the chain to its page
 // numbers and the join of its wavefronts, which for heads of 256 no second workgroup of
 // the compute unit fills.  (96 rows of 0 .. 16384 keys of 256, us: 32 KB 78, 64 KB 64,
@@ -105,7 +94,7 @@ template <typename T, int HD> struct Line {
         bool bad;
         row = i < a.n ? a.index[i] : -1;
         keys = entry_keys(a, row, i < a.n ? a.positions[i] : -1, bad);
-        end = wave_scan(length(keys));
+        end = (uint32_t)wave_scan((int)length(keys));
         all = __builtin_amdgcn_readlane(end, kWave - 1);
     }
     // the whole line; leaves the first chunk in place

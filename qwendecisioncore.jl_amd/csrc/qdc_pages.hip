@@ -33,25 +33,15 @@ __device__ __forceinline__ int load_past_l1(const int32_t *p) {
 
 // Exclusive prefix sum over the workgroup and the whole; `parts` is LDS scratch.
 __device__ __forceinline__ int block_scan(int v, int *parts, int &all) {
-    const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
-    int inc = v;
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        const int o = __shfl_up(inc, d, kWave);
-        if (l >= d) inc += o;
-    }
+    static_assert(kBookWaves == 16, "a row of lanes");
+    const int l = threadIdx.x % kWave, wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int inc = wave_scan(v);
     __syncthreads();  // the scratch is free
     if (l == kWave - 1) parts[wv] = inc;
     __syncthreads();
-    int before = 0;
-    all = 0;
-#pragma unroll
-    for (int w = 0; w < kBookWaves; ++w) {
-        const int p = parts[w];
-        if (w < wv) before += p;
-        all += p;
-    }
-    return before + inc - v;
+    const int ends = row_scan(parts[l % kBookWaves]);
+    all = __builtin_amdgcn_readlane(ends, kBookWaves - 1);
+    return (wv ? __builtin_amdgcn_readlane(ends, wv - 1) : 0) + inc - v;
 }
 
 // Whether any thread says so, with the sum of v (below 2^31) over all of them.
