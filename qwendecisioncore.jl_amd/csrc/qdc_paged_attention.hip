@@ -4,11 +4,11 @@
 //
 // Every key and value is read once for the (up to 16) query heads that share it, so
 // the reads of the pages are all that it has to cost.  The work is cut by what is
-// there, not by what could be: the keys of all entries, head after head, are one row
-// of tiles (32 keys bf16, 16 fp32) that the workgroups share out evenly, whatever the
-// lengths are.  Each workgroup finds its tiles from the positions by itself; a piece
-// that begins and ends within a head's keys leaves its maximum, sum and unnormalised
-// output in the workspace, and a second launch joins the pieces of a head in order.
+// there, not by what could be: the keys of all entries, head after head, in tiles (32
+// keys bf16, 16 fp32), are dealt to the workgroups in even parts whatever the lengths
+// are.  Each workgroup finds its tiles from the positions by itself; a piece that is not
+// all of a head's keys leaves its maximum, sum and unnormalised output in the workspace,
+// and a second launch joins the pieces of a head in order.
 //
 // Scores are formed transposed, S^T = K Q^T on the matrix cores: a lane then holds
 // the scores of one head for some keys, the operand layout of O^T = V^T P^T, and the
@@ -24,7 +24,7 @@
 // MB, each byte fetched once) 123 us = 6.7 TB/s with its join of 4.6 us behind it, of 7.0
 // that a plain streaming read reaches; 96 rows of 0 .. 16384 keys (333 MB) 56 us = 6.0
 // TB/s.  Where little is read the chain positions -> pages -> K -> scores -> join counts: 8
-// rows of 2048 keys (34 MB) 12.2 + 4.0 us, one row of 411 keys (0.4 MB, in one launch) 8.9.
+// rows of 2048 keys (34 MB) 11.2 + 4.0 us, one row of 411 keys (0.4 MB, in one launch) 8.6.
 #include <cfloat>
 #include <type_traits>
 
@@ -74,19 +74,32 @@ __device__ __forceinline__ int entry_keys(const PagedAttention &a, int row, int 
 // 128 KB 56, 256 KB 57; 200 rows of 1 .. 4000 of 64: 17.9, 17.1, 20.0, 24.6.)
 constexpr int begin_bytes(int head_dim) { return head_dim > 128 ? 131072 : 65536; }
 
-// The work of the call is a line: entry by entry, unit by unit (KV head and group of its
-// query heads), kBegin tiles' worth for beginning a unit and then its tiles.  A
-// wavefront sees 64 entries at a time: lane l holds entry first + l.
+// How the call's work, entry by entry and unit by unit (KV head and group of its query
+// heads), is dealt to the workgroups.  Of up to 64 entries a unit is cut into parts of up
+// to `share` tiles, a workgroup each, where that takes no more than the workgroups and no
+// more rounds of a tile a wavefront than an even split would.  Anything else is a line
+// that is cut evenly: a unit is kBegin tiles' worth for beginning it and then its tiles.
+// (us, shares / line: 8 rows of 2048 keys of 256 11.2 / 12.1, 32 of 1000 16.2 /
+// 17.1.)
+// A wavefront sees 64 entries at a time: lane l holds entry first + l.
 template <typename T, int HD> struct Line {
     static constexpr int TILE = tile_keys<T>();
     static constexpr uint32_t kBegin = begin_bytes(HD) / (TILE * HD * 2 * (int)sizeof(T));
     const PagedAttention &a;
     const uint32_t units;
     int first, row, keys;
-    uint32_t end, before, all;  // this entry's end within the chunk; earlier chunks; this one
+    uint32_t span, end;    // places of a unit of this entry; the entry's end within the chunk
+    uint32_t before, all;  // places of earlier chunks; of this one
+    uint32_t share;        // 0: a line
 
-    __device__ __forceinline__ uint32_t length(int keys) const {
-        return keys ? ((uint32_t)(keys + TILE - 1) / TILE + kBegin) * units : 0u;
+    static __device__ __forceinline__ uint32_t tiles_of(int keys) {
+        return (uint32_t)(keys + TILE - 1) / TILE;
+    }
+    __device__ __forceinline__ void add_up() {
+        const uint32_t tiles = tiles_of(keys);
+        span = share ? (tiles + share - 1) / share : keys ? tiles + kBegin : 0u;
+        end = (uint32_t)wave_scan((int)(span * units));
+        all = __builtin_amdgcn_readlane(end, kWave - 1);
     }
     __device__ __forceinline__ void load(int at) {
         first = at;
@@ -94,15 +107,27 @@ template <typename T, int HD> struct Line {
         bool bad;
         row = i < a.n ? a.index[i] : -1;
         keys = entry_keys(a, row, i < a.n ? a.positions[i] : -1, bad);
-        end = (uint32_t)wave_scan((int)length(keys));
-        all = __builtin_amdgcn_readlane(end, kWave - 1);
     }
-    // the whole line; leaves the first chunk in place
+    // all places of the call; leaves the first chunk in place
     __device__ __forceinline__ uint32_t total() {
         before = 0;
+        if (a.n <= kWave) {
+            load(0);
+            const uint32_t tiles = __builtin_amdgcn_readlane(
+                wave_scan((int)(tiles_of(keys) * units)), kWave - 1);
+            const uint32_t wgs = 1u << a.log_wgs;
+            share = max((tiles + wgs - 1) >> a.log_wgs, kMinTiles);
+            for (const uint32_t most = (share + kWaves - 1) / kWaves * kWaves; share <= most;
+                 ++share) {
+                add_up();
+                if (all <= wgs) return all;
+            }
+        }
+        share = 0;
         uint32_t sum = 0;
         for (int at = (a.n - 1) / kWave * kWave; at >= 0; at -= kWave) {
             load(at);
+            add_up();
             sum += all;
         }
         return sum;
@@ -110,6 +135,7 @@ template <typename T, int HD> struct Line {
     __device__ __forceinline__ void next() {
         before += all;
         load(first + kWave);
+        add_up();
     }
 };
 
@@ -226,7 +252,8 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     const uint32_t off_k = (uint32_t)(lr * HD + L::V * lg) * (uint32_t)sizeof(T);
     const uint32_t off_v = (uint32_t)(4 * lg * HD + L::VD * lr) * (uint32_t)sizeof(T);
     L x;
-    const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
+    const int kvh = a.head_groups == 1 ? unit : unit / a.head_groups;
+    const int hg = unit - kvh * a.head_groups;
     const int head0 = kvh * a.group + hg * kHeads;
     const int gu = min(kHeads, a.group - hg * kHeads);
     const int32_t *pages = a.table + (int64_t)row * a.width;
@@ -462,10 +489,13 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
     constexpr int TILE = tile_keys<T>();
     Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
-    const int lw = log_workers(a.log_wgs, all);
-    if (blockIdx.x >> lw) return;
-    uint32_t t = (uint32_t)(((uint64_t)all * blockIdx.x) >> lw);
-    const uint32_t t_end = (uint32_t)(((uint64_t)all * (blockIdx.x + 1)) >> lw);
+    uint32_t t = blockIdx.x, t_end = t + (t < all);  // with shares a place is a workgroup's
+    if (!line.share) {
+        const int lw = log_workers(a.log_wgs, all);
+        if (blockIdx.x >> lw) return;
+        t = (uint32_t)(((uint64_t)all * blockIdx.x) >> lw);
+        t_end = (uint32_t)(((uint64_t)all * (blockIdx.x + 1)) >> lw);
+    }
     while (t < t_end) {
         while (line.before + line.all <= t && line.first + kWave < a.n) line.next();
         // the entry and unit that hold place t, and the tiles of it up to t_end
@@ -474,13 +504,22 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
         const int el = __builtin_ctzll(past);
         const int keys = __builtin_amdgcn_readlane(line.keys, el);
         const int row = __builtin_amdgcn_readlane(line.row, el);
-        const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE, span = tiles + line.kBegin;
+        const uint32_t tiles = line.tiles_of(keys);
+        const uint32_t span = __builtin_amdgcn_readlane(line.span, el);
         const uint32_t rel = t - (line.before + __builtin_amdgcn_readlane(line.end, el) -
-                                  line.length(keys));
+                                  span * line.units);
         const uint32_t unit = rel / span, p0 = rel - unit * span, p1 = min(span, p0 + (t_end - t));
+        uint32_t j0, j1;
         t += p1 - p0;
-        if (p1 <= line.kBegin) continue;
-        const uint32_t j0 = p0 > line.kBegin ? p0 - line.kBegin : 0, j1 = p1 - line.kBegin;
+        if (line.share) {  // part p0 of span
+            const uint32_t each = tiles / span, more = tiles - each * span;
+            j0 = p0 * each + min(p0, more);
+            j1 = j0 + each + (p0 < more);
+        } else {
+            if (p1 <= line.kBegin) continue;
+            j0 = p0 > line.kBegin ? p0 - line.kBegin : 0;
+            j1 = p1 - line.kBegin;
+        }
         attend<T, HD, kWaves>(a, line.first + el, row, keys, (int)unit, (int)j0, (int)j1,
                               j0 == 0 && j1 == tiles, 2 * (int64_t)blockIdx.x + (j0 == 0));
     }
@@ -507,11 +546,13 @@ __global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short
 }
 
 // A workgroup per (entry, head): the pieces of its keys, in order; zeros for an entry
-// without keys; nothing where one workgroup had them all.
-template <typename T, int HD>
-__global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a) {
+// without keys; nothing where one workgroup had them all.  (us, 256 / 512 threads: 128
+// pieces a head 6.7 / 5.5, 32 5.0 / 4.9, few pieces of 200 x 8 heads 6.2 / 9.2.)
+constexpr int64_t kManyPieces = 64;
+template <typename T, int HD, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_attention_join(PagedAttention a) {
     constexpr int TILE = tile_keys<T>();
-    constexpr int LPP = HD / 4, PARTS = kBlock / LPP;  // lanes of a piece's row, rows at a time
+    constexpr int LPP = HD / 4, PARTS = THREADS / LPP;  // lanes of a piece's row, rows at a time
     __shared__ float top_of[PARTS], sum_of[PARTS];
     __shared__ __align__(16) float so[PARTS][HD];
     const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
@@ -535,14 +576,20 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join(PagedAttention a)
         if (wv == 0) store_zero<T, HD, HD / kWave>(a, entry, h, dim);
         return;
     }
-    const int lw = log_workers(a.log_wgs, all);
-    const uint32_t first = line.before + __builtin_amdgcn_readlane(line.end, entry - line.first) -
-                           line.length(keys) + line.kBegin +
-                           (uint32_t)(kvh * a.head_groups + hg) * (tiles + line.kBegin);
-    // the workgroups that hold its first and its last tile: that of place t is the last
-    // with all * w / 2^lw <= t
-    const uint32_t w0 = (uint32_t)((((uint64_t)(first + 1) << lw) - 1) / all);
-    const uint32_t w1 = (uint32_t)((((uint64_t)(first + tiles) << lw) - 1) / all);
+    const uint32_t unit = (uint32_t)(kvh * a.head_groups + hg);
+    const uint32_t span = __builtin_amdgcn_readlane(line.span, entry - line.first);
+    const uint32_t start = line.before + __builtin_amdgcn_readlane(line.end, entry - line.first) -
+                           span * line.units + unit * span;
+    uint32_t w0, w1;  // the workgroups that hold its first and its last tile
+    if (line.share) {
+        w0 = start;
+        w1 = start + span - 1;
+    } else {  // that of place t is the last with all * w / 2^lw <= t
+        const int lw = log_workers(a.log_wgs, all);
+        const uint32_t first = start + line.kBegin;
+        w0 = (uint32_t)((((uint64_t)(first + 1) << lw) - 1) / all);
+        w1 = (uint32_t)((((uint64_t)(first + tiles) << lw) - 1) / all);
+    }
     if (w0 == w1) return;
     const int parts = (int)(w1 - w0) + 1;
     auto slot = [&](int p) {
@@ -719,6 +766,7 @@ extern "C" int32_t qdc_paged_attention(
     const bool brief = need == 0;
     const dim3 grid(brief ? (uint32_t)(n * kv_heads * a.head_groups) : 1u << a.log_wgs);
     const dim3 join((uint32_t)(n * heads)), block(kBlock);
+    const bool many = kManyPieces * n * kv_heads * a.head_groups <= grid.x;
     a.pieces = reinterpret_cast<float *>(workspace);
     a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;
 #define QDC_PAGED(T, HD)                                                                       \
@@ -731,7 +779,12 @@ extern "C" int32_t qdc_paged_attention(
         hipLaunchKernelGGL((paged_attention<T, HD>), grid, block, 0, stream, a);               \
         const int32_t status = launch_status();                                                \
         if (status != QDC_OK) return status;                                                   \
-        hipLaunchKernelGGL((paged_attention_join<T, HD>), join, block, 0, stream, a);          \
+        if (many)                                                                              \
+            hipLaunchKernelGGL((paged_attention_join<T, HD, 2 * kBlock>), join,                \
+                               dim3(2 * kBlock), 0, stream, a);                                \
+        else                                                                                   \
+            hipLaunchKernelGGL((paged_attention_join<T, HD, kBlock>), join, block, 0, stream,  \
+                               a);                                                             \
         return launch_status();                                                                \
     }
     if (dtype == QDC_BF16) {

@@ -452,6 +452,20 @@ def test_paged_attention_long(H, KV, hd, lengths, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,lengths", [
+    (8, 2, 256, [1000] * 8),                # an even share each, the last tile not full
+    (4, 2, 64, [700] * 64), (4, 2, 64, [700] * 65),   # as many as a wavefront sees, one more
+    (16, 16, 64, [20 + i for i in range(60)] + [2500]),  # more units than workgroups
+    (40, 2, 64, [1500, 0, 1, 1033]),        # two groups of heads a KV head, one not full
+    (8, 2, 256, [16001])])                  # many pieces of one row
+def test_paged_attention_dealt(H, KV, hd, lengths, dtype):
+    """Keys that go to the workgroups in even shares and as one line."""
+    case = attend_case(len(lengths) + hd, H, KV, hd, 16, lengths, dtype)
+    assert attend_check(case, np.array(lengths) - 1, 16, dtype, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_attention_rising_scores(dtype):
     """Scores that rise along the keys by hundreds, so that begun sums are rescaled,
     and a last key far below: its weight is nothing."""
