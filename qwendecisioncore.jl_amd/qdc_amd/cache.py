@@ -5,11 +5,13 @@ keeps what the next token needs -- keys and values in pages, the states and
 convolution inputs of the linear attention layers -- so that a prompt is run once
 (:meth:`~BackboneCache.prefill`), then continued (:meth:`~BackboneCache.step`) and
 branched into candidate continuations that share its pages
-(:meth:`~BackboneCache.fork`).  The layers run as in :mod:`qdc_amd.backbone`, with the
+(:meth:`~BackboneCache.fork`).  :class:`graphs.StepGraphs` serves steps from recorded
+HIP graphs.  The layers run as in :mod:`qdc_amd.backbone`, with the
 operators of :mod:`qdc_amd.cache_ops` for what the cache holds.
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import threading
 
@@ -24,7 +26,7 @@ def _call(method):
     """A call of the cache: alone, on the model's device, without gradients."""
     @functools.wraps(method)
     def call(self, *args, **kwargs):
-        with self._lock, torch.cuda.device(self.model.device), torch.no_grad():
+        with self._alone():
             return method(self, *args, **kwargs)
     return call
 
@@ -135,21 +137,7 @@ class BackboneCache:
     def step(self, rows, ids) -> np.ndarray:
         """One more token for each of ``rows`` (distinct rows in use): the
         final-normalised hidden states after it, ``[n, hidden]`` fp32."""
-        rows = self._in_use(rows)
-        ids = np.asarray(ids, np.int64).reshape(-1)
-        if ids.size != len(rows) or not rows:
-            raise ValueError("One token ID for each row is required.")
-        ops.check_ids(ids, self.model.vocab)
-        if any(self._lengths[r] >= self.max_tokens for r in rows):
-            raise ValueError(f"A sequence holds at most {self.max_tokens} tokens.")
-        d_rows, d_ids = self._ints(np.asarray(rows), ids)
-        try:
-            at = cache_ops.extend_pages(self.book, d_rows, error_flag=self._flag)
-            out = _host(self._token(d_ids, d_rows, at))
-        except Exception:
-            self._abandon(rows, d_rows)
-            raise
-        return self._finish(out, [], None, {r: self._lengths[r] + 1 for r in rows})
+        return self._step(*self._check_step(rows, ids))
 
     @_call
     def fork(self, rows) -> list:
@@ -185,6 +173,39 @@ class BackboneCache:
         cache_ops.compact_pages(self.book, self._pool())
 
     # --------------------------------------------------------- bookkeeping --
+    @contextlib.contextmanager
+    def _alone(self):
+        """One call at a time, on the model's device, without gradients."""
+        with self._lock, torch.cuda.device(self.model.device), torch.no_grad():
+            yield
+
+    def _check_step(self, rows, ids):
+        rows = self._in_use(rows)
+        ids = np.asarray(ids, np.int64).reshape(-1)
+        if ids.size != len(rows) or not rows:
+            raise ValueError("One token ID for each row is required.")
+        ops.check_ids(ids, self.model.vocab)
+        if any(self._lengths[r] >= self.max_tokens for r in rows):
+            raise ValueError(f"A sequence holds at most {self.max_tokens} tokens.")
+        return rows, ids
+
+    def _step(self, rows, ids) -> np.ndarray:
+        d_rows, d_ids = self._ints(np.asarray(rows), ids)
+        try:
+            out = _host(self._advance(d_rows, d_ids))
+        except Exception:
+            self._abandon(rows, d_rows)
+            raise
+        return self._stepped(out, rows)
+
+    def _advance(self, rows, ids):
+        """One more token of each row; an entry with row -1 is none."""
+        at = cache_ops.extend_pages(self.book, rows, error_flag=self._flag)
+        return self._token(ids, rows, at)
+
+    def _stepped(self, out, rows, flagged=None) -> np.ndarray:
+        return self._finish(out, [], None, {r: self._lengths[r] + 1 for r in rows}, flagged)
+
     def _heads(self) -> bool:
         return self.pool.shape[0] > 0
 
@@ -227,9 +248,9 @@ class BackboneCache:
         dev = torch.from_numpy(packed).to(self.model.device)
         return tuple(dev[end - -(-a.size // 4) * 4:][:a.size] for a, end in zip(flat, ends))
 
-    def _finish(self, out, taken, result, lengths):
+    def _finish(self, out, taken, result, lengths, flagged=None):
         """Waits for the call, and takes it back if a kernel flagged it."""
-        if int(self._flag.item()) != 0:
+        if int(self._flag.item() if flagged is None else flagged) != 0:
             self._flag.zero_()
             self._unused += taken[::-1]
             raise RuntimeError("Too few free pages.")

@@ -1,5 +1,5 @@
 """HIP-graph replay of the last-token forward, for a decision model that scores
-one prompt after another.
+one prompt after another, and of a cache's step.
 
 A short single sequence is launch-bound: one forward of a 4-layer hybrid model
 is ~48 kernel launches of a few microseconds each, and the host work of
@@ -15,6 +15,10 @@ Each key is recorded with both of torch's GEMM libraries on ROCm and the
 recording that replays faster is kept: at a few hundred tokens the products
 are small, and the library whose kernels are tiled for large problems can
 leave most of the chip idle.
+
+:class:`StepGraphs` does the same for :meth:`cache.BackboneCache.step`, one recording for
+each number of rows: which page is whose is kept on the device, so the same launches
+serve any rows at any positions.
 
 Every captured graph is inspected before first use: a graph holding a memset
 node is dropped and its key served eagerly, since memset nodes in replayed
@@ -89,18 +93,10 @@ def node_types(graph: int) -> list:
     return types
 
 
-class _Entry:
-    """One recorded forward: static inputs, the graph, its output and a pinned
-    host copy of it."""
+class _Recording:
+    """A graph with the output it writes."""
 
-    def __init__(self, model: bb.QwenBackbone, seq_len: int, masked: bool):
-        dev = model.device
-        self.ids = torch.zeros((1, seq_len), dtype=torch.int32, device=dev)
-        self.mask = torch.ones((1, seq_len), dtype=torch.int32, device=dev) if masked else None
-        self.ids_host = torch.zeros((1, seq_len), dtype=torch.int32, pin_memory=True)
-        self.mask_host = (torch.ones((1, seq_len), dtype=torch.int32, pin_memory=True)
-                          if masked else None)
-        self.out_host = torch.empty(model.cfg.hidden, dtype=torch.float32, pin_memory=True)
+    def __init__(self):
         self.graph = None
         self.out = None
         self.nodes = []
@@ -108,7 +104,126 @@ class _Entry:
         self.replay_ms = None   # its measured replay time
 
 
-class LastHiddenGraphs:
+class _Entry(_Recording):
+    """One recorded forward: static inputs, the graph, its output and a pinned
+    host copy of it."""
+
+    def __init__(self, model: bb.QwenBackbone, seq_len: int, masked: bool):
+        super().__init__()
+        dev = model.device
+        self.ids = torch.zeros((1, seq_len), dtype=torch.int32, device=dev)
+        self.mask = torch.ones((1, seq_len), dtype=torch.int32, device=dev) if masked else None
+        self.ids_host = torch.zeros((1, seq_len), dtype=torch.int32, pin_memory=True)
+        self.mask_host = (torch.ones((1, seq_len), dtype=torch.int32, pin_memory=True)
+                          if masked else None)
+        self.out_host = torch.empty(model.cfg.hidden, dtype=torch.float32, pin_memory=True)
+
+
+class _StepEntry(_Recording):
+    """One recorded step of ``n`` rows: the row numbers and, from a multiple of 16 bytes
+    on, the token ids, as one static device vector with its pinned host copy; what the
+    recording runs itself is steps of no token (rows -1), which leave a cache as it is."""
+
+    def __init__(self, cache, n: int):
+        super().__init__()
+        ids = -(-n // 4) * 4
+        self.host = torch.zeros(ids + n, dtype=torch.int32, pin_memory=True)
+        self.host[:n] = -1
+        self.inputs = self.host.to(cache.model.device)
+        self.rows, self.ids = self.inputs[:n], self.inputs[ids:]
+        self.rows_host, self.ids_host = self.host[:n].numpy(), self.host[ids:].numpy()
+        self.out_host = torch.empty((n, cache.model.cfg.hidden), dtype=torch.float32,
+                                    pin_memory=True)
+        self.flag_host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+
+
+class _Recordings:
+    """Recorded forwards of a model by key: recorded on first use with each of
+    ``gemm_libraries``, the fastest kept, least recently used first out."""
+
+    def __init__(self, model: bb.QwenBackbone, max_graphs: int, gemm_libraries, trials: int):
+        if max_graphs < 1:
+            raise ValueError("max_graphs must be at least 1.")
+        if trials < 1:
+            raise ValueError("trials must be at least 1.")
+        self.model = model
+        self.max_graphs = max_graphs
+        self.gemm_libraries = tuple(gemm_libraries) if gemm_libraries else None
+        self.trials = trials
+        self._entries: OrderedDict = OrderedDict()
+        self.eager_keys: set = set()
+        self._lock = threading.Lock()
+        self._stream = None   # the recording stream, made at the first recording
+
+    def _record_one(self, *key) -> _Recording:
+        e = self._new(*key)
+        if self._stream is None:
+            self._stream = torch.cuda.Stream(device=self.model.device)
+        cur = torch.cuda.current_stream(self.model.device)
+        self._stream.wait_stream(cur)
+        with torch.cuda.stream(self._stream):
+            for _ in range(2):    # library handles, RoPE tables and workspaces first
+                self._forward(e)
+        cur.wait_stream(self._stream)
+        torch.cuda.synchronize(self.model.device)
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph, stream=self._stream):
+            e.out = self._forward(e)
+        e.nodes = node_types(graph.raw_cuda_graph())
+        graph.instantiate()
+        e.graph = graph
+        return e
+
+    def _replay_ms(self, e: _Recording) -> float:
+        stream = torch.cuda.current_stream(self.model.device)
+        e.graph.replay()                       # first replay: uploads the graph
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record(stream)
+        for _ in range(self.trials):
+            e.graph.replay()
+        end.record(stream)
+        end.synchronize()
+        return start.elapsed_time(end) / self.trials
+
+    def _record(self, *key):
+        """The fastest usable recording of this key over the GEMM libraries, or
+        None when every recording holds a memset node."""
+        backends = torch.backends.cuda
+        previous = backends.preferred_blas_library()
+        best = None
+        try:
+            with torch.cuda.device(self.model.device):
+                for library in self.gemm_libraries or (previous,):
+                    backends.preferred_blas_library(library)
+                    e = self._record_one(*key)
+                    if MEMSET_NODE in e.nodes:
+                        continue
+                    e.library = str(library)
+                    e.replay_ms = self._replay_ms(e)
+                    if best is None or e.replay_ms < best.replay_ms:
+                        best = e
+        finally:
+            backends.preferred_blas_library(previous)
+        return best
+
+    def _entry(self, *key):
+        """The recording for this key (made now if needed), None where it is served
+        eagerly."""
+        if key in self.eager_keys:
+            return None
+        e = self._entries.get(key)
+        if e is None:
+            e = self._record(*key)
+            if e is None:
+                self.eager_keys.add(key)
+                return None
+            self._entries[key] = e
+            while len(self._entries) > self.max_graphs:
+                self._entries.popitem(last=False)
+        self._entries.move_to_end(key)
+        return e
+
+class LastHiddenGraphs(_Recordings):
     """``backbone_last_hidden`` served from recorded HIP graphs.
 
     ``graphs(ids, mask)`` returns what ``backbone.backbone_last_hidden(model,
@@ -134,90 +249,18 @@ class LastHiddenGraphs:
 
     def __init__(self, model: bb.QwenBackbone, max_graphs: int = 8,
                  gemm_libraries=("cublaslt", "cublas"), trials: int = 5):
-        if max_graphs < 1:
-            raise ValueError("max_graphs must be at least 1.")
-        if trials < 1:
-            raise ValueError("trials must be at least 1.")
-        self.model = model
-        self.max_graphs = max_graphs
-        self.gemm_libraries = tuple(gemm_libraries) if gemm_libraries else None
-        self.trials = trials
-        self._entries: OrderedDict = OrderedDict()
-        self.eager_keys: set = set()
-        self._lock = threading.Lock()
-        self._stream = None   # the recording stream, made at the first recording
+        super().__init__(model, max_graphs, gemm_libraries, trials)
 
     def _forward(self, e: _Entry) -> torch.Tensor:
         return self.model.forward(e.ids, e.mask, last_only=True)[0]
 
-    def _record_one(self, seq_len: int, masked: bool) -> _Entry:
-        e = _Entry(self.model, seq_len, masked)
-        if self._stream is None:
-            self._stream = torch.cuda.Stream(device=self.model.device)
-        cur = torch.cuda.current_stream(self.model.device)
-        self._stream.wait_stream(cur)
-        with torch.cuda.stream(self._stream):
-            for _ in range(2):    # library handles, RoPE tables and workspaces first
-                self._forward(e)
-        cur.wait_stream(self._stream)
-        torch.cuda.synchronize(self.model.device)
-        graph = torch.cuda.CUDAGraph(keep_graph=True)
-        with torch.cuda.graph(graph, stream=self._stream):
-            e.out = self._forward(e)
-        e.nodes = node_types(graph.raw_cuda_graph())
-        graph.instantiate()
-        e.graph = graph
-        return e
-
-    def _replay_ms(self, e: _Entry) -> float:
-        stream = torch.cuda.current_stream(self.model.device)
-        e.graph.replay()                       # first replay: uploads the graph
-        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        start.record(stream)
-        for _ in range(self.trials):
-            e.graph.replay()
-        end.record(stream)
-        end.synchronize()
-        return start.elapsed_time(end) / self.trials
-
-    def _record(self, seq_len: int, masked: bool):
-        """The fastest usable recording of this key over the GEMM libraries, or
-        None when every recording holds a memset node."""
-        backends = torch.backends.cuda
-        previous = backends.preferred_blas_library()
-        best = None
-        try:
-            with torch.cuda.device(self.model.device):
-                for library in self.gemm_libraries or (previous,):
-                    backends.preferred_blas_library(library)
-                    e = self._record_one(seq_len, masked)
-                    if MEMSET_NODE in e.nodes:
-                        continue
-                    e.library = str(library)
-                    e.replay_ms = self._replay_ms(e)
-                    if best is None or e.replay_ms < best.replay_ms:
-                        best = e
-        finally:
-            backends.preferred_blas_library(previous)
-        return best
+    def _new(self, seq_len: int, masked: bool) -> _Entry:
+        return _Entry(self.model, seq_len, masked)
 
     def entry(self, seq_len: int, masked: bool):
         """The recorded forward for this key (recording it now if needed), or
         None when the key is served eagerly."""
-        key = (seq_len, masked)
-        if key in self.eager_keys:
-            return None
-        e = self._entries.get(key)
-        if e is None:
-            e = self._record(seq_len, masked)
-            if e is None:
-                self.eager_keys.add(key)
-                return None
-            self._entries[key] = e
-            while len(self._entries) > self.max_graphs:
-                self._entries.popitem(last=False)
-        self._entries.move_to_end(key)
-        return e
+        return self._entry(seq_len, masked)
 
     def __call__(self, ids, mask) -> np.ndarray:
         ids, mask = bb._host_sequence(self.model, ids, mask)
@@ -237,3 +280,45 @@ class LastHiddenGraphs:
                 e.out_host.copy_(e.out.float(), non_blocking=True)
                 stream.synchronize()
                 return e.out_host.numpy().copy()
+
+
+class StepGraphs(_Recordings):
+    """``cache.step`` of a :class:`cache.BackboneCache` served from recorded HIP graphs.
+
+    ``graphs(rows, ids)`` does what ``cache.step(rows, ids)`` does, with the same checks
+    and errors, and may take turns with it and with the cache's other calls.  One graph
+    for each number of rows is recorded on first use and kept, least recently used first
+    out beyond ``max_graphs``; the GEMMs are recorded, and results compare with the eager
+    step's, as for :class:`LastHiddenGraphs`.  The cache's lock makes it one call at a
+    time for the cache."""
+
+    def __init__(self, cache, max_graphs: int = 8, gemm_libraries=("cublaslt", "cublas"),
+                 trials: int = 5):
+        super().__init__(cache.model, max_graphs, gemm_libraries, trials)
+        self.cache = cache
+
+    def _new(self, n: int) -> _StepEntry:
+        return _StepEntry(self.cache, n)
+
+    def _forward(self, e: _StepEntry) -> torch.Tensor:
+        return self.cache._advance(e.rows, e.ids)
+
+    def __call__(self, rows, ids) -> np.ndarray:
+        cache = self.cache
+        with cache._alone():
+            rows, ids = cache._check_step(rows, ids)
+            e = self._entry(len(rows))
+            if e is None:
+                return cache._step(rows, ids)
+            e.rows_host[:] = rows
+            e.ids_host[:] = ids
+            try:
+                e.inputs.copy_(e.host, non_blocking=True)
+                e.graph.replay()
+                e.out_host.copy_(e.out.float(), non_blocking=True)
+                e.flag_host.copy_(cache._flag, non_blocking=True)
+                torch.cuda.current_stream(self.model.device).synchronize()
+            except Exception:
+                cache._abandon(rows, *cache._ints(np.asarray(rows)))
+                raise
+            return cache._stepped(e.out_host.numpy().copy(), rows, int(e.flag_host[0]))

@@ -175,6 +175,72 @@ def test_a_call_that_raises_leaves_no_flag_and_no_rows(monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["f32", "mlp"])
+def test_step_graphs(mode):
+    """Recorded steps beside eager ones of a second cache: the same bits with the same
+    GEMM library, over page borders, forks, a move, other row counts and eager steps
+    between, and too few pages raise and leave everything."""
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.graphs import StepGraphs
+    model = model_of(mode)
+    new = lambda: BackboneCache(model, rows=6, pages=13, page_size=16)  # noqa: E731
+    cache, twin = new(), new()
+    graphs = StepGraphs(cache, max_graphs=2, gemm_libraries=None)
+    rng = np.random.default_rng(8)
+    ids = rng.integers(0, model.vocab, (2, 30))
+    (a, b), _ = cache.prefill(ids)
+    assert twin.prefill(ids)[0] == [a, b]
+    held = {a: ids[0].tolist(), b: ids[1].tolist()}
+
+    def step(rows, eager=False):
+        tokens = rng.integers(0, model.vocab, len(rows))
+        got = (cache.step if eager else graphs)(rows, tokens)
+        assert np.array_equal(got, twin.step(rows, tokens))
+        for r, t in zip(rows, tokens):
+            held[r].append(int(t))
+        assert cache.lengths() == twin.lengths() == {r: len(t) for r, t in held.items()}
+        return got
+
+    for i in range(4):
+        got = step([b, a], eager=i == 2)                  # 32 and on: another page each
+    for r, g in zip((b, a), got):
+        assert normwise(g, whole(model, held[r])) <= BARS[mode]
+    kids = cache.fork([a, b])
+    assert twin.fork([a, b]) == kids
+    held.update({k: list(held[p]) for k, p in zip(kids, (a, b))})
+    for _ in range(3):
+        step(kids + [a, b])
+    step([a])                                             # a third key: the first is dropped
+    assert list(graphs._entries) == [(4,), (1,)] and not graphs.eager_keys
+    cache.free([b]), twin.free([b])
+    del held[b]
+    cache.compact()
+    for _ in range(2):
+        got = step([kids[1], a])
+    assert normwise(got[0], whole(model, held[kids[1]])) <= BARS[mode]
+    for c in (cache, twin):                               # the pages that are left
+        c.prefill(np.ones(16 * c.free_page_count()))
+    full, = set(cache.lengths()) - set(held)
+    held[full] = [1] * cache.lengths()[full]
+    before = cache.lengths()
+    for call in (graphs, cache.step):
+        with pytest.raises(RuntimeError):
+            call([full, a], [1, 2])
+        assert cache.lengths() == before
+    step([a])
+    for bad in (lambda: graphs([a], [model.vocab]), lambda: graphs([a, a], [1, 2]),
+                lambda: graphs([5], [1]), lambda: graphs([], [])):
+        with pytest.raises(ValueError):
+            bad()
+    both = StepGraphs(cache, trials=2)                    # the faster of the two libraries
+    got = both([a], [3])
+    held[a].append(3)
+    assert normwise(got[0], whole(model, held[a])) <= BARS[mode]
+    with pytest.raises(ValueError):
+        StepGraphs(cache, max_graphs=0)
+
+
+@pytest.mark.gpu
 def test_refusals():
     import dataclasses
 
