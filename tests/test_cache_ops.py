@@ -1030,6 +1030,60 @@ def test_captured_step():
 
 
 @pytest.mark.gpu
+def test_two_captured_graphs():
+    """Two caches' graphs that end, fork, move and continue rows through workspaces of
+    their own, replayed in turn, with eager work between."""
+    H, KV, hd, page, width, pages = 8, 2, 256, 64, 12, 60
+    parents, children, rows = ints([0, 1, 2]), ints([3, 4, 5]), ints(range(6))
+
+    def inputs(seed):
+        rng = np.random.default_rng(seed)
+        t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32)).bfloat16().to(DEV)  # noqa: E731
+        book = cache_ops.page_table(6, width, pages, page, DEV)
+        cache_ops.extend_pages(book, parents, ints([300, 511, 70 + seed]))
+        return dict(q=t(6, H, hd), k=t(6, KV, hd), v=t(6, KV, hd), gate=t(6, H, hd),
+                    norm=t(hd) * 0.1, pool=t(2, pages, KV, page, hd), book=book, rows=rows,
+                    tables=ops.rope_tables(width * page, 16, 1e4, DEV), flag=flag())
+
+    def cycle(s):
+        cache_ops.free_pages(s["book"], children, error_flag=s["flag"])
+        cache_ops.fork_pages(s["book"], parents, children, s["pool"], error_flag=s["flag"])
+        cache_ops.compact_pages(s["book"], s["pool"])
+        cache_ops.copy_pages(s["pool"], ints_50, ints_51, error_flag=s["flag"])
+        return decode_step(s)
+
+    ints_50, ints_51 = ints([0, -1, 7]), ints([51, 3, 52])     # pages beyond those in use
+    lib = cache_ops.lib()
+    assert lib.qdc_pages_fork_workspace(3, page, 2, KV, 2 * hd) > 0
+    assert lib.qdc_paged_attention_workspace(6, H, KV, hd, width, page, BF16) > 0
+    twins, held = [inputs(0), inputs(1)], [inputs(0), inputs(1)]
+    stream = torch.cuda.Stream()
+    graphs, outs, eager = [], [], []
+    with torch.cuda.stream(stream):
+        for h, w in zip(held, twins):
+            cycle(h)
+            eager.append(cycle(w))
+    torch.cuda.synchronize()
+    for h in held:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(cycle(h))
+        graphs.append(graph)
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+        got = [o.clone() for o in outs]
+        torch.cuda.synchronize()
+        for g, h, w in zip(got, held, twins):
+            assert torch.equal(g, cycle(w)) and torch.isfinite(g).all()
+            for x, y in zip(h["book"][:4], w["book"][:4]):
+                assert torch.equal(x, y)
+            assert torch.equal(h["pool"], w["pool"])
+            assert h["flag"].item() == w["flag"].item() == 0
+    assert not torch.equal(got[0], got[1])
+
+
+@pytest.mark.gpu
 def test_other_stream_and_same_results():
     """On a side stream the kernels wait for that stream's work alone, and two runs give
     the same bits."""
@@ -1045,6 +1099,25 @@ def test_other_stream_and_same_results():
         got = decode_step(s)
     torch.cuda.current_stream().wait_stream(stream)
     assert torch.equal(want, got)
+
+
+@pytest.mark.gpu
+def test_two_threads():
+    """Two host threads, each with a stream and a cache of its own."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    def steps(seed):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            s = decode_inputs(seed)
+            out = [decode_step(s) for _ in range(30)]
+        stream.synchronize()
+        return torch.stack(out)
+
+    want = [steps(3), steps(4)]
+    with ThreadPoolExecutor(2) as pool:
+        got = list(pool.map(steps, (3, 4)))
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
 @pytest.mark.gpu
