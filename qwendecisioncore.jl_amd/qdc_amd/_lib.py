@@ -2,7 +2,8 @@
 
 The library is loaded from ``qwendecisioncore.jl_amd/lib/`` (built in-tree by
 ``make -C qwendecisioncore.jl_amd/csrc``).  There is no fallback: a missing
-library is an error.  Status codes map to exceptions the way the reference maps
+library is an error.  ``lib/qdc_calls.so``, built with it, calls the cache's operators
+for PyTorch tensors.  Status codes map to exceptions the way the reference maps
 bad input to ``ArgumentError`` / ``DimensionMismatch``: a negative status raises
 ``ValueError`` (argument error found on the host before any launch), a positive
 one ``RuntimeError`` (HIP launch failure).
@@ -10,10 +11,13 @@ one ``RuntimeError`` (HIP launch failure).
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libqdc_hip.so")
+CALLS_PATH = os.path.join(os.path.dirname(_HERE), "lib", "qdc_calls.so")
 
 QDC_F32 = 0
 QDC_BF16 = 1
@@ -122,6 +126,27 @@ def lib():
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_calls = None
+
+
+def calls():
+    """The module ``qdc_calls`` (loads it, and the library that it calls, on first use)."""
+    global _calls
+    if _calls is None:
+        import torch  # noqa: F401  (the module's symbols)
+        lib()
+        if not os.path.exists(CALLS_PATH):
+            raise RuntimeError(f"{CALLS_PATH} is not built; run `make -C "
+                               "qwendecisioncore.jl_amd/csrc` or __graft_entry__.build()")
+        loader = importlib.machinery.ExtensionFileLoader("qdc_calls", CALLS_PATH)
+        module = importlib.util.module_from_spec(
+            importlib.util.spec_from_file_location("qdc_calls", CALLS_PATH, loader=loader))
+        loader.exec_module(module)
+        module.on_failure(check)
+        _calls = module
+    return _calls
 
 
 def status_string(status: int) -> str:

@@ -26,13 +26,10 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._lib import check, lib
-from .ops import _DTYPES, _device, _is_split
+from ._lib import calls
+from .ops import _DTYPES, _is_split
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
-_I32, _F32 = torch.int32, torch.float32
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class PageTable(NamedTuple):
@@ -60,99 +57,9 @@ def page_table(rows: int, width: int, pages: int, page_size: int, device) -> Pag
                      torch.zeros(pages, **i32), free, page_size)
 
 
-# The host's part of a call is the whole cost of a small one, so each check below is one
-# expression of plain attributes (a device as its index, get_device, in 0.04 us where
-# comparing device objects takes 0.12; new_empty of sizes in 1.0 where empty takes 1.7).
-def _call(dev: int, name: str, fn, *args) -> None:
-    """``fn(*args, stream)`` on device ``dev``, made the current one for the launch if it
-    is not."""
-    if _current_device() == dev:
-        status = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev))
-    if status:
-        check(status, name)
-
-
-def _on(t: torch.Tensor) -> int:
-    """The index of a call's device, that of its first tensor."""
-    dev = t.get_device()
-    if dev < 0:
-        _device(t)
-    return dev
-
-
-def _ints(t: torch.Tensor, dev: int, name: str, n: int) -> int:
-    """Pointer of a contiguous int32 vector of ``n`` entries (-1: any number)."""
-    shape = t.shape
-    if t.dtype is not _I32 or len(shape) != 1 or (n >= 0 and shape[0] != n) \
-            or t.get_device() != dev or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 vector"
-                         + (f" of {n} entries" if n >= 0 else "") + " on the call's device")
-    return t.data_ptr()
-
-
-def _flag(error_flag: torch.Tensor | None, dev: int) -> int:
-    if error_flag is None:
-        return 0
-    if error_flag.get_device() != dev or error_flag.dtype is not _I32 or error_flag.numel() < 1:
-        raise ValueError("error_flag must be an int32 tensor on the call's device")
-    return error_flag.data_ptr()
-
-
-def _table(table: torch.Tensor, dev: int) -> tuple:
-    shape = table.shape
-    if table.dtype is not _I32 or len(shape) != 2 or table.get_device() != dev \
-            or not table.is_contiguous():
-        raise ValueError("table must be a contiguous int32 [rows, width] tensor on the call's "
-                         "device")
-    return shape
-
-
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, like: torch.Tensor, dev: int):
-    """Shape of a layer's page tensors."""
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype is not like.dtype \
-            or v_pages.dtype is not like.dtype or k_pages.get_device() != dev \
-            or v_pages.get_device() != dev or not k_pages.is_contiguous() \
-            or not v_pages.is_contiguous():
-        raise ValueError("k_pages and v_pages must be contiguous [pages, kv_heads, page_size, "
-                         "head_dim] tensors of q's dtype and device")
-    return shape
-
-
-def _rows(t: torch.Tensor, like: torch.Tensor, dev: int, name: str):
-    """Shape and (token, head) strides of a ``[n, heads, head_dim]`` view."""
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 3 or strides[2] != 1 or t.dtype is not like.dtype or t.get_device() != dev:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim] with contiguous rows, of q's "
-                         "dtype and device")
-    return shape, (strides[0] if shape[0] > 1 else shape[1] * shape[2],
-                   strides[1] if shape[1] > 1 else shape[2])
-
-
-def _rope(tables, rotary_dim: int, dev: int) -> tuple:
-    """(cos pointer, sin pointer, length) of the rotation tables."""
-    if not rotary_dim:
-        return 0, 0, 0
-    if tables is None or len(tables) != 2:
-        raise ValueError("rotation needs the (cos, sin) tables of rope_tables")
-    cos, sin = tables
-    shape = cos.shape
-    if len(shape) != 2 or shape[1] != rotary_dim // 2 or sin.shape != shape \
-            or cos.dtype is not _F32 or sin.dtype is not _F32 or cos.get_device() != dev \
-            or sin.get_device() != dev or not cos.is_contiguous() or not sin.is_contiguous():
-        raise ValueError("cos and sin must be contiguous float32 [n_pos, rotary_dim//2] tables of "
-                         "one shape on the call's device")
-    return cos.data_ptr(), sin.data_ptr(), shape[0]
-
-
-def _code(t: torch.Tensor) -> int:
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise ValueError(f"unsupported dtype {t.dtype}; expected float32 or bfloat16")
-    return code
+# The host's part of a call is the whole cost of a small one, so the tensors are checked and
+# the entry points called by a compiled module, csrc/qdc_calls.cpp (5 to 7 us a call less
+# than the same in Python).
 
 
 # --------------------------------------------------------------- attention ---
@@ -171,39 +78,9 @@ def prepare_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: tor
     and not stored; the same, with ``error_flag`` set, for one whose position is beyond
     the rotation tables or the row's pages.  Of two tokens at one position of one row,
     either may be stored, or pieces of both.  head_dim 64, 128 or 256."""
-    dev, code = _on(q), _code(q)
-    (T, H, hd), q_strides = _rows(q, q, dev, "q")
-    k_shape, k_strides = _rows(k, q, dev, "k")
-    v_shape, v_strides = _rows(v, q, dev, "v")
-    KV = k_shape[1]
-    if v_shape != k_shape or k_shape[0] != T or k_shape[2] != hd:
-        raise ValueError("q must be [T, H, hd] and k, v [T, KV, hd]")
-    for w in (q_norm, k_norm):
-        if w.dtype is not q.dtype or w.numel() != hd or w.get_device() != dev \
-                or not w.is_contiguous():
-            raise ValueError(f"q_norm and k_norm must be contiguous vectors of {hd} elements, of "
-                             "q's dtype and device")
-    page_shape = _pages(k_pages, v_pages, q, dev)
-    if page_shape[1] != KV or page_shape[3] != hd:
-        raise ValueError("k_pages and v_pages must hold k's heads")
-    cos, sin, table_len = _rope(tables, rotary_dim, dev)
-    n_rows, width = _table(table, dev)
-    index, at = _ints(rows, dev, "rows", T), _ints(positions, dev, "positions", T)
-    if q_out is None:
-        q_out = q.new_empty(T, H, hd)
-    elif q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.get_device() != dev \
-            or not q_out.is_contiguous():
-        raise ValueError("q_out must be a contiguous tensor of q's shape, dtype and device")
-    if k_out is not None and (k_out.shape != k_shape or k_out.dtype is not q.dtype
-                              or k_out.get_device() != dev or not k_out.is_contiguous()):
-        raise ValueError("k_out must be a contiguous tensor of k's shape, dtype and device")
-    _call(dev, "prepare_paged", lib().qdc_prepare_paged, q_out.data_ptr(),
-          0 if k_out is None else k_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-          q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
-          cos, sin, index, at, table.data_ptr(), T, H, KV, hd, rotary_dim, table_len, n_rows, width,
-          page_shape[0], page_shape[2], *q_strides, *k_strides, *v_strides, eps, code,
-          _flag(error_flag, dev))
-    return q_out
+    cos, sin = (None, None) if tables is None or not rotary_dim else tables
+    return calls().prepare_paged(q, k, v, q_norm, k_norm, cos, sin, rotary_dim, eps, rows, positions,
+                                 table, k_pages, v_pages, q_out, k_out, error_flag)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -218,35 +95,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``[n, 2*H*hd]``).  Entries that are no token give zeros; positions behind the
     table's width and pages that are none count as masked and set ``error_flag``.
     ``scale`` positive; head_dim 64, 128 or 256."""
-    dev, code = _on(q), _code(q)
-    (n, H, hd), q_strides = _rows(q, q, dev, "q")
-    pages, KV, page, page_hd = _pages(k_pages, v_pages, q, dev)
-    if page_hd != hd or KV == 0 or H % KV:
-        raise ValueError("q's heads must be a multiple of those of k_pages, of one head_dim")
-    n_rows, width = _table(table, dev)
-    index, at = _ints(rows, dev, "rows", n), _ints(positions, dev, "positions", n)
-    gate_at, gate_strides = 0, (0, hd)
-    if gate is not None:
-        gate_shape, gate_strides = _rows(gate, q, dev, "gate")
-        if gate_shape != q.shape:
-            raise ValueError("gate must be a view like q")
-        gate_at = gate.data_ptr()
-    if out_dtype is None:
-        split, out_code, odt = False, code, q.dtype
-    else:
-        split = _is_split(out_dtype)
-        odt = torch.bfloat16 if split else out_dtype
-        out_code = _lib.QDC_BF16X2 if split else _DTYPES.get(odt)
-        if out_code is None:
+    code = -1
+    if out_dtype is not None:
+        code = _lib.QDC_BF16X2 if _is_split(out_dtype) else _DTYPES.get(out_dtype)
+        if code is None:
             raise ValueError("out_dtype must be float32, bfloat16 or BF16X2")
-    out = q.new_empty(n, 2 * H * hd if split else H * hd, dtype=odt)
-    need = lib().qdc_paged_attention_workspace(n, H, KV, hd, width, page, code)
-    work = q.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    _call(dev, "paged_attention", lib().qdc_paged_attention, out.data_ptr(), out_code,
-          q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), gate_at, table.data_ptr(), index,
-          at, n, H, KV, hd, n_rows, width, pages, page, *q_strides, *gate_strides, H * hd, scale,
-          code, 0 if work is None else work.data_ptr(), need, _flag(error_flag, dev))
-    return out
+    return calls().paged_attention(q, k_pages, v_pages, table, rows, positions, scale, gate, code,
+                                   error_flag)
 
 
 # ------------------------------------------------------------------- pages ---
@@ -282,15 +137,7 @@ def extend_pages(book: PageTable, rows: torch.Tensor, counts: torch.Tensor | Non
     cannot be done whole -- a row out of range or named twice, a negative count, a row
     longer than its table, too few free pages -- does nothing but set every position
     to -1 and ``error_flag``."""
-    dev, at, sizes = _book(book)
-    index = _ints(rows, dev, "rows", -1)
-    n = rows.shape[0]
-    many = 0 if counts is None else _ints(counts, dev, "counts", n)
-    if positions is None:
-        positions = rows.new_empty(n)
-    _call(dev, "extend_pages", lib().qdc_pages_extend, _ints(positions, dev, "positions", n), *at,
-          index, many, n, *sizes, _flag(error_flag, dev))
-    return positions
+    return calls().extend_pages(*book, rows, counts, positions, error_flag)
 
 
 def free_pages(book: PageTable, rows: torch.Tensor,
@@ -298,9 +145,7 @@ def free_pages(book: PageTable, rows: torch.Tensor,
     """Rows give up their pages and are empty; pages that no other row shares are free
     again (an empty row: nothing).  Negative rows are left out; a row out of range or
     named twice: nothing is done and ``error_flag`` is set."""
-    dev, at, sizes = _book(book)
-    _call(dev, "free_pages", lib().qdc_pages_free, *at, _ints(rows, dev, "rows", -1),
-          rows.shape[0], *sizes, _flag(error_flag, dev))
+    calls().free_pages(*book, rows, error_flag)
 
 
 def fork_pages(book: PageTable, parents: torch.Tensor, children: torch.Tensor,
@@ -312,33 +157,14 @@ def fork_pages(book: PageTable, parents: torch.Tensor, children: torch.Tensor,
     negative row are left out.  A child that is not empty, named twice or also a
     parent, a row out of range, too few free pages: nothing is done and ``error_flag``
     is set."""
-    dev, at, sizes = _book(book)
-    src = _ints(parents, dev, "parents", -1)
-    n = parents.shape[0]
-    dst = _ints(children, dev, "children", n)
-    pool_at, planes, _ = _pool(pool, sizes[2], dev)
-    heads = token = 0
-    if pool is not None:
-        shape = pool.shape
-        if len(shape) != 5 or shape[3] != book.page_size:
-            raise ValueError("pool must be [planes, pages, kv_heads, page_size, head_dim]")
-        heads, token = shape[2], shape[4] * pool.element_size()
-    need = lib().qdc_pages_fork_workspace(n, sizes[3], planes, heads, token)
-    work = parents.new_empty(need, dtype=torch.uint8) if need else None
-    _call(dev, "fork_pages", lib().qdc_pages_fork, *at, src, dst, n, *sizes, pool_at, planes,
-          heads, token, work.data_ptr() if need else 0, need, _flag(error_flag, dev))
+    calls().fork_pages(*book, parents, children, pool, error_flag)
 
 
 def compact_pages(book: PageTable, pool: torch.Tensor | None = None) -> None:
     """The pages in use move to the low end, in every plane of ``pool [planes, pages,
     ...]``: with ``m`` of them, the k-th free page below ``m`` takes the k-th page in
     use from ``m`` on.  Tables and refs follow; the stack holds the rest, lowest on top."""
-    dev, at, (rows, width, pages, _) = _book(book)
-    pool_at, planes, nbytes = _pool(pool, pages, dev)
-    need = lib().qdc_pages_compact_workspace(pages)
-    work = book.table.new_empty(need, dtype=torch.uint8)
-    _call(dev, "compact_pages", lib().qdc_pages_compact, at[0], at[2], at[3], rows, width, pages,
-          pool_at, planes, nbytes, work.data_ptr(), need)
+    calls().compact_pages(*book, pool)
 
 
 def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -348,13 +174,7 @@ def copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
     rows.  Pairs with a negative index are left out; a pair out of range, or whose
     ``dst`` is an earlier pair's or any pair's ``src``, is not copied and sets
     ``error_flag``.  At most 4096 pairs a call."""
-    dev = _on(pool)
-    index = _ints(src, dev, "src", -1)
-    n = src.shape[0]
-    items = pool.shape[1] if pool.dim() > 1 else -1
-    at, planes, nbytes = _pool(pool, items, dev)
-    _call(dev, "copy_pages", lib().qdc_copy_pages, at, index, _ints(dst, dev, "dst", n), n, planes,
-          items, nbytes, _flag(error_flag, dev))
+    calls().copy_pages(pool, src, dst, error_flag)
 
 
 # -------------------------------------------------------- linear attention ---
@@ -375,45 +195,10 @@ def delta_step(proj: torch.Tensor, conv: torch.Tensor, a_decay: torch.Tensor,
     token give zeros and leave the cache; so does a row out of range or that of an
     earlier token of the call, which sets ``error_flag``.  key_dim 32, 64 or 128,
     value_dim a multiple of 16 up to 256, up to 8 taps."""
-    dev, code, dtype = _on(proj), _code(proj), proj.dtype
-    vw = value_heads * value_dim
-    channels = 2 * key_heads * key_dim + vw
-    n, width = proj.shape if proj.dim() == 2 else (0, -1)
-    if width < channels + vw + 2 * value_heads or proj.stride(1) != 1:
-        raise ValueError("proj must be [n, width] with contiguous rows of the q|k|v|z|a|b blocks")
-    taps = conv.shape[-1]
-    if conv.shape != (channels, taps) or conv.dtype is not _F32 or conv.get_device() != dev \
-            or not conv.is_contiguous():
-        raise ValueError(f"conv must be a contiguous float32 [{channels}, taps] tensor (the q|k|v "
-                         "channels) on proj's device")
-    for t in (a_decay, dt_bias):
-        if t.dtype is not _F32 or t.numel() != value_heads or t.get_device() != dev \
-                or not t.is_contiguous():
-            raise ValueError(f"a_decay and dt_bias must be contiguous float32 vectors of "
-                             f"{value_heads} elements on proj's device")
-    if norm.dtype is not dtype or norm.numel() != value_dim or norm.get_device() != dev \
-            or not norm.is_contiguous():
-        raise ValueError(f"norm must be a contiguous vector of {value_dim} elements of proj's "
-                         "dtype and device")
-    cache_rows = state.shape[0]
-    if state.shape != (cache_rows, value_heads, value_dim, key_dim) or state.dtype is not _F32 \
-            or state.get_device() != dev or not state.is_contiguous():
-        raise ValueError("state must be a contiguous float32 [cache rows, value_heads, value_dim, "
-                         "key_dim] tensor on proj's device")
-    if ring.shape != (cache_rows, taps, channels) or ring.dtype is not dtype \
-            or ring.get_device() != dev or not ring.is_contiguous():
-        raise ValueError(f"ring must be a contiguous [cache rows, {taps}, {channels}] tensor of "
-                         "proj's dtype and device")
-    index, at = _ints(rows, dev, "rows", n), _ints(positions, dev, "positions", n)
     split = out_dtype is not None and _is_split(out_dtype)
-    if split and dtype is not torch.bfloat16:
+    if split and proj.dtype is not torch.bfloat16:
         raise ValueError("the split output takes a bfloat16 proj")
-    if not split and out_dtype not in (None, dtype):
+    if not split and out_dtype not in (None, proj.dtype):
         raise ValueError("out_dtype must be proj's dtype or BF16X2")
-    out = proj.new_empty(n, 2 * vw if split else vw)
-    _call(dev, "delta_step", lib().qdc_delta_step, out.data_ptr(),
-          _lib.QDC_BF16X2 if split else code, proj.data_ptr(), code,
-          proj.stride(0) if n > 1 else width, conv.data_ptr(), taps, a_decay.data_ptr(),
-          dt_bias.data_ptr(), norm.data_ptr(), ring.data_ptr(), state.data_ptr(), index, at, n,
-          cache_rows, key_heads, key_dim, value_heads, value_dim, eps, _flag(error_flag, dev))
-    return out
+    return calls().delta_step(proj, conv, a_decay, dt_bias, norm, eps, ring, state, rows, positions,
+                              key_heads, key_dim, value_heads, value_dim, split, error_flag)

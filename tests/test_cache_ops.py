@@ -1053,7 +1053,7 @@ def test_two_captured_graphs():
         return decode_step(s)
 
     ints_50, ints_51 = ints([0, -1, 7]), ints([51, 3, 52])     # pages beyond those in use
-    lib = cache_ops.lib()
+    lib = _lib.lib()
     assert lib.qdc_pages_fork_workspace(3, page, 2, KV, 2 * hd) > 0
     assert lib.qdc_paged_attention_workspace(6, H, KV, hd, width, page, BF16) > 0
     twins, held = [inputs(0), inputs(1)], [inputs(0), inputs(1)]
