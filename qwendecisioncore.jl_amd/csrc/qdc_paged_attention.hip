@@ -24,7 +24,7 @@
 // MB, each byte fetched once) 123 us = 6.7 TB/s with its join of 4.6 us behind it, of 7.0
 // that a plain streaming read reaches; 96 rows of 0 .. 16384 keys (333 MB) 56 us = 6.0
 // TB/s.  Where little is read the chain positions -> pages -> K -> scores -> join counts: 8
-// rows of 2048 keys (34 MB) 11.2 + 4.0 us, one row of 411 keys (0.4 MB, in one launch) 8.6.
+// rows of 2048 keys (34 MB) 11.2 + 4.0 us, one row of 411 keys (0.4 MB, in one launch) 6.9.
 #include <cfloat>
 #include <type_traits>
 
@@ -209,11 +209,29 @@ template <typename P> __device__ __forceinline__ P load_page(const char *p) {
     return __builtin_nontemporal_load(reinterpret_cast<const P *>(p));
 }
 
+// Moves within each row of 16 lanes (by 4, 8) and each quad (its lane I to all four).
+template <int N> __device__ __forceinline__ float row_rotate(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
+}
+template <int I> __device__ __forceinline__ float quad_lane(float v) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x55 * I, 0xf, 0xf, true));
+}
+
 // One wavefront's operands and sums over its tiles of one head group.
 //   K: lane (lr, lg) holds values DS s + V lg .. of key 16 sub + lr.
 //   V: values 16 VD c + VD lr .. of keys 16 sub + 4 lg + r.
 //   S^T, P: head lr, keys 16 sub + 4 lg + r.   O^T[c][j]: head lr, values
 //   16 VD c + VD (4 lg + r) + j.
+// FEW, for fp32 and up to 4 heads: sixteen 4 x 4 products with one key's or value's step
+// each in place of one of 16 x 16, of which 4 columns would be in use: a quarter of the
+// matrix cores' time, which short rows wait for (us, 16 x 16 / 4 x 4: a row of 500 keys of
+// 64 9.1 / 7.7, 8 rows of 256 of 128 11.7 / 10.5, 410 MB of 256 134 / 127).  Quad g = lane / 4 %
+// 4 and j = lane % 4:
+//   K as above, each lg a part of the sum.  S^T, P: head j, keys 4 g + r, the same for all
+//   lg.  V: values 16 VD c + VD (4 lg + j) .. of keys 4 g + r.   O[c][e]: head r, values 16
+//   VD c + VD (4 lg + j) + e over the keys of quad g.
 template <typename T, int HD> struct Lanes {
     static constexpr bool BF = sizeof(T) == 2;
     static constexpr int V = Elem<T>::kVec, SUBS = BF ? 2 : 1, DS = 4 * V, STEPS = HD / DS;
@@ -237,7 +255,7 @@ template <typename T, int HD> struct Lanes {
 
 // Tiles j0 .. j1 - 1 of a unit (KV head and group of its query heads) of an entry, by
 // WAVES wavefronts: its outputs, when `whole`, or a piece in slot `slot`.
-template <typename T, int HD, int WAVES>
+template <typename T, int HD, int WAVES, bool FEW>
 __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int row, int keys,
                                        int unit, int j0, int j1, bool whole, int64_t slot) {
     typedef Lanes<T, HD> L;
@@ -250,7 +268,8 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     const int lr = l % 16, lg = l / 16;
     const int mask = (1 << a.shift) - 1;
     const uint32_t off_k = (uint32_t)(lr * HD + L::V * lg) * (uint32_t)sizeof(T);
-    const uint32_t off_v = (uint32_t)(4 * lg * HD + L::VD * lr) * (uint32_t)sizeof(T);
+    const int vk = FEW ? lr / 4 : lg, vp = FEW ? l % 4 + 4 * lg : lr;  // V's keys, its piece
+    const uint32_t off_v = (uint32_t)(4 * vk * HD + L::VD * vp) * (uint32_t)sizeof(T);
     L x;
     const int kvh = a.head_groups == 1 ? unit : unit / a.head_groups;
     const int hg = unit - kvh * a.head_groups;
@@ -315,7 +334,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     for (int i = threadIdx.x; i < L::STEPS * kWave; i += WAVES * kWave) {
         const int s = i / kWave, ln = i % kWave;
         sq[s][ln] = load_raw((const T *)a.q + (int64_t)entry * a.q_tok +
-                             (int64_t)(head0 + min(ln % 16, gu - 1)) * a.q_head + L::DS * s +
+                             (int64_t)(head0 + min(ln % (FEW ? 4 : 16), gu - 1)) * a.q_head + L::DS * s +
                              L::V * (ln / 16));
     }
     __syncthreads();
@@ -324,23 +343,40 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     // registers they fill (in a branch of their own they would be waited for there)
     auto step = [&](int k, auto more) {
         f32x4 sc[L::SUBS];
+        if constexpr (FEW) {
+            f32x4 part[4];  // chains beside each other
 #pragma unroll
-        for (int s = 0; s < L::SUBS; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; ++e) part[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < L::STEPS; ++i) {
-            const u32x4 qf = sq[i][l];
+            for (int i = 0; i < L::STEPS; ++i) {
+                const u32x4 qf = sq[i][l];
 #pragma unroll
-            for (int s = 0; s < L::SUBS; ++s) {
-                if constexpr (L::BF) {
-                    sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, x.k[s][i]), __builtin_bit_cast(bf16x8, qf),
-                        sc[s], 0, 0, 0);
-                } else {
+                for (int e = 0; e < 4; ++e)
+                    part[e] = __builtin_amdgcn_mfma_f32_4x4x1f32(
+                        __uint_as_float(x.k[0][i][e]), __uint_as_float(qf[e]), part[e], 0, 0, 0);
+            }
+            sc[0] = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            __uint_as_float(x.k[s][i][e]), __uint_as_float(qf[e]), sc[s], 0, 0,
-                            0);
+            for (int r = 0; r < 4; ++r) sc[0][r] = swap_sum32(swap_sum16(sc[0][r]));
+        } else {
+#pragma unroll
+            for (int s = 0; s < L::SUBS; ++s) sc[s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < L::STEPS; ++i) {
+                const u32x4 qf = sq[i][l];
+#pragma unroll
+                for (int s = 0; s < L::SUBS; ++s) {
+                    if constexpr (L::BF) {
+                        sc[s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8, x.k[s][i]), __builtin_bit_cast(bf16x8, qf),
+                            sc[s], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            sc[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                __uint_as_float(x.k[s][i][e]), __uint_as_float(qf[e]), sc[s], 0,
+                                0, 0);
+                    }
                 }
             }
         }
@@ -359,7 +395,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
             for (int s = 0; s < L::SUBS; ++s)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (4 * lg + r < now[s]) continue;
+                    if (4 * vk + r < now[s]) continue;
                     sc[s][r] = -__builtin_inff();
 #pragma unroll
                     for (int c = 0; c < L::VC; ++c)  // 0 times what lies there may be NaN
@@ -371,14 +407,23 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
         for (int s = 0; s < L::SUBS; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[s][r]);
-        top = fmaxf(swap_max(top) * a.scale_log2, x.base);
+        if constexpr (FEW) {
+            top = fmaxf(top, row_rotate<8>(top));
+            top = fmaxf(top, row_rotate<4>(top));
+        } else {
+            top = swap_max(top);
+        }
+        top = fmaxf(top * a.scale_log2, x.base);
         if (__any(top > x.base)) {
             const float f = __builtin_amdgcn_exp2f(x.base - top);
+            const f32x4 fs = FEW ? f32x4{quad_lane<0>(f), quad_lane<1>(f), quad_lane<2>(f),
+                                         quad_lane<3>(f)}
+                                 : f32x4{f, f, f, f};
             x.sum *= f;
 #pragma unroll
             for (int c = 0; c < L::VC; ++c)
 #pragma unroll
-                for (int j = 0; j < L::VD; ++j) x.o[c][j] *= f;
+                for (int j = 0; j < L::VD; ++j) x.o[c][j] *= fs;
             x.base = top;
         }
         float p[L::SUBS][4];
@@ -422,9 +467,15 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
 #pragma unroll
                 for (int j = 0; j < L::VD; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            __uint_as_float(x.v[0][r][c][j]), p[0][r], x.o[c][j], 0, 0, 0);
+                    for (int r = 0; r < 4; ++r) {
+                        const float vf = __uint_as_float(x.v[0][r][c][j]);
+                        if constexpr (FEW)
+                            x.o[c][j] = __builtin_amdgcn_mfma_f32_4x4x1f32(p[0][r], vf, x.o[c][j],
+                                                                           0, 0, 0);
+                        else
+                            x.o[c][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, p[0][r],
+                                                                             x.o[c][j], 0, 0, 0);
+                    }
         }
         if constexpr (decltype(more)::value) {
             __builtin_amdgcn_sched_barrier(0);
@@ -434,15 +485,36 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     for (int k = 0; k + 1 < cnt; ++k) step(k, std::true_type{});
     if (cnt) step(cnt - 1, std::false_type{});
     // the wavefronts' sums together, four heads at a time
-    x.sum = swap_sum32(swap_sum16(x.sum));
-    if (lg == 0) {
-        sm[wv][lr] = x.base;
-        sl[wv][lr] = x.sum;
+    if constexpr (FEW) {
+        x.sum += row_rotate<8>(x.sum);
+        x.sum += row_rotate<4>(x.sum);
+    } else {
+        x.sum = swap_sum32(swap_sum16(x.sum));
+    }
+    if (l < (FEW ? 4 : kHeads)) {
+        sm[wv][l] = x.base;
+        sl[wv][l] = x.sum;
     }
     for (int h0 = 0; h0 < gu; h0 += 4) {
         const int hh = lr - h0;
         if (h0 && whole && wv < min(gu - h0, 4)) load_gate(a, entry, head0 + h0 + wv, dim, gate);
-        if (hh >= 0 && hh < 4)
+        if constexpr (FEW) {  // the quads' sums, quad g's lanes for head g
+#pragma unroll
+            for (int c = 0; c < L::VC; ++c) {
+                f32x4 mine;
+#pragma unroll
+                for (int j = 0; j < L::VD; ++j) {
+                    f32x4 o = x.o[c][j];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        o[r] += row_rotate<8>(o[r]);
+                        o[r] += row_rotate<4>(o[r]);
+                    }
+                    mine[j] = vk < 2 ? (vk ? o[1] : o[0]) : (vk == 2 ? o[2] : o[3]);
+                }
+                *reinterpret_cast<f32x4 *>(&so[wv][vk][16 * L::VD * c + L::VD * vp]) = mine;
+            }
+        } else if (hh >= 0 && hh < 4) {
 #pragma unroll
             for (int c = 0; c < L::VC; ++c)
 #pragma unroll
@@ -450,6 +522,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         so[wv][hh][16 * L::VD * c + L::VD * (4 * lg + r) + j] = x.o[c][j][r];
+        }
         __syncthreads();
         const int h = h0 + wv;
         if (h < gu && wv < 4) {
@@ -484,9 +557,8 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
     }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool FEW>
 __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(PagedAttention a) {
-    constexpr int TILE = tile_keys<T>();
     Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
     uint32_t t = blockIdx.x, t_end = t + (t < all);  // with shares a place is a workgroup's
@@ -520,13 +592,13 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
             j0 = p0 > line.kBegin ? p0 - line.kBegin : 0;
             j1 = p1 - line.kBegin;
         }
-        attend<T, HD, kWaves>(a, line.first + el, row, keys, (int)unit, (int)j0, (int)j1,
+        attend<T, HD, kWaves, FEW>(a, line.first + el, row, keys, (int)unit, (int)j0, (int)j1,
                               j0 == 0 && j1 == tiles, 2 * (int64_t)blockIdx.x + (j0 == 0));
     }
 }
 
 // The same where every row is short: a workgroup for a unit, whole, and no join.
-template <typename T, int HD>
+template <typename T, int HD, bool FEW>
 __global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short(PagedAttention a) {
     constexpr int TILE = tile_keys<T>(), WAVES = short_waves(HD), VEC = HD / kWave;
     const int units = a.kv * a.head_groups;
@@ -536,7 +608,7 @@ __global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short
     const int keys = entry_keys(a, row, a.positions[entry], bad);
     if (bad && unit == 0 && threadIdx.x == 0) raise_flag(a.error_flag);
     if (keys) {
-        attend<T, HD, WAVES>(a, entry, row, keys, unit, 0, (keys + TILE - 1) / TILE, true, 0);
+        attend<T, HD, WAVES, FEW>(a, entry, row, keys, unit, 0, (keys + TILE - 1) / TILE, true, 0);
         return;
     }
     const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
@@ -763,20 +835,20 @@ extern "C" int32_t qdc_paged_attention(
     a.log_wgs = log_workgroups(line, head_dim);
     a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
-    const bool brief = need == 0;
+    const bool brief = need == 0, few = dtype == QDC_F32 && a.group <= 4;
     const dim3 grid(brief ? (uint32_t)(n * kv_heads * a.head_groups) : 1u << a.log_wgs);
     const dim3 join((uint32_t)(n * heads)), block(kBlock);
     const bool many = kManyPieces * n * kv_heads * a.head_groups <= grid.x;
     a.pieces = reinterpret_cast<float *>(workspace);
     a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;
-#define QDC_PAGED(T, HD)                                                                       \
-    if (head_dim == HD) {                                                                      \
+#define QDC_PAGED(T, HD, FEW)                                                                  \
+    if (head_dim == HD && few == FEW) {                                                                      \
         if (brief) {                                                                           \
-            hipLaunchKernelGGL((paged_attention_short<T, HD>), grid,                           \
+            hipLaunchKernelGGL((paged_attention_short<T, HD, FEW>), grid,                           \
                                dim3(short_waves(HD) * kWave), 0, stream, a);                   \
             return launch_status();                                                            \
         }                                                                                      \
-        hipLaunchKernelGGL((paged_attention<T, HD>), grid, block, 0, stream, a);               \
+        hipLaunchKernelGGL((paged_attention<T, HD, FEW>), grid, block, 0, stream, a);               \
         const int32_t status = launch_status();                                                \
         if (status != QDC_OK) return status;                                                   \
         if (many)                                                                              \
@@ -788,13 +860,16 @@ extern "C" int32_t qdc_paged_attention(
         return launch_status();                                                                \
     }
     if (dtype == QDC_BF16) {
-        QDC_PAGED(bf16_t, 64)
-        QDC_PAGED(bf16_t, 128)
-        QDC_PAGED(bf16_t, 256)
+        QDC_PAGED(bf16_t, 64, false)
+        QDC_PAGED(bf16_t, 128, false)
+        QDC_PAGED(bf16_t, 256, false)
     }
-    QDC_PAGED(float, 64)
-    QDC_PAGED(float, 128)
-    QDC_PAGED(float, 256)
+    QDC_PAGED(float, 64, true)
+    QDC_PAGED(float, 64, false)
+    QDC_PAGED(float, 128, true)
+    QDC_PAGED(float, 128, false)
+    QDC_PAGED(float, 256, true)
+    QDC_PAGED(float, 256, false)
 #undef QDC_PAGED
     return QDC_ERR_SHAPE;
 }
