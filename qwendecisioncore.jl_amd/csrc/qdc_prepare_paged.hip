@@ -8,16 +8,22 @@
 // one K and V head: one position, rotation and place for all of them, every row's loads
 // before the first is used, and a row's sum one lane-group reduction.  A lane with a
 // rotary chunk reads its partner chunk, half a rotary block away, from the same row a
-// second time: it is in the cache line the group is fetching anyway.
+// second time: it is in the cache line the group is fetching anyway, and the other
+// lanes read one line there together.
 //
 // Bound by memory: 16384 tokens of 8 + 2 heads of 256 (bf16, 105 MB read, 105 written)
-// 38.4 us = 5.5 TB/s, of 6.5 for a copy: what is between is the chain position -> page ->
+// 36.3 us = 5.8 TB/s, of 6.5 for a copy: what is between is the chain position -> page ->
 // place in front of the K and V stores and the stores' scatter over the pages.  One token
 // 2.7 us, a launch and three dependent loads.
 #include "qdc_cache.hpp"
 
 namespace qdc {
 namespace {
+
+// Small workgroups let stores begin while other rows load (us, 16384 tokens of 8 + 2 heads of
+// 256 in bf16, 64 / 128 / 256 / 512 threads: 40.9 / 36.3 / 37.3 / 42.8; other sizes within
+// 4% between 64 and 256).
+constexpr int kThreads = 128;
 
 struct PreparePaged {
     void *q_out, *k_out, *k_pages, *v_pages;
@@ -102,8 +108,8 @@ __device__ __forceinline__ void norm_rope(const PreparePaged &a, const Turn<T> &
 }
 
 template <typename T, int HD, int RPG, bool WHOLE>
-__global__ __launch_bounds__(kBlock) void prepare_paged(PreparePaged a) {
-    constexpr int V = Elem<T>::kVec, LPR = HD / V, GPB = kBlock / LPR;
+__global__ __launch_bounds__(kThreads) void prepare_paged(PreparePaged a) {
+    constexpr int V = Elem<T>::kVec, LPR = HD / V, GPB = kThreads / LPR;
     const int lane = threadIdx.x % LPR;
     const int64_t unit = (int64_t)blockIdx.x * GPB + threadIdx.x / LPR;
     if (unit >= a.total) return;  // uniform per lane group
@@ -120,14 +126,14 @@ __global__ __launch_bounds__(kBlock) void prepare_paged(PreparePaged a) {
     const bool paired = WHOLE && turn.rotary;
     float w[V], wp[V];
     load_chunk(norm + turn.e0, w);
-    load_chunk(norm + (paired ? turn.ep : turn.e0), wp);
+    load_chunk(norm + (paired ? turn.ep : 0), wp);
     u32x4 raw[RPG], other[RPG], value = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < RPG; ++i) {
         if (i && !is_q) continue;  // uniform per lane group
         const T *x = src + i * a.q_head;
         raw[i] = load_stream(x + turn.e0);
-        other[i] = load_raw(x + (paired ? turn.ep : turn.e0));
+        other[i] = load_raw(x + (paired ? turn.ep : 0));  // unused: one line for all lanes
     }
     if (!is_q)
         value = load_stream((const T *)a.v + (int64_t)t * a.v_tok + (int64_t)h * a.v_head + turn.e0);
@@ -260,9 +266,9 @@ extern "C" int32_t qdc_prepare_paged(
     a.eps = eps;
 #define QDC_PREPARE_ROWS(T, HD, RPG, WHOLE)                                                    \
     if (rpg == RPG && whole == WHOLE) {                                                        \
-        constexpr int64_t gpb = kBlock / (HD / Elem<T>::kVec);                                 \
+        constexpr int64_t gpb = kThreads / (HD / Elem<T>::kVec);                                 \
         hipLaunchKernelGGL((prepare_paged<T, HD, RPG, WHOLE>),                                 \
-                           dim3((uint32_t)ceil_div(a.total, gpb)), dim3(kBlock), 0, stream, a);\
+                           dim3((uint32_t)ceil_div(a.total, gpb)), dim3(kThreads), 0, stream, a);\
         return launch_status();                                                                \
     }
 #define QDC_PREPARE(T, HD)                                                                     \
