@@ -274,6 +274,11 @@ class BackboneCache:
         keep = None if mask is None else mask.view(-1)
         token_rows = rows.repeat_interleave(S)
         token_at = at.reshape(-1)
+        # the convolution inputs that the rings keep (padding has a projection of zeros)
+        last = min(S, cfg.conv_kernel)
+        held = rows.long()
+        slots = (held[:, None] * cfg.conv_kernel
+                 + at[:, -last:].long() % cfg.conv_kernel).view(-1)
 
         def mix(i, layer, proj):
             a = self.plane[i]
@@ -296,10 +301,9 @@ class BackboneCache:
             state = torch.empty((B, vh, vd, kd), dtype=torch.float32, device=proj.device)
             x = ops.delta_scan(q.view(B, S, kh, kd), k.view(B, S, kh, kd), v.view(B, S, vh, vd),
                                beta.view(B, S, vh), decay.view(B, S, vh), model.dtype, state=state)
-            self.states[a][rows.long()] = state
-            last = min(S, cfg.conv_kernel)   # padding has a projection of zeros
-            self.rings[a][rows.long()[:, None], at[:, -last:].long() % cfg.conv_kernel] = \
-                proj.view(B, S, -1)[:, -last:, :channels]
+            self.states[a].index_copy_(0, held, state)
+            self.rings[a].view(-1, channels).index_copy_(
+                0, slots, proj.view(B, S, -1)[:, -last:, :channels].reshape(-1, channels))
             z = proj[:, channels:channels + vw].view(-1, vh, vd)
             return ops.native_gated_rms(x.view(-1, vh, vd), z, layer["norm"], cfg.eps,
                                         out_dtype=model.gemm_in).view(B * S, -1)
@@ -340,6 +344,8 @@ class BackboneCache:
         h, normed = ops.native_gather_rms(model.embedding, ids, model.layers[0]["input_norm"],
                                           cfg.eps, token_mask=masked(0),
                                           normed_dtype=model.gemm_in)
+        if model.fused_f32 and ops.linear_f32_takes(ids.shape[0], cfg.hidden, cfg.intermediate):
+            return self._through_small(h, normed, masked, mix, last_rows)
         for i, layer in enumerate(model.layers):
             attention = layer["kind"] == "full_attention"
             mixed = mix(i, layer, model._mm(normed, layer["qkv" if attention else "proj"]))
@@ -357,3 +363,22 @@ class BackboneCache:
                                                 token_mask=None if last else masked(i + 1),
                                                 out_dtype=None if last else model.gemm_in)
         return normed
+
+    def _through_small(self, h, normed, masked, mix, last_rows):
+        """``QwenBackbone._forward_small`` around the layers' mixing step."""
+        model, eps = self.model, self.model.cfg.eps
+        due = None  # the MLP output not yet added to h
+        for i, layer in enumerate(model.layers):
+            w = layer["qkv" if layer["kind"] == "full_attention" else "proj"]
+            if due is None:
+                proj = ops.linear_f32(normed, w)
+            else:
+                h, proj = ops.linear_f32(h, w, add=due, weight=layer["input_norm"], eps=eps,
+                                         token_mask=masked(i))
+            mixed = mix(i, layer, proj)
+            if i + 1 == len(model.layers):
+                h, mixed = last_rows(h), last_rows(mixed)
+            h, act = ops.linear_f32(h, layer["gate_up"], add=ops.linear_f32(mixed, layer["out"]),
+                                    weight=layer["post_norm"], eps=eps, swiglu=True)
+            due = ops.linear_f32(act, layer["down"])
+        return ops.native_residual_rms(h, due, model.final_norm, eps)[1]

@@ -128,6 +128,7 @@ def test_too_few_pages_leaves_everything():
 
 @pytest.mark.gpu
 def test_a_call_that_raises_ends_its_rows(monkeypatch):
+    from qdc_amd import ops
     from qdc_amd.cache import BackboneCache
     model = model_of("f32")
     cache = BackboneCache(model, rows=4, pages=20, page_size=16)
@@ -138,7 +139,7 @@ def test_a_call_that_raises_ends_its_rows(monkeypatch):
 
     for call in (lambda: cache.prefill([1, 2, 3]), lambda: cache.step([b], [5])):
         with monkeypatch.context() as m:
-            m.setattr(model, "_project_add_norm", fail)
+            m.setattr(ops, "native_residual_rms", fail)
             with pytest.raises(MemoryError):
                 call()
     assert cache.lengths() == {a: 30} and cache.free_page_count() == 18
