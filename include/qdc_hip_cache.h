@@ -163,8 +163,8 @@ int32_t qdc_copy_pages(void *pool, const int32_t *src, const int32_t *dst, int64
  * type, or QDC_BF16X2 for bf16): the gated norm's result.  An entry that is no token
  * gives zeros and leaves ring and state; so does one whose row is not below `rows` or
  * is that of an earlier token of the call (error_flag).  key_dim 32, 64 or 128,
- * value_dim a multiple of 16 up to 256, taps up to 8; state 16-byte aligned
- * (QDC_ERR_SHAPE otherwise). */
+ * value_dim a multiple of 16 up to 256, taps up to 8, n * value_heads below 2^22; state
+ * 16-byte aligned (QDC_ERR_SHAPE otherwise). */
 int32_t qdc_delta_step(void *out, int32_t out_dtype, const void *proj, int32_t proj_dtype,
                        int64_t ld, const float *conv, int64_t taps, const float *a_decay,
                        const float *dt_bias, const void *norm, void *ring, float *state,

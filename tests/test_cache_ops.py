@@ -207,6 +207,15 @@ def test_host_tensors_are_refused():
     for bad in ((0, 1, 1, 16), (1, 0, 1, 16), (1, 1, 0, 16), (1, 1, 1, 24)):
         with pytest.raises(ValueError):
             cache_ops.page_table(*bad, "cpu")
+    for call in (lambda: cache_ops.copy_pages([1.0], i, i), lambda: cache_ops.free_pages((i, 2, 3, 4, 5), i),
+                 lambda: cache_ops.delta_step(z(2, 600), z(384, 4), z(4), z(4), z(32), 1e-6,
+                                              z(2, 4, 384), z(2, 4, 32, 64), i, i, 2.5, 64, 4, 32),
+                 lambda: cache_ops.paged_attention(None, i, i, i, i, i, 0.1)):
+        with pytest.raises((TypeError, ValueError)):      # no tensor, no integer
+            call()
+    with pytest.raises(ValueError, match="split output"):
+        cache_ops.delta_step(z(2, 600), z(384, 4), z(4), z(4), z(32), 1e-6, z(2, 4, 384),
+                             z(2, 4, 32, 64), i, i, 2, 64, 4, 32, out_dtype=ops.BF16X2)
 
 
 # ------------------------------------------------------------------ helpers --
