@@ -52,7 +52,7 @@ struct PagedAttention {
     int32_t *error_flag;
     float *pieces, *stats;  // [2 workgroups][heads of a unit][head_dim], [..][2]
     int64_t q_tok, q_head, gate_tok, gate_head, out_tok, width;
-    int n, heads, kv, group, unit_heads, head_groups, rows, pages, shift, log_wgs;
+    int n, heads, kv, group, unit_heads, head_groups, rows, pages, shift, log_wgs, join_heads;
     int out_dtype;
     float scale_log2;       // scale * log2(e)
 };
@@ -617,10 +617,14 @@ __global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short
                                VEC * (threadIdx.x % kWave));
 }
 
-// A workgroup per (entry, head): the pieces of its keys, in order; zeros for an entry
-// without keys; nothing where one workgroup had them all.  (us, 256 / 512 threads: 128
+// A workgroup per entry and head, or join_heads of its heads: the pieces of their keys, in
+// order; zeros for an entry without keys; nothing where one workgroup had them all.  (us, 256 / 512 threads: 128
 // pieces a head 6.7 / 5.5, 32 5.0 / 4.9, few pieces of 200 x 8 heads 6.2 / 9.2.)
 constexpr int64_t kManyPieces = 64;
+// Entries times heads from which on a workgroup takes all heads of its entry, so that the
+// line is added up once for them.  (us of the whole call, a head each / all: 128 x 8 23.6 /
+// 30.1, 512 x 8 67.1 / 62.5, 1024 x 8 147 / 123.)
+constexpr int64_t kJoinWgs = 2048;
 template <typename T, int HD, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_attention_join(PagedAttention a) {
     constexpr int TILE = tile_keys<T>();
@@ -628,82 +632,90 @@ __global__ __launch_bounds__(THREADS) void paged_attention_join(PagedAttention a
     __shared__ float top_of[PARTS], sum_of[PARTS];
     __shared__ __align__(16) float so[PARTS][HD];
     const int l = threadIdx.x % kWave, wv = threadIdx.x / kWave;
-    const int entry = blockIdx.x / a.heads, h = blockIdx.x - entry * a.heads;
-    const int kvh = h / a.group, in_group = h - kvh * a.group;
-    const int hg = in_group / kHeads, hu = in_group - hg * kHeads;
+    const int per_entry = a.heads / a.join_heads, entry = blockIdx.x / per_entry;
+    const int h0 = (blockIdx.x - entry * per_entry) * a.join_heads, h1 = h0 + a.join_heads;
     const int dim = HD / kWave * l;
     T gate[HD / kWave] = {};
-    if (wv == 0) load_gate(a, entry, h, dim, gate);
+    if (wv == 0) load_gate(a, entry, h0, dim, gate);
     Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
     while (line.first + kWave <= entry) line.next();
     const int keys = __builtin_amdgcn_readlane(line.keys, entry - line.first);
     const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE;
-    if (h == 0 && threadIdx.x == 0) {
+    if (h0 == 0 && threadIdx.x == 0) {
         bool bad;
         entry_keys(a, a.index[entry], a.positions[entry], bad);
         if (bad) raise_flag(a.error_flag);
     }
     if (tiles == 0) {
-        if (wv == 0) store_zero<T, HD, HD / kWave>(a, entry, h, dim);
+        if (wv == 0)
+            for (int h = h0; h < h1; ++h) store_zero<T, HD, HD / kWave>(a, entry, h, dim);
         return;
     }
-    const uint32_t unit = (uint32_t)(kvh * a.head_groups + hg);
     const uint32_t span = __builtin_amdgcn_readlane(line.span, entry - line.first);
     const uint32_t start = line.before + __builtin_amdgcn_readlane(line.end, entry - line.first) -
-                           span * line.units + unit * span;
-    uint32_t w0, w1;  // the workgroups that hold its first and its last tile
-    if (line.share) {
-        w0 = start;
-        w1 = start + span - 1;
-    } else {  // that of place t is the last with all * w / 2^lw <= t
-        const int lw = log_workers(a.log_wgs, all);
-        const uint32_t first = start + line.kBegin;
-        w0 = (uint32_t)((((uint64_t)(first + 1) << lw) - 1) / all);
-        w1 = (uint32_t)((((uint64_t)(first + tiles) << lw) - 1) / all);
-    }
-    if (w0 == w1) return;
-    const int parts = (int)(w1 - w0) + 1;
-    auto slot = [&](int p) {
-        return ((2 * (int64_t)(w0 + p) + (p == 0)) * a.unit_heads + hu);
-    };
-    // Each group of LPP lanes runs over every PARTS-th piece, its maximum and sum beside
-    // the rows, so that nothing waits for a first pass over the maxima.
-    const int part = threadIdx.x / LPP, d4 = 4 * (threadIdx.x % LPP);
-    float top = -FLT_MAX, sum = 0.0f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+                           span * line.units;
+    for (int h = h0; h < h1; ++h) {
+        const int kvh = h / a.group, in_group = h - kvh * a.group;
+        const int hg = in_group / kHeads, hu = in_group - hg * kHeads;
+        const uint32_t at = start + (uint32_t)(kvh * a.head_groups + hg) * span;
+        uint32_t w0, w1;  // the workgroups that hold its first and its last tile
+        if (line.share) {
+            w0 = at;
+            w1 = at + span - 1;
+        } else {  // that of place t is the last with all * w / 2^lw <= t
+            const int lw = log_workers(a.log_wgs, all);
+            const uint32_t first = at + line.kBegin;
+            w0 = (uint32_t)((((uint64_t)(first + 1) << lw) - 1) / all);
+            w1 = (uint32_t)((((uint64_t)(first + tiles) << lw) - 1) / all);
+        }
+        if (w0 == w1) continue;
+        if (h != h0) {
+            __syncthreads();  // the scratch is free
+            if (wv == 0) load_gate(a, entry, h, dim, gate);
+        }
+        const int parts = (int)(w1 - w0) + 1;
+        auto slot = [&](int p) {
+            return ((2 * (int64_t)(w0 + p) + (p == 0)) * a.unit_heads + hu);
+        };
+        // Each group of LPP lanes runs over every PARTS-th piece, its maximum and sum beside
+        // the rows, so that nothing waits for a first pass over the maxima.
+        const int part = threadIdx.x / LPP, d4 = 4 * (threadIdx.x % LPP);
+        float top = -FLT_MAX, sum = 0.0f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int p = part; p < parts; p += PARTS) {
-        const f32x4 o = *reinterpret_cast<const f32x4 *>(a.pieces + slot(p) * HD + d4);
-        const f32x2 s = *reinterpret_cast<const f32x2 *>(a.stats + 2 * slot(p));
-        const float m = fmaxf(top, s[0]);
-        const float f = __builtin_amdgcn_exp2f(top - m), g = __builtin_amdgcn_exp2f(s[0] - m);
-        top = m;
-        sum = __builtin_fmaf(g, s[1], f * sum);
+        for (int p = part; p < parts; p += PARTS) {
+            const f32x4 o = *reinterpret_cast<const f32x4 *>(a.pieces + slot(p) * HD + d4);
+            const f32x2 s = *reinterpret_cast<const f32x2 *>(a.stats + 2 * slot(p));
+            const float m = fmaxf(top, s[0]);
+            const float f = __builtin_amdgcn_exp2f(top - m), g = __builtin_amdgcn_exp2f(s[0] - m);
+            top = m;
+            sum = __builtin_fmaf(g, s[1], f * sum);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(g, o[e], f * acc[e]);
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(g, o[e], f * acc[e]);
+        }
+        *reinterpret_cast<f32x4 *>(&so[part][d4]) = acc;
+        if (d4 == 0) {
+            top_of[part] = top;
+            sum_of[part] = sum;
+        }
+        __syncthreads();
+        if (wv) continue;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) top = fmaxf(top, top_of[p]);
+        float total = 0.0f, o[HD / kWave] = {};
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            const float f = __builtin_amdgcn_exp2f(top_of[p] - top);
+            total = __builtin_fmaf(f, sum_of[p], total);
+#pragma unroll
+            for (int e = 0; e < HD / kWave; ++e) o[e] = __builtin_fmaf(f, so[p][dim + e], o[e]);
+        }
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
+#pragma unroll
+        for (int e = 0; e < HD / kWave; ++e) o[e] *= inv;
+        store_out<T, HD, HD / kWave>(a, entry, h, dim, o, a.gate, gate);
     }
-    *reinterpret_cast<f32x4 *>(&so[part][d4]) = acc;
-    if (d4 == 0) {
-        top_of[part] = top;
-        sum_of[part] = sum;
-    }
-    __syncthreads();
-    if (wv) return;
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) top = fmaxf(top, top_of[p]);
-    float total = 0.0f, o[HD / kWave] = {};
-#pragma unroll
-    for (int p = 0; p < PARTS; ++p) {
-        const float f = __builtin_amdgcn_exp2f(top_of[p] - top);
-        total = __builtin_fmaf(f, sum_of[p], total);
-#pragma unroll
-        for (int e = 0; e < HD / kWave; ++e) o[e] = __builtin_fmaf(f, so[p][dim + e], o[e]);
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // 0: no key seen
-#pragma unroll
-    for (int e = 0; e < HD / kWave; ++e) o[e] *= inv;
-    store_out<T, HD, HD / kWave>(a, entry, h, dim, o, a.gate, gate);
 }
 
 // The longest line that a call of these sizes can have, 0 when it is too long or the
@@ -837,7 +849,8 @@ extern "C" int32_t qdc_paged_attention(
     a.scale_log2 = scale * 1.4426950408889634f;
     const bool brief = need == 0, few = dtype == QDC_F32 && a.group <= 4;
     const dim3 grid(brief ? (uint32_t)(n * kv_heads * a.head_groups) : 1u << a.log_wgs);
-    const dim3 join((uint32_t)(n * heads)), block(kBlock);
+    a.join_heads = n * heads >= kJoinWgs ? (int)heads : 1;
+    const dim3 join((uint32_t)(n * heads / a.join_heads)), block(kBlock);
     const bool many = kManyPieces * n * kv_heads * a.head_groups <= grid.x;
     a.pieces = reinterpret_cast<float *>(workspace);
     a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;

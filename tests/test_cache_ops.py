@@ -466,6 +466,7 @@ def test_paged_attention_long(H, KV, hd, lengths, dtype):
     (4, 2, 64, [700] * 64), (4, 2, 64, [700] * 65),   # as many as a wavefront sees, one more
     (16, 16, 64, [20 + i for i in range(60)] + [2500]),  # more units than workgroups
     (40, 2, 64, [1500, 0, 1, 1033]),        # two groups of heads a KV head, one not full
+    (12, 3, 64, [(37 * i) % 700 for i in range(181)]),   # all heads of an entry joined together
     (8, 2, 256, [16001])])                  # many pieces of one row
 def test_paged_attention_dealt(H, KV, hd, lengths, dtype):
     """Keys that go to the workgroups in even shares and as one line."""
