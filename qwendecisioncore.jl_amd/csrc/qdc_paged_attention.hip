@@ -82,12 +82,14 @@ constexpr int begin_bytes(int head_dim) { return head_dim > 128 ? 131072 : 65536
 // (us, shares / line: 8 rows of 2048 keys of 256 11.2 / 12.1, 32 of 1000 16.2 /
 // 17.1.)
 // A wavefront sees 64 entries at a time: lane l holds entry first + l.
-template <typename T, int HD> struct Line {
+// With FIRST it also holds each entry's first page.
+template <typename T, int HD, bool FIRST> struct Line {
     static constexpr int TILE = tile_keys<T>();
     static constexpr uint32_t kBegin = begin_bytes(HD) / (TILE * HD * 2 * (int)sizeof(T));
     const PagedAttention &a;
     const uint32_t units;
     int first, row, keys;
+    int32_t page;
     uint32_t span, end;    // places of a unit of this entry; the entry's end within the chunk
     uint32_t before, all;  // places of earlier chunks; of this one
     uint32_t share;        // 0: a line
@@ -107,6 +109,7 @@ template <typename T, int HD> struct Line {
         bool bad;
         row = i < a.n ? a.index[i] : -1;
         keys = entry_keys(a, row, i < a.n ? a.positions[i] : -1, bad);
+        if constexpr (FIRST) page = keys ? a.table[(int64_t)row * a.width] : -1;
     }
     // all places of the call; leaves the first chunk in place
     __device__ __forceinline__ uint32_t total() {
@@ -201,12 +204,14 @@ __device__ __forceinline__ void store_zero(const PagedAttention &a, int i, int h
     store_out<T, HD, N>(a, i, h, dim, zero, false, gate);
 }
 
-// Pages stream by: read as such they come at up to 6.7 TB/s, with plain loads at 5.6.
-// (Rows that share pages read them again from a cache, which this makes the most of in
-// neither way: 40 rows over 8 prompts of 2000 tokens 34 us, 36 with plain loads; 64 rows
-// over 4 prompts of 8000, 2.1 GB of reads of 131 MB, 215 and 157 us.)
-template <typename P> __device__ __forceinline__ P load_page(const char *p) {
-    return __builtin_nontemporal_load(reinterpret_cast<const P *>(p));
+// Pages stream by: read as such they come at up to 6.7 TB/s, with plain loads at 5.6.  Rows
+// that share pages, such as continuations of one prompt, find them in a cache again: plain
+// loads keep them there.  (us, as a stream / plain: 40 prompts of 2000 tokens 34.6 / 37.8;
+// 8 with 5 rows each 33.7 / 32.4, 16 of 4000 with 4 rows 71.9 / 53.0, 4 of 8000 with 16
+// rows 107 / 80.)
+template <bool SHARED, typename P> __device__ __forceinline__ P load_page(const char *p) {
+    const P *q = reinterpret_cast<const P *>(p);
+    return SHARED ? *q : __builtin_nontemporal_load(q);
 }
 
 // Moves within each row of 16 lanes (by 4, 8) and each quad (its lane I to all four).
@@ -253,17 +258,25 @@ template <typename T, int HD> struct Lanes {
     }
 };
 
+// What the wavefronts of a workgroup share: the queries, and their sums in the end.
+template <typename T, int HD, int WAVES> struct Scratch {
+    u32x4 q[Lanes<T, HD>::STEPS][kWave];
+    float out[WAVES][4][HD + 4], top[WAVES][kHeads], sum[WAVES][kHeads];
+};
+
 // Tiles j0 .. j1 - 1 of a unit (KV head and group of its query heads) of an entry, by
 // WAVES wavefronts: its outputs, when `whole`, or a piece in slot `slot`.
-template <typename T, int HD, int WAVES, bool FEW>
+template <typename T, int HD, int WAVES, bool FEW, bool SHARED>
 __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int row, int keys,
-                                       int unit, int j0, int j1, bool whole, int64_t slot) {
+                                       int unit, int j0, int j1, bool whole, int64_t slot,
+                                       Scratch<T, HD, WAVES> &scratch) {
     typedef Lanes<T, HD> L;
     constexpr int TILE = tile_keys<T>(), KT = kWave / L::SUBS;
     constexpr int VEC = HD / kWave;  // outputs of a thread per pass of 4 heads
-    __shared__ __align__(16) u32x4 sq[L::STEPS][kWave];
-    __shared__ __align__(16) float so[WAVES][4][HD + 4];
-    __shared__ float sm[WAVES][kHeads], sl[WAVES][kHeads];
+    auto &sq = scratch.q;
+    auto &so = scratch.out;
+    auto &sm = scratch.top;
+    auto &sl = scratch.sum;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
     const int lr = l % 16, lg = l / 16;
     const int mask = (1 << a.shift) - 1;
@@ -311,7 +324,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
         for (int s = 0; s < L::SUBS; ++s)
 #pragma unroll
             for (int i = 0; i < L::STEPS; ++i)
-                x.k[s][i] = load_page<u32x4>((const char *)a.k + from[s] + off_k +
+                x.k[s][i] = load_page<SHARED, u32x4>((const char *)a.k + from[s] + off_k +
                                              L::DS * (int)sizeof(T) * i);
     };
     auto load_v = [&] {
@@ -321,7 +334,7 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int c = 0; c < L::VC; ++c)
-                    x.v[s][r][c] = load_page<typename L::piece>(
+                    x.v[s][r][c] = load_page<SHARED, typename L::piece>(
                         (const char *)a.v + from[s] + off_v +
                         (r * HD + 16 * L::VD * c) * (int)sizeof(T));
     };
@@ -559,7 +572,8 @@ __device__ __forceinline__ void attend(const PagedAttention &a, int entry, int r
 
 template <typename T, int HD, bool FEW>
 __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(PagedAttention a) {
-    Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
+    __shared__ __align__(16) Scratch<T, HD, kWaves> scratch;
+    Line<T, HD, true> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
     uint32_t t = blockIdx.x, t_end = t + (t < all);  // with shares a place is a workgroup's
     if (!line.share) {
@@ -592,8 +606,18 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
             j0 = p0 > line.kBegin ? p0 - line.kBegin : 0;
             j1 = p1 - line.kBegin;
         }
-        attend<T, HD, kWaves, FEW>(a, line.first + el, row, keys, (int)unit, (int)j0, (int)j1,
-                              j0 == 0 && j1 == tiles, 2 * (int64_t)blockIdx.x + (j0 == 0));
+        // another entry of the 64 begins with the same page
+        const int32_t page = __builtin_amdgcn_readlane(line.page, el);
+        const uint64_t same = __ballot(line.page == page);
+        const int entry = line.first + el;
+        const bool whole = j0 == 0 && j1 == tiles;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (j0 == 0);
+        if (same & (same - 1))
+            attend<T, HD, kWaves, FEW, true>(a, entry, row, keys, (int)unit, (int)j0, (int)j1,
+                                             whole, slot, scratch);
+        else
+            attend<T, HD, kWaves, FEW, false>(a, entry, row, keys, (int)unit, (int)j0, (int)j1,
+                                              whole, slot, scratch);
     }
 }
 
@@ -601,6 +625,7 @@ __global__ __launch_bounds__(kBlock, HD > 128 ? 1 : 2) void paged_attention(Page
 template <typename T, int HD, bool FEW>
 __global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short(PagedAttention a) {
     constexpr int TILE = tile_keys<T>(), WAVES = short_waves(HD), VEC = HD / kWave;
+    __shared__ __align__(16) Scratch<T, HD, WAVES> scratch;
     const int units = a.kv * a.head_groups;
     const int entry = blockIdx.x / units, unit = blockIdx.x - entry * units;
     const int row = a.index[entry];
@@ -608,7 +633,8 @@ __global__ __launch_bounds__(short_waves(HD) * kWave) void paged_attention_short
     const int keys = entry_keys(a, row, a.positions[entry], bad);
     if (bad && unit == 0 && threadIdx.x == 0) raise_flag(a.error_flag);
     if (keys) {
-        attend<T, HD, WAVES, FEW>(a, entry, row, keys, unit, 0, (keys + TILE - 1) / TILE, true, 0);
+        attend<T, HD, WAVES, FEW, false>(a, entry, row, keys, unit, 0, (keys + TILE - 1) / TILE,
+                                         true, 0, scratch);
         return;
     }
     const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
@@ -637,7 +663,7 @@ __global__ __launch_bounds__(THREADS) void paged_attention_join(PagedAttention a
     const int dim = HD / kWave * l;
     T gate[HD / kWave] = {};
     if (wv == 0) load_gate(a, entry, h0, dim, gate);
-    Line<T, HD> line{a, (uint32_t)(a.kv * a.head_groups)};
+    Line<T, HD, false> line{a, (uint32_t)(a.kv * a.head_groups)};
     const uint32_t all = line.total();
     while (line.first + kWave <= entry) line.next();
     const int keys = __builtin_amdgcn_readlane(line.keys, entry - line.first);

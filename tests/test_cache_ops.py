@@ -476,6 +476,21 @@ def test_paged_attention_dealt(H, KV, hd, lengths, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 256), (4, 2, 64), (12, 4, 128), (10, 2, 64)])
+def test_paged_attention_shared_pages(H, KV, hd, dtype):
+    """Rows that hold the same pages, some only the first of them, beside one that does not."""
+    lengths = [900, 900, 611, 900, 640]
+    case = attend_case(hd + H, H, KV, hd, 16, lengths, dtype)
+    table = case[4].copy()
+    table[1] = table[0]
+    table[4, :20] = table[0, :20]
+    pos = np.array(lengths) - 1
+    pos[1] = 555
+    assert attend_check(case, pos, 16, dtype, None, table=table) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_attention_rising_scores(dtype):
     """Scores that rise along the keys by hundreds, so that begun sums are rescaled,
     and a last key far below: its weight is nothing."""
