@@ -280,18 +280,27 @@ class BackboneCache:
         slots = (held[:, None] * cfg.conv_kernel
                  + at[:, -last:].long() % cfg.conv_kernel).view(-1)
 
+        last_row = lambda t: t.view(B, S, *t.shape[1:])[:, -1]  # noqa: E731
+
         def mix(i, layer, proj):
             a = self.plane[i]
+            final = i + 1 == len(model.layers)   # of it only the last tokens go on
             if layer["kind"] == "full_attention":
                 q, k, v, gate = self._split_proj(proj)
-                k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+                keys, values = self.pool[2 * a], self.pool[2 * a + 1]
+                k_out = None if final else torch.empty(k.shape, dtype=k.dtype, device=k.device)
                 q = cache_ops.prepare_paged(q, k, v, layer["q_norm"], layer["k_norm"], self.tables,
                                             cfg.rotary_dim if self.tables else 0, cfg.eps,
-                                            token_rows, token_at, self.book.table,
-                                            self.pool[2 * a], self.pool[2 * a + 1], k_out=k_out,
-                                            error_flag=self._flag)
+                                            token_rows, token_at, self.book.table, keys, values,
+                                            k_out=k_out, error_flag=self._flag)
+                out_dtype = model.gemm_in or model.dtype
+                if final:
+                    return cache_ops.paged_attention(last_row(q), keys, values, self.book.table,
+                                                     rows, at[:, -1].contiguous(), self.scale,
+                                                     gate=last_row(gate), out_dtype=out_dtype,
+                                                     error_flag=self._flag)
                 return ops.attention_fused(q, k_out, v, gate, mask, self.scale, B,
-                                           out_dtype=model.gemm_in or model.dtype)
+                                           out_dtype=out_dtype)
             kd, kh, vd, vh = cfg.key_dim, cfg.key_heads, cfg.value_dim, cfg.value_heads
             kw, vw = kd * kh, vd * vh
             channels = 2 * kw + vw
@@ -305,11 +314,12 @@ class BackboneCache:
             self.rings[a].view(-1, channels).index_copy_(
                 0, slots, proj.view(B, S, -1)[:, -last:, :channels].reshape(-1, channels))
             z = proj[:, channels:channels + vw].view(-1, vh, vd)
-            return ops.native_gated_rms(x.view(-1, vh, vd), z, layer["norm"], cfg.eps,
-                                        out_dtype=model.gemm_in).view(B * S, -1)
+            x = ops.native_gated_rms(x.view(-1, vh, vd), z, layer["norm"], cfg.eps,
+                                     out_dtype=model.gemm_in).view(B * S, -1)
+            return last_row(x).contiguous() if final else x
 
         return self._through(ids.reshape(-1).contiguous(), keep, mix,
-                             lambda t: t.view(B, S, -1)[:, -1].contiguous())
+                             lambda h: last_row(h).contiguous())
 
     def _token(self, ids, rows, at):
         """One token of each row from and into the cache."""
@@ -336,8 +346,8 @@ class BackboneCache:
         return self._through(ids, None, mix, lambda t: t)
 
     def _through(self, ids, keep, mix, last_rows):
-        """``QwenBackbone.forward`` around the layers' mixing step: ``last_rows`` of the
-        last layer alone go on after it."""
+        """``QwenBackbone.forward`` around the layers' mixing step; in the last layer it
+        gives the rows that go on, of whose residuals ``last_rows`` takes the same."""
         model, cfg = self.model, self.model.cfg
         count = len(model.layers)
         masked = lambda i: keep if model.layers[i]["kind"] != "full_attention" else None  # noqa: E731
@@ -351,7 +361,7 @@ class BackboneCache:
             mixed = mix(i, layer, model._mm(normed, layer["qkv" if attention else "proj"]))
             last = i + 1 == count
             if last:
-                h, mixed = last_rows(h), last_rows(mixed)
+                h = last_rows(h)
             h, normed = self._project_add_norm(h, mixed, layer, "out", layer["post_norm"],
                                                out_dtype=model.mlp_in)
             gate_up = (model._mm32 if model.split else model._mm)(normed, layer["gate_up"])
@@ -392,7 +402,7 @@ class BackboneCache:
                                          token_mask=masked(i))
             mixed = mix(i, layer, proj)
             if i + 1 == len(model.layers):
-                h, mixed = last_rows(h), last_rows(mixed)
+                h = last_rows(h)
             h, act = ops.linear_f32(h, layer["gate_up"], add=ops.linear_f32(mixed, layer["out"]),
                                     weight=layer["post_norm"], eps=eps, swiglu=True)
             due = ops.linear_f32(act, layer["down"])
