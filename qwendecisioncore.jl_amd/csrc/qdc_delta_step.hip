@@ -76,7 +76,7 @@ __global__ __launch_bounds__(step_threads(STREAM)) void delta_step(DeltaStep a) 
     // an address within the cache, whatever the entry holds; what comes from there is
     // used only once the entry has been checked
     const int64_t safe = min(max(row, 0), a.rows - 1);
-    const int p0 = max(pos, 0);
+    const uint32_t p0 = (uint32_t)max(pos, 0);
 
     // everything a thread reads, the small things first: the token's channels of this
     // head (q | k | v), their window, the gates, and then the state
@@ -96,7 +96,8 @@ __global__ __launch_bounds__(step_threads(STREAM)) void delta_step(DeltaStep a) 
 #pragma unroll
         for (int lag = 0; lag < W; ++lag) {  // tap taps - 1 - lag
             if (!TAPS && lag >= taps) continue;
-            if (lag) window[lag] = ring[(int64_t)((p0 + taps - lag) % taps) * cq + c];
+            // (without a sign: the sum may pass 2^31)
+            if (lag) window[lag] = ring[(p0 + (uint32_t)(taps - lag)) % (uint32_t)taps * cq + c];
             conv[lag] = a.conv[c * taps + (taps - 1 - lag)];
         }
     }

@@ -919,6 +919,21 @@ def test_delta_step_rows(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("taps", [3, 4, 8])
+def test_delta_step_last_positions(taps):
+    """The largest positions there are: the window's slots are those of the tokens before,
+    whatever their sum with the taps passes."""
+    KH, H, kd, vd, n = 2, 4, 32, 32, 9
+    s = step_case(taps, KH, H, kd, vd, taps, n, n, torch.float32)
+    s["pos"] = [2 ** 31 - 1 - i for i in range(n)]
+    s["rows"] = list(range(n))          # the largest in the first row
+    f = flag()
+    got = step_run(s, KH, H, kd, vd, error_flag=f)
+    step_near(got, step_exact(s, KH, kd, H, vd, taps), KH, kd, vd, torch.float32)
+    assert f.item() == 0
+
+
+@pytest.mark.gpu
 def test_delta_step_large_state():
     """A state of 128 MB and more is streamed: the same bits as rows a few at a time."""
     KH, H, kd, vd, n = 16, 32, 128, 128, 70
