@@ -121,10 +121,11 @@ class BackboneCache:
         if self._heads() and not ops.attention_fused_takes(self.model.dtype, cfg.head_dim, B, S,
                                                            cfg.heads, cfg.kv_heads):
             raise ValueError("Too many or too long prompts for one call.")
-        rows = self._take(B)
+        rows = self._next(B)
         d_ids, d_mask = bb._upload(self.model, ids, mask)
         at = np.arange(S) - (S - counts[:, None])
         d_rows, d_counts, d_at = self._ints(np.asarray(rows), counts, at)
+        self._take(B)
         try:
             cache_ops.extend_pages(self.book, d_rows, d_counts, error_flag=self._flag)
             out = _host(self._prompt(d_ids, d_mask, d_rows, d_at.view(B, S)))
@@ -146,8 +147,9 @@ class BackboneCache:
         parents = self._in_use(rows, distinct=False)
         if not parents:
             return []
-        children = self._take(len(parents))
+        children = self._next(len(parents))
         src, dst = self._ints(np.asarray(parents), np.asarray(children))
+        self._take(len(children))
         try:
             cache_ops.fork_pages(self.book, src, dst, self._pool(), error_flag=self._flag)
             if self.states.shape[0]:
@@ -220,10 +222,14 @@ class BackboneCache:
             raise ValueError("A row is named twice.")
         return rows
 
-    def _take(self, n: int) -> list:
+    def _next(self, n: int) -> list:
+        """The rows that :meth:`_take` takes: a call that raises before it has lost none."""
         if n > len(self._unused):
             raise RuntimeError("Too few free rows.")
-        return [self._unused.pop() for _ in range(n)]
+        return self._unused[len(self._unused) - n:][::-1]
+
+    def _take(self, n: int) -> None:
+        del self._unused[len(self._unused) - n:]
 
     def _end(self, rows, d_rows) -> None:
         cache_ops.free_pages(self.book, d_rows)

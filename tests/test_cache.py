@@ -176,6 +176,33 @@ def test_a_call_that_raises_leaves_no_flag_and_no_rows(monkeypatch):
 
 
 @pytest.mark.gpu
+def test_an_upload_that_raises_changes_nothing(monkeypatch):
+    """No memory for a call's own numbers: every row, free or not, is what it was."""
+    from qdc_amd import backbone
+    from qdc_amd.cache import BackboneCache
+    model = model_of("f32")
+    cache = BackboneCache(model, rows=4, pages=20, page_size=16)
+    (a,), _ = cache.prefill(np.arange(30))
+
+    def fail(*args, **kwargs):
+        raise MemoryError("none left")
+
+    prompt = lambda: cache.prefill([1, 2, 3])  # noqa: E731
+    for where, name, call in ((backbone, "_upload", prompt), (BackboneCache, "_ints", prompt),
+                              (BackboneCache, "_ints", lambda: cache.fork([a, a])),
+                              (BackboneCache, "_ints", lambda: cache.step([a], [1])),
+                              (BackboneCache, "_ints", lambda: cache.free([a]))):
+        with monkeypatch.context() as m:
+            m.setattr(where, name, fail)
+            with pytest.raises(MemoryError):
+                call()
+        assert cache.lengths() == {a: 30} and cache.free_page_count() == 18
+    assert sorted([a] + cache.fork([a, a, a])) == [0, 1, 2, 3]
+    got = cache.step([a], [7])
+    assert normwise(got[0], whole(model, list(range(30)) + [7])) <= BARS["f32"]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("mode", ["f32", "mlp"])
 def test_step_graphs(mode):
     """Recorded steps beside eager ones of a second cache: the same bits with the same
