@@ -43,7 +43,7 @@ class BackboneCache:
     :meth:`free`.  Invalid ids, masks and rows raise ``ValueError`` before anything
     runs; too few free pages (or rows) raise ``RuntimeError``, and every sequence is
     as it was before the call.  (Where torch itself raises within a call, for want of
-    memory say, the rows that the call was at are ended.)  One call at a time per
+    memory say, or the call is interrupted, the rows that it was at are ended.)  One call at a time per
     instance (a lock), all of them on one stream, the device's current one; prefill,
     step and fork wait for their result.  The cache takes
     ``2 * attention layers * pages * kv_heads * page_size * head_dim`` values in the
@@ -121,18 +121,18 @@ class BackboneCache:
         if self._heads() and not ops.attention_fused_takes(self.model.dtype, cfg.head_dim, B, S,
                                                            cfg.heads, cfg.kv_heads):
             raise ValueError("Too many or too long prompts for one call.")
-        rows = self._next(B)
+        rows = self._next(B)            # none is taken before the call is done
         d_ids, d_mask = bb._upload(self.model, ids, mask)
         at = np.arange(S) - (S - counts[:, None])
         d_rows, d_counts, d_at = self._ints(np.asarray(rows), counts, at)
-        self._take(B)
         try:
             cache_ops.extend_pages(self.book, d_rows, d_counts, error_flag=self._flag)
             out = _host(self._prompt(d_ids, d_mask, d_rows, d_at.view(B, S)))
-        except Exception:
+            done = self._settle(rows, counts)
+        except BaseException:
             self._abandon(rows, d_rows)
             raise
-        return self._finish(out, rows, rows, {r: int(c) for r, c in zip(rows, counts)})
+        return self._answer(done, (rows, out))
 
     @_call
     def step(self, rows, ids) -> np.ndarray:
@@ -149,18 +149,17 @@ class BackboneCache:
             return []
         children = self._next(len(parents))
         src, dst = self._ints(np.asarray(parents), np.asarray(children))
-        self._take(len(children))
         try:
             cache_ops.fork_pages(self.book, src, dst, self._pool(), error_flag=self._flag)
             if self.states.shape[0]:
                 for part in zip(src.split(4096), dst.split(4096)):
                     cache_ops.copy_pages(self.states, *part)
                     cache_ops.copy_pages(self.rings, *part)
-        except Exception:
+            done = self._settle(children, [self._lengths[p] for p in parents])
+        except BaseException:
             self._abandon(children, dst)
             raise
-        return self._finish(None, children, children,
-                            {c: self._lengths[p] for p, c in zip(parents, children)})
+        return self._answer(done, children)
 
     @_call
     def free(self, rows) -> None:
@@ -168,6 +167,7 @@ class BackboneCache:
         rows = self._in_use(rows)
         if rows:
             self._end(rows, *self._ints(np.asarray(rows)))
+            self._unused += rows[::-1]
 
     @_call
     def compact(self) -> None:
@@ -195,18 +195,16 @@ class BackboneCache:
         d_rows, d_ids = self._ints(np.asarray(rows), ids)
         try:
             out = _host(self._advance(d_rows, d_ids))
-        except Exception:
+            done = self._settle_step(rows)
+        except BaseException:
             self._abandon(rows, d_rows)
             raise
-        return self._stepped(out, rows)
+        return self._answer(done, out)
 
     def _advance(self, rows, ids):
         """One more token of each row; an entry with row -1 is none."""
         at = cache_ops.extend_pages(self.book, rows, error_flag=self._flag)
         return self._token(ids, rows, at)
-
-    def _stepped(self, out, rows, flagged=None) -> np.ndarray:
-        return self._finish(out, [], None, {r: self._lengths[r] + 1 for r in rows}, flagged)
 
     def _heads(self) -> bool:
         return self.pool.shape[0] > 0
@@ -223,24 +221,46 @@ class BackboneCache:
         return rows
 
     def _next(self, n: int) -> list:
-        """The rows that :meth:`_take` takes: a call that raises before it has lost none."""
+        """The free rows that a call of ``n`` new sequences is to take."""
         if n > len(self._unused):
             raise RuntimeError("Too few free rows.")
         return self._unused[len(self._unused) - n:][::-1]
 
-    def _take(self, n: int) -> None:
-        del self._unused[len(self._unused) - n:]
+    def _settle(self, rows, lengths, flagged=None) -> bool:
+        """Waits for a call and writes down what its rows hold now, new ones being those
+        of :meth:`_next`; nothing, and False, where a kernel flagged it."""
+        if int(self._flag.item() if flagged is None else flagged) != 0:
+            self._flag.zero_()
+            return False
+        new = sum(r not in self._lengths for r in rows)
+        self._lengths.update({r: int(n) for r, n in zip(rows, lengths)})
+        del self._unused[len(self._unused) - new:]
+        return True
 
-    def _end(self, rows, d_rows) -> None:
-        cache_ops.free_pages(self.book, d_rows)
+    def _settle_step(self, rows, flagged=None) -> bool:
+        return self._settle(rows, [self._lengths[r] + 1 for r in rows], flagged)
+
+    @staticmethod
+    def _answer(done, result):
+        if not done:
+            raise RuntimeError("Too few free pages.")
+        return result
+
+    def _end(self, rows, d_rows=None) -> None:
+        # the host first: were what follows to raise, the rows would be lost, and not taken
+        # for something that the device does not hold
         for r in rows:
             self._lengths.pop(r, None)
-        self._unused += rows[::-1]
+        cache_ops.free_pages(self.book, self._ints(np.asarray(rows))[0] if d_rows is None
+                             else d_rows)
 
-    def _abandon(self, rows, d_rows) -> None:
-        """Ends the rows of a call that raised; what it flagged is not the next call's."""
+    def _abandon(self, rows, d_rows=None) -> None:
+        """Ends the rows of a call that raised, wherever it did; what it flagged is not the
+        next call's."""
         self._end(rows, d_rows)
         self._flag.zero_()
+        free = set(self._unused)
+        self._unused += [r for r in rows[::-1] if r not in free]
 
     def _ints(self, *arrays):
         """Host arrays to the device as int32 vectors, in one copy (what follows starts
@@ -253,17 +273,6 @@ class BackboneCache:
             packed[start:start + a.size] = a
         dev = torch.from_numpy(packed).to(self.model.device)
         return tuple(dev[end - -(-a.size // 4) * 4:][:a.size] for a, end in zip(flat, ends))
-
-    def _finish(self, out, taken, result, lengths, flagged=None):
-        """Waits for the call, and takes it back if a kernel flagged it."""
-        if int(self._flag.item() if flagged is None else flagged) != 0:
-            self._flag.zero_()
-            self._unused += taken[::-1]
-            raise RuntimeError("Too few free pages.")
-        self._lengths.update(lengths)
-        if result is None:
-            return out
-        return result if out is None else (result, out)
 
     # -------------------------------------------------------------- layers --
     def _split_proj(self, proj):

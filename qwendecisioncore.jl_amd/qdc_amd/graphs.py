@@ -318,7 +318,9 @@ class StepGraphs(_Recordings):
                 e.out_host.copy_(e.out.float(), non_blocking=True)
                 e.flag_host.copy_(cache._flag, non_blocking=True)
                 torch.cuda.current_stream(self.model.device).synchronize()
-            except Exception:
-                cache._abandon(rows, *cache._ints(np.asarray(rows)))
+                out = e.out_host.numpy().copy()
+                done = cache._settle_step(rows, int(e.flag_host[0]))
+            except BaseException:
+                cache._abandon(rows)
                 raise
-            return cache._stepped(e.out_host.numpy().copy(), rows, int(e.flag_host[0]))
+            return cache._answer(done, out)

@@ -202,6 +202,100 @@ def test_an_upload_that_raises_changes_nothing(monkeypatch):
     assert normwise(got[0], whole(model, list(range(30)) + [7])) <= BARS["f32"]
 
 
+def interrupted(wait):
+    """``wait`` with an interrupt that arrives while it waits, once."""
+    left = [1]
+
+    def call(*args, **kwargs):
+        out = wait(*args, **kwargs)
+        if left:
+            left.pop()
+            raise KeyboardInterrupt
+        return out
+    return call
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["prefill", "step", "fork", "graphs"])
+@pytest.mark.parametrize("wait", ["cpu", "item", "synchronize"])
+def test_an_interrupted_call_ends_its_rows(monkeypatch, what, wait):
+    """An interrupt while a call waits for the device: the rows that it was at are ended
+    or, where it did not wait so, as the call leaves them; no row has tokens that
+    ``lengths`` does not say, and every row and page can be taken again."""
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.graphs import StepGraphs
+    model = model_of("f32")
+    cache = BackboneCache(model, rows=4, pages=12, page_size=16)
+    graphs = StepGraphs(cache, gemm_libraries=None)
+    rng = np.random.default_rng(3)
+    prompts = rng.integers(0, model.vocab, (2, 31))
+    (a, b), _ = cache.prefill(prompts)
+    held = {a: prompts[0].tolist(), b: prompts[1].tolist()}
+    graphs([a], [1]), held[a].append(1)
+    where = torch.cuda.Stream if wait == "synchronize" else torch.Tensor
+    with monkeypatch.context() as m:
+        m.setattr(where, wait, interrupted(getattr(where, wait)))
+        try:
+            if what == "prefill":
+                rows, _ = cache.prefill(prompts[0, :20])
+                held[rows[0]] = prompts[0, :20].tolist()
+            elif what == "fork":
+                kid, = cache.fork([b])
+                held[kid] = list(held[b])
+            else:
+                (cache.step if what == "step" else graphs)([b], [5])
+                held[b].append(5)
+            stopped = False
+        except KeyboardInterrupt:
+            stopped = True
+    if stopped and what in ("step", "graphs"):
+        del held[b]
+    assert stopped == ((wait, what) in (("cpu", "prefill"), ("cpu", "step"), ("item", "prefill"),
+                                        ("item", "step"), ("item", "fork"),
+                                        ("synchronize", "graphs")))
+    assert cache.lengths() == {r: len(t) for r, t in held.items()}
+    lengths = cache.book.lengths.tolist()
+    assert lengths == [len(held.get(r, [])) for r in range(4)]
+    for r in held:
+        got = cache.step([r], [9])
+        held[r].append(9)
+        assert normwise(got[0], whole(model, held[r])) <= BARS["f32"]
+    rest = 4 - len(held)
+    rows, got = cache.prefill(np.tile(prompts[1], (rest, 1)))
+    assert sorted(rows + list(held)) == [0, 1, 2, 3]
+    for g in got:
+        assert normwise(g, whole(model, prompts[1])) <= BARS["f32"]
+    cache.free(list(cache.lengths()))
+    assert cache.free_page_count() == 12
+
+
+@pytest.mark.gpu
+def test_an_interrupted_replay_without_memory(monkeypatch):
+    """Where the rows of an interrupted call cannot be ended either, they are out of use."""
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.graphs import StepGraphs
+    model = model_of("f32")
+    cache = BackboneCache(model, rows=3, pages=12, page_size=16)
+    graphs = StepGraphs(cache, gemm_libraries=None)
+    (a, b), _ = cache.prefill([[1, 2, 3], [4, 5, 6]])
+    graphs([a], [1])
+
+    def fail(*args, **kwargs):
+        raise MemoryError("none left")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda.Stream, "synchronize", interrupted(torch.cuda.Stream.synchronize))
+        m.setattr(BackboneCache, "_ints", fail)
+        with pytest.raises((MemoryError, KeyboardInterrupt)):
+            graphs([b], [1])
+    assert cache.lengths() == {a: 4}
+    for call in (graphs, cache.step):
+        with pytest.raises(ValueError):
+            call([b], [2])
+    got = cache.step([a], [7])
+    assert normwise(got[0], whole(model, [1, 2, 3, 1, 7])) <= BARS["f32"]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("mode", ["f32", "mlp"])
 def test_step_graphs(mode):
