@@ -437,4 +437,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "qdc_calls", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_qdc_calls() { return PyModule_Create(&module); }
+// version: of the header whose entry points the functions call
+PyMODINIT_FUNC PyInit_qdc_calls() {
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "version", QDC_HIP_CACHE_VERSION) == 0) return m;
+    Py_XDECREF(m);
+    return nullptr;
+}

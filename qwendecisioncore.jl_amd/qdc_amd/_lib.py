@@ -2,8 +2,8 @@
 
 The library is loaded from ``qwendecisioncore.jl_amd/lib/`` (built in-tree by
 ``make -C qwendecisioncore.jl_amd/csrc``).  There is no fallback: a missing
-library is an error.  ``lib/qdc_calls.so``, built with it, calls the cache's operators
-for PyTorch tensors.  Status codes map to exceptions the way the reference maps
+library is an error.  ``lib/qdc_calls.so`` (``make -C qwendecisioncore.jl_amd/csrc
+python``) calls the cache's operators for PyTorch tensors.  Status codes map to exceptions the way the reference maps
 bad input to ``ArgumentError`` / ``DimensionMismatch``: a negative status raises
 ``ValueError`` (argument error found on the host before any launch), a positive
 one ``RuntimeError`` (HIP launch failure).
@@ -139,11 +139,15 @@ def calls():
         lib()
         if not os.path.exists(CALLS_PATH):
             raise RuntimeError(f"{CALLS_PATH} is not built; run `make -C "
-                               "qwendecisioncore.jl_amd/csrc` or __graft_entry__.build()")
+                               "qwendecisioncore.jl_amd/csrc python` or __graft_entry__.build()")
         loader = importlib.machinery.ExtensionFileLoader("qdc_calls", CALLS_PATH)
         module = importlib.util.module_from_spec(
             importlib.util.spec_from_file_location("qdc_calls", CALLS_PATH, loader=loader))
         loader.exec_module(module)
+        version = lib().qdc_cache_version().decode()
+        if module.version != version:   # the arguments may be others
+            raise RuntimeError(f"{CALLS_PATH} was built for {module.version!r}, the library is "
+                               f"{version!r}; run `make -C qwendecisioncore.jl_amd/csrc python`")
         module.on_failure(check)
         _calls = module
     return _calls

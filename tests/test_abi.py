@@ -528,3 +528,34 @@ def test_c_host_program_host_only(tmp_path):
     r = subprocess.run([str(exe), "--host-only"], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "all checks passed" in r.stdout
+
+
+def test_the_library_builds_without_torch():
+    """A C or Julia host's build is the library alone; what needs torch is a target of its
+    own."""
+    directory = os.path.join(ROOT, "qwendecisioncore.jl_amd", "csrc")
+
+    def commands(*targets):  # of a build from nothing, with a Python that has no torch
+        return subprocess.run(["make", "-n", "-B", "-C", directory, "PYTHON=/bin/false", *targets],
+                              check=True, capture_output=True, text=True).stdout
+
+    alone = commands()
+    assert "libqdc_hip.so" in alone and "qdc_pages.hip" in alone
+    assert "qdc_calls" not in alone and "torch" not in alone
+    assert "qdc_calls.cpp" in commands("python") and "libqdc_hip.so" in commands("python")
+
+
+def test_calls_are_of_the_library_s_version(monkeypatch):
+    """The module that calls the cache's operators is refused beside a library with other
+    entry points."""
+    assert _lib.calls().version == _lib.lib().qdc_cache_version().decode()
+
+    class Other:
+        @staticmethod
+        def qdc_cache_version():
+            return b"qdc_hip_cache 9.9.9"
+
+    monkeypatch.setattr(_lib, "_calls", None)
+    monkeypatch.setattr(_lib, "lib", lambda: Other)
+    with pytest.raises(RuntimeError, match="9.9.9"):
+        _lib.calls()
