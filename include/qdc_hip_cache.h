@@ -14,7 +14,8 @@
  *   lengths int32 [rows]: positions that a row holds;
  *   refs    int32 [pages]: rows that share a page;
  *   free    int32 [1 + pages]: a count c, then the free pages as a stack, its top at c.
- * A page that is not full belongs to one row alone.
+ * A page that is not full belongs to one row alone.  pages and rows * width are at most
+ * 2^31 - 1024, width * page_size below 2^31 (QDC_ERR_SHAPE otherwise).
  *
  * A call's tokens are named by `index` (the row of the cache, int32 [n]) and
  * `positions` (int32 [n]).  An entry whose row or position is negative is no token:

@@ -17,6 +17,8 @@ namespace {
 constexpr int kBook = 1024;              // threads of the bookkeeping workgroup
 constexpr int kBookWaves = kBook / kWave;
 constexpr int kMaxRows = 1 << 18;        // rows of a cache: a bit each in LDS
+// pages, and places of a table: lists of them are walked in steps of kBook, in 32 bits
+constexpr int64_t kMaxPages = ((int64_t)1 << 31) - kBook;
 
 struct Book {
     int32_t *table, *lengths, *refs, *free_pages;
@@ -528,8 +530,8 @@ int32_t check_book(const int32_t *table, const int32_t *lengths, const int32_t *
                    int64_t pages, int64_t page_size) {
     const int64_t lim = (int64_t)1 << 31;
     if (n < 0 || n >= ((int64_t)1 << 24) || rows <= 0 || rows >= kMaxRows || width <= 0 ||
-        pages <= 0 || pages >= lim - 1 || page_shift(page_size) < 0 || width >= lim / page_size ||
-        rows * width >= lim)
+        pages <= 0 || pages > kMaxPages || page_shift(page_size) < 0 ||
+        width >= lim / page_size || rows * width > kMaxPages)
         return QDC_ERR_SHAPE;
     if (n && (!table || !lengths || !refs || !free_pages)) return QDC_ERR_NULL;
     return QDC_OK;
@@ -648,7 +650,7 @@ extern "C" int32_t qdc_pages_fork(int32_t *table, int32_t *lengths, int32_t *ref
 }
 
 extern "C" int64_t qdc_pages_compact_workspace(int64_t pages) {
-    return pages <= 0 || pages >= ((int64_t)1 << 31) - 1 ? 0 : 16 + 12 * pages;
+    return pages <= 0 || pages > kMaxPages ? 0 : 16 + 12 * pages;
 }
 
 extern "C" int32_t qdc_pages_compact(int32_t *table, int32_t *refs, int32_t *free_pages,

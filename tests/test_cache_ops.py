@@ -151,6 +151,31 @@ def test_pages_validation():
     assert copy(n=4096, planes=1024, nbytes=65536) == -2
 
 
+def test_pages_largest_counts():
+    """Lists of pages are walked 1024 at a time in 32 bits: the sizes that a step past their
+    end would leave are refused, the last before them are taken (by what each refuses next:
+    a missing index or workspace)."""
+    lib, most = _lib.lib(), 2 ** 31 - 1024
+    T, L, R, S, W = (FAR << i for i in range(5))
+    wide = 2 ** 27 - 1                      # 16 rows of it are 2^31 - 16 places
+
+    def calls(rows, width, pages):
+        at = (T, L, R, S)
+        size = (rows, width, pages, 16)
+        return (lib.qdc_pages_extend(FAKE, *at, None, None, 4, *size, None, None),
+                lib.qdc_pages_free(*at, None, 4, *size, None, None),
+                lib.qdc_pages_fork(*at, None, None, 4, *size, None, 0, 0, 0, None, 0, None, None))
+
+    assert calls(5, 6, most) == calls(15, wide, 7) == (-1, -1, -1)
+    for bad in ((5, 6, most + 1), (5, 6, 2 ** 31 - 2), (16, wide, 7)):
+        assert calls(*bad) == (-2, -2, -2), bad
+    need = lib.qdc_pages_compact_workspace(most)
+    assert need == 16 + 12 * most and lib.qdc_pages_compact_workspace(most + 1) == 0
+    compact = lambda pages, nbytes: lib.qdc_pages_compact(T, R, S, 5, 6, pages, None, 0, 0, None,  # noqa: E731
+                                                          nbytes, None)
+    assert compact(most, need) == -1 and compact(most + 1, 1 << 40) == -2
+
+
 def test_delta_step_validation():
     names = ("proj", "conv", "a_decay", "dt_bias", "norm", "ring", "state", "index", "positions")
 
