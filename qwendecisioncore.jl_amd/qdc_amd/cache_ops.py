@@ -46,9 +46,13 @@ class PageTable(NamedTuple):
 
 def page_table(rows: int, width: int, pages: int, page_size: int, device) -> PageTable:
     """An empty :class:`PageTable` of ``rows`` rows of up to ``width`` pages each, the
-    lowest of ``pages`` free pages on top of the stack."""
+    lowest of ``pages`` free pages on top of the stack.  ``rows`` below 2^18, ``width *
+    page_size`` below 2^31, ``pages`` and ``rows * width`` at most 2^31 - 1024."""
     if rows <= 0 or width <= 0 or pages <= 0 or page_size not in PAGE_SIZES:
         raise ValueError(f"rows, width and pages must be positive, page_size one of {PAGE_SIZES}")
+    most = 2 ** 31 - 1024
+    if rows >= 2 ** 18 or width * page_size >= 2 ** 31 or pages > most or rows * width > most:
+        raise ValueError("too many rows or pages, or too wide a table, for the operators")
     i32 = dict(dtype=torch.int32, device=device)
     free = torch.empty(1 + pages, **i32)
     free[0] = pages

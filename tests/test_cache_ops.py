@@ -176,6 +176,17 @@ def test_pages_largest_counts():
     assert compact(most, need) == -1 and compact(most + 1, 1 << 40) == -2
 
 
+def test_page_table_limits():
+    """A table that the operators would refuse at every call is not made."""
+    for rows, width, pages, page in ((2 ** 18, 1, 1, 16), (1, 2 ** 23, 1, 256), (1, 2 ** 27, 1, 16),
+                                     (1, 1, 2 ** 31 - 1023, 16), (2 ** 17, 2 ** 14, 1, 16)):
+        with pytest.raises(ValueError, match="too many rows"):
+            cache_ops.page_table(rows, width, pages, page, "meta")
+    for rows, width, pages, page in ((2 ** 18 - 1, 1, 1, 16), (1, 2 ** 23 - 1, 1, 256),
+                                     (1, 1, 2 ** 31 - 1024, 16), (2 ** 17, 2 ** 14 - 1, 1, 16)):
+        assert cache_ops.page_table(rows, width, pages, page, "meta").table.shape == (rows, width)
+
+
 def test_delta_step_validation():
     names = ("proj", "conv", "a_decay", "dt_bias", "norm", "ring", "state", "index", "positions")
 
