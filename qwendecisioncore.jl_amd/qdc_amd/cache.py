@@ -18,7 +18,7 @@ import threading
 import numpy as np
 import torch
 
-from . import backbone as bb
+from . import _lib, backbone as bb
 from . import cache_ops, ops
 
 
@@ -68,6 +68,14 @@ class BackboneCache:
                              "of a multiple of 16 up to 256 and at most 8 convolution taps.")
         self.model, self.rows, self.max_tokens = model, rows, max_tokens
         dev, width = model.device, -(-max_tokens // page_size)
+        # rows of one call, of which attention takes fewer the more tokens they may hold
+        self._most = rows
+        while attention and self._most and _lib.lib().qdc_paged_attention_workspace(
+                self._most, cfg.heads, cfg.kv_heads, cfg.head_dim, width, page_size,
+                ops._DTYPES[model.dtype]) < 0:
+            self._most //= 2
+        if not self._most:
+            raise ValueError("max_tokens is too large.")
         self.book = cache_ops.page_table(rows, width, pages, page_size, dev)
         # planes 2 a and 2 a + 1: K and V of attention layer a
         self.pool = torch.zeros((2 * len(attention), pages, cfg.kv_heads, page_size, cfg.head_dim),
@@ -117,6 +125,7 @@ class BackboneCache:
         counts = mask.sum(1)
         if counts.max() > self.max_tokens:
             raise ValueError(f"A sequence holds at most {self.max_tokens} tokens.")
+        self._check_count(B)
         cfg = self.model.cfg
         if self._heads() and not ops.attention_fused_takes(self.model.dtype, cfg.head_dim, B, S,
                                                            cfg.heads, cfg.kv_heads):
@@ -189,7 +198,13 @@ class BackboneCache:
         ops.check_ids(ids, self.model.vocab)
         if any(self._lengths[r] >= self.max_tokens for r in rows):
             raise ValueError(f"A sequence holds at most {self.max_tokens} tokens.")
+        self._check_count(len(rows))
         return rows, ids
+
+    def _check_count(self, n: int) -> None:
+        if n > self._most:
+            raise ValueError(f"With {self.max_tokens} tokens a sequence a call takes at most "
+                             f"{self._most} of them.")
 
     def _step(self, rows, ids) -> np.ndarray:
         d_rows, d_ids = self._ints(np.asarray(rows), ids)

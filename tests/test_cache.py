@@ -402,6 +402,40 @@ def test_refusals():
 
 
 @pytest.mark.gpu
+def test_more_rows_than_a_call_takes():
+    """Where sequences may be so long that attention does not take all rows at once, a call
+    of too many is refused before anything runs, and its rows go on."""
+    import dataclasses
+
+    from qdc_amd import _lib, backbone
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.config import synthetic_inference_config
+    from qdc_amd.graphs import StepGraphs
+    from qdc_amd.weights import random_weights
+    cfg = dataclasses.replace(synthetic_inference_config(), layer_types=("full_attention",),
+                              rotary_dim=0)
+    model = backbone.QwenBackbone.from_weights(random_weights(cfg, seed=2), cfg)
+    tokens, rows = 2 ** 26, 300
+    takes = lambda n, t=tokens: _lib.lib().qdc_paged_attention_workspace(  # noqa: E731
+        n, cfg.heads, cfg.kv_heads, 64, t // 256, 256, _lib.QDC_F32) >= 0
+    assert takes(150) and not takes(rows) and not takes(1, 2 ** 31)
+    cache = BackboneCache(model, rows=rows, pages=rows, page_size=256, max_tokens=tokens)
+    ids = np.arange(rows)[:, None] % cfg.vocab
+    held, _ = cache.prefill(ids[:150])
+    held += cache.prefill(ids[150:])[0]
+    for call in (lambda: cache.step(held, ids), lambda: StepGraphs(cache)(held, ids),
+                 lambda: cache.prefill(ids)):
+        with pytest.raises(ValueError, match="at most 150"):
+            call()
+        assert cache.lengths() == {r: 1 for r in range(rows)}
+    got = cache.step(held[100:250], ids[100:250])
+    assert np.isfinite(got).all() and cache.book.lengths.tolist() == [
+        1 + (r in held[100:250]) for r in range(rows)]
+    with pytest.raises(ValueError, match="max_tokens"):
+        BackboneCache(model, rows=1, pages=1, page_size=256, max_tokens=2 ** 31)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kinds", [("full_attention",), ("linear_attention", "linear_attention")])
 def test_one_kind_of_layer(kinds):
     """Models with no state to keep, or with no pages."""
