@@ -43,9 +43,10 @@ class BackboneCache:
     :meth:`free`.  Invalid ids, masks and rows raise ``ValueError`` before anything
     runs; too few free pages (or rows) raise ``RuntimeError``, and every sequence is
     as it was before the call.  (Where torch itself raises within a call, for want of
-    memory say, or the call is interrupted, the rows that it was at are ended.)  One call at a time per
-    instance (a lock), all of them on one stream, the device's current one; prefill,
-    step and fork wait for their result.  The cache takes
+    memory say, or the call is interrupted, the rows that it was at are ended.)  One
+    call at a time per instance (a lock), all of them on one stream, the device's
+    current one, whichever the cache was made on; prefill, step and fork wait for their
+    result.  The cache takes
     ``2 * attention layers * pages * kv_heads * page_size * head_dim`` values in the
     model's dtype, and per row and linear attention layer ``value_heads * value_dim *
     key_dim`` float32 values and ``conv_kernel`` rows of the convolution's channels."""
@@ -93,6 +94,8 @@ class BackboneCache:
         self._unused = list(range(rows - 1, -1, -1))
         self._lengths = {}     # tokens of every row in use
         self._lock = threading.Lock()
+        # the calls may run on another stream than the one that has filled all this
+        torch.cuda.current_stream(dev).synchronize()
 
     # ------------------------------------------------------------- calls --
     @_call

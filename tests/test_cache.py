@@ -436,6 +436,45 @@ def test_more_rows_than_a_call_takes():
 
 
 @pytest.mark.gpu
+def test_made_on_another_stream(monkeypatch):
+    """A cache made on a stream that has much to do, then used on another one: it is whole
+    before the first call."""
+    import dataclasses
+
+    from qdc_amd import backbone
+    from qdc_amd import cache as module
+    from qdc_amd.config import synthetic_inference_config
+    from qdc_amd.weights import random_weights
+    # (no attention layer: the upload of rotation tables would wait for the stream)
+    cfg = dataclasses.replace(synthetic_inference_config(), layer_types=("linear_attention",) * 2)
+    model = backbone.QwenBackbone.from_weights(random_weights(cfg, seed=2), cfg)
+    ids = np.arange(40)
+    want = whole(model, ids)
+    new = lambda: module.BackboneCache(model, rows=3, pages=8, page_size=16)  # noqa: E731
+    new()                                                 # (new memory might wait as well)
+    big, busy, table = torch.randn(8192, 8192, device="cuda:0"), torch.cuda.Event(), \
+        module.cache_ops.page_table
+
+    def slow(*args):
+        out, x = table(*args), big
+        for _ in range(30):
+            x = x @ big * 1e-3
+        busy.record()
+        return out
+
+    slow(3, 8, 8, 16, "cuda:0")
+    torch.cuda.synchronize()
+    monkeypatch.setattr(module.cache_ops, "page_table", slow)
+    cache = new()
+    assert busy.query()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        (row,), got = cache.prefill(ids[:-1])
+        got = cache.step([row], ids[-1:])
+        assert cache.free_page_count() == 5
+    assert normwise(got[0], want) <= BARS["f32"]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kinds", [("full_attention",), ("linear_attention", "linear_attention")])
 def test_one_kind_of_layer(kinds):
     """Models with no state to keep, or with no pages."""
