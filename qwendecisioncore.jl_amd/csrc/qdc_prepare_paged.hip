@@ -257,7 +257,6 @@ extern "C" int32_t qdc_prepare_paged(
     a.per_token = make_fastdiv((uint32_t)(heads / rpg + kv_heads));
     a.heads = (int)heads;
     a.kv = (int)kv_heads;
-    a.half = (int)(rotary_dim / 2);
     a.rows = (int)rows;
     a.pages = (int)pages;
     a.shift = shift;

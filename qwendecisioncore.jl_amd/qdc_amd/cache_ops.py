@@ -109,29 +109,6 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 # ------------------------------------------------------------------- pages ---
-def _book(book: PageTable) -> tuple:
-    """Of a page table: the device, (four pointers), (rows, width, pages, page size)."""
-    table, lengths, refs, free, size = book
-    dev = _on(table)
-    rows, width = _table(table, dev)
-    at = (table.data_ptr(), _ints(lengths, dev, "lengths", rows), _ints(refs, dev, "refs", -1),
-          _ints(free, dev, "free", 1 + refs.shape[0]))
-    return dev, at, (rows, width, refs.shape[0], size)
-
-
-def _pool(pool: torch.Tensor | None, items: int, dev: int):
-    """``(pointer, planes, bytes of an item)`` of a contiguous ``[planes, items, ...]``."""
-    if pool is None:
-        return 0, 0, 0
-    shape = pool.shape
-    if len(shape) < 3 or shape[1] != items or pool.get_device() != dev or not pool.is_contiguous():
-        raise ValueError(f"pool must be a contiguous [planes, {items}, ...] tensor on the call's "
-                         "device")
-    # (strides of axes of one entry may be anything)
-    return (pool.data_ptr(), shape[0],
-            pool.numel() // max(1, shape[0] * items) * pool.element_size())
-
-
 def extend_pages(book: PageTable, rows: torch.Tensor, counts: torch.Tensor | None = None,
                  positions: torch.Tensor | None = None,
                  error_flag: torch.Tensor | None = None) -> torch.Tensor:
