@@ -94,6 +94,111 @@ def test_sequences(mode, config):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", list(MODES))
+def test_long_sequences(mode):
+    """Rows that may hold some thousands of tokens, so that attention is dealt out by what
+    they hold: a long and a short one, forks and a move, eager and recorded steps."""
+    from qdc_amd import _lib
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.graphs import StepGraphs
+    model = model_of(mode)
+    cfg, dtype = model.cfg, _lib.QDC_F32 if mode == "f32" else _lib.QDC_BF16
+    cache = BackboneCache(model, rows=6, pages=150, page_size=16)
+    assert _lib.lib().qdc_paged_attention_workspace(1, cfg.heads, cfg.kv_heads, cfg.head_dim, 150,
+                                                    16, dtype) > 0
+    graphs = StepGraphs(cache, gemm_libraries=None)
+    rng = np.random.default_rng(6)
+    ids = rng.integers(0, model.vocab, (2, 1205))
+    mask = np.ones_like(ids)
+    mask[1, :-3] = 0
+    (a, b), got = cache.prefill(ids, mask)
+    held = {a: ids[0].tolist(), b: ids[1, -3:].tolist()}
+
+    def check(rows, got):
+        for r, g in zip(rows, got):
+            exp = whole(model, held[r])
+            assert normwise(g, exp) <= BARS[mode], (r, len(held[r]), normwise(g, exp))
+
+    check((a, b), got)
+    kids = cache.fork([a, b, a])
+    held.update({k: list(held[p]) for k, p in zip(kids, (a, b, a))})
+    for i in range(4):
+        if i == 2:
+            cache.free([kids[0]])
+            del held[kids[0]]
+            cache.compact()
+        rows = list(held)[::-1]
+        tokens = rng.integers(0, model.vocab, len(rows))
+        got = (graphs if i % 2 else cache.step)(rows, tokens)
+        for r, t in zip(rows, tokens):
+            held[r].append(int(t))
+        check(rows, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["mlp", "all"])
+@pytest.mark.parametrize("intermediate,parts", [(1536, 8), (2560, 16), (3584, 16)])
+def test_few_rows_of_split_inputs(mode, intermediate, parts):
+    """The wide inner product of a step's MLP through the product cut in parts, from 1 to 63
+    rows, beside the whole product, which takes the others; then steps of such a model."""
+    import dataclasses
+
+    from oracle import qdc_oracle as O
+    from qdc_amd import backbone, ops
+    from qdc_amd.cache import BackboneCache
+    from qdc_amd.config import synthetic_inference_config
+    from qdc_amd.weights import random_weights
+    cfg = dataclasses.replace(synthetic_inference_config(), intermediate=intermediate)
+    weights = {k: O.round_bf16(v) for k, v in random_weights(cfg, seed=4).items()}
+    model = backbone.QwenBackbone.from_weights(weights, cfg, "cuda:0", torch.bfloat16,
+                                               split_gemm_inputs=mode)
+    cache = BackboneCache(model, rows=8, pages=60, page_size=16)
+    layer, norm = model.layers[1], model.layers[2]["input_norm"]
+    w = layer["down_rows"]
+    assert w.shape == (cfg.hidden, intermediate)
+    used = []
+    cut = ops.linear_residual_rms
+
+    def record(*args, **kwargs):
+        used.append(args[5])
+        return cut(*args, **kwargs)
+
+    g = torch.Generator(device="cuda:0").manual_seed(intermediate)
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(ops, "linear_residual_rms", record)
+        for n in (1, 2, 33, 63, 64):
+            t = lambda *s: torch.randn(s, generator=g, device="cuda:0")  # noqa: E731
+            h = t(n, cfg.hidden)
+            act = ops.native_mlp_gate(t(n, intermediate), t(n, intermediate), out_dtype=ops.BF16X2)
+            keep = torch.ones(n, dtype=torch.int32, device="cuda:0")
+            keep[n // 2] = int(n == 1)
+            used.clear()
+            got = cache._project_add_norm(h, act, layer, "down", norm, token_mask=keep,
+                                          out_dtype=ops.BF16X2)
+            assert used == ([parts] if n < 64 else used)
+            # fp32 sums of exact products of bf16, two a value of the input
+            x = ops.join_split(act).double()
+            exp = h.double() + x @ w.double().t()
+            tol = (2 * intermediate + 20) * 2.0 ** -24 * (h.double().abs() + x.abs() @ w.double().abs().t())
+            assert ((got[0].double() - exp).abs() <= tol).all()
+            scale = 1 / torch.sqrt(exp.square().mean(-1, keepdim=True) + cfg.eps)
+            out = exp * scale * (1 + norm.double()) * keep[:, None]
+            # the norm's sum and root add 300 half steps at most; the split form 2^-17
+            tol = (tol + exp.abs() * tol.amax(-1, keepdim=True) * scale) * scale * 2 \
+                + (300 * 2.0 ** -24 + 2.0 ** -17) * out.abs()
+            assert ((ops.join_split(got[1]).double() - out).abs() <= tol).all()
+            assert (got[1][keep == 0] == 0).all()
+        used.clear()
+        ids = np.arange(8 * 5).reshape(8, 5)
+        rows, _ = cache.prefill(ids)
+        used.clear()
+        got = cache.step(rows, np.arange(8))
+        assert used.count(parts) == len(model.layers)
+    for i, out in enumerate(got):
+        assert normwise(out, whole(model, ids[i].tolist() + [i])) <= BARS[mode]
+
+
+@pytest.mark.gpu
 def test_too_few_pages_leaves_everything():
     """A prompt, a step or a fork that does not fit raises, and what was there goes on."""
     from qdc_amd.cache import BackboneCache

@@ -353,6 +353,57 @@ def test_prepare_paged(T, H, KV, hd, rd, page, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,H,KV,hd,rd,dtype", [
+    (8209, 8, 2, 256, 64, torch.bfloat16),     # from 32 MB of bf16 queries on four heads at a time
+    (2731, 24, 3, 256, 32, torch.bfloat16),
+    (11003, 12, 4, 128, 128, torch.bfloat16),
+    (43691, 6, 1, 64, 0, torch.bfloat16),      # no multiple of four: two
+    (10923, 6, 2, 128, 16, torch.float32)])
+def test_prepare_paged_many_tokens(T, H, KV, hd, rd, dtype):
+    """As above with the tolerance of above, for prompts of tens of MB."""
+    assert T * H * hd * dtype.itemsize >= 32 << 20
+    g = torch.Generator(device=DEV).manual_seed(T)
+    page, rows = 32, 7
+    reach = -(-T // rows)
+    table, pages = scattered(np.random.default_rng(T), [reach] * rows, page)
+    table = torch.from_numpy(table).to(DEV)
+    t = lambda *s: torch.randn(s, generator=g, device=DEV).to(dtype)  # noqa: E731
+    qg, kv, qn, kn = t(T, H, 2, hd), t(T, 2, KV, hd), t(hd) * 0.1, t(hd) * 0.1
+    place = torch.randperm(T, generator=g, device=DEV)
+    index, pos = (place // reach).int(), (place % reach).int()
+    pos[7::1000], index[9::1000] = -1, -1
+    live = (index >= 0) & (pos >= 0)
+    tables = ops.rope_tables(reach, rd, 1e4, DEV) if rd else None
+    store = torch.full((2, pages, KV, page, hd), float("nan"), dtype=dtype, device=DEV)
+    k_out, f = torch.empty((T, KV, hd), dtype=dtype, device=DEV), flag()
+    got = cache_ops.prepare_paged(qg[:, :, 0], kv[:, 0], kv[:, 1], qn, kn, tables, rd, 1e-6, index, pos,
+                                  table, store[0], store[1], k_out=k_out, error_flag=f)
+
+    def near(got, x, w):
+        x = x.double()
+        x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+        tol = (hd + 16) * 2.0 ** -24 * x.abs().amax(-1, keepdim=True)
+        if rd:
+            keep = live[:, None, None]
+            cos, sin = (c.double()[torch.where(live, pos, 0).long()][:, None] for c in tables)
+            cos, sin = torch.where(keep, cos, 1.0), torch.where(keep, sin, 0.0)
+            a, b = x[..., :rd // 2], x[..., rd // 2:rd]
+            x = torch.cat([a * cos - b * sin, b * cos + a * sin, x[..., rd:]], -1)
+        if dtype == torch.bfloat16:
+            tol = tol + HALF[dtype] * x.abs()
+        assert ((got.double() - x).abs() <= tol).all()
+
+    near(got, qg[:, :, 0], qn)
+    near(k_out, kv[:, 0], kn)
+    assert f.item() == 0
+    at, row = pos[live].long(), index[live].long()
+    p, o = table[row, at // page].long(), at % page
+    assert torch.equal(store[0, p, :, o], k_out[live]) and torch.equal(store[1, p, :, o], kv[live, 1])
+    store[:, p, :, o] = float("nan")
+    assert torch.isnan(store).all()
+
+
+@pytest.mark.gpu
 def test_prepare_paged_refusals():
     z = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt, device=DEV)  # noqa: E731
     i, q, k, n, pg = ints([0, 1]), z(2, 4, 64), z(2, 2, 64), z(64), z(4, 2, 16, 64)
@@ -572,6 +623,157 @@ def test_paged_attention_nan_and_inf(dtype):
     assert torch.isfinite(got[1, 2:, :7]).all() and torch.isfinite(got[3]).all()
     exp, _ = attend_exact(q, k, v, table, index, [49, 59, 69, 79], 0.125, None, 16)
     assert normwise(got[2, 0], exp.view(4, 4, 64)[2, 0]) <= 2 * HALF[dtype] + 1e-5
+
+
+def short(n, H, KV, hd, table, page, dtype):
+    """Whether such a call is one launch, of a workgroup for each entry and head group."""
+    need = _lib.lib().qdc_paged_attention_workspace(n, H, KV, hd, table.shape[1], page,
+                                                    F32 if dtype == torch.float32 else BF16)
+    assert need >= 0
+    return need == 0
+
+
+def widen(table, places, page):
+    """The same rows in a table of ``places`` positions and more, -1 behind them."""
+    more = max(0, -(-places // page) - table.shape[1])
+    return np.pad(table, ((0, 0), (0, more)), constant_values=-1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,page", [(4, 2, 64, 16), (8, 2, 256, 64), (5, 1, 128, 32),
+                                          (16, 1, 64, 16), (20, 1, 128, 16), (3, 3, 256, 128),
+                                          (34, 2, 64, 256), (12, 3, 256, 16)])
+def test_paged_attention_rows_of_a_wide_table(H, KV, hd, page, dtype):
+    """Short rows whose table could hold long ones: work is dealt out by what is there."""
+    case = attend_case(H * hd + page, H, KV, hd, page, LENGTHS, dtype,
+                       order=np.random.default_rng(H).permutation(len(LENGTHS)))
+    pos, table = np.array(LENGTHS)[case[-1]] - 1, widen(case[4], 2000, page)
+    assert not short(len(pos), H, KV, hd, table, page, dtype)
+    for out, gated in ((None, True), (torch.float32, False), (ops.BF16X2, True)):
+        assert attend_check(case, pos, page, dtype, out, gated, table=table) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,page", [(8, 2, 256, 16), (3, 1, 256, 64), (20, 1, 256, 32),
+                                          (12, 4, 128, 16), (17, 1, 128, 128), (6, 1, 64, 32)])
+def test_paged_attention_short_rows(H, KV, hd, page, dtype):
+    """Tables of so few positions that a workgroup takes a unit whole, up to their last."""
+    most = {64: 16, 128: 8, 256: 4}[hd] * 2 * (32 if dtype == torch.bfloat16 else 16)
+    lengths = [n for n in LENGTHS if n < most] + [most, most - 1]
+    case = attend_case(H * hd + page, H, KV, hd, page, lengths, dtype)
+    assert short(len(lengths), H, KV, hd, case[4], page, dtype)
+    assert case[4].shape[1] * page == most
+    assert not short(1, H, KV, hd, widen(case[4], most + 1, page), page, dtype)
+    for out, gated in ((None, True), (torch.float32, False), (ops.BF16X2, True)):
+        assert attend_check(case, np.array(lengths) - 1, page, dtype, out, gated) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,rows,n", [
+    (4, 2, 64, 40, 65),          # one entry more than a wavefront sees
+    (8, 2, 256, 30, 151),
+    (12, 4, 128, 60, 171),       # 2052 heads: all of an entry joined by one workgroup
+    (8, 1, 64, 90, 300),
+    (20, 1, 64, 50, 128)])       # the same, two groups of heads
+def test_paged_attention_many_entries_of_a_wide_table(H, KV, hd, rows, n, dtype):
+    """More entries than a wavefront sees at once, dealt out as one line, several of one
+    row at positions of their own, entries that are no token among them."""
+    rng = np.random.default_rng(n + hd)
+    lengths = [int(x) for x in rng.integers(0, 90, rows)]
+    lengths[:3] = [700, 1, 0]
+    order = rng.integers(0, rows, n)
+    order[:2] = 0
+    case = attend_case(n, H, KV, hd, 16, lengths, dtype, order=order)
+    pos = np.array([rng.integers(-1, lengths[r]) if lengths[r] else -1 for r in order])
+    pos[0] = 699
+    case[-1][[3, 63, 64, n - 1]] = -1
+    table = widen(case[4], 1100, 16)
+    assert not short(n, H, KV, hd, table, 16, dtype)
+    assert attend_check(case, pos, 16, dtype, None, table=table) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (8, 2, 256), (10, 1, 128)])
+def test_paged_attention_shared_pages_of_a_wide_table(H, KV, hd, dtype):
+    """Rows that hold the same pages, in the kernel that keeps those in the caches."""
+    lengths = [900, 900, 611, 900, 640, 900]
+    case = attend_case(hd + H, H, KV, hd, 16, lengths, dtype)
+    table = widen(case[4], 1100, 16)
+    table[1] = table[0]
+    table[4, :20] = table[0, :20]
+    pos = np.array(lengths) - 1
+    pos[1], pos[5] = 555, -1
+    assert not short(len(pos), H, KV, hd, table, 16, dtype)
+    assert attend_check(case, pos, 16, dtype, None, table=table) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,n", [(4, 1, 64, 1500), (8, 1, 256, 2500), (20, 1, 128, 1100)])
+def test_paged_attention_rising_scores_over_pieces(H, KV, hd, n, dtype):
+    """Scores that rise along the keys by hundreds, from piece to piece of a row, and a
+    last key far below."""
+    q, gate, k, v, table, index = case = attend_case(9, H, KV, hd, 16, [n], dtype)
+    for j in range(n):
+        k[table[0, j // 16], 0, j % 16] = torch.where(q[0, 0] > 0, 1.0, -1.0) * (j * 10.0 / n)
+    k[table[0, (n - 1) // 16], 0, (n - 1) % 16] *= -1
+    assert not short(1, H, KV, hd, table, 16, dtype)
+    assert attend_check(case, np.array([n - 1]), 16, dtype, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (8, 2, 256), (17, 1, 128)])
+@pytest.mark.parametrize("others", [0, 61])
+def test_paged_attention_bad_long_tables(H, KV, hd, others, dtype):
+    """Pages that are none within long rows, a row of nothing but such, positions behind
+    the table and rows that are none: left out and flagged, in the shares of few entries
+    and in the line of many."""
+    lengths = [1500, 1300, 700, 40, 9] + [7] * others
+    n = len(lengths)
+    order = np.arange(n)
+    order[4] = n + 3                                        # no row
+    case = attend_case(11, H, KV, hd, 16, lengths, dtype, order=order)
+    table = widen(case[4], 1600, 16)
+    assert not short(n, H, KV, hd, table, 16, dtype)
+    table[0, 2], table[0, 70:], table[2, :] = -1, case[2].shape[0], 1 << 30
+    pos = np.array(lengths) - 1
+    pos[4] = 10
+    assert attend_check(case, pos, 16, dtype, None, table=table) == 1
+    full = [1600, 1600, 33]                                 # every place of the table held
+    case = attend_case(12, H, KV, hd, 16, full, dtype)
+    assert attend_check(case, np.array([1650, 2 ** 31 - 1, 32]), 16, dtype, None) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (8, 2, 256), (6, 2, 128)])
+def test_paged_attention_nan_and_inf_in_long_rows(H, KV, hd, dtype):
+    """A NaN or infinity in one piece of a long row shows in that row's heads alone; a score
+    of minus infinity is a weight of nothing."""
+    lengths = [1500, 1600, 1700, 1100]
+    q, gate, k, v, table, index = attend_case(13, H, KV, hd, 16, lengths, dtype)
+    k[table[0, 41], 0, 3, 5] = float("nan")
+    v[table[1, 52], 1, 4, 7] = float("inf")
+    q[2, 0, 0] = 1.0
+    k[table[2, 60], 0, 2, 0] = -float("inf")          # head 0 of entry 2: one key masked
+    assert not short(4, H, KV, hd, table, 16, dtype)
+    d, scale, G = lambda x: x.to(DEV), hd ** -0.5, H // KV  # noqa: E731
+    pos = [x - 1 for x in lengths]
+    got = cache_ops.paged_attention(d(q), d(k), d(v), d(torch.from_numpy(table)), ints(index),
+                                    ints(pos), scale).float().cpu().view(4, H, hd)
+    assert torch.isnan(got[0, :G]).all() and torch.isfinite(got[0, G:]).all()
+    assert torch.isfinite(got[1, :G]).all() and (got[1, G:, 7] == float("inf")).all()
+    rest = [i for i in range(hd) if i != 7]
+    assert torch.isfinite(got[1, G:][:, rest]).all() and torch.isfinite(got[3]).all()
+    exp, _ = attend_exact(q, k, v, table, index, pos, scale, None, 16)
+    exp = exp.view(4, H, hd)
+    for i, h in ((2, 0), (1, 0), (3, H - 1)):
+        assert normwise(got[i, h], exp[i, h]) <= 2 * HALF[dtype] + 1e-5
 
 
 @pytest.mark.gpu
