@@ -789,6 +789,56 @@ int64_t unit_heads(int64_t heads, int64_t kv_heads) {
     return g < kHeads ? g : kHeads;
 }
 
+// Entries of a slice.  Every workgroup adds up its call's line, so a call's time would grow
+// with the square of its entries: from twice this many on it is launched slice by slice,
+// evenly, of so many entries and more.  (ms, whole / in slices of 1024 / 2048 / 4096, bf16 rows
+// of up to 40 keys: 4096 x 4 heads of 64 .172 / .147 / .147 / .170, 131072 65.5 / 5.07 / 4.98 /
+// 5.61, 131072 x 8 heads of 256 68.4 / 9.00 / 8.55 / 9.32; up to 600 keys, 3000 x 8 heads of
+// 256 .353 / .388 / .373 / .356.)
+constexpr int64_t kSlice = 2048;
+
+int32_t launch(PagedAttention a, int64_t head_dim, int32_t dtype, bool brief, bool few,
+               void *workspace, hipStream_t stream) {
+    const int64_t n = a.n, units = (int64_t)a.kv * a.head_groups;
+    const dim3 grid(brief ? (uint32_t)(n * units) : 1u << a.log_wgs);
+    a.join_heads = n * a.heads >= kJoinWgs ? a.heads : 1;
+    const dim3 join((uint32_t)(n * a.heads / a.join_heads)), block(kBlock);
+    const bool many = kManyPieces * n * units <= grid.x;
+    a.pieces = reinterpret_cast<float *>(workspace);
+    a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;
+#define QDC_PAGED(T, HD, FEW)                                                                  \
+    if (head_dim == HD && few == FEW) {                                                        \
+        if (brief) {                                                                           \
+            hipLaunchKernelGGL((paged_attention_short<T, HD, FEW>), grid,                      \
+                               dim3(short_waves(HD) * kWave), 0, stream, a);                   \
+            return launch_status();                                                            \
+        }                                                                                      \
+        hipLaunchKernelGGL((paged_attention<T, HD, FEW>), grid, block, 0, stream, a);          \
+        const int32_t status = launch_status();                                                \
+        if (status != QDC_OK) return status;                                                   \
+        if (many)                                                                              \
+            hipLaunchKernelGGL((paged_attention_join<T, HD, 2 * kBlock>), join,                \
+                               dim3(2 * kBlock), 0, stream, a);                                \
+        else                                                                                   \
+            hipLaunchKernelGGL((paged_attention_join<T, HD, kBlock>), join, block, 0, stream,  \
+                               a);                                                             \
+        return launch_status();                                                                \
+    }
+    if (dtype == QDC_BF16) {
+        QDC_PAGED(bf16_t, 64, false)
+        QDC_PAGED(bf16_t, 128, false)
+        QDC_PAGED(bf16_t, 256, false)
+    }
+    QDC_PAGED(float, 64, true)
+    QDC_PAGED(float, 64, false)
+    QDC_PAGED(float, 128, true)
+    QDC_PAGED(float, 128, false)
+    QDC_PAGED(float, 256, true)
+    QDC_PAGED(float, 256, false)
+#undef QDC_PAGED
+    return QDC_ERR_SHAPE;
+}
+
 }  // namespace
 }  // namespace qdc
 
@@ -846,14 +896,9 @@ extern "C" int32_t qdc_paged_attention(
         {index, n * 4}, {positions, n * 4}};
     if (any_alias(outs, 3, ins, 7)) return QDC_ERR_ALIAS;
     PagedAttention a{};
-    a.out = out;
-    a.q = q;
     a.k = k_pages;
     a.v = v_pages;
-    a.gate = gate;
     a.table = table;
-    a.index = index;
-    a.positions = positions;
     a.error_flag = error_flag;
     a.q_tok = q_tok;
     a.q_head = q_head;
@@ -861,7 +906,6 @@ extern "C" int32_t qdc_paged_attention(
     a.gate_head = gate_head;
     a.out_tok = out_tok;
     a.width = width;
-    a.n = (int)n;
     a.heads = (int)heads;
     a.kv = (int)kv_heads;
     a.group = (int)(heads / kv_heads);
@@ -870,45 +914,22 @@ extern "C" int32_t qdc_paged_attention(
     a.rows = (int)rows;
     a.pages = (int)pages;
     a.shift = page_shift(page_size);
-    a.log_wgs = log_workgroups(line, head_dim);
     a.out_dtype = out_dtype;
     a.scale_log2 = scale * 1.4426950408889634f;
     const bool brief = need == 0, few = dtype == QDC_F32 && a.group <= 4;
-    const dim3 grid(brief ? (uint32_t)(n * kv_heads * a.head_groups) : 1u << a.log_wgs);
-    a.join_heads = n * heads >= kJoinWgs ? (int)heads : 1;
-    const dim3 join((uint32_t)(n * heads / a.join_heads)), block(kBlock);
-    const bool many = kManyPieces * n * kv_heads * a.head_groups <= grid.x;
-    a.pieces = reinterpret_cast<float *>(workspace);
-    a.stats = a.pieces + (int64_t)2 * grid.x * a.unit_heads * head_dim;
-#define QDC_PAGED(T, HD, FEW)                                                                  \
-    if (head_dim == HD && few == FEW) {                                                                      \
-        if (brief) {                                                                           \
-            hipLaunchKernelGGL((paged_attention_short<T, HD, FEW>), grid,                           \
-                               dim3(short_waves(HD) * kWave), 0, stream, a);                   \
-            return launch_status();                                                            \
-        }                                                                                      \
-        hipLaunchKernelGGL((paged_attention<T, HD, FEW>), grid, block, 0, stream, a);               \
-        const int32_t status = launch_status();                                                \
-        if (status != QDC_OK) return status;                                                   \
-        if (many)                                                                              \
-            hipLaunchKernelGGL((paged_attention_join<T, HD, 2 * kBlock>), join,                \
-                               dim3(2 * kBlock), 0, stream, a);                                \
-        else                                                                                   \
-            hipLaunchKernelGGL((paged_attention_join<T, HD, kBlock>), join, block, 0, stream,  \
-                               a);                                                             \
-        return launch_status();                                                                \
+    const int64_t slices = brief || n < 2 * kSlice ? 1 : n / kSlice;
+    for (int64_t i = 0; i < slices; ++i) {
+        const int64_t i0 = n * i / slices, m = n * (i + 1) / slices - i0;
+        a.out = (char *)out + i0 * out_tok * oes;
+        a.q = (const char *)q + i0 * q_tok * es;
+        a.gate = gate ? (const char *)gate + i0 * gate_tok * es : nullptr;
+        a.index = index + i0;
+        a.positions = positions + i0;
+        a.n = (int)m;
+        a.log_wgs = log_workgroups(
+            longest_line(m, heads, kv_heads, head_dim, width, page_size, dtype), head_dim);
+        const int32_t status = launch(a, head_dim, dtype, brief, few, workspace, stream);
+        if (status != QDC_OK) return status;
     }
-    if (dtype == QDC_BF16) {
-        QDC_PAGED(bf16_t, 64, false)
-        QDC_PAGED(bf16_t, 128, false)
-        QDC_PAGED(bf16_t, 256, false)
-    }
-    QDC_PAGED(float, 64, true)
-    QDC_PAGED(float, 64, false)
-    QDC_PAGED(float, 128, true)
-    QDC_PAGED(float, 128, false)
-    QDC_PAGED(float, 256, true)
-    QDC_PAGED(float, 256, false)
-#undef QDC_PAGED
-    return QDC_ERR_SHAPE;
+    return QDC_OK;
 }

@@ -697,6 +697,50 @@ def test_paged_attention_many_entries_of_a_wide_table(H, KV, hd, rows, n, dtype)
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,KV,hd,n,out", [(2, 1, 64, 4095, None), (2, 1, 64, 4096, ops.BF16X2),
+                                           (3, 3, 128, 6201, None)])
+def test_paged_attention_thousands_of_entries(H, KV, hd, n, out, dtype):
+    """Entries on both sides of where a call is launched in slices, each of its own row of
+    the arguments."""
+    rng = np.random.default_rng(n)
+    lengths = [int(x) for x in rng.integers(0, 40, 50)]
+    lengths[0] = 300
+    order = rng.integers(1, 50, n)
+    order[[0, n // 2, n - 1]] = 0
+    case = attend_case(n, H, KV, hd, 16, lengths, dtype, order=order)
+    pos = np.array([lengths[r] - 1 for r in order])
+    case[-1][rng.integers(1, n // 2, 20)] = -1
+    table = widen(case[4], 1100, 16)
+    assert not short(n, H, KV, hd, table, 16, dtype)
+    assert attend_check(case, pos, 16, dtype, out, table=table) == 0
+
+
+@pytest.mark.gpu
+def test_paged_attention_time_of_many_entries():
+    """Eight times the entries take eight times as long, not sixty-four."""
+    pages = torch.zeros(64, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    table = torch.full((64, 80), -1, dtype=torch.int32, device=DEV)
+    table[:, 0] = torch.arange(64, device=DEV)
+
+    def best(n):
+        q = torch.zeros(n, 4, 64, dtype=torch.bfloat16, device=DEV)
+        rows, pos = ints(np.arange(n) % 64), ints(np.arange(n) % 16)
+        times = []
+        for _ in range(4):
+            start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            start.record()
+            cache_ops.paged_attention(q, pages, pages, table, rows, pos, 0.1)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+
+    few, many = best(8192), best(65536)     # whole: 0.45 and 17.3 ms
+    assert many < 16 * few, (few, many)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,KV,hd", [(4, 2, 64), (8, 2, 256), (10, 1, 128)])
 def test_paged_attention_shared_pages_of_a_wide_table(H, KV, hd, dtype):
     """Rows that hold the same pages, in the kernel that keeps those in the caches."""
