@@ -209,9 +209,11 @@ __global__ __launch_bounds__(step_threads(STREAM)) void delta_step(DeltaStep a) 
 
 template <typename T, int KD> int32_t launch(const DeltaStep &a, int64_t n, hipStream_t stream) {
     const dim3 grid((uint32_t)n, (uint32_t)a.heads);
-    // Bytes of state from which on it is a stream: half of the last-level cache of 256 MB.
-    // us, replayed, cached / streamed, 67 MB 23.7 / 28.2 (with 1 GB of other layers' states
-    // between two calls 33.0 / 28.9), 134 MB 55.9 / 51.1, 317 MB 130.7 / 114.8.
+    // Bytes of state from which on it is a stream: half of the last-level cache of 256 MB,
+    // which is right for calls repeated on one state (us, replayed, cached / streamed: 67 MB
+    // 23.7 / 28.2, 134 MB 55.9 / 51.1, 317 MB 130.7 / 114.8).  What passes between two calls
+    // is not known here: with 1 GB of other layers' states in between 67 MB would be ahead as
+    // a stream too (33.0 / 28.9).
     const bool stream_state =
         a.taps == 4 && n * a.heads * a.value_dim * KD * 4 >= ((int64_t)128 << 20);
     const dim3 block(step_threads(stream_state));

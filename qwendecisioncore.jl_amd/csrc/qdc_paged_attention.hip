@@ -22,9 +22,11 @@
 //
 // It is bound by the reads of K and V: 2 rows of 100003 keys of 4 heads of 256 (bf16, 819
 // MB, each byte fetched once) 123 us = 6.7 TB/s with its join of 4.6 us behind it, of 7.0
-// that a plain streaming read reaches; 96 rows of 0 .. 16384 keys (333 MB) 56 us = 6.0
-// TB/s.  Where little is read the chain positions -> pages -> K -> scores -> join counts: 8
-// rows of 2048 keys (34 MB) 11.2 + 4.0 us, one row of 411 keys (0.4 MB, in one launch) 6.9.
+// that a plain streaming read reaches; 2 rows of 100000 of 2 heads of 256 in fp32 (819 MB)
+// 128 + 5.2; 96 rows of 0 .. 16384 keys (333 MB) 56 us = 6.0 TB/s.  Where little is read the
+// chain positions -> pages -> K -> scores -> join counts: 8 rows of 2048 keys (34 MB) 10.5 +
+// 4.0 us, one row of 411 keys (0.4 MB) 5.0 + 3.3, or 6.9 in one launch where the table is so
+// narrow that every row must be short.
 #include <cfloat>
 #include <type_traits>
 
@@ -232,7 +234,7 @@ template <int I> __device__ __forceinline__ float quad_lane(float v) {
 // FEW, for fp32 and up to 4 heads: sixteen 4 x 4 products with one key's or value's step
 // each in place of one of 16 x 16, of which 4 columns would be in use: a quarter of the
 // matrix cores' time, which short rows wait for (us, 16 x 16 / 4 x 4: a row of 500 keys of
-// 64 9.1 / 7.7, 8 rows of 256 of 128 11.7 / 10.5, 410 MB of 256 134 / 127).  Quad g = lane / 4 %
+// 64 9.1 / 7.7, 8 rows of 256 of 128 11.7 / 10.5, 819 MB of 256 134 / 127).  Quad g = lane / 4 %
 // 4 and j = lane % 4:
 //   K as above, each lg a part of the sum.  S^T, P: head j, keys 4 g + r, the same for all
 //   lg.  V: values 16 VD c + VD (4 lg + j) .. of keys 4 g + r.   O[c][e]: head r, values 16
@@ -763,8 +765,11 @@ int64_t longest_line(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_di
     return span >= lim / units / n ? 0 : span * units * n;
 }
 
-// Whether rows of `width` pages are short: at most kShortTiles tiles a wavefront.  (The
-// grid of a workgroup for each unit stays below 2^32 work-items.)
+// Whether rows of `width` pages are short: at most kShortTiles tiles a wavefront.  The host
+// knows the table's width and not the rows: short rows of a wider table are dealt out and
+// joined (us a call, a row of 411 keys of 2 fp32 heads of 64: 7.1 in a table of 416 places,
+// 8.5 in one of 32768; 8 rows of 2048 of 256, dealt out in both, 12.9 and 13.1).  (The grid
+// of a workgroup for each unit stays below 2^32 work-items.)
 bool short_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t width,
                 int64_t page_size, int32_t dtype) {
     const int64_t tile = dtype == QDC_BF16 ? tile_keys<bf16_t>() : tile_keys<float>();

@@ -62,8 +62,8 @@ def page_table(rows: int, width: int, pages: int, page_size: int, device) -> Pag
 
 
 # The host's part of a call is the whole cost of a small one, so the tensors are checked and
-# the entry points called by a compiled module, csrc/qdc_calls.cpp (5 to 7 us a call less
-# than the same in Python).
+# the entry points called by a compiled module, csrc/qdc_calls.cpp (4.6 to 4.9 us of the
+# host's time for a call of one launch, 5 to 7 less than the same in Python).
 
 
 # --------------------------------------------------------------- attention ---
