@@ -3,8 +3,9 @@
 The library is loaded from ``qwendecisioncore.jl_amd/lib/`` (built in-tree by
 ``make -C qwendecisioncore.jl_amd/csrc``).  There is no fallback: a missing
 library is an error.  ``lib/qdc_calls.so`` (``make -C qwendecisioncore.jl_amd/csrc
-python``) calls the cache's operators for PyTorch tensors.  Status codes map to exceptions the way the reference maps
-bad input to ``ArgumentError`` / ``DimensionMismatch``: a negative status raises
+python``) calls the cache's operators for PyTorch tensors.  Status codes map to
+exceptions the way the reference maps bad input to ``ArgumentError`` /
+``DimensionMismatch``: a negative status raises
 ``ValueError`` (argument error found on the host before any launch), a positive
 one ``RuntimeError`` (HIP launch failure).
 """

@@ -128,12 +128,12 @@ class BackboneCache:
         counts = mask.sum(1)
         if counts.max() > self.max_tokens:
             raise ValueError(f"A sequence holds at most {self.max_tokens} tokens.")
-        self._check_count(B)
         cfg = self.model.cfg
         if self._heads() and not ops.attention_fused_takes(self.model.dtype, cfg.head_dim, B, S,
                                                            cfg.heads, cfg.kv_heads):
             raise ValueError("Too many or too long prompts for one call.")
         rows = self._next(B)            # none is taken before the call is done
+        self._check_count(B)
         d_ids, d_mask = bb._upload(self.model, ids, mask)
         at = np.arange(S) - (S - counts[:, None])
         d_rows, d_counts, d_at = self._ints(np.asarray(rows), counts, at)

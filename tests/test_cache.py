@@ -528,14 +528,20 @@ def test_more_rows_than_a_call_takes():
     ids = np.arange(rows)[:, None] % cfg.vocab
     held, _ = cache.prefill(ids[:150])
     held += cache.prefill(ids[150:])[0]
-    for call in (lambda: cache.step(held, ids), lambda: StepGraphs(cache)(held, ids),
-                 lambda: cache.prefill(ids)):
+    for call in (lambda: cache.step(held, ids), lambda: StepGraphs(cache)(held, ids)):
         with pytest.raises(ValueError, match="at most 150"):
             call()
         assert cache.lengths() == {r: 1 for r in range(rows)}
     got = cache.step(held[100:250], ids[100:250])
     assert np.isfinite(got).all() and cache.book.lengths.tolist() == [
         1 + (r in held[100:250]) for r in range(rows)]
+    cache.free(held)
+    with pytest.raises(ValueError, match="at most 150"):
+        cache.prefill(ids)
+    for many in (ids, np.tile(ids, (2, 1))):              # more than are free, than there are
+        with pytest.raises(RuntimeError, match="free rows"):
+            BackboneCache(model, rows=150, pages=rows, page_size=256).prefill(many)
+    assert not cache.lengths() and cache.free_page_count() == rows
     with pytest.raises(ValueError, match="max_tokens"):
         BackboneCache(model, rows=1, pages=1, page_size=256, max_tokens=2 ** 31)
 
