@@ -97,7 +97,7 @@ template <typename T, int HD, bool FIRST> struct Line {
     uint32_t share;        // 0: a line
 
     static __device__ __forceinline__ uint32_t tiles_of(int keys) {
-        return (uint32_t)(keys + TILE - 1) / TILE;
+        return ((uint32_t)keys + TILE - 1) / TILE;  // (keys may be 2^31 - 16)
     }
     __device__ __forceinline__ void add_up() {
         const uint32_t tiles = tiles_of(keys);
@@ -655,7 +655,6 @@ constexpr int64_t kManyPieces = 64;
 constexpr int64_t kJoinWgs = 2048;
 template <typename T, int HD, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_attention_join(PagedAttention a) {
-    constexpr int TILE = tile_keys<T>();
     constexpr int LPP = HD / 4, PARTS = THREADS / LPP;  // lanes of a piece's row, rows at a time
     __shared__ float top_of[PARTS], sum_of[PARTS];
     __shared__ __align__(16) float so[PARTS][HD];
@@ -669,7 +668,7 @@ __global__ __launch_bounds__(THREADS) void paged_attention_join(PagedAttention a
     const uint32_t all = line.total();
     while (line.first + kWave <= entry) line.next();
     const int keys = __builtin_amdgcn_readlane(line.keys, entry - line.first);
-    const uint32_t tiles = (uint32_t)(keys + TILE - 1) / TILE;
+    const uint32_t tiles = line.tiles_of(keys);
     if (h0 == 0 && threadIdx.x == 0) {
         bool bad;
         entry_keys(a, a.index[entry], a.positions[entry], bad);

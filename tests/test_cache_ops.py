@@ -716,6 +716,38 @@ def test_paged_attention_thousands_of_entries(H, KV, hd, n, out, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_attention_widest_table(dtype):
+    """A row of 2^31 - 16 keys, all but the last 20 of them one page again and again.  The
+    last page's scores are 22 and the others' 1 at most, so it has 0.7 of the weight or
+    more.  Sums over 2^27 tiles of 2048 wavefronts: chains of 65536 additions, 2^-24 each,
+    of the weights and of their products, and as many again for the rescaling: 2^-6."""
+    width, hd = 2 ** 27 - 1, 64
+    rng = np.random.default_rng(1)
+    t = lambda *s: torch.from_numpy(rng.standard_normal(s, dtype=np.float32)).to(dtype)  # noqa: E731
+    q = torch.ones(1, 1, hd, dtype=dtype)
+    k, v = t(3, 1, 16, hd) * 0.05, t(3, 1, 16, hd)
+    k[2] = 2.75                                             # 64 of it / 8: 22
+    table = torch.zeros((1, width), dtype=torch.int32, device=DEV)
+    table[0, -2], table[0, -1] = 1, 2
+    last = width * 16 - 1 - 12                              # 4 keys of the last page
+    f = flag()
+    got = cache_ops.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), table, ints([0]), ints([last]),
+                                    0.125, out_dtype=torch.float32, error_flag=f)
+    assert f.item() == 0
+    s = (k.double()[:, 0].sum(-1) * 0.125)                  # [3, 16]
+    assert s[:2].max() < 1 and (s[2] == 22).all()
+    times = torch.ones(3, 16, dtype=torch.float64)
+    times[0], times[2, 4:] = width - 2, 0
+    w = times * torch.exp(s)
+    w /= w.sum()
+    assert 0.7 < w[2].sum() < 0.95
+    exp = (w[..., None] * v.double()[:, 0]).sum((0, 1))
+    tol = (2.0 ** -6 + 2.0 ** -16) * (w[..., None] * v.double()[:, 0].abs()).sum((0, 1))
+    assert ((got.double().cpu()[0] - exp).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 def test_paged_attention_time_of_many_entries():
     """Eight times the entries take eight times as long, not sixty-four."""
     pages = torch.zeros(64, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
