@@ -325,8 +325,8 @@ def _plain_pack(s):
     group = s["case"]["group"]
     out, inner = s["w"].shape
     w = torch.nn.functional.pad(s["w"].float(), (0, -inner % group)).view(out, -1, group)
-    scale = (w.abs().amax(-1, keepdim=True) / 7.0).bfloat16().float()
-    # in 64 bits, as a quotient next to a half would be rounded to it in 32
+    # quotients in 64 bits, as one next to a half would be rounded to it in 32
+    scale = (w.abs().amax(-1, keepdim=True).double() / 7.0).bfloat16().float()
     q = torch.where(scale > 0, w.double() / scale.double(), 0.0).round().clamp(-7, 7)
     return (q.float() * scale).flatten(1)[:, :inner].contiguous()
 
