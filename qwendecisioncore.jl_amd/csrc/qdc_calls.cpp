@@ -1,12 +1,13 @@
-// qdc_calls.cpp -- the host side of the cache's operators: the checks of their tensors and
-// the call of the entry point (include/qdc_hip_cache.h), as functions of a Python module.
+// qdc_calls.cpp -- the host side of the cache's operators and of those on 4-bit weights: the
+// checks of their tensors and the call of the entry point (include/qdc_hip_cache.h,
+// include/qdc_hip_quant.h), as functions of a Python module.
 //
 // A step is many small calls, and their host side is what they cost.  The host's time for a
 // call, its launch of 2.6 us and the output's allocation within it, with some fifteen tensors
 // to look at and up to 46 arguments to convert, in Python / here: a token stored 12.1 / 4.9
 // us, one attended to in one launch 10.8 / 4.6, its step of the recurrence 9.9 / 4.8.
-// The functions take exactly the arguments that qdc_amd.cache_ops passes them, by position;
-// it documents what they do and refuse.
+// The functions take exactly the arguments that qdc_amd.cache_ops and qdc_amd.quant_ops pass
+// them, by position; those document what they do and refuse.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/python_numbers.h>
@@ -16,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include "qdc_hip_cache.h"
+#include "qdc_hip_quant.h"
 
 namespace {
 
@@ -409,6 +411,210 @@ PyObject *delta_step(Args a) {
     return THPVariable_Wrap(out);
 }
 
+// A matrix with contiguous rows, ld elements apart.
+struct Matrix {
+    const at::Tensor &t;
+    int64_t rows, width, ld;
+
+    Matrix(const Call &call, PyObject *o, const char *name) : t(tensor(o, name)) {
+        TORCH_CHECK_VALUE(t.dim() == 2 && call.here(t) && (t.size(1) < 2 || t.stride(1) == 1),
+                          name, " must be a matrix with contiguous rows on the call's device");
+        rows = t.size(0);
+        width = t.size(1);
+        ld = rows > 1 ? t.stride(0) : (width + 7) / 8 * 8;
+    }
+};
+
+// Rows in 8 bits: values and the scales of their groups.
+struct Rows8 {
+    const at::Tensor &values, &scales;
+    int64_t rows, width;
+
+    Rows8(const Call &call, PyObject *v, PyObject *s)
+        : values(tensor(v, "values")), scales(tensor(s, "scales")) {
+        TORCH_CHECK_VALUE(values.dim() == 2 && call.plain(values, at::kChar) && scales.dim() == 2 &&
+                              call.plain(scales, at::kFloat) &&
+                              scales.size(0) == values.size(0) &&
+                              scales.size(1) == (values.size(1) + 127) / 128,
+                          "8-bit rows are contiguous int8 values [rows, width] and float32 scales "
+                          "[rows, ceil(width / 128)] of one device");
+        rows = values.size(0);
+        width = values.size(1);
+    }
+};
+
+// A weight in 4 bits: a[0..5] packed, scales, out, inner, group, gated.
+struct Weight4 {
+    const at::Tensor &packed, &scales;
+    int64_t out, inner, group;
+    bool gated;
+
+    Weight4(const Call &call, Args a)
+        : packed(tensor(a[0], "packed")), scales(tensor(a[1], "scales")), out(integer(a[2])),
+          inner(integer(a[3])), group(integer(a[4])), gated(PyObject_IsTrue(a[5]) == 1) {
+        TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128,
+                          "group must be 32, 64 or 128");
+        TORCH_CHECK_VALUE(out > 0 && inner > 0 && (!gated || out % 2 == 0),
+                          "out and inner must be positive, a gated weight's out even");
+        const int64_t nb = gated ? 2 * ((out / 2 + 15) / 16) : (out + 15) / 16;
+        const int64_t kb = (inner + 127) / 128;
+        TORCH_CHECK_VALUE(packed.dim() == 4 && packed.size(0) == nb && packed.size(1) == kb &&
+                              packed.size(2) == 64 && packed.size(3) == 4 &&
+                              call.plain(packed, at::kInt) && scales.dim() == 3 &&
+                              scales.size(0) == nb && scales.size(1) == kb * (128 / group) &&
+                              scales.size(2) == 16 && call.plain(scales, at::kBFloat16),
+                          "a 4-bit weight is a contiguous int32 [", nb, ", ", kb,
+                          ", 64, 4] tensor and contiguous bfloat16 scales [", nb, ", ",
+                          kb * (128 / group), ", 16] on the call's device");
+    }
+};
+
+at::Tensor q8_scales(const at::Tensor &like, int64_t rows, int64_t width) {
+    return at::empty({rows, (width + 127) / 128}, like.options().dtype(at::kFloat));
+}
+PyObject *pair(const at::Tensor &a, const at::Tensor &b) {
+    THPObjectPtr x(THPVariable_Wrap(a)), y(THPVariable_Wrap(b));
+    PyObject *t = x && y ? PyTuple_Pack(2, x.get(), y.get()) : nullptr;
+    if (!t) throw python_error();
+    return t;
+}
+at::ScalarType type_of(int64_t code) { return code == QDC_F32 ? at::kFloat : at::kBFloat16; }
+
+PyObject *pack_w4(Args a) {
+    const Call call(tensor(a[0], "w"));
+    const Matrix w(call, a[0], "w");
+    const int32_t code = dtype_code(w.t);
+    const int64_t group = integer(a[1]);
+    const bool gated = PyObject_IsTrue(a[2]) == 1;
+    TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
+    TORCH_CHECK_VALUE(w.rows > 0 && w.width > 0 && w.width % 8 == 0 && (!gated || w.rows % 2 == 0),
+                      "w must be [out, inner] with inner a multiple of 8, a gated one's out even");
+    const int64_t nb = gated ? 2 * ((w.rows / 2 + 15) / 16) : (w.rows + 15) / 16;
+    const int64_t kb = (w.width + 127) / 128;
+    const at::Tensor packed = at::empty({nb, kb, 64, 4}, w.t.options().dtype(at::kInt));
+    const at::Tensor scales =
+        at::empty({nb, kb * (128 / group), 16}, w.t.options().dtype(at::kBFloat16));
+    call.run("pack_w4", [&](hipStream_t stream) {
+        return qdc_pack_w4(packed.data_ptr(), scales.data_ptr(), w.t.data_ptr(), w.rows, w.width,
+                           w.ld, group, gated, code, stream);
+    });
+    return pair(packed, scales);
+}
+
+// a[6]: the output's dtype code
+PyObject *unpack_w4(Args a) {
+    const Call call(tensor(a[0], "packed"));
+    const Weight4 w(call, a);
+    const int32_t code = (int32_t)integer(a[6]);
+    const at::Tensor out =
+        at::empty({w.out, w.inner}, w.packed.options().dtype(type_of(code)));
+    call.run("unpack_w4", [&](hipStream_t stream) {
+        return qdc_unpack_w4(out.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), w.out,
+                             w.inner, w.group, w.gated, code, stream);
+    });
+    return THPVariable_Wrap(out);
+}
+
+PyObject *quantize_q8(Args a) {
+    const Call call(tensor(a[0], "x"));
+    const Matrix x(call, a[0], "x");
+    const int32_t code = dtype_code(x.t);
+    const at::Tensor values = at::empty({x.rows, x.width}, x.t.options().dtype(at::kChar));
+    const at::Tensor scales = q8_scales(x.t, x.rows, x.width);
+    call.run("quantize_q8", [&](hipStream_t stream) {
+        return qdc_quantize_q8(values.data_ptr(), data<float>(scales), x.t.data_ptr(), x.rows,
+                               x.width, x.ld, code, stream);
+    });
+    return pair(values, scales);
+}
+
+PyObject *dequantize_q8(Args a) {
+    const Call call(tensor(a[0], "values"));
+    const Rows8 q(call, a[0], a[1]);
+    const int32_t code = (int32_t)integer(a[2]);
+    const at::Tensor out =
+        at::empty({q.rows, q.width}, q.values.options().dtype(type_of(code)));
+    call.run("dequantize_q8", [&](hipStream_t stream) {
+        return qdc_dequantize_q8(out.data_ptr(), q.values.data_ptr(), data<const float>(q.scales),
+                                 q.rows, q.width, code, stream);
+    });
+    return THPVariable_Wrap(out);
+}
+
+PyObject *residual_rms_q8(Args a) {
+    const at::Tensor &x = tensor(a[0], "x");
+    const Call call(x);
+    TORCH_CHECK_VALUE(x.dim() == 2 && call.plain(x, at::kFloat),
+                      "x must be a contiguous float32 matrix");
+    const int64_t rows = x.size(0), width = x.size(1);
+    const float *add = nullptr;
+    if (a[1] != Py_None) {
+        const at::Tensor &t = tensor(a[1], "add");
+        TORCH_CHECK_VALUE(t.sizes() == x.sizes() && call.plain(t, at::kFloat),
+                          "add must be a contiguous float32 tensor like x");
+        add = data<const float>(t);
+    }
+    const at::Tensor &norm = tensor(a[2], "weight");
+    const int32_t code = dtype_code(norm);
+    TORCH_CHECK_VALUE(norm.numel() == width && call.here(norm) && norm.is_contiguous(),
+                      "weight must be a contiguous vector of ", width, " elements on x's device");
+    const float eps = real(a[3]);
+    const int32_t *mask = nullptr;
+    if (a[4] != Py_None) mask = call.ints(a[4], "token_mask", rows);
+    const at::Tensor residual = add ? at::empty({rows, width}, x.options()) : x;
+    const at::Tensor values = at::empty({rows, width}, x.options().dtype(at::kChar));
+    const at::Tensor scales = q8_scales(x, rows, width);
+    call.run("residual_rms_q8", [&](hipStream_t stream) {
+        return qdc_residual_rmsnorm_q8(add ? data<float>(residual) : nullptr, values.data_ptr(),
+                                       data<float>(scales), data<const float>(x), add,
+                                       norm.data_ptr(), mask, rows, width, eps, code, stream);
+    });
+    THPObjectPtr r(THPVariable_Wrap(residual)), v(THPVariable_Wrap(values)),
+        s(THPVariable_Wrap(scales));
+    PyObject *t = r && v && s ? PyTuple_Pack(3, r.get(), v.get(), s.get()) : nullptr;
+    if (!t) throw python_error();
+    return t;
+}
+
+// a[0], a[1]: x, or the values and scales of 8-bit rows (a[1] not None); a[2..7]: the weight;
+// a[8]: the output's dtype code, -1 for x's
+PyObject *linear_w4(Args a) {
+    const at::Tensor &x0 = tensor(a[0], "x");
+    const Call call(x0);
+    const Weight4 w(call, a + 2);
+    int64_t rows, width, ld;
+    int32_t code = QDC_Q8;
+    const float *x_scales = nullptr;
+    if (a[1] != Py_None) {
+        const Rows8 x(call, a[0], a[1]);
+        rows = x.rows;
+        width = ld = x.width;
+        x_scales = data<const float>(x.scales);
+    } else {
+        const Matrix x(call, a[0], "x");
+        code = dtype_code(x0);
+        rows = x.rows;
+        width = x.width;
+        ld = x.ld;
+    }
+    TORCH_CHECK_VALUE(width == w.inner, "x has rows of ", width, " values, the weight takes ",
+                      w.inner);
+    int32_t out_code = (int32_t)integer(a[8]);
+    if (out_code < 0) out_code = code == QDC_Q8 ? QDC_BF16 : code;
+    const int64_t cols = w.gated ? w.out / 2 : w.out;
+    const at::Tensor y = at::empty(
+        {rows, cols},
+        x0.options().dtype(out_code == QDC_Q8 ? at::kChar : type_of(out_code)));
+    const at::Tensor y_scales = out_code == QDC_Q8 ? q8_scales(x0, rows, cols) : at::Tensor();
+    call.run(w.gated ? "gated_w4" : "linear_w4", [&](hipStream_t stream) {
+        return qdc_linear_w4(y.data_ptr(), out_code == QDC_Q8 ? data<float>(y_scales) : nullptr,
+                             out_code, x0.data_ptr(), x_scales, code, w.packed.data_ptr(),
+                             w.scales.data_ptr(), rows, w.out, w.inner, w.group, ld, w.gated,
+                             stream);
+    });
+    return out_code == QDC_Q8 ? pair(y, y_scales) : THPVariable_Wrap(y);
+}
+
 template <PyObject *(*F)(Args), Py_ssize_t N>
 PyObject *function(PyObject *, Args args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -430,6 +636,9 @@ PyMethodDef methods[] = {QDC_FUNCTION(prepare_paged, 17), QDC_FUNCTION(paged_att
                          QDC_FUNCTION(extend_pages, 9), QDC_FUNCTION(free_pages, 7),
                          QDC_FUNCTION(fork_pages, 9), QDC_FUNCTION(compact_pages, 6),
                          QDC_FUNCTION(copy_pages, 4), QDC_FUNCTION(delta_step, 16),
+                         QDC_FUNCTION(pack_w4, 3), QDC_FUNCTION(unpack_w4, 7),
+                         QDC_FUNCTION(quantize_q8, 1), QDC_FUNCTION(dequantize_q8, 3),
+                         QDC_FUNCTION(residual_rms_q8, 5), QDC_FUNCTION(linear_w4, 9),
                          {"on_failure", on_failure, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 #undef QDC_FUNCTION
@@ -438,10 +647,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "qdc_calls", nullptr, -1, methods};
 
 }  // namespace
 
-// version: of the header whose entry points the functions call
+// version, quant_version: of the headers whose entry points the functions call
 PyMODINIT_FUNC PyInit_qdc_calls() {
     PyObject *m = PyModule_Create(&module);
-    if (m && PyModule_AddStringConstant(m, "version", QDC_HIP_CACHE_VERSION) == 0) return m;
+    if (m && PyModule_AddStringConstant(m, "version", QDC_HIP_CACHE_VERSION) == 0 &&
+        PyModule_AddStringConstant(m, "quant_version", QDC_HIP_QUANT_VERSION) == 0)
+        return m;
     Py_XDECREF(m);
     return nullptr;
 }

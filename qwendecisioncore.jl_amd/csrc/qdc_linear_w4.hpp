@@ -1,0 +1,470 @@
+// qdc_linear_w4.hpp -- the product of rows with 4-bit weights, for rows of one type.
+//
+// y[m, n] = sum over groups g of s[n, g] * sum over k in g of q[n, k] x[m, k].  The whole
+// numbers enter the matrix instructions as they are (an 8-bit one holds 16 q, a bf16 one
+// 16 q exactly), so the only roundings are those of fp32 sums: a group's sum is scaled and
+// added in fp32, and the factor 16 taken out of the result.  fp32 rows enter as three bf16
+// terms that hold all 24 bits (8 each, by truncation); 8-bit rows as they are, with whole
+// sums, their own scale joining the weight's.
+//
+// A block of weights is 16 outputs x 128 inputs, 16 bytes a lane in the order of the
+// instruction's first operand; x is the second, so that a lane holds one row of the result
+// and 4 consecutive outputs.
+#pragma once
+
+#include "qdc_quant.hpp"
+
+namespace qdc {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+enum { kF32, kBf16, kQ8 };  // types of x
+
+// 8 bf16 values, of 4 + 4 signed bytes 16 q in the upper halves of a word's bytes.
+__device__ __forceinline__ bf16x8 widen(uint32_t word) {
+    const uint32_t lo = (word << 4) & 0xf0f0f0f0u, hi = word & 0xf0f0f0f0u;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t b = i ? hi : lo;
+        const float v0 = (float)(int8_t)b, v1 = (float)(int8_t)(b >> 8);
+        const float v2 = (float)(int8_t)(b >> 16), v3 = (float)(int8_t)(b >> 24);
+        // exact in bf16: the upper halves of the fp32 values
+        r[2 * i] = __builtin_amdgcn_perm(__float_as_uint(v1), __float_as_uint(v0), 0x07060302u);
+        r[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(v3), __float_as_uint(v2), 0x07060302u);
+    }
+    return __builtin_bit_cast(bf16x8, r);
+}
+
+// The three bf16 terms of fp32 values, each the upper half of what is left: hi + mid + lo
+// is v.  An infinity or NaN is its first term.
+__device__ __forceinline__ void terms(const float (&v)[8], u32x4 (&r)[3]) {
+    uint32_t h[8], m[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t b = __float_as_uint(v[i]);
+        const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+        h[i] = b | (!finite && (b & 0xffffu) ? 0x400000u : 0u);  // a NaN stays one
+        const float rest = finite ? v[i] - __uint_as_float(b & 0xffff0000u) : 0.0f;
+        m[i] = __float_as_uint(rest);
+        l[i] = __float_as_uint(rest - __uint_as_float(m[i] & 0xffff0000u));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[0][i] = __builtin_amdgcn_perm(h[2 * i + 1], h[2 * i], 0x07060302u);
+        r[1][i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u);
+        r[2][i] = __builtin_amdgcn_perm(l[2 * i + 1], l[2 * i], 0x07060302u);
+    }
+}
+
+// 4 scales as fp32.
+__device__ __forceinline__ f32x4 scales4(u32x2 s) {
+    return f32x4{__uint_as_float(s[0] << 16), __uint_as_float(s[0] & 0xffff0000u),
+                 __uint_as_float(s[1] << 16), __uint_as_float(s[1] & 0xffff0000u)};
+}
+
+// The operand of x for 32 inputs of a block: raw words as they are loaded or staged.
+template <int X> struct Piece {
+    static constexpr int kTerms = X == kF32 ? 3 : 1;
+    u32x4 t[kTerms];  // 8 values in bf16; kQ8: 8 bytes in the first two words
+};
+
+// total += the block's products.  piece(t): x for the inputs 32 t + 8 (lane / 16) + 0..7.
+template <int X, int G, typename F>
+__device__ __forceinline__ void block_product(f32x4 &total, u32x4 words, const u32x2 *scales,
+                                              float x_scale, F piece) {
+    if constexpr (X == kQ8) {
+#pragma unroll
+        for (int g = 0; g < 128 / G; ++g) {
+            i32x4 sum = {0, 0, 0, 0};
+            if constexpr (G == 32) {
+                const uint32_t w = words[g];
+                const u32x2 a = {(w << 4) & 0xf0f0f0f0u, w & 0xf0f0f0f0u};
+                const u32x4 x = piece(g).t[0];
+                sum = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                    __builtin_bit_cast(long, a), __builtin_bit_cast(long, u32x2{x[0], x[1]}), sum,
+                    0, 0, 0);
+            } else {
+#pragma unroll
+                for (int u = g * G / 64; u < (g + 1) * G / 64; ++u) {
+                    const uint32_t w0 = words[2 * u], w1 = words[2 * u + 1];
+                    const u32x4 a = {(w0 << 4) & 0xf0f0f0f0u, w0 & 0xf0f0f0f0u,
+                                     (w1 << 4) & 0xf0f0f0f0u, w1 & 0xf0f0f0f0u};
+                    const u32x4 x0 = piece(2 * u).t[0], x1 = piece(2 * u + 1).t[0];
+                    sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                        __builtin_bit_cast(i32x4, a),
+                        __builtin_bit_cast(i32x4, u32x4{x0[0], x0[1], x1[0], x1[1]}), sum, 0, 0, 0);
+                }
+            }
+            const f32x4 s = scales4(scales[g]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                total[r] = __builtin_fmaf((float)sum[r], s[r] * x_scale, total[r]);
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < 128 / G; ++g) {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int t = g * G / 32; t < (g + 1) * G / 32; ++t) {
+                const bf16x8 w = widen(words[t]);
+                const Piece<X> x = piece(t);
+#pragma unroll
+                for (int n = Piece<X>::kTerms - 1; n >= 0; --n)  // the smallest first
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        w, __builtin_bit_cast(bf16x8, x.t[n]), sum, 0, 0, 0);
+            }
+            const f32x4 s = scales4(scales[g]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) total[r] = __builtin_fmaf(sum[r], s[r], total[r]);
+        }
+    }
+}
+
+// 8 values of x from memory, zeros where there are none.
+template <int X> __device__ __forceinline__ Piece<X> load_piece(const void *row, int k, bool in) {
+    Piece<X> r{};
+    if (!in) return r;
+    if constexpr (X == kF32) {
+        float v[8];
+        unpack(load_frag<float, 8>(reinterpret_cast<const float *>(row) + k), v);
+        terms(v, r.t);
+    } else if constexpr (X == kBf16) {
+        r.t[0] = load_raw(reinterpret_cast<const bf16_t *>(row) + k);
+    } else {
+        const u32x2 h = *reinterpret_cast<const u32x2 *>(reinterpret_cast<const char *>(row) + k);
+        r.t[0] = u32x4{h[0], h[1], 0u, 0u};
+    }
+    return r;
+}
+template <int X> constexpr int kXBytes = X == kF32 ? 4 : X == kBf16 ? 2 : 1;
+
+// 4 consecutive outputs of a row, n the first; what is behind the last column is left out.
+template <typename T>
+__device__ __forceinline__ void put4(T *y, int row, int n, int cols, const float (&v)[4]) {
+    T *at = y + (int64_t)row * cols + n;
+    if ((cols & 3) == 0) {  // uniform
+        if (n < cols) store_frag<4>(at, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (n + j < cols) at[j] = from_f32<T>(v[j]);
+}
+__device__ __forceinline__ void put4(const W4Product &p, int32_t dtype, int row, int n,
+                                     const float (&v)[4]) {
+    if (dtype == QDC_F32) put4(reinterpret_cast<float *>(p.y), row, n, p.cols, v);
+    else put4(reinterpret_cast<bf16_t *>(p.y), row, n, p.cols, v);
+}
+
+// ---------------------------------------------------------------- few rows ---
+// A workgroup per block of outputs (two, gate and up, where gated) and 16 * MT rows, whose
+// wavefronts take the blocks of inputs in turn and add up at the end: bound by the weights'
+// way from memory and, for a row or two, by one trip there, so every load of a wavefront's
+// block leaves at once and x comes straight from the caches.
+template <int X, int G, int MT, bool GATED, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_dtype) {
+    constexpr int NB = GATED ? 2 : 1;
+    __shared__ f32x4 parts[WAVES][NB][MT][kWave];
+    const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int quarter = l / 16, b0 = blockIdx.x * NB, m0 = blockIdx.y * 16 * MT;
+    f32x4 total[NB][MT];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) total[b][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = wave; c < p.kb; c += WAVES) {
+        u32x4 words[NB];
+        u32x2 s[NB][128 / G];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int64_t unit = (int64_t)(b0 + b) * p.kb + c;
+            words[b] = load_stream(p.packed + unit * kWave + l);
+#pragma unroll
+            for (int g = 0; g < 128 / G; ++g)
+                s[b][g] = p.scales[(unit * (128 / G) + g) * 4 + quarter];
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int row = m0 + 16 * i + l % 16;
+            const bool in = row < p.rows;
+            const char *src = reinterpret_cast<const char *>(p.x) +
+                              (int64_t)(in ? row : 0) * p.ld_x * kXBytes<X>;
+            Piece<X> x[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int k = c * kW4Inputs + 32 * t + 8 * quarter;
+                x[t] = load_piece<X>(src, k, in && k < p.inner);
+            }
+            float xs = 0.0f;
+            if constexpr (X == kQ8)
+                if (in) xs = p.x_scales[(int64_t)row * p.q8_groups + c];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                block_product<X, G>(total[b][i], words[b], s[b], xs,
+                                    [&](int t) -> const Piece<X> & { return x[t]; });
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) parts[wave][b][i][l] = total[b][i];
+    __syncthreads();
+    if (wave >= MT) return;
+    const int row = m0 + 16 * wave + l % 16;
+    if (row >= p.rows) return;
+    f32x4 sum[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        sum[b] = parts[0][b][wave][l];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) sum[b] += parts[w][b][wave][l];
+    }
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        v[r] = sum[0][r] * 0.0625f;
+        if constexpr (GATED) v[r] = silu(v[r]) * (sum[1][r] * 0.0625f);
+    }
+    put4(p, y_dtype, row, 16 * (int)blockIdx.x + 4 * quarter, v);
+}
+
+// --------------------------------------------------------------- many rows ---
+// A workgroup of 4 x NWM wavefronts takes 256 outputs (16 blocks) by 16 * MT * NWM rows, a
+// wavefront 64 by 16 * MT.  x goes through LDS, a step of 128 inputs while the step before
+// is multiplied; the weights, read once or twice by a workgroup and in operand order
+// already, go to registers.  OUT8: the 256 outputs are gate and up of the 128 columns that
+// share a scale of an 8-bit row, whose maximum four wavefronts find together.
+template <int X, int MT, int NWM> struct Staged {
+    static constexpr int kRows = 16 * MT * NWM;
+    static constexpr int kThreads = 256 * NWM;
+    static constexpr int kTerms = Piece<X>::kTerms;
+    static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
+    static constexpr int kBytes = kRows * kLd * kTerms;
+};
+
+template <int X, int G, int MT, int NWM, bool GATED, bool OUT8>
+__global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dtype) {
+    typedef Staged<X, MT, NWM> S;
+    __shared__ __align__(16) char tile[2][S::kBytes];
+    const int tid = threadIdx.x, l = tid % kWave, wave = tid / kWave;
+    const int quarter = l / 16, wn = wave % 4, wm = wave / 4;
+    const int m0 = blockIdx.y * S::kRows, b0 = blockIdx.x * 16 + wn * 4;
+
+    // this thread's pieces of 8 values: the same columns of MT rows
+    const int k8 = tid % 16;
+    const char *src[MT];
+    bool in[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int row = m0 + tid / 16 + i * (S::kThreads / 16);
+        in[i] = row < p.rows;
+        src[i] = reinterpret_cast<const char *>(p.x) +
+                 (int64_t)(in[i] ? row : 0) * p.ld_x * kXBytes<X>;
+    }
+    // a step's raw values on their way
+    constexpr int RAW = X == kF32 ? 2 : 1;
+    u32x4 raw[MT][RAW];
+    auto load_x = [&](int c) {
+        const int k = c * kW4Inputs + 8 * k8;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const bool ok = in[i] && k < p.inner;
+#pragma unroll
+            for (int h = 0; h < RAW; ++h) raw[i][h] = u32x4{0u, 0u, 0u, 0u};
+            if (!ok) continue;
+            const char *at = src[i] + (int64_t)k * kXBytes<X>;
+            if constexpr (X == kQ8) {
+                const u32x2 v = *reinterpret_cast<const u32x2 *>(at);
+                raw[i][0] = u32x4{v[0], v[1], 0u, 0u};
+            } else {
+#pragma unroll
+                for (int h = 0; h < RAW; ++h) raw[i][h] = load_raw(at + 16 * h);
+            }
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            char *dst = tile[buf] + (tid / 16 + i * (S::kThreads / 16)) * S::kLd;
+            if constexpr (X == kQ8) {
+                // the two pieces that an instruction's lane takes lie side by side
+                *reinterpret_cast<u32x2 *>(dst + 64 * (k8 / 8) + 16 * (k8 % 4) +
+                                           8 * (k8 / 4 % 2)) = u32x2{raw[i][0][0], raw[i][0][1]};
+            } else if constexpr (X == kBf16) {
+                *reinterpret_cast<u32x4 *>(dst + 16 * k8) = raw[i][0];
+            } else {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(raw[i][e / 4][e % 4]);
+                u32x4 t[3];
+                terms(v, t);
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    *reinterpret_cast<u32x4 *>(dst + n * S::kRows * S::kLd + 16 * k8) = t[n];
+            }
+        }
+    };
+    u32x4 words[2][4];
+    u32x2 scales[2][4][128 / G];
+    float xs[2][MT];
+    auto load_w = [&](int c, int set) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // behind the last block: loaded, not stored
+            const int64_t unit = (int64_t)min(b0 + j, p.nb - 1) * p.kb + c;
+            words[set][j] = load_raw(p.packed + unit * kWave + l);
+#pragma unroll
+            for (int g = 0; g < 128 / G; ++g)
+                scales[set][j][g] = p.scales[(unit * (128 / G) + g) * 4 + quarter];
+        }
+        if constexpr (X == kQ8)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int row = m0 + wm * 16 * MT + 16 * i + l % 16;
+                xs[set][i] = p.x_scales[(int64_t)min(row, p.rows - 1) * p.q8_groups + c];
+            }
+    };
+
+    f32x4 total[4][MT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) total[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](int buf) {
+        const char *mine = tile[buf] + (wm * 16 * MT + l % 16) * S::kLd;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                block_product<X, G>(
+                    total[j][i], words[buf][j], scales[buf][j], X == kQ8 ? xs[buf][i] : 0.0f,
+                    [&](int t) {
+                        Piece<X> r{};
+                        const char *at = mine + 16 * i * S::kLd;
+                        if constexpr (X == kQ8) {
+                            const u32x2 h = *reinterpret_cast<const u32x2 *>(
+                                at + 64 * (t / 2) + 16 * quarter + 8 * (t % 2));
+                            r.t[0] = u32x4{h[0], h[1], 0u, 0u};
+                        } else {
+#pragma unroll
+                            for (int n = 0; n < S::kTerms; ++n)
+                                r.t[n] = *reinterpret_cast<const u32x4 *>(
+                                    at + n * S::kRows * S::kLd + 64 * t + 16 * quarter);
+                        }
+                        return r;
+                    });
+    };
+    load_x(0);
+    load_w(0, 0);
+    stage(0);
+    __syncthreads();
+    for (int c = 0; c < p.kb; c += 2)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // step c + h: buffer and set h
+            if (c + h >= p.kb) break;  // uniform
+            const bool more = c + h + 1 < p.kb;
+            if (more) {
+                load_x(c + h + 1);
+                load_w(c + h + 1, h ^ 1);
+            }
+            multiply(h);
+            if (more) stage(h ^ 1);  // read a step ago, a barrier back
+            __syncthreads();
+        }
+
+    constexpr int NB = GATED ? 2 : 1;
+    uint32_t(*most)[S::kRows] = reinterpret_cast<uint32_t(*)[S::kRows]>(tile[0]);
+    float act[4 / NB][MT][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int at = wm * 16 * MT + 16 * i + l % 16, row = m0 + at;
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4 / NB; ++j) {
+            const int n = (b0 / NB + j) * kW4Outputs + 4 * quarter;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = total[NB * j][i][r] * 0.0625f;
+                if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * 0.0625f);
+                act[j][i][r] = v;
+                if (OUT8 && n < p.cols) m = max(m, size_bits(v));
+            }
+            if constexpr (!OUT8)
+                if (row < p.rows) put4(p, y_dtype, row, n, act[j][i]);
+        }
+        if constexpr (OUT8) {  // over the quarters, then the wavefronts
+            const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+            m = max(a[0], a[1]);
+            const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+            m = max(b[0], b[1]);
+            if (quarter == 0) most[wn][at] = m;
+        }
+    }
+    if constexpr (OUT8) {
+        __syncthreads();
+        const int groups = (p.cols + kQ8Group - 1) / kQ8Group;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int at = wm * 16 * MT + 16 * i + l % 16, row = m0 + at;
+            if (row >= p.rows) continue;
+            const Q8Scale s(max(max(most[0][at], most[1][at]), max(most[2][at], most[3][at])));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = (b0 / 2 + j) * kW4Outputs + 4 * quarter;
+                if (n >= p.cols) continue;
+                *reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.y) +
+                                              (int64_t)row * p.cols + n) =
+                    pack_bytes(s.value(act[j][i][0]), s.value(act[j][i][1]), s.value(act[j][i][2]),
+                               s.value(act[j][i][3]));
+            }
+            if (wn == 0 && quarter == 0)
+                p.y_scales[(int64_t)row * groups + blockIdx.x] = s.scale;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- dispatch ---
+template <int X, int G, int MT, bool GATED, int WAVES>
+int32_t launch_rows(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    const dim3 grid((uint32_t)(p.nb / (GATED ? 2 : 1)),
+                    (uint32_t)ceil_div((int64_t)p.rows, (int64_t)16 * MT));
+    hipLaunchKernelGGL((w4_rows<X, G, MT, GATED, WAVES>), grid, dim3(WAVES * kWave), 0, s, p,
+                       y_dtype);
+    return launch_status();
+}
+template <int X, int G, int MT, int NWM, bool GATED, bool OUT8>
+int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    const dim3 grid((uint32_t)ceil_div((int64_t)p.nb, (int64_t)16),
+                    (uint32_t)ceil_div((int64_t)p.rows, (int64_t)16 * MT * NWM));
+    hipLaunchKernelGGL((w4_tiles<X, G, MT, NWM, GATED, OUT8>), grid, dim3(256 * NWM), 0, s, p,
+                       y_dtype);
+    return launch_status();
+}
+
+template <int X, int G, bool GATED>
+int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    constexpr int BIG = X == kF32 ? 2 : 4;  // fp32: three terms a row in LDS
+    if constexpr (GATED)
+        if (y_dtype == QDC_Q8) {
+            if (p.rows <= 16) return launch_tiles<X, G, 1, 1, true, true>(p, y_dtype, s);
+            if (p.rows <= 512) return launch_tiles<X, G, 2, 1, true, true>(p, y_dtype, s);
+            return launch_tiles<X, G, BIG, 2, true, true>(p, y_dtype, s);
+        }
+    if (p.rows <= 16) return launch_rows<X, G, 1, GATED, 8>(p, y_dtype, s);
+    if (p.rows <= 64) return launch_rows<X, G, 2, GATED, 8>(p, y_dtype, s);
+    if (p.rows <= 512) return launch_tiles<X, G, 2, 1, GATED, false>(p, y_dtype, s);
+    return launch_tiles<X, G, BIG, 2, GATED, false>(p, y_dtype, s);
+}
+
+template <int X>
+int32_t linear_w4(const W4Product &p, int group, bool gated, int32_t y_dtype, hipStream_t s) {
+    if (group == 32) return gated ? launch<X, 32, true>(p, y_dtype, s) : launch<X, 32, false>(p, y_dtype, s);
+    if (group == 64) return gated ? launch<X, 64, true>(p, y_dtype, s) : launch<X, 64, false>(p, y_dtype, s);
+    return gated ? launch<X, 128, true>(p, y_dtype, s) : launch<X, 128, false>(p, y_dtype, s);
+}
+
+}  // namespace
+}  // namespace qdc

@@ -1,0 +1,10 @@
+// qdc_linear_w4_q8.hip -- the kernels of qdc_linear_w4.hpp for rows in 8 bits.
+#include "qdc_linear_w4.hpp"
+
+namespace qdc {
+
+int32_t linear_w4_q8(const W4Product &p, int group, bool gated, int32_t y_dtype, hipStream_t s) {
+    return linear_w4<kQ8>(p, group, gated, y_dtype, s);
+}
+
+}  // namespace qdc

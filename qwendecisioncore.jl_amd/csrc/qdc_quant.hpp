@@ -1,0 +1,122 @@
+// qdc_quant.hpp -- what the kernels on 4-bit weights and 8-bit rows share.
+#pragma once
+
+#include "qdc_common.hpp"
+#include "qdc_hip_quant.h"
+
+namespace qdc {
+
+constexpr int kQ8Group = 128;   // columns of an 8-bit row that share a scale
+constexpr int kW4Outputs = 16;  // of a block of 4-bit weights: a matrix instruction's rows,
+constexpr int kW4Inputs = 128;  // and as many inputs as make it 16 bytes a lane
+constexpr int kW4Words = 256;
+
+// |v| as an integer that orders like it, NaN above infinity.
+__device__ __forceinline__ uint32_t size_bits(float v) {
+    return __float_as_uint(v) & 0x7fffffffu;
+}
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true));
+}
+// The maximum over aligned groups of N lanes (as group_sum's sum).
+template <int N> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    if constexpr (N >= 2) v = dpp_max<0xB1>(v);
+    if constexpr (N >= 4) v = dpp_max<0x4E>(v);
+    if constexpr (N >= 8) v = dpp_max<0x141>(v);
+    if constexpr (N >= 16) v = dpp_max<0x140>(v);
+    if constexpr (N >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = max(r[0], r[1]);
+    }
+    if constexpr (N >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = max(r[0], r[1]);
+    }
+    return v;
+}
+
+// The scale of a group of 8-bit values whose largest size is `most`, and values under it.
+struct Q8Scale {
+    float scale, inverse;
+    bool plain;  // whether a product with the inverse will do
+
+    __device__ explicit Q8Scale(uint32_t most) {
+        scale = __uint_as_float(most) / 127.0f;
+        // below 2^-100 the inverse may overflow; infinities and NaN: every value is 0
+        plain = most >= 0x0d800000u && most < 0x7f800000u;
+        inverse = plain ? 1.0f / scale : 0.0f;
+    }
+    // within -127..127: |v| <= most, and the product is off by 2 roundings at most
+    __device__ __forceinline__ int value(float v) const {
+        if (plain) return (int)__builtin_rintf(v * inverse);
+        if (!(scale > 0.0f && scale < __builtin_inff())) return 0;
+        return (int)fminf(fmaxf(__builtin_rintf(v / scale), -127.0f), 127.0f);
+    }
+};
+
+__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
+    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 |
+           (uint32_t)d << 24;
+}
+
+static inline bool w4_group(int64_t group) { return group == 32 || group == 64 || group == 128; }
+// Blocks of outputs and of inputs.
+static inline int64_t w4_rows(int64_t out, int32_t gated) {
+    return gated ? 2 * ceil_div(out / 2, (int64_t)kW4Outputs) : ceil_div(out, (int64_t)kW4Outputs);
+}
+static inline int64_t w4_cols(int64_t inner) { return ceil_div(inner, (int64_t)kW4Inputs); }
+
+// A weight's sizes: within 2^24 outputs and inputs, 2^31 words.
+static inline bool w4_shape(int64_t out, int64_t inner, int64_t group, int32_t gated) {
+    const int64_t lim = (int64_t)1 << 24;
+    return out > 0 && inner > 0 && out < lim && inner < lim && inner % 8 == 0 && w4_group(group) &&
+           (!gated || out % 2 == 0) &&
+           w4_rows(out, gated) * w4_cols(inner) < ((int64_t)1 << 31) / kW4Words;
+}
+static inline int64_t w4_bytes(int64_t out, int64_t inner, int32_t gated) {
+    return w4_rows(out, gated) * w4_cols(inner) * kW4Words * 4;
+}
+static inline int64_t w4_scale_bytes(int64_t out, int64_t inner, int64_t group, int32_t gated) {
+    return w4_rows(out, gated) * w4_cols(inner) * (kW4Inputs / group) * kW4Outputs * 2;
+}
+static inline int64_t q8_groups(int64_t width) { return ceil_div(width, (int64_t)kQ8Group); }
+
+struct QuantRange {
+    const void *p;
+    int64_t bytes;
+};
+// Whether an output overlaps an input or another output (null: nothing there).
+static inline bool quant_alias(const QuantRange *outs, int n_outs, const QuantRange *ins,
+                               int n_ins) {
+    for (int i = 0; i < n_outs; ++i) {
+        if (!outs[i].p) continue;
+        for (int j = 0; j < n_ins; ++j)
+            if (ins[j].p && overlaps(outs[i].p, outs[i].bytes, ins[j].p, ins[j].bytes)) return true;
+        for (int j = 0; j < i; ++j)
+            if (outs[j].p && overlaps(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes))
+                return true;
+    }
+    return false;
+}
+
+// What the kernels of the product are given.
+struct W4Product {
+    const void *x;
+    const float *x_scales;
+    const u32x4 *packed;
+    const u32x2 *scales;  // 4 bf16 scales each
+    void *y;
+    float *y_scales;
+    int64_t ld_x;
+    int rows, cols;  // of y
+    int inner, kb;   // inputs, blocks of inputs
+    int nb;          // blocks of outputs
+    int q8_groups;   // of a row of x
+};
+
+// The products of x in one type; y_dtype QDC_F32, QDC_BF16 or, gated, QDC_Q8.
+int32_t linear_w4_f32(const W4Product &p, int group, bool gated, int32_t y_dtype, hipStream_t s);
+int32_t linear_w4_bf16(const W4Product &p, int group, bool gated, int32_t y_dtype, hipStream_t s);
+int32_t linear_w4_q8(const W4Product &p, int group, bool gated, int32_t y_dtype, hipStream_t s);
+
+}  // namespace qdc

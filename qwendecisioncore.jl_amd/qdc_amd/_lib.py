@@ -3,7 +3,7 @@
 The library is loaded from ``qwendecisioncore.jl_amd/lib/`` (built in-tree by
 ``make -C qwendecisioncore.jl_amd/csrc``).  There is no fallback: a missing
 library is an error.  ``lib/qdc_calls.so`` (``make -C qwendecisioncore.jl_amd/csrc
-python``) calls the cache's operators for PyTorch tensors.  Status codes map to
+python``) calls the operators of the cache and on 4-bit weights for PyTorch tensors.  Status codes map to
 exceptions the way the reference maps bad input to ``ArgumentError`` /
 ``DimensionMismatch``: a negative status raises
 ``ValueError`` (argument error found on the host before any launch), a positive
@@ -23,6 +23,7 @@ CALLS_PATH = os.path.join(os.path.dirname(_HERE), "lib", "qdc_calls.so")
 QDC_F32 = 0
 QDC_BF16 = 1
 QDC_BF16X2 = 2  # output only: two bf16 terms per fp32 value
+QDC_Q8 = 3      # rows in 8 bits with scales, of the operators on 4-bit weights
 
 STATUS = {0: "QDC_OK", -1: "QDC_ERR_NULL", -2: "QDC_ERR_SHAPE", -3: "QDC_ERR_DTYPE",
           -4: "QDC_ERR_RANGE", -5: "QDC_ERR_ALIAS"}
@@ -104,6 +105,18 @@ CACHE_SIGNATURES = {
     "qdc_delta_scan_state": (_i32, [_vp, _i32] + [_vp] * 6 + [_i64] * 8 + [_vp, _i64, _vp]),
 }
 
+# the entry points of include/qdc_hip_quant.h, likewise
+QUANT_SIGNATURES = {
+    "qdc_quant_version": (ctypes.c_char_p, []),
+    "qdc_pack_w4": (_i32, [_vp] * 3 + [_i64] * 4 + [_i32, _i32, _vp]),
+    "qdc_unpack_w4": (_i32, [_vp] * 3 + [_i64] * 3 + [_i32, _i32, _vp]),
+    "qdc_quantize_q8": (_i32, [_vp] * 3 + [_i64] * 3 + [_i32, _vp]),
+    "qdc_dequantize_q8": (_i32, [_vp] * 3 + [_i64] * 2 + [_i32, _vp]),
+    "qdc_residual_rmsnorm_q8": (_i32, [_vp] * 7 + [_i64] * 2 + [_f32, _i32, _vp]),
+    "qdc_linear_w4": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp] + [_i64] * 5
+                      + [_i32, _vp]),
+}
+
 _lib = None
 
 
@@ -120,8 +133,8 @@ def lib():
                 f"{LIB_PATH} is not built; run `make -C qwendecisioncore.jl_amd/csrc` "
                 "or __graft_entry__.build()")
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in (SIGNATURES | WORKSPACE_SIGNATURES
-                                  | CACHE_SIGNATURES).items():
+        for name, (res, args) in (SIGNATURES | WORKSPACE_SIGNATURES | CACHE_SIGNATURES
+                                  | QUANT_SIGNATURES).items():
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
@@ -145,10 +158,11 @@ def calls():
         module = importlib.util.module_from_spec(
             importlib.util.spec_from_file_location("qdc_calls", CALLS_PATH, loader=loader))
         loader.exec_module(module)
-        version = lib().qdc_cache_version().decode()
-        if module.version != version:   # the arguments may be others
-            raise RuntimeError(f"{CALLS_PATH} was built for {module.version!r}, the library is "
-                               f"{version!r}; run `make -C qwendecisioncore.jl_amd/csrc python`")
+        for built, version in ((module.version, lib().qdc_cache_version().decode()),
+                               (module.quant_version, lib().qdc_quant_version().decode())):
+            if built != version:   # the arguments may be others
+                raise RuntimeError(f"{CALLS_PATH} was built for {built!r}, the library is "
+                                   f"{version!r}; run `make -C qwendecisioncore.jl_amd/csrc python`")
         module.on_failure(check)
         _calls = module
     return _calls
