@@ -12,6 +12,8 @@
 // and 4 consecutive outputs.
 #pragma once
 
+#include <type_traits>
+
 #include "qdc_quant.hpp"
 
 namespace qdc {
@@ -248,51 +250,50 @@ template <int X, int MT, int NWM> struct Staged {
 template <int X, int G, int MT, int NWM, bool GATED, bool OUT8>
 __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dtype) {
     typedef Staged<X, MT, NWM> S;
+    constexpr int NG = 128 / G;  // groups of a step
     __shared__ __align__(16) char tile[2][S::kBytes];
     const int tid = threadIdx.x, l = tid % kWave, wave = tid / kWave;
     const int quarter = l / 16, wn = wave % 4, wm = wave / 4;
     const int m0 = blockIdx.y * S::kRows, b0 = blockIdx.x * 16 + wn * 4;
 
-    // this thread's pieces of 8 values: the same columns of MT rows
+    // this thread's pieces of 8 values: the same columns of MT rows (behind the last row:
+    // the first one's, which is not stored)
     const int k8 = tid % 16;
     const char *src[MT];
-    bool in[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int row = m0 + tid / 16 + i * (S::kThreads / 16);
-        in[i] = row < p.rows;
         src[i] = reinterpret_cast<const char *>(p.x) +
-                 (int64_t)(in[i] ? row : 0) * p.ld_x * kXBytes<X>;
+                 (int64_t)(row < p.rows ? row : 0) * p.ld_x * kXBytes<X>;
     }
     // a step's raw values on their way
     constexpr int RAW = X == kF32 ? 2 : 1;
-    u32x4 raw[MT][RAW];
+    typedef typename std::conditional<X == kQ8, u32x2, u32x4>::type Raw;
+    Raw raw[MT][RAW];
     auto load_x = [&](int c) {
         const int k = c * kW4Inputs + 8 * k8;
+        const int64_t at = k < p.inner ? (int64_t)k * kXBytes<X> : 0;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const bool ok = in[i] && k < p.inner;
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int h = 0; h < RAW; ++h) raw[i][h] = u32x4{0u, 0u, 0u, 0u};
-            if (!ok) continue;
-            const char *at = src[i] + (int64_t)k * kXBytes<X>;
-            if constexpr (X == kQ8) {
-                const u32x2 v = *reinterpret_cast<const u32x2 *>(at);
-                raw[i][0] = u32x4{v[0], v[1], 0u, 0u};
-            } else {
-#pragma unroll
-                for (int h = 0; h < RAW; ++h) raw[i][h] = load_raw(at + 16 * h);
-            }
-        }
+            for (int h = 0; h < RAW; ++h)
+                raw[i][h] = *reinterpret_cast<const Raw *>(src[i] + at + 16 * h);
     };
-    auto stage = [&](int buf) {
+    auto stage = [&](int buf, int c) {
+        // zeros behind the last input, where the weights are 0 but x might be infinite
+        const bool ok = c * kW4Inputs + 8 * k8 < p.inner;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             char *dst = tile[buf] + (tid / 16 + i * (S::kThreads / 16)) * S::kLd;
+#pragma unroll
+            for (int h = 0; h < RAW; ++h)
+#pragma unroll
+                for (int e = 0; e < (X == kQ8 ? 2 : 4); ++e)
+                    raw[i][h][e] = ok ? raw[i][h][e] : 0u;
             if constexpr (X == kQ8) {
                 // the two pieces that an instruction's lane takes lie side by side
                 *reinterpret_cast<u32x2 *>(dst + 64 * (k8 / 8) + 16 * (k8 % 4) +
-                                           8 * (k8 / 4 % 2)) = u32x2{raw[i][0][0], raw[i][0][1]};
+                                           8 * (k8 / 4 % 2)) = raw[i][0];
             } else if constexpr (X == kBf16) {
                 *reinterpret_cast<u32x4 *>(dst + 16 * k8) = raw[i][0];
             } else {
@@ -307,24 +308,24 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
             }
         }
     };
-    u32x4 words[2][4];
-    u32x2 scales[2][4][128 / G];
-    float xs[2][MT];
-    auto load_w = [&](int c, int set) {
+    // a step's weights on their way, then as they are multiplied
+    u32x4 words[4];
+    u32x2 scales[4][NG];
+    float xs[MT];
+    auto load_w = [&](int c) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             // behind the last block: loaded, not stored
             const int64_t unit = (int64_t)min(b0 + j, p.nb - 1) * p.kb + c;
-            words[set][j] = load_raw(p.packed + unit * kWave + l);
+            words[j] = load_raw(p.packed + unit * kWave + l);
 #pragma unroll
-            for (int g = 0; g < 128 / G; ++g)
-                scales[set][j][g] = p.scales[(unit * (128 / G) + g) * 4 + quarter];
+            for (int g = 0; g < NG; ++g) scales[j][g] = p.scales[(unit * NG + g) * 4 + quarter];
         }
         if constexpr (X == kQ8)
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const int row = m0 + wm * 16 * MT + 16 * i + l % 16;
-                xs[set][i] = p.x_scales[(int64_t)min(row, p.rows - 1) * p.q8_groups + c];
+                xs[i] = p.x_scales[(int64_t)min(row, p.rows - 1) * p.q8_groups + c];
             }
     };
 
@@ -333,47 +334,156 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
     for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) total[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto multiply = [&](int buf) {
-        const char *mine = tile[buf] + (wm * 16 * MT + l % 16) * S::kLd;
+
+    // A step's products, in units of four instructions or more whose sums are scaled and
+    // added while the next unit's are multiplied: the scheduler, left to itself, starts them
+    // all and runs out of registers.
+    auto multiply_whole = [&](int buf, auto &&next) {
+        const char *mine = tile[buf] + (wm * 16 * MT + l % 16) * S::kLd + 16 * quarter;
+        u32x4 a[4][2];
+        f32x4 s[4][NG];
+        float own[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int j = 0; j < 4; ++j) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                block_product<X, G>(
-                    total[j][i], words[buf][j], scales[buf][j], X == kQ8 ? xs[buf][i] : 0.0f,
-                    [&](int t) {
-                        Piece<X> r{};
-                        const char *at = mine + 16 * i * S::kLd;
-                        if constexpr (X == kQ8) {
-                            const u32x2 h = *reinterpret_cast<const u32x2 *>(
-                                at + 64 * (t / 2) + 16 * quarter + 8 * (t % 2));
-                            r.t[0] = u32x4{h[0], h[1], 0u, 0u};
-                        } else {
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t w0 = words[j][2 * u], w1 = words[j][2 * u + 1];
+                a[j][u] = u32x4{(w0 << 4) & 0xf0f0f0f0u, w0 & 0xf0f0f0f0u, (w1 << 4) & 0xf0f0f0f0u,
+                                w1 & 0xf0f0f0f0u};
+            }
 #pragma unroll
-                            for (int n = 0; n < S::kTerms; ++n)
-                                r.t[n] = *reinterpret_cast<const u32x4 *>(
-                                    at + n * S::kRows * S::kLd + 64 * t + 16 * quarter);
-                        }
-                        return r;
-                    });
+            for (int g = 0; g < NG; ++g) s[j][g] = scales4(scales[j][g]);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) own[i] = xs[i];
+        next();
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4 x[2][2];
+        auto read = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                x[i % 2][u] =
+                    *reinterpret_cast<const u32x4 *>(mine + 16 * i * S::kLd + 64 * u);
+        };
+        read(0);
+        i32x4 sum[2][4];
+        f32x4 block[4];
+#pragma unroll
+        for (int n = 0; n <= MT * NG; ++n) {
+            if (n < MT * NG) {
+                const int i = n / NG, g = n % NG;
+                if (g == 0 && i + 1 < MT) read(i + 1);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    i32x4 &to = sum[n % 2][j];
+                    to = i32x4{0, 0, 0, 0};
+                    if constexpr (G == 32) {
+                        const u32x4 w = a[j][g / 2], v = x[i % 2][g / 2];
+                        const int h = g % 2 * 2;
+                        to = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                            __builtin_bit_cast(long, u32x2{w[h], w[h + 1]}),
+                            __builtin_bit_cast(long, u32x2{v[h], v[h + 1]}), to, 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int u = g * (G / 64); u < (g + 1) * (G / 64); ++u)
+                            to = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                                __builtin_bit_cast(i32x4, a[j][u]),
+                                __builtin_bit_cast(i32x4, x[i % 2][u]), to, 0, 0, 0);
+                    }
+                }
+            }
+            if (n > 0) {
+                const int i = (n - 1) / NG, g = (n - 1) % NG;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = (float)sum[(n - 1) % 2][j][r];
+                        block[j][r] = g == 0 ? v * s[j][g][r]
+                                             : __builtin_fmaf(v, s[j][g][r], block[j][r]);
+                        if (g == NG - 1)
+                            total[j][i][r] = __builtin_fmaf(block[j][r], own[i], total[j][i][r]);
+                    }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto multiply_float = [&](int buf, auto &&next) {
+        const char *mine = tile[buf] + (wm * 16 * MT + l % 16) * S::kLd + 16 * quarter;
+        constexpr int KEEP = G == 128 ? MT : 2;  // sums alive: all rows' over two halves
+        constexpr int UG = G == 32 ? 2 : 1;      // groups in a half
+        f32x4 sum[KEEP][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            bf16x8 a[4][2];
+            f32x4 s[4][UG];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) a[j][t] = widen(words[j][2 * half + t]);
+#pragma unroll
+                for (int g = 0; g < UG; ++g) s[j][g] = scales4(scales[j][G == 128 ? 0 : half * UG + g]);
+            }
+            if (half == 1) next();
+            __builtin_amdgcn_sched_barrier(0);
+            u32x4 x[2][2][S::kTerms];
+            auto read = [&](int i) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int n = 0; n < S::kTerms; ++n)
+                        x[i % 2][t][n] = *reinterpret_cast<const u32x4 *>(
+                            mine + n * S::kRows * S::kLd + 16 * i * S::kLd + 64 * (2 * half + t));
+            };
+            read(0);
+#pragma unroll
+            for (int n = 0; n <= MT * UG; ++n) {
+                if (n < MT * UG) {
+                    const int i = n / UG, g = n % UG;
+                    if (g == 0 && i + 1 < MT) read(i + 1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        f32x4 &to = sum[n % KEEP][j];
+                        if (G != 128 || half == 0) to = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int t = UG == 2 ? g : 0; t < (UG == 2 ? g + 1 : 2); ++t)
+#pragma unroll
+                            for (int k = S::kTerms - 1; k >= 0; --k)  // the smallest first
+                                to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    a[j][t], __builtin_bit_cast(bf16x8, x[i % 2][t][k]), to, 0, 0,
+                                    0);
+                    }
+                }
+                if (n > 0 && (G != 128 || half == 1)) {
+                    const int i = (n - 1) / UG, g = (n - 1) % UG;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            total[j][i][r] = __builtin_fmaf(sum[(n - 1) % KEEP][j][r], s[j][g][r],
+                                                            total[j][i][r]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     };
     load_x(0);
-    load_w(0, 0);
-    stage(0);
+    load_w(0);
+    stage(0, 0);
     __syncthreads();
-    for (int c = 0; c < p.kb; c += 2)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {  // step c + h: buffer and set h
-            if (c + h >= p.kb) break;  // uniform
-            const bool more = c + h + 1 < p.kb;
-            if (more) {
-                load_x(c + h + 1);
-                load_w(c + h + 1, h ^ 1);
-            }
-            multiply(h);
-            if (more) stage(h ^ 1);  // read a step ago, a barrier back
-            __syncthreads();
-        }
+    // One block of code: after a branch, the last step's sums would be scaled behind it, all
+    // of them held until then.  (So the last step loads and stages itself once more.)
+    for (int c = 0; c < p.kb; ++c) {
+        const int after = min(c + 1, p.kb - 1);
+        auto next = [&] {
+            load_w(after);
+            load_x(after);
+        };
+        if constexpr (X == kQ8) multiply_whole(c & 1, next);
+        else multiply_float(c & 1, next);
+        stage(~c & 1, after);  // read a step ago, a barrier back
+        __syncthreads();
+    }
 
     constexpr int NB = GATED ? 2 : 1;
     uint32_t(*most)[S::kRows] = reinterpret_cast<uint32_t(*)[S::kRows]>(tile[0]);
