@@ -67,6 +67,14 @@ __device__ __forceinline__ f32x4 scales4(u32x2 s) {
                  __uint_as_float(s[1] << 16), __uint_as_float(s[1] & 0xffff0000u)};
 }
 
+// Whole sums as fp32 by a subtraction: they start at 1.5 * 2^23, whose last bit as a float is
+// 1, and stay within the 2^22 to either side (128 products of 128 * 127 at most).  Four times
+// as fast as a conversion.
+constexpr int kWhole = 0x4b400000;
+__device__ __forceinline__ float whole(int sum) {
+    return __int_as_float(sum) - __int_as_float(kWhole);
+}
+
 // The operand of x for 32 inputs of a block: raw words as they are loaded or staged.
 template <int X> struct Piece {
     static constexpr int kTerms = X == kF32 ? 3 : 1;
@@ -80,7 +88,7 @@ __device__ __forceinline__ void block_product(f32x4 &total, u32x4 words, const u
     if constexpr (X == kQ8) {
 #pragma unroll
         for (int g = 0; g < 128 / G; ++g) {
-            i32x4 sum = {0, 0, 0, 0};
+            i32x4 sum = {kWhole, kWhole, kWhole, kWhole};
             if constexpr (G == 32) {
                 const uint32_t w = words[g];
                 const u32x2 a = {(w << 4) & 0xf0f0f0f0u, w & 0xf0f0f0f0u};
@@ -103,7 +111,7 @@ __device__ __forceinline__ void block_product(f32x4 &total, u32x4 words, const u
             const f32x4 s = scales4(scales[g]);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                total[r] = __builtin_fmaf((float)sum[r], s[r] * x_scale, total[r]);
+                total[r] = __builtin_fmaf(whole(sum[r]), s[r] * x_scale, total[r]);
         }
     } else {
 #pragma unroll
@@ -143,22 +151,26 @@ template <int X> __device__ __forceinline__ Piece<X> load_piece(const void *row,
 }
 template <int X> constexpr int kXBytes = X == kF32 ? 4 : X == kBf16 ? 2 : 1;
 
-// 4 consecutive outputs of a row, n the first; what is behind the last column is left out.
+// 4 consecutive outputs from `at` on, of which `left` lie within the row.
 template <typename T>
-__device__ __forceinline__ void put4(T *y, int row, int n, int cols, const float (&v)[4]) {
-    T *at = y + (int64_t)row * cols + n;
-    if ((cols & 3) == 0) {  // uniform
-        if (n < cols) store_frag<4>(at, v);
+__device__ __forceinline__ void put4(T *at, int left, bool whole, const float (&v)[4]) {
+    if (whole) {  // uniform
+        // an ordinary store: the cache joins what the wavefront's next ones write of a line
+        if (left <= 0) return;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4 *>(at) = pack(v);
+        else *reinterpret_cast<u32x2 *>(at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
         return;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (n + j < cols) at[j] = from_f32<T>(v[j]);
+        if (j < left) at[j] = from_f32<T>(v[j]);
 }
-__device__ __forceinline__ void put4(const W4Product &p, int32_t dtype, int row, int n,
-                                     const float (&v)[4]) {
-    if (dtype == QDC_F32) put4(reinterpret_cast<float *>(p.y), row, n, p.cols, v);
-    else put4(reinterpret_cast<bf16_t *>(p.y), row, n, p.cols, v);
+// N pieces of 4 outputs of a row, 16 apart, n the first output.
+template <typename T, int N>
+__device__ __forceinline__ void put(const W4Product &p, int row, int n, const float (&v)[N][4]) {
+    T *at = reinterpret_cast<T *>(p.y) + (int64_t)row * p.cols + n;
+#pragma unroll
+    for (int j = 0; j < N; ++j) put4(at + 16 * j, p.cols - n - 16 * j, (p.cols & 3) == 0, v[j]);
 }
 
 // ---------------------------------------------------------------- few rows ---
@@ -224,67 +236,93 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_d
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) sum[b] += parts[w][b][wave][l];
     }
-    float v[4];
+    float v[1][4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-        v[r] = sum[0][r] * 0.0625f;
-        if constexpr (GATED) v[r] = silu(v[r]) * (sum[1][r] * 0.0625f);
+        v[0][r] = sum[0][r] * 0.0625f;
+        if constexpr (GATED) v[0][r] = silu(v[0][r]) * (sum[1][r] * 0.0625f);
     }
-    put4(p, y_dtype, row, 16 * (int)blockIdx.x + 4 * quarter, v);
+    const int n = 16 * (int)blockIdx.x + 4 * quarter;
+    if (y_dtype == QDC_F32) put<float>(p, row, n, v);
+    else put<bf16_t>(p, row, n, v);
 }
 
 // --------------------------------------------------------------- many rows ---
-// A workgroup of 4 x NWM wavefronts takes 256 outputs (16 blocks) by 16 * MT * NWM rows, a
-// wavefront 64 by 16 * MT.  x goes through LDS, a step of 128 inputs while the step before
-// is multiplied; the weights, read once or twice by a workgroup and in operand order
-// already, go to registers.  OUT8: the 256 outputs are gate and up of the 128 columns that
+// A workgroup of 4 wavefronts takes tiles of 256 outputs (16 blocks) by 16 * MT rows, a
+// wavefront 64 outputs of them.  x goes through LDS, a step of 128 inputs while the step
+// before is multiplied; the weights, each for one wavefront and in operand order already,
+// go to registers.  OUT8: the 256 outputs are gate and up of the 128 columns that
 // share a scale of an 8-bit row, whose maximum four wavefronts find together.
-template <int X, int MT, int NWM> struct Staged {
-    static constexpr int kRows = 16 * MT * NWM;
-    static constexpr int kThreads = 256 * NWM;
+template <int X, int MT> struct Staged {
+    static constexpr int kRows = 16 * MT;
     static constexpr int kTerms = Piece<X>::kTerms;
     static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
     static constexpr int kBytes = kRows * kLd * kTerms;
 };
 
-template <int X, int G, int MT, int NWM, bool GATED, bool OUT8>
-__global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dtype) {
-    typedef Staged<X, MT, NWM> S;
+// The tiles of a workgroup.  Workgroups go to the 8 dies in turn, each with a cache of its
+// own: a die takes a range of tiles, 8 tiles of rows by all outputs, then the next 8, so
+// that it reads its rows once and the weights an eighth as often as it has tiles of rows.
+struct Tiles {
+    uint32_t first, count, step, at;  // of the die; step: its workgroups
+
+    __device__ explicit Tiles(const W4Product &p) {
+        const uint32_t die = blockIdx.x % 8, all = p.tiles;
+        first = die * (all / 8) + min(die, all % 8);
+        count = all / 8 + (die < all % 8);
+        step = gridDim.x / 8 + (die < gridDim.x % 8);
+        at = blockIdx.x / 8;  // below count, as the launch has at most a workgroup per tile
+    }
+    __device__ void place(const W4Product &p, uint32_t i, int &n, int &m) const {
+        const uint32_t strip = fastdiv(first + i, p.strip), in = first + i - strip * p.strip.d;
+        const uint32_t tall = min(8u, (uint32_t)p.tiles_m - 8 * strip);
+        n = (int)(in / tall);
+        m = (int)(8 * strip + in % tall);
+    }
+};
+
+template <int X, int G, int MT, bool GATED, bool OUT8>
+__global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype) {
+    typedef Staged<X, MT> S;
     constexpr int NG = 128 / G;  // groups of a step
     __shared__ __align__(16) char tile[2][S::kBytes];
-    const int tid = threadIdx.x, l = tid % kWave, wave = tid / kWave;
-    const int quarter = l / 16, wn = wave % 4, wm = wave / 4;
-    const int m0 = blockIdx.y * S::kRows, b0 = blockIdx.x * 16 + wn * 4;
+    const int tid = threadIdx.x, l = tid % kWave;
+    // known to be one of a wavefront, so that its addresses are scalar
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int quarter = l / 16;
 
-    // this thread's pieces of 8 values: the same columns of MT rows (behind the last row:
-    // the first one's, which is not stored)
+    // this thread's pieces of 8 values: the same columns of MT rows.  Offsets are 32 bits from
+    // the tile's first row; rows behind the last one are the last one, and not stored.
     const int k8 = tid % 16;
-    const char *src[MT];
+    const uint32_t row_bytes = (uint32_t)p.ld_x * kXBytes<X>, q8_bytes = 4 * (uint32_t)p.q8_groups;
+    uint32_t x_at[MT], xs_at[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int row = m0 + tid / 16 + i * (S::kThreads / 16);
-        src[i] = reinterpret_cast<const char *>(p.x) +
-                 (int64_t)(row < p.rows ? row : 0) * p.ld_x * kXBytes<X>;
+        x_at[i] = (uint32_t)(tid / 16 + 16 * i) * row_bytes;
+        xs_at[i] = (uint32_t)(16 * i + l % 16) * q8_bytes;
     }
     // a step's raw values on their way
     constexpr int RAW = X == kF32 ? 2 : 1;
     typedef typename std::conditional<X == kQ8, u32x2, u32x4>::type Raw;
     Raw raw[MT][RAW];
-    auto load_x = [&](int c) {
-        const int k = c * kW4Inputs + 8 * k8;
-        const int64_t at = k < p.inner ? (int64_t)k * kXBytes<X> : 0;
+    auto load_x = [&](int m, int c) {
+        const int m0 = m * S::kRows, k = c * kW4Inputs + 8 * k8;
+        const char *base = reinterpret_cast<const char *>(p.x) + (int64_t)m0 * row_bytes;
+        const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows) * row_bytes;
+        const uint32_t col = k < p.inner ? (uint32_t)k * kXBytes<X> : 0u;
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
-                raw[i][h] = *reinterpret_cast<const Raw *>(src[i] + at + 16 * h);
+                raw[i][h] =
+                    *reinterpret_cast<const Raw *>(base + (min(x_at[i], most) + col + 16 * h));
     };
     auto stage = [&](int buf, int c) {
         // zeros behind the last input, where the weights are 0 but x might be infinite
         const bool ok = c * kW4Inputs + 8 * k8 < p.inner;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            char *dst = tile[buf] + (tid / 16 + i * (S::kThreads / 16)) * S::kLd;
+            char *dst = tile[buf] + (tid / 16 + 16 * i) * S::kLd;
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
 #pragma unroll
@@ -312,34 +350,35 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
     u32x4 words[4];
     u32x2 scales[4][NG];
     float xs[MT];
-    auto load_w = [&](int c) {
+    const uint32_t word_at = 16 * l, scale_at = 8 * quarter;  // from a scalar address
+    auto load_w = [&](int n, int m, int c) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             // behind the last block: loaded, not stored
-            const int64_t unit = (int64_t)min(b0 + j, p.nb - 1) * p.kb + c;
-            words[j] = load_raw(p.packed + unit * kWave + l);
+            const int64_t unit = (int64_t)min(16 * n + 4 * wave + j, p.nb - 1) * p.kb + c;
+            words[j] = load_raw(reinterpret_cast<const char *>(p.packed + unit * kWave) + word_at);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) scales[j][g] = p.scales[(unit * NG + g) * 4 + quarter];
+            for (int g = 0; g < NG; ++g)
+                scales[j][g] = *reinterpret_cast<const u32x2 *>(
+                    reinterpret_cast<const char *>(p.scales + (unit * NG + g) * 4) + scale_at);
         }
-        if constexpr (X == kQ8)
+        if constexpr (X == kQ8) {
+            const int m0 = m * S::kRows;
+            const char *base =
+                reinterpret_cast<const char *>(p.x_scales + (int64_t)m0 * p.q8_groups + c);
+            const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows) * q8_bytes;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int row = m0 + wm * 16 * MT + 16 * i + l % 16;
-                xs[i] = p.x_scales[(int64_t)min(row, p.rows - 1) * p.q8_groups + c];
-            }
+            for (int i = 0; i < MT; ++i)
+                xs[i] = *reinterpret_cast<const float *>(base + min(xs_at[i], most));
+        }
     };
 
     f32x4 total[4][MT];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) total[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    // A step's products, in units of four instructions or more whose sums are scaled and
-    // added while the next unit's are multiplied: the scheduler, left to itself, starts them
-    // all and runs out of registers.
+    // A step's products, in units of two blocks by 16 rows whose sums are scaled and added
+    // while the next unit's are multiplied: the scheduler, left to itself, starts them all
+    // and runs out of registers.
     auto multiply_whole = [&](int buf, auto &&next) {
-        const char *mine = tile[buf] + (wm * 16 * MT + l % 16) * S::kLd + 16 * quarter;
+        const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
         u32x4 a[4][2];
         f32x4 s[4][NG];
         float own[MT];
@@ -366,19 +405,19 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
                     *reinterpret_cast<const u32x4 *>(mine + 16 * i * S::kLd + 64 * u);
         };
         read(0);
-        i32x4 sum[2][4];
-        f32x4 block[4];
+        i32x4 sum[2][2];
+        f32x4 block[2];
 #pragma unroll
-        for (int n = 0; n <= MT * NG; ++n) {
-            if (n < MT * NG) {
-                const int i = n / NG, g = n % NG;
-                if (g == 0 && i + 1 < MT) read(i + 1);
+        for (int n = 0; n <= MT * 2 * NG; ++n) {
+            if (n < MT * 2 * NG) {
+                const int i = n / (2 * NG), j0 = n / NG % 2 * 2, g = n % NG;
+                if (n % (2 * NG) == 0 && i + 1 < MT) read(i + 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
                     i32x4 &to = sum[n % 2][j];
-                    to = i32x4{0, 0, 0, 0};
+                    to = i32x4{kWhole, kWhole, kWhole, kWhole};
                     if constexpr (G == 32) {
-                        const u32x4 w = a[j][g / 2], v = x[i % 2][g / 2];
+                        const u32x4 w = a[j0 + j][g / 2], v = x[i % 2][g / 2];
                         const int h = g % 2 * 2;
                         to = __builtin_amdgcn_mfma_i32_16x16x32_i8(
                             __builtin_bit_cast(long, u32x2{w[h], w[h + 1]}),
@@ -387,32 +426,33 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
 #pragma unroll
                         for (int u = g * (G / 64); u < (g + 1) * (G / 64); ++u)
                             to = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                                __builtin_bit_cast(i32x4, a[j][u]),
+                                __builtin_bit_cast(i32x4, a[j0 + j][u]),
                                 __builtin_bit_cast(i32x4, x[i % 2][u]), to, 0, 0, 0);
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);  // their results are a unit away
             if (n > 0) {
-                const int i = (n - 1) / NG, g = (n - 1) % NG;
+                const int m = n - 1, i = m / (2 * NG), j0 = m / NG % 2 * 2, g = m % NG;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float v = (float)sum[(n - 1) % 2][j][r];
-                        block[j][r] = g == 0 ? v * s[j][g][r]
-                                             : __builtin_fmaf(v, s[j][g][r], block[j][r]);
+                        const float v = whole(sum[m % 2][j][r]), w = s[j0 + j][g][r];
+                        block[j][r] = g == 0 ? v * w : __builtin_fmaf(v, w, block[j][r]);
                         if (g == NG - 1)
-                            total[j][i][r] = __builtin_fmaf(block[j][r], own[i], total[j][i][r]);
+                            total[j0 + j][i][r] =
+                                __builtin_fmaf(block[j][r], own[i], total[j0 + j][i][r]);
                     }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     auto multiply_float = [&](int buf, auto &&next) {
-        const char *mine = tile[buf] + (wm * 16 * MT + l % 16) * S::kLd + 16 * quarter;
-        constexpr int KEEP = G == 128 ? MT : 2;  // sums alive: all rows' over two halves
+        const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
+        constexpr int KEEP = G == 128 ? 2 * MT : 2;  // sums alive: all rows' over two halves
         constexpr int UG = G == 32 ? 2 : 1;      // groups in a half
-        f32x4 sum[KEEP][4];
+        f32x4 sum[KEEP][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             bf16x8 a[4][2];
@@ -437,12 +477,12 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
             };
             read(0);
 #pragma unroll
-            for (int n = 0; n <= MT * UG; ++n) {
-                if (n < MT * UG) {
-                    const int i = n / UG, g = n % UG;
-                    if (g == 0 && i + 1 < MT) read(i + 1);
+            for (int n = 0; n <= MT * 2 * UG; ++n) {
+                if (n < MT * 2 * UG) {
+                    const int i = n / (2 * UG), j0 = n / UG % 2 * 2, g = n % UG;
+                    if (n % (2 * UG) == 0 && i + 1 < MT) read(i + 1);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < 2; ++j) {
                         f32x4 &to = sum[n % KEEP][j];
                         if (G != 128 || half == 0) to = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -450,89 +490,116 @@ __global__ __launch_bounds__(256 * NWM) void w4_tiles(W4Product p, int32_t y_dty
 #pragma unroll
                             for (int k = S::kTerms - 1; k >= 0; --k)  // the smallest first
                                 to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                    a[j][t], __builtin_bit_cast(bf16x8, x[i % 2][t][k]), to, 0, 0,
-                                    0);
+                                    a[j0 + j][t], __builtin_bit_cast(bf16x8, x[i % 2][t][k]), to,
+                                    0, 0, 0);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);  // their results are a unit away
                 if (n > 0 && (G != 128 || half == 1)) {
-                    const int i = (n - 1) / UG, g = (n - 1) % UG;
+                    const int m = n - 1, i = m / (2 * UG), j0 = m / UG % 2 * 2, g = m % UG;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            total[j][i][r] = __builtin_fmaf(sum[(n - 1) % KEEP][j][r], s[j][g][r],
-                                                            total[j][i][r]);
+                            total[j0 + j][i][r] = __builtin_fmaf(
+                                sum[m % KEEP][j][r], s[j0 + j][g][r], total[j0 + j][i][r]);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
     };
-    load_x(0);
-    load_w(0);
-    stage(0, 0);
-    __syncthreads();
-    // One block of code: after a branch, the last step's sums would be scaled behind it, all
-    // of them held until then.  (So the last step loads and stages itself once more.)
-    for (int c = 0; c < p.kb; ++c) {
-        const int after = min(c + 1, p.kb - 1);
-        auto next = [&] {
-            load_w(after);
-            load_x(after);
-        };
-        if constexpr (X == kQ8) multiply_whole(c & 1, next);
-        else multiply_float(c & 1, next);
-        stage(~c & 1, after);  // read a step ago, a barrier back
-        __syncthreads();
-    }
-
     constexpr int NB = GATED ? 2 : 1;
-    uint32_t(*most)[S::kRows] = reinterpret_cast<uint32_t(*)[S::kRows]>(tile[0]);
-    float act[4 / NB][MT][4];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int at = wm * 16 * MT + 16 * i + l % 16, row = m0 + at;
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 4 / NB; ++j) {
-            const int n = (b0 / NB + j) * kW4Outputs + 4 * quarter;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float v = total[NB * j][i][r] * 0.0625f;
-                if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * 0.0625f);
-                act[j][i][r] = v;
-                if (OUT8 && n < p.cols) m = max(m, size_bits(v));
-            }
-            if constexpr (!OUT8)
-                if (row < p.rows) put4(p, y_dtype, row, n, act[j][i]);
-        }
-        if constexpr (OUT8) {  // over the quarters, then the wavefronts
-            const auto a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
-            m = max(a[0], a[1]);
-            const auto b = __builtin_amdgcn_permlane32_swap(m, m, false, false);
-            m = max(b[0], b[1]);
-            if (quarter == 0) most[wn][at] = m;
-        }
-    }
-    if constexpr (OUT8) {
-        __syncthreads();
-        const int groups = (p.cols + kQ8Group - 1) / kQ8Group;
+    __shared__ uint32_t sizes[OUT8 ? 4 : 1][OUT8 ? S::kRows : 1];
+    auto finish = [&](int n, int m) {
+        const int n0 = (16 * n + 4 * wave) / NB * kW4Outputs + 4 * quarter;
+        float act[MT][4 / NB][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const int at = wm * 16 * MT + 16 * i + l % 16, row = m0 + at;
-            if (row >= p.rows) continue;
-            const Q8Scale s(max(max(most[0][at], most[1][at]), max(most[2][at], most[3][at])));
+            const int at = 16 * i + l % 16, row = m * S::kRows + at;
+            uint32_t most = 0;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int n = (b0 / 2 + j) * kW4Outputs + 4 * quarter;
-                if (n >= p.cols) continue;
-                *reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.y) +
-                                              (int64_t)row * p.cols + n) =
-                    pack_bytes(s.value(act[j][i][0]), s.value(act[j][i][1]), s.value(act[j][i][2]),
-                               s.value(act[j][i][3]));
+            for (int j = 0; j < 4 / NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = total[NB * j][i][r] * 0.0625f;
+                    if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * 0.0625f);
+                    act[i][j][r] = v;
+                    if (OUT8 && n0 + 16 * j < p.cols) most = max(most, size_bits(v));
+                }
+            if constexpr (!OUT8)
+                if (row < p.rows) {
+                    if (y_dtype == QDC_F32) put<float>(p, row, n0, act[i]);
+                    else put<bf16_t>(p, row, n0, act[i]);
+                }
+            if constexpr (OUT8) {  // over the quarters, then the wavefronts
+                const auto a = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+                most = max(a[0], a[1]);
+                const auto b = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+                most = max(b[0], b[1]);
+                if (quarter == 0) sizes[wave][at] = most;
             }
-            if (wn == 0 && quarter == 0)
-                p.y_scales[(int64_t)row * groups + blockIdx.x] = s.scale;
         }
+        if constexpr (OUT8) {
+            __syncthreads();  // before the next tile's sizes there is another, if only a step's
+            const int groups = (p.cols + kQ8Group - 1) / kQ8Group;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int at = 16 * i + l % 16, row = m * S::kRows + at;
+                if (row >= p.rows) continue;
+                const Q8Scale s(
+                    max(max(sizes[0][at], sizes[1][at]), max(sizes[2][at], sizes[3][at])));
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (n0 + 16 * j >= p.cols) continue;
+                    *reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.y) +
+                                                  (int64_t)row * p.cols + n0 + 16 * j) =
+                        pack_bytes(s.value(act[i][j][0]), s.value(act[i][j][1]),
+                                   s.value(act[i][j][2]), s.value(act[i][j][3]));
+                }
+                if (wave == 0 && quarter == 0)
+                    p.y_scales[(int64_t)row * groups + n] = s.scale;
+            }
+        }
+    };
+
+    Tiles mine(p);
+    int n, m, buf = 0;
+    mine.place(p, mine.at, n, m);
+    load_x(m, 0);
+    load_w(n, m, 0);
+    stage(0, 0);
+    __syncthreads();
+    for (;;) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) total[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // The next tile's first step is loaded with this one's last, so that memory is not
+        // waited for between tiles.  (Behind the last tile: its own again.)
+        const uint32_t after = mine.at + mine.step;
+        const bool more = after < mine.count;
+        int n1, m1;
+        mine.place(p, more ? after : mine.at, n1, m1);
+        // One block of code: after a branch, the last step's sums would be scaled behind it,
+        // all of them held until then.
+        for (int c = 0; c < p.kb; ++c) {
+            const bool within = c + 1 < p.kb;
+            const int c1 = within ? c + 1 : 0;
+            auto next = [&] {
+                load_w(within ? n : n1, within ? m : m1, c1);
+                load_x(within ? m : m1, c1);
+            };
+            if constexpr (X == kQ8) multiply_whole(buf, next);
+            else multiply_float(buf, next);
+            stage(buf ^ 1, c1);  // read a step ago, a barrier back
+            buf ^= 1;
+            __syncthreads();
+        }
+        finish(n, m);
+        if (!more) return;
+        mine.at = after;
+        n = n1;
+        m = m1;
     }
 }
 
@@ -545,12 +612,17 @@ int32_t launch_rows(const W4Product &p, int32_t y_dtype, hipStream_t s) {
                        y_dtype);
     return launch_status();
 }
-template <int X, int G, int MT, int NWM, bool GATED, bool OUT8>
+template <int X, int G, int MT, bool GATED, bool OUT8>
 int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
-    const dim3 grid((uint32_t)ceil_div((int64_t)p.nb, (int64_t)16),
-                    (uint32_t)ceil_div((int64_t)p.rows, (int64_t)16 * MT * NWM));
-    hipLaunchKernelGGL((w4_tiles<X, G, MT, NWM, GATED, OUT8>), grid, dim3(256 * NWM), 0, s, p,
-                       y_dtype);
+    W4Product q = p;
+    const int64_t tiles_n = ceil_div((int64_t)p.nb, (int64_t)16);
+    q.tiles_m = (int)ceil_div((int64_t)p.rows, (int64_t)16 * MT);
+    q.strip = make_fastdiv((uint32_t)(8 * tiles_n));
+    const int64_t tiles = tiles_n * q.tiles_m;
+    if (tiles >= (int64_t)1 << 30) return QDC_ERR_SHAPE;
+    q.tiles = (uint32_t)tiles;
+    const uint32_t grid = tiles < 512 ? (uint32_t)tiles : 512;  // two a compute unit
+    hipLaunchKernelGGL((w4_tiles<X, G, MT, GATED, OUT8>), dim3(grid), dim3(256), 0, s, q, y_dtype);
     return launch_status();
 }
 
@@ -559,14 +631,14 @@ int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     constexpr int BIG = X == kF32 ? 2 : 4;  // fp32: three terms a row in LDS
     if constexpr (GATED)
         if (y_dtype == QDC_Q8) {
-            if (p.rows <= 16) return launch_tiles<X, G, 1, 1, true, true>(p, y_dtype, s);
-            if (p.rows <= 512) return launch_tiles<X, G, 2, 1, true, true>(p, y_dtype, s);
-            return launch_tiles<X, G, BIG, 2, true, true>(p, y_dtype, s);
+            if (p.rows <= 16) return launch_tiles<X, G, 1, true, true>(p, y_dtype, s);
+            if (p.rows <= 512) return launch_tiles<X, G, 2, true, true>(p, y_dtype, s);
+            return launch_tiles<X, G, BIG, true, true>(p, y_dtype, s);
         }
     if (p.rows <= 16) return launch_rows<X, G, 1, GATED, 8>(p, y_dtype, s);
     if (p.rows <= 64) return launch_rows<X, G, 2, GATED, 8>(p, y_dtype, s);
-    if (p.rows <= 512) return launch_tiles<X, G, 2, 1, GATED, false>(p, y_dtype, s);
-    return launch_tiles<X, G, BIG, 2, GATED, false>(p, y_dtype, s);
+    if (p.rows <= 512) return launch_tiles<X, G, 2, GATED, false>(p, y_dtype, s);
+    return launch_tiles<X, G, BIG, GATED, false>(p, y_dtype, s);
 }
 
 template <int X>

@@ -112,6 +112,10 @@ struct W4Product {
     int inner, kb;   // inputs, blocks of inputs
     int nb;          // blocks of outputs
     int q8_groups;   // of a row of x
+    // of a launch by tiles: how many, how many of rows, and tiles in 8 of those
+    uint32_t tiles;
+    int tiles_m;
+    FastDiv strip;
 };
 
 // The products of x in one type; y_dtype QDC_F32, QDC_BF16 or, gated, QDC_Q8.
