@@ -249,15 +249,17 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_d
 
 // --------------------------------------------------------------- many rows ---
 // A workgroup of 4 wavefronts takes tiles of 256 outputs (16 blocks) by 16 * MT rows, a
-// wavefront 64 outputs of them.  x goes through LDS, a step of 128 inputs while the step
-// before is multiplied; the weights, each for one wavefront and in operand order already,
-// go to registers.  OUT8: the 256 outputs are gate and up of the 128 columns that
+// wavefront 64 outputs of them.  x and the scales go through LDS, a step of 128 inputs while
+// the step before is multiplied; the weights, each for one wavefront and in operand order
+// already, go to registers.  OUT8: the 256 outputs are gate and up of the 128 columns that
 // share a scale of an 8-bit row, whose maximum four wavefronts find together.
-template <int X, int MT> struct Staged {
+template <int X, int G, int MT> struct Staged {
     static constexpr int kRows = 16 * MT;
     static constexpr int kTerms = Piece<X>::kTerms;
     static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
-    static constexpr int kBytes = kRows * kLd * kTerms;
+    static constexpr int kX = kRows * kLd * kTerms;         // x, then the weights' scales
+    static constexpr int kScales = 16 * (128 / G) * 32;     // (a block's groups, 16 bf16 each),
+    static constexpr int kBytes = kX + kScales + 4 * kRows;  // then those of 8-bit rows
 };
 
 // The tiles of a workgroup.  Workgroups go to the 8 dies in turn, each with a cache of its
@@ -283,7 +285,7 @@ struct Tiles {
 
 template <int X, int G, int MT, bool GATED, bool OUT8>
 __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype) {
-    typedef Staged<X, MT> S;
+    typedef Staged<X, G, MT> S;
     constexpr int NG = 128 / G;  // groups of a step
     __shared__ __align__(16) char tile[2][S::kBytes];
     const int tid = threadIdx.x, l = tid % kWave;
@@ -294,17 +296,44 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     // this thread's pieces of 8 values: the same columns of MT rows.  Offsets are 32 bits from
     // the tile's first row; rows behind the last one are the last one, and not stored.
     const int k8 = tid % 16;
-    const uint32_t row_bytes = (uint32_t)p.ld_x * kXBytes<X>, q8_bytes = 4 * (uint32_t)p.q8_groups;
-    uint32_t x_at[MT], xs_at[MT];
+    const uint32_t row_bytes = (uint32_t)p.ld_x * kXBytes<X>;
+    uint32_t x_at[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        x_at[i] = (uint32_t)(tid / 16 + 16 * i) * row_bytes;
-        xs_at[i] = (uint32_t)(16 * i + l % 16) * q8_bytes;
-    }
+    for (int i = 0; i < MT; ++i) x_at[i] = (uint32_t)(tid / 16 + 16 * i) * row_bytes;
+    // and 1/16 of a block's scales (2, 4 or 8 bytes), and a row's
+    const uint32_t block_bytes = (uint32_t)p.kb * (32 * NG), q8_bytes = 4 * (uint32_t)p.q8_groups;
+    const uint32_t scale_at = (uint32_t)(tid / 16) * block_bytes;
+    const uint32_t xs_at = (uint32_t)(tid % S::kRows) * q8_bytes;
+    typedef typename std::conditional<
+        NG == 1, uint16_t, typename std::conditional<NG == 2, uint32_t, u32x2>::type>::type Scales;
     // a step's raw values on their way
     constexpr int RAW = X == kF32 ? 2 : 1;
     typedef typename std::conditional<X == kQ8, u32x2, u32x4>::type Raw;
     Raw raw[MT][RAW];
+    Scales raw_scales;
+    float raw_xs = 0.0f;
+    u32x4 words[4];
+    const uint32_t word_at = 16 * l;
+    auto load_w = [&](int n, int m, int c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // behind the last block: loaded, not stored
+            const int64_t unit = (int64_t)min(16 * n + 4 * wave + j, p.nb - 1) * p.kb + c;
+            words[j] = load_raw(reinterpret_cast<const char *>(p.packed + unit * kWave) + word_at);
+        }
+        const char *base = reinterpret_cast<const char *>(p.scales) +
+                           ((int64_t)16 * n * p.kb + c) * (32 * NG);
+        const uint32_t most = (uint32_t)min(p.nb - 1 - 16 * n, 16) * block_bytes;
+        raw_scales = *reinterpret_cast<const Scales *>(
+            base + (min(scale_at, most) + (uint32_t)(tid % 16 * sizeof(Scales))));
+        if constexpr (X == kQ8) {
+            const int m0 = m * S::kRows;
+            const char *from =
+                reinterpret_cast<const char *>(p.x_scales + (int64_t)m0 * p.q8_groups + c);
+            raw_xs = *reinterpret_cast<const float *>(
+                from + min(xs_at, (uint32_t)min(p.rows - 1 - m0, S::kRows) * q8_bytes));
+        }
+    };
     auto load_x = [&](int m, int c) {
         const int m0 = m * S::kRows, k = c * kW4Inputs + 8 * k8;
         const char *base = reinterpret_cast<const char *>(p.x) + (int64_t)m0 * row_bytes;
@@ -320,6 +349,10 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     auto stage = [&](int buf, int c) {
         // zeros behind the last input, where the weights are 0 but x might be infinite
         const bool ok = c * kW4Inputs + 8 * k8 < p.inner;
+        *reinterpret_cast<Scales *>(tile[buf] + S::kX + tid * sizeof(Scales)) = raw_scales;
+        if constexpr (X == kQ8)
+            *reinterpret_cast<float *>(tile[buf] + S::kX + S::kScales + 4 * (tid % S::kRows)) =
+                raw_xs;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             char *dst = tile[buf] + (tid / 16 + 16 * i) * S::kLd;
@@ -346,31 +379,10 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             }
         }
     };
-    // a step's weights on their way, then as they are multiplied
-    u32x4 words[4];
-    u32x2 scales[4][NG];
-    float xs[MT];
-    const uint32_t word_at = 16 * l, scale_at = 8 * quarter;  // from a scalar address
-    auto load_w = [&](int n, int m, int c) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // behind the last block: loaded, not stored
-            const int64_t unit = (int64_t)min(16 * n + 4 * wave + j, p.nb - 1) * p.kb + c;
-            words[j] = load_raw(reinterpret_cast<const char *>(p.packed + unit * kWave) + word_at);
-#pragma unroll
-            for (int g = 0; g < NG; ++g)
-                scales[j][g] = *reinterpret_cast<const u32x2 *>(
-                    reinterpret_cast<const char *>(p.scales + (unit * NG + g) * 4) + scale_at);
-        }
-        if constexpr (X == kQ8) {
-            const int m0 = m * S::kRows;
-            const char *base =
-                reinterpret_cast<const char *>(p.x_scales + (int64_t)m0 * p.q8_groups + c);
-            const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows) * q8_bytes;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-                xs[i] = *reinterpret_cast<const float *>(base + min(xs_at[i], most));
-        }
+    // the scales of 4 outputs of the wavefront's block j in group g of a step
+    auto scales = [&](int buf, int j, int g) {
+        return scales4(*reinterpret_cast<const u32x2 *>(
+            tile[buf] + S::kX + ((4 * wave + j) * NG + g) * 32 + 8 * quarter));
     };
 
     f32x4 total[4][MT];
@@ -379,8 +391,16 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     // and runs out of registers.
     auto multiply_whole = [&](int buf, auto &&next) {
         const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
+        u32x4 x[2][2];
+        auto read = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                x[i % 2][u] =
+                    *reinterpret_cast<const u32x4 *>(mine + 16 * i * S::kLd + 64 * u);
+        };
+        read(0);
         u32x4 a[4][2];
-        f32x4 s[4][NG];
+        f32x4 s[4][NG], bias[4];
         float own[MT];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -391,20 +411,18 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
                                 w1 & 0xf0f0f0f0u};
             }
 #pragma unroll
-            for (int g = 0; g < NG; ++g) s[j][g] = scales4(scales[j][g]);
+            for (int g = 0; g < NG; ++g) s[j][g] = scales(buf, j, g);
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) own[i] = xs[i];
+        for (int i = 0; i < MT; ++i)
+            own[i] = *reinterpret_cast<const float *>(tile[buf] + S::kX + S::kScales +
+                                                      4 * (16 * i + l % 16));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[j][r] = s[j][0][r] * -__int_as_float(kWhole);
         next();
         __builtin_amdgcn_sched_barrier(0);
-        u32x4 x[2][2];
-        auto read = [&](int i) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-                x[i % 2][u] =
-                    *reinterpret_cast<const u32x4 *>(mine + 16 * i * S::kLd + 64 * u);
-        };
-        read(0);
         i32x4 sum[2][2];
         f32x4 block[2];
 #pragma unroll
@@ -438,8 +456,13 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float v = whole(sum[m % 2][j][r]), w = s[j0 + j][g][r];
-                        block[j][r] = g == 0 ? v * w : __builtin_fmaf(v, w, block[j][r]);
+                        const float w = s[j0 + j][g][r];
+                        const int v = sum[m % 2][j][r];
+                        // the first group's subtraction is part of its product: 3 * 2^22 of a
+                        // scale's 8 bits is exact
+                        block[j][r] =
+                            g == 0 ? __builtin_fmaf(__int_as_float(v), w, bias[j0 + j][r])
+                                   : __builtin_fmaf(whole(v), w, block[j][r]);
                         if (g == NG - 1)
                             total[j0 + j][i][r] =
                                 __builtin_fmaf(block[j][r], own[i], total[j0 + j][i][r]);
@@ -462,7 +485,8 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) a[j][t] = widen(words[j][2 * half + t]);
 #pragma unroll
-                for (int g = 0; g < UG; ++g) s[j][g] = scales4(scales[j][G == 128 ? 0 : half * UG + g]);
+                for (int g = 0; g < UG; ++g)
+                    s[j][g] = scales(buf, j, G == 128 ? 0 : half * UG + g);
             }
             if (half == 1) next();
             __builtin_amdgcn_sched_barrier(0);
@@ -562,6 +586,9 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         }
     };
 
+    // Of the two workgroups of a compute unit one goes first, so that they do not come to
+    // their barriers and stores at the same time.
+    if (blockIdx.x / 256 % 2) __builtin_amdgcn_s_setprio(1);
     Tiles mine(p);
     int n, m, buf = 0;
     mine.place(p, mine.at, n, m);
