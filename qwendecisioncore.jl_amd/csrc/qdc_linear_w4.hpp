@@ -257,8 +257,8 @@ template <int X, int G, int MT> struct Staged {
     static constexpr int kRows = 16 * MT;
     static constexpr int kTerms = Piece<X>::kTerms;
     static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
-    static constexpr int kX = kRows * kLd * kTerms;         // x, then the weights' scales
-    static constexpr int kScales = 16 * (128 / G) * 32;     // (a block's groups, 16 bf16 each),
+    static constexpr int kX = kRows * kLd * kTerms;          // x, then the weights' scales
+    static constexpr int kScales = 16 * (128 / G) * 64;      // (a block's groups, 16 fp32 each),
     static constexpr int kBytes = kX + kScales + 4 * kRows;  // then those of 8-bit rows
 };
 
@@ -347,9 +347,14 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
                     *reinterpret_cast<const Raw *>(base + (min(x_at[i], most) + col + 16 * h));
     };
     auto stage = [&](int buf, int c) {
-        // zeros behind the last input, where the weights are 0 but x might be infinite
-        const bool ok = c * kW4Inputs + 8 * k8 < p.inner;
-        *reinterpret_cast<Scales *>(tile[buf] + S::kX + tid * sizeof(Scales)) = raw_scales;
+        // zeros behind the last input, where the weights are 0 but a float might be infinite
+        const bool ok = X == kQ8 || c * kW4Inputs + 8 * k8 < p.inner;
+        float *s = reinterpret_cast<float *>(tile[buf] + S::kX) + tid * NG;
+        if constexpr (NG == 1) *s = to_f32(raw_scales);
+        else if constexpr (NG == 2)
+            *reinterpret_cast<f32x2 *>(s) = f32x2{__uint_as_float(raw_scales << 16),
+                                                  __uint_as_float(raw_scales & 0xffff0000u)};
+        else *reinterpret_cast<f32x4 *>(s) = scales4(raw_scales);
         if constexpr (X == kQ8)
             *reinterpret_cast<float *>(tile[buf] + S::kX + S::kScales + 4 * (tid % S::kRows)) =
                 raw_xs;
@@ -381,8 +386,8 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     };
     // the scales of 4 outputs of the wavefront's block j in group g of a step
     auto scales = [&](int buf, int j, int g) {
-        return scales4(*reinterpret_cast<const u32x2 *>(
-            tile[buf] + S::kX + ((4 * wave + j) * NG + g) * 32 + 8 * quarter));
+        return *reinterpret_cast<const f32x4 *>(tile[buf] + S::kX +
+                                                ((4 * wave + j) * NG + g) * 64 + 16 * quarter);
     };
 
     f32x4 total[4][MT];
@@ -586,9 +591,6 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         }
     };
 
-    // Of the two workgroups of a compute unit one goes first, so that they do not come to
-    // their barriers and stores at the same time.
-    if (blockIdx.x / 256 % 2) __builtin_amdgcn_s_setprio(1);
     Tiles mine(p);
     int n, m, buf = 0;
     mine.place(p, mine.at, n, m);
@@ -655,7 +657,8 @@ int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
 
 template <int X, int G, bool GATED>
 int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
-    constexpr int BIG = X == kF32 ? 2 : 4;  // fp32: three terms a row in LDS
+    // fp32: three terms a row in LDS; groups of 32: the scales fill the registers
+    constexpr int BIG = X == kF32 || (X == kQ8 && G == 32) ? 2 : 4;
     if constexpr (GATED)
         if (y_dtype == QDC_Q8) {
             if (p.rows <= 16) return launch_tiles<X, G, 1, true, true>(p, y_dtype, s);
