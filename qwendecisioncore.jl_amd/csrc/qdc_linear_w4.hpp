@@ -174,13 +174,12 @@ __device__ __forceinline__ void put(const W4Product &p, int row, int n, const fl
 }
 
 // ---------------------------------------------------------------- few rows ---
-// A workgroup per block of outputs (two, gate and up, where gated) and 16 * MT rows, whose
-// wavefronts take the blocks of inputs in turn and add up at the end: bound by the weights'
-// way from memory and, for a row or two, by one trip there, so every load of a wavefront's
-// block leaves at once and x comes straight from the caches.
-template <int X, int G, int MT, bool GATED, int WAVES>
+// A workgroup per NB blocks of outputs (pairs of gate and up where gated) and 16 * MT rows,
+// whose wavefronts take the blocks of inputs in turn and add up at the end: bound by the
+// weights' way from memory and, for a row or two, by one trip there, so every load of a
+// wavefront's block leaves at once and x comes straight from the caches.
+template <int X, int G, int MT, int NB, bool GATED, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_dtype) {
-    constexpr int NB = GATED ? 2 : 1;
     __shared__ f32x4 parts[WAVES][NB][MT][kWave];
     const int l = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int quarter = l / 16, b0 = blockIdx.x * NB, m0 = blockIdx.y * 16 * MT;
@@ -194,7 +193,7 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_d
         u32x2 s[NB][128 / G];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int64_t unit = (int64_t)(b0 + b) * p.kb + c;
+            const int64_t unit = (int64_t)min(b0 + b, p.nb - 1) * p.kb + c;
             words[b] = load_stream(p.packed + unit * kWave + l);
 #pragma unroll
             for (int g = 0; g < 128 / G; ++g)
@@ -236,13 +235,16 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_d
 #pragma unroll
         for (int w = 1; w < WAVES; ++w) sum[b] += parts[w][b][wave][l];
     }
-    float v[1][4];
+    constexpr int PER = GATED ? 2 : 1;
+    float v[NB / PER][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        v[0][r] = sum[0][r] * 0.0625f;
-        if constexpr (GATED) v[0][r] = silu(v[0][r]) * (sum[1][r] * 0.0625f);
-    }
-    const int n = 16 * (int)blockIdx.x + 4 * quarter;
+    for (int b = 0; b < NB / PER; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v[b][r] = sum[PER * b][r] * 0.0625f;
+            if constexpr (GATED) v[b][r] = silu(v[b][r]) * (sum[2 * b + 1][r] * 0.0625f);
+        }
+    const int n = b0 / PER * kW4Outputs + 4 * quarter;
     if (y_dtype == QDC_F32) put<float>(p, row, n, v);
     else put<bf16_t>(p, row, n, v);
 }
@@ -633,11 +635,11 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
 }
 
 // ---------------------------------------------------------------- dispatch ---
-template <int X, int G, int MT, bool GATED, int WAVES>
+template <int X, int G, int MT, int NB, bool GATED, int WAVES>
 int32_t launch_rows(const W4Product &p, int32_t y_dtype, hipStream_t s) {
-    const dim3 grid((uint32_t)(p.nb / (GATED ? 2 : 1)),
+    const dim3 grid((uint32_t)ceil_div((int64_t)p.nb, (int64_t)NB),
                     (uint32_t)ceil_div((int64_t)p.rows, (int64_t)16 * MT));
-    hipLaunchKernelGGL((w4_rows<X, G, MT, GATED, WAVES>), grid, dim3(WAVES * kWave), 0, s, p,
+    hipLaunchKernelGGL((w4_rows<X, G, MT, NB, GATED, WAVES>), grid, dim3(WAVES * kWave), 0, s, p,
                        y_dtype);
     return launch_status();
 }
@@ -655,19 +657,40 @@ int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     return launch_status();
 }
 
+// The kernel with the smallest tile of which the chip's 256 units take one each, the largest
+// where none is large enough.  us for 1024 -> 5120 of bf16 rows, groups of 64, tiles of 16 x
+// 16 / 16 x 32 / 32 x 32 / 32 x 64 / by tiles of 16, 32, 64 rows x 256 (workgroups in
+// brackets): 16 rows 4.7 (320) / 4.4 (160) / 4.5 / - / -, 32 rows 6.0 / 5.5 (320) / 5.2
+// (160) / 6.4 / -, 96 rows - / 8.1 / 7.4 (480) / 6.6 (240) / 10.6, 256 rows - / - / 14.7 /
+// 16.1 / 16.1 (320), 13.9 (160), 18, 512 rows: - / - / 26.5 / 27.1 / 23.3, 19.1 (320),
+// 18.8 (160).
 template <int X, int G, bool GATED>
 int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    auto fits = [&](int rows, int blocks) {
+        return ceil_div((int64_t)p.rows, (int64_t)rows) * ceil_div((int64_t)p.nb, (int64_t)blocks) <=
+               256;
+    };
     // fp32: three terms a row in LDS; groups of 32: the scales fill the registers
     constexpr int BIG = X == kF32 || (X == kQ8 && G == 32) ? 2 : 4;
     if constexpr (GATED)
-        if (y_dtype == QDC_Q8) {
-            if (p.rows <= 16) return launch_tiles<X, G, 1, true, true>(p, y_dtype, s);
-            if (p.rows <= 512) return launch_tiles<X, G, 2, true, true>(p, y_dtype, s);
+        if (y_dtype == QDC_Q8) {  // 128 columns are a tile's
+            if (fits(16, 16)) return launch_tiles<X, G, 1, true, true>(p, y_dtype, s);
+            if (BIG == 2 || fits(32, 16)) return launch_tiles<X, G, 2, true, true>(p, y_dtype, s);
             return launch_tiles<X, G, BIG, true, true>(p, y_dtype, s);
         }
-    if (p.rows <= 16) return launch_rows<X, G, 1, GATED, 8>(p, y_dtype, s);
-    if (p.rows <= 64) return launch_rows<X, G, 2, GATED, 8>(p, y_dtype, s);
-    if (p.rows <= 512) return launch_tiles<X, G, 2, GATED, false>(p, y_dtype, s);
+    if constexpr (!GATED)
+        if (fits(16, 1)) {
+            // a wavefront for each 128 inputs, up to 16: 3584 -> 1024, one row of bf16, 4.1
+            // us, of fp32 8.7, with 8 wavefronts 4.3 and 10.4; 256 -> 768 with 4 2.3, 8 2.4
+            if (p.kb <= 4) return launch_rows<X, G, 1, 1, false, 4>(p, y_dtype, s);
+            if (p.kb < 16) return launch_rows<X, G, 1, 1, false, 8>(p, y_dtype, s);
+            return launch_rows<X, G, 1, 1, false, 16>(p, y_dtype, s);
+        }
+    if (fits(16, 2)) return launch_rows<X, G, 1, 2, GATED, 8>(p, y_dtype, s);
+    if (fits(32, 2)) return launch_rows<X, G, 2, 2, GATED, 8>(p, y_dtype, s);
+    if (fits(32, 4)) return launch_rows<X, G, 2, 4, GATED, 8>(p, y_dtype, s);
+    if (fits(16, 16)) return launch_tiles<X, G, 1, GATED, false>(p, y_dtype, s);
+    if (BIG == 2 || fits(32, 16)) return launch_tiles<X, G, 2, GATED, false>(p, y_dtype, s);
     return launch_tiles<X, G, BIG, GATED, false>(p, y_dtype, s);
 }
 
