@@ -68,8 +68,9 @@ int32_t qdc_residual_rmsnorm_q8(float *residual, void *q, float *scales, const f
 
 /* y = x w^T, or with gated != 0 y = silu(x gate^T) * (x up^T): y [rows, out] ([rows, out / 2])
  * contiguous, fp32 or bf16, and of a gated product also QDC_Q8 (y_scales; out / 2 a multiple
- * of 16).  x [rows, inner] is fp32, bf16 (rows ld_x elements apart, a multiple of 8) or
- * QDC_Q8 (x_scales; inner a multiple of 16, ld_x = inner).  Sums are fp32 (whole numbers
+ * of 16).  x [rows, inner], at most 2^20 - 16 rows, is fp32, bf16 (rows ld_x elements apart, a
+ * multiple of 8, at most 2^26 bytes) or QDC_Q8 (x_scales; inner a multiple of 16, ld_x =
+ * inner).  Sums are fp32 (whole numbers
  * within a group of 8-bit rows), the scale applied to each group's sum: q * x is summed
  * before it, so an fp32 or bf16 x beyond 2^116 may overflow where q * s * x would not.
  * x_scales and y_scales are ignored where they are not used. */

@@ -325,7 +325,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         }
         const char *base = reinterpret_cast<const char *>(p.scales) +
                            ((int64_t)16 * n * p.kb + c) * (32 * NG);
-        const uint32_t most = (uint32_t)min(p.nb - 1 - 16 * n, 16) * block_bytes;
+        const uint32_t most = (uint32_t)min(p.nb - 1 - 16 * n, 15) * block_bytes;
         raw_scales = *reinterpret_cast<const Scales *>(
             base + (min(scale_at, most) + (uint32_t)(tid % 16 * sizeof(Scales))));
         if constexpr (X == kQ8) {
@@ -333,13 +333,13 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             const char *from =
                 reinterpret_cast<const char *>(p.x_scales + (int64_t)m0 * p.q8_groups + c);
             raw_xs = *reinterpret_cast<const float *>(
-                from + min(xs_at, (uint32_t)min(p.rows - 1 - m0, S::kRows) * q8_bytes));
+                from + min(xs_at, (uint32_t)min(p.rows - 1 - m0, S::kRows - 1) * q8_bytes));
         }
     };
     auto load_x = [&](int m, int c) {
         const int m0 = m * S::kRows, k = c * kW4Inputs + 8 * k8;
         const char *base = reinterpret_cast<const char *>(p.x) + (int64_t)m0 * row_bytes;
-        const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows) * row_bytes;
+        const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows - 1) * row_bytes;
         const uint32_t col = k < p.inner ? (uint32_t)k * kXBytes<X> : 0u;
 #pragma unroll
         for (int i = 0; i < MT; ++i)

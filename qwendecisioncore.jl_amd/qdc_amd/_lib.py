@@ -158,8 +158,9 @@ def calls():
         module = importlib.util.module_from_spec(
             importlib.util.spec_from_file_location("qdc_calls", CALLS_PATH, loader=loader))
         loader.exec_module(module)
-        for built, version in ((module.version, lib().qdc_cache_version().decode()),
-                               (module.quant_version, lib().qdc_quant_version().decode())):
+        for built, name in ((module.version, "qdc_cache_version"),
+                            (module.quant_version, "qdc_quant_version")):
+            version = getattr(lib(), name)().decode()
             if built != version:   # the arguments may be others
                 raise RuntimeError(f"{CALLS_PATH} was built for {built!r}, the library is "
                                    f"{version!r}; run `make -C qwendecisioncore.jl_amd/csrc python`")

@@ -40,6 +40,11 @@ for SwiGLU; the attention and DeltaNet projections, q/k, the probabilities and
 the recurrence output stay bf16.  ``split_gemm_inputs="mlp"`` splits only the
 two MLP inputs (the post-attention norm and the SwiGLU output), where bf16
 rounding is amplified most, and leaves the other GEMMs at their bf16 size.
+
+``weight_format="w4"`` holds every projection in 4 bits (``quant_ops.pack_w4``) and
+multiplies with the framework's own kernels, SwiGLU within the gate/up product;
+``"w4a8"`` also holds the rows that the norms and SwiGLU write in 8 bits.  Norms,
+convolution, recurrence, attention and the embedding are as without it.
 """
 from __future__ import annotations
 
@@ -48,10 +53,10 @@ import os
 import numpy as np
 import torch
 
-from . import ops
+from . import ops, quant_ops
 from .config import BackboneConfig, load_config
+from .quant_ops import Q8, W4
 from .weights import read_checkpoint_tensors
-
 
 
 class QwenBackbone:
@@ -60,14 +65,20 @@ class QwenBackbone:
     model, and a tensor in ``layers`` is not to be changed by itself."""
 
     def __init__(self, cfg: BackboneConfig, weights: dict, device="cuda:0",
-                 dtype: torch.dtype = torch.float32, split_gemm_inputs: bool | str = False):
+                 dtype: torch.dtype = torch.float32, split_gemm_inputs: bool | str = False,
+                 weight_format: str | None = None, weight_group: int = 64):
         """``dtype`` is the storage type of weights and GEMM activations; the
         residual stream and the returned hidden states are fp32 either way.
         ``split_gemm_inputs`` (bfloat16 only: False, True / ``"all"``, or
         ``"mlp"``) selects the split GEMM inputs described in the module
         docstring.  A bfloat16 model holds a projection into the residual stream
         twice, transposed and as the checkpoint has it, where some number of rows
-        takes the product cut into parts (``ops.linear_parts_fits``)."""
+        takes the product cut into parts (``ops.linear_parts_fits``).
+        ``weight_format`` (None, ``"w4"`` or ``"w4a8"``, without split inputs): the
+        projections in 4 bits with a scale for each ``weight_group`` inputs (32, 64 or
+        128), as the module docstring says; inner widths are multiples of 8, and with
+        ``"w4a8"`` hidden and intermediate of 16.  ``dtype`` is then that of the
+        activations, the embedding and the norms."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be float32 or bfloat16")
         modes = {False: None, None: None, "none": None, True: "all", "all": "all", "mlp": "mlp"}
@@ -76,6 +87,20 @@ class QwenBackbone:
         self.split = modes[split_gemm_inputs]
         if self.split and dtype != torch.bfloat16:
             raise ValueError("split GEMM inputs are a bfloat16 mode")
+        if weight_format not in (None, "w4", "w4a8"):
+            raise ValueError("weight_format must be None, 'w4' or 'w4a8'")
+        if weight_format:
+            inner = (cfg.hidden, cfg.intermediate, cfg.heads * cfg.head_dim,
+                     cfg.value_heads * cfg.value_dim)
+            if self.split:
+                raise ValueError("weights in 4 bits take no split GEMM inputs")
+            if weight_group not in quant_ops.GROUPS:
+                raise ValueError(f"weight_group must be one of {quant_ops.GROUPS}")
+            if any(w % 8 for w in inner) or (weight_format == "w4a8"
+                                             and any(w % 16 for w in inner[:2])):
+                raise ValueError("weights in 4 bits need inner widths of multiples of 8, 8-bit "
+                                 f"rows hidden and intermediate of 16; got {inner}")
+        self.weight_format, self.weight_group = weight_format, weight_group
         self.cfg, self.dtype = cfg, dtype
         # a split row holds whole groups of 4 elements
         widths = {"mlp": (cfg.hidden, cfg.intermediate),
@@ -87,6 +112,10 @@ class QwenBackbone:
         # and every other GEMM input
         self.mlp_in = ops.BF16X2 if self.split else None
         self.gemm_in = ops.BF16X2 if self.split == "all" else None
+        # of the norm before an attention or DeltaNet projection
+        self.norm_in = self.gemm_in
+        if weight_format == "w4a8":
+            self.mlp_in = self.norm_in = Q8
         self.device = torch.device(device)
         self._tables = {}
 
@@ -94,16 +123,19 @@ class QwenBackbone:
             t = x if isinstance(x, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(x))
             return t.to(self.device).to(dt or dtype).contiguous()
 
-        def gemm_weight(w, split):  # [out, in] -> [in, out] (input rows repeated when split)
+        def gemm_weight(w, split, gated=False):
+            # [out, in] -> [in, out] (input rows repeated when split), or in 4 bits
+            if weight_format:
+                return quant_ops.pack_w4(w, weight_group, gated)
             w = w.t().contiguous()
             return ops.split_weight(w) if split else w
 
-        def lin(*names, pad_to=1, mlp=False):  # packed, transposed [in, out] for y = x @ W
+        def lin(*names, pad_to=1, mlp=False):  # packed, for y = x @ W; mlp: gate and up
             w = torch.cat([dev(weights[n]) for n in names], 0)
             extra = -w.shape[0] % pad_to
             if extra:  # zero output columns: the GEMM runs a tile-aligned width
                 w = torch.cat([w, w.new_zeros((extra, w.shape[1]))], 0)
-            return gemm_weight(w, self.mlp_in if mlp else self.gemm_in)
+            return gemm_weight(w, self.mlp_in if mlp else self.gemm_in, gated=mlp)
 
         def residual_stream(key, name, split):
             """A projection into the residual stream: transposed for the library's
@@ -112,7 +144,7 @@ class QwenBackbone:
             src = weights[name]
             w = dev(src)
             layer[key] = gemm_weight(w, split)
-            if dtype == torch.bfloat16 and ops.linear_parts_fits(w.shape[1], w.shape[0],
+            if dtype == torch.bfloat16 and not weight_format and ops.linear_parts_fits(w.shape[1], w.shape[0],
                                                                  bool(split)):
                 shared = isinstance(src, torch.Tensor) and w.data_ptr() == src.data_ptr()
                 layer[key + "_rows"] = w.clone() if shared else w
@@ -173,13 +205,15 @@ class QwenBackbone:
     @classmethod
     def from_weights(cls, weights: dict, cfg: BackboneConfig, device="cuda:0",
                      dtype: torch.dtype = torch.float32,
-                     split_gemm_inputs: bool | str = False) -> "QwenBackbone":
-        return cls(cfg, weights, device, dtype, split_gemm_inputs)
+                     split_gemm_inputs: bool | str = False, weight_format: str | None = None,
+                     weight_group: int = 64) -> "QwenBackbone":
+        return cls(cfg, weights, device, dtype, split_gemm_inputs, weight_format, weight_group)
 
     @classmethod
     def from_directory(cls, directory: str, device="cuda:0",
                        dtype: torch.dtype = torch.float32,
-                       split_gemm_inputs: bool | str = False) -> "QwenBackbone":
+                       split_gemm_inputs: bool | str = False, weight_format: str | None = None,
+                       weight_group: int = 64) -> "QwenBackbone":
         """A local safetensors checkpoint directory (no network access).  Tensors
         load straight onto ``device`` in their stored dtype; with ``dtype=bfloat16``
         a BF16 checkpoint is never widened to fp32 (the packed projection weights
@@ -189,15 +223,19 @@ class QwenBackbone:
         cfg = BackboneConfig(**{**cfg.as_dict(), "vocab": weights["embed_tokens.weight"].shape[0],
                                 "intermediate": weights["layers.0.mlp.gate_proj.weight"].shape[0],
                                 "layer_types": cfg.layer_types})
-        return cls(cfg, weights, device, dtype, split_gemm_inputs)
+        return cls(cfg, weights, device, dtype, split_gemm_inputs, weight_format, weight_group)
 
     def _mm(self, a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
         """A projection whose result feeds a row kernel, in the model dtype."""
+        if isinstance(b, W4):
+            return quant_ops.linear_w4(a, b, out_dtype=self.dtype)
         return a @ b
 
     def _mm32(self, a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
         """A GEMM whose result feeds the fp32 residual stream: fp32 output even
         from bf16 operands (hipBLASLt accumulates in fp32 either way)."""
+        if isinstance(b, W4):
+            return quant_ops.linear_w4(a, b, out_dtype=torch.float32)
         if a.dtype == torch.float32:
             return a @ b
         return torch.mm(a, b, out_dtype=torch.float32)
@@ -240,13 +278,14 @@ class QwenBackbone:
                                           self.layers[0]["input_norm"], cfg.eps,
                                           token_mask=delta_keep(0), error_flag=error_flag,
                                           normed_dtype=self.gemm_in)
+        normed = self._first_rows(h, normed, delta_keep(0))
         if self.fused_f32 and ops.linear_f32_takes(B * S, self.cfg.hidden, self.cfg.intermediate):
             return self._forward_small(h, normed, mask32, delta_keep, B, S, last_only)
         for i, layer in enumerate(self.layers):
             last = i + 1 == len(self.layers)
             # the last-token forward's last attention layer attends from the
             # last query only (its attention output comes back as [B, hidden])
-            final_query = last and last_only and layer["kind"] == "full_attention"
+            final_query = last and last_only and self._takes_final_query(layer)
             if final_query:
                 mixed = self._final_query_attention(layer, normed, mask32, B, S)
             elif layer["kind"] == "full_attention":
@@ -258,30 +297,59 @@ class QwenBackbone:
                 if not final_query:
                     mixed = mixed.view(B, S, -1)[:, -1].contiguous()
             if final_query:
-                residual, normed = ops.native_residual_rms(h, mixed, layer["post_norm"], cfg.eps,
-                                                           out_dtype=self.mlp_in)
+                residual, normed = self._add_norm(h, mixed, layer["post_norm"],
+                                                  out_dtype=self.mlp_in)
             else:
                 residual, normed = self._project_add_norm(h, mixed, layer, "out",
                                                           layer["post_norm"],
                                                           out_dtype=self.mlp_in)
-            # split inputs: fp32 gate/up for SwiGLU (bf16 there costs ~6x the
-            # end-to-end error of the whole split pipeline)
-            gate_up = (self._mm32 if self.split else self._mm)(normed, layer["gate_up"])
-            inter = gate_up.shape[1] // 2
-            act = ops.native_mlp_gate(gate_up[:, :inter], gate_up[:, inter:],
-                                      out_dtype=self.mlp_in)
+            act = self._activate(normed, layer["gate_up"])
             nxt = self.final_norm if last else self.layers[i + 1]["input_norm"]
             # residual add of the MLP fused with the next RMSNorm
             h, normed = self._project_add_norm(residual, act, layer, "down", nxt,
                                                token_mask=None if last else delta_keep(i + 1),
-                                               out_dtype=None if last else self.gemm_in)
+                                               out_dtype=None if last else self.norm_in)
         return normed
+
+    def _first_rows(self, h, normed, token_mask):
+        """The first layer's normalised rows as its projection takes them, from what
+        ``ops.native_gather_rms`` gives."""
+        if self.norm_in is not Q8:
+            return normed
+        return quant_ops.residual_rms_q8(h, None, self.layers[0]["input_norm"], self.cfg.eps,
+                                         token_mask=token_mask)[1]
+
+    def _activate(self, normed, w):
+        """SwiGLU of the gate and up projections, what the down projection takes."""
+        if isinstance(w, W4):
+            return quant_ops.gated_w4(normed, w, out_dtype=self.mlp_in or self.dtype)
+        # split inputs: fp32 gate/up for SwiGLU (bf16 there costs ~6x the
+        # end-to-end error of the whole split pipeline)
+        gate_up = (self._mm32 if self.split else self._mm)(normed, w)
+        inter = gate_up.shape[1] // 2
+        return ops.native_mlp_gate(gate_up[:, :inter], gate_up[:, inter:], out_dtype=self.mlp_in)
+
+    def _add_norm(self, h, mixed, norm, token_mask=None, out_dtype=None):
+        """``(h + mixed, rms(h + mixed))``, the second as the next projection takes it."""
+        if out_dtype is Q8:
+            return quant_ops.residual_rms_q8(h, mixed, norm, self.cfg.eps, token_mask=token_mask)
+        return ops.native_residual_rms(h, mixed, norm, self.cfg.eps, token_mask=token_mask,
+                                       out_dtype=out_dtype)
+
+    def _takes_final_query(self, layer) -> bool:
+        """Whether a last layer attends from the last query alone: a full-attention one
+        whose key and value projections can be taken by themselves (4-bit weights go by
+        16 outputs)."""
+        cfg = self.cfg
+        return layer["kind"] == "full_attention" and (
+            not self.weight_format or (cfg.heads * cfg.head_dim % 16 == 0
+                                       and 2 * cfg.kv_heads * cfg.head_dim % 16 == 0))
 
     def _fused_f32_fits(self) -> bool:
         """Whether every projection of this model has the widths, types and alignments
         of ``ops.linear_f32``."""
         cfg = self.cfg
-        if self.dtype != torch.float32 or not self.layers:
+        if self.dtype != torch.float32 or not self.layers or self.weight_format:
             return False
         # z is the column block of the packed projection after 2 keys and a value
         if any("proj" in layer for layer in self.layers) and (
@@ -348,8 +416,7 @@ class QwenBackbone:
             if parts:
                 return ops.linear_residual_rms(h, a, rows, norm, self.cfg.eps, parts,
                                                token_mask=token_mask, out_dtype=out_dtype)
-        return ops.native_residual_rms(h, self._mm32(a, layer[name]), norm, self.cfg.eps,
-                                       token_mask=token_mask, out_dtype=out_dtype)
+        return self._add_norm(h, self._mm32(a, layer[name]), norm, token_mask, out_dtype)
 
     def _attention_context(self, layer, x, mask32, B, S):
         """What the output projection of a full-attention layer multiplies:
@@ -406,8 +473,12 @@ class QwenBackbone:
         G = H // KV
         T = B * S
         w = layer["qkv"]                                     # [in, q | k | v | gate]
-        kv = self._mm(x, w[:, H * hd:(H + 2 * KV) * hd])    # [T, k | v] of every token
-        proj = self._mm(x.view(B, S, -1)[:, -1], w)          # [B, q | k | v | gate], last rows
+        w_kv = w.outputs(H * hd, (H + 2 * KV) * hd) if isinstance(w, W4) else \
+            w[:, H * hd:(H + 2 * KV) * hd]
+        kv = self._mm(x, w_kv)                               # [T, k | v] of every token
+        last = Q8(*(t.view(B, S, -1)[:, -1].contiguous() for t in x)) if isinstance(x, Q8) else \
+            x.view(B, S, -1)[:, -1].contiguous()
+        proj = self._mm(last, w)                             # [B, q | k | v | gate], last rows
         tables = self.rope_tables(S) if cfg.rotary_dim else None
         _, kt, v = ops.attention_prepare(None, kv[:, :KV * hd].view(T, KV, hd),
                                          kv[:, KV * hd:].view(T, KV, hd), None, layer["k_norm"],

@@ -387,6 +387,7 @@ class BackboneCache:
         h, normed = ops.native_gather_rms(model.embedding, ids, model.layers[0]["input_norm"],
                                           cfg.eps, token_mask=masked(0),
                                           normed_dtype=model.gemm_in)
+        normed = model._first_rows(h, normed, masked(0))
         if model.fused_f32 and ops.linear_f32_takes(ids.shape[0], cfg.hidden, cfg.intermediate):
             return self._through_small(h, normed, masked, mix, last_rows)
         for i, layer in enumerate(model.layers):
@@ -397,14 +398,11 @@ class BackboneCache:
                 h = last_rows(h)
             h, normed = self._project_add_norm(h, mixed, layer, "out", layer["post_norm"],
                                                out_dtype=model.mlp_in)
-            gate_up = (model._mm32 if model.split else model._mm)(normed, layer["gate_up"])
-            inter = gate_up.shape[1] // 2
-            act = ops.native_mlp_gate(gate_up[:, :inter], gate_up[:, inter:],
-                                      out_dtype=model.mlp_in)
+            act = model._activate(normed, layer["gate_up"])
             norm = model.final_norm if last else model.layers[i + 1]["input_norm"]
             h, normed = self._project_add_norm(h, act, layer, "down", norm,
                                                token_mask=None if last else masked(i + 1),
-                                               out_dtype=None if last else model.gemm_in)
+                                               out_dtype=None if last else model.norm_in)
         return normed
 
     def _project_add_norm(self, h, a, layer, name, norm, token_mask=None, out_dtype=None):

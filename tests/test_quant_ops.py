@@ -95,7 +95,7 @@ def test_linear_validation():
     for bad in (dict(rows=-1), dict(rows=(1 << 20) - 15), dict(out=0), dict(inner=252),
                 dict(group=48), dict(ld=248), dict(ld=260), dict(out=95, gated=1),
                 dict(out=2 * 40, gated=1, yt=Q8), dict(xt=Q8, inner=248, ld=248),
-                dict(xt=Q8, ld=272)):
+                dict(xt=Q8, ld=272), dict(ld=(1 << 25) + 8), dict(xt=F32, ld=(1 << 24) + 8)):
         assert f(**bad) == -2, bad
     for n in ("y", "x", "p", "s"):
         assert f(**{n: None}) == -1 and f(**{n: FAR + (9 << 40) + 8}) == -2, n
