@@ -285,6 +285,8 @@ struct Tiles {
     }
 };
 
+template <int N> __device__ __forceinline__ int round_up(int v) { return (v + N - 1) / N * N; }
+
 template <int X, int G, int MT, bool GATED, bool OUT8>
 __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype) {
     typedef Staged<X, G, MT> S;
@@ -308,35 +310,39 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     const uint32_t xs_at = (uint32_t)(tid % S::kRows) * q8_bytes;
     typedef typename std::conditional<
         NG == 1, uint16_t, typename std::conditional<NG == 2, uint32_t, u32x2>::type>::type Scales;
-    // a step's raw values on their way
+    // The raw values of a step on their way, or of two where the registers have room: alone
+    // on its unit a workgroup would wait for memory at every step.
     constexpr int RAW = X == kF32 ? 2 : 1;
+    constexpr int SETS = MT == 1 || (MT == 2 && !(X == kQ8 && G == 32)) ? 2 : 1;
     typedef typename std::conditional<X == kQ8, u32x2, u32x4>::type Raw;
-    Raw raw[MT][RAW];
-    Scales raw_scales;
-    float raw_xs = 0.0f;
-    u32x4 words[4];
+    Raw raw[SETS][MT][RAW];
+    Scales raw_scales[SETS];
+    float raw_xs[SETS];
+    u32x4 words[SETS][4];
     const uint32_t word_at = 16 * l;
-    auto load_w = [&](int n, int m, int c) {
+    auto load_w = [&](auto set, int n, int m, int c) {
+        c = min(c, p.kb - 1);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             // behind the last block: loaded, not stored
             const int64_t unit = (int64_t)min(16 * n + 4 * wave + j, p.nb - 1) * p.kb + c;
-            words[j] = load_raw(reinterpret_cast<const char *>(p.packed + unit * kWave) + word_at);
+            words[set][j] =
+                load_raw(reinterpret_cast<const char *>(p.packed + unit * kWave) + word_at);
         }
         const char *base = reinterpret_cast<const char *>(p.scales) +
                            ((int64_t)16 * n * p.kb + c) * (32 * NG);
         const uint32_t most = (uint32_t)min(p.nb - 1 - 16 * n, 15) * block_bytes;
-        raw_scales = *reinterpret_cast<const Scales *>(
+        raw_scales[set] = *reinterpret_cast<const Scales *>(
             base + (min(scale_at, most) + (uint32_t)(tid % 16 * sizeof(Scales))));
         if constexpr (X == kQ8) {
             const int m0 = m * S::kRows;
             const char *from =
                 reinterpret_cast<const char *>(p.x_scales + (int64_t)m0 * p.q8_groups + c);
-            raw_xs = *reinterpret_cast<const float *>(
+            raw_xs[set] = *reinterpret_cast<const float *>(
                 from + min(xs_at, (uint32_t)min(p.rows - 1 - m0, S::kRows - 1) * q8_bytes));
         }
     };
-    auto load_x = [&](int m, int c) {
+    auto load_x = [&](auto set, int m, int c) {
         const int m0 = m * S::kRows, k = c * kW4Inputs + 8 * k8;
         const char *base = reinterpret_cast<const char *>(p.x) + (int64_t)m0 * row_bytes;
         const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows - 1) * row_bytes;
@@ -345,21 +351,22 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
-                raw[i][h] =
+                raw[set][i][h] =
                     *reinterpret_cast<const Raw *>(base + (min(x_at[i], most) + col + 16 * h));
     };
-    auto stage = [&](int buf, int c) {
+    auto stage = [&](auto set, int buf, int c) {
+        Raw(&mine)[MT][RAW] = raw[set];
         // zeros behind the last input, where the weights are 0 but a float might be infinite
-        const bool ok = X == kQ8 || c * kW4Inputs + 8 * k8 < p.inner;
+        const bool ok = (X == kQ8 && SETS == 1) || c * kW4Inputs + 8 * k8 < p.inner;
         float *s = reinterpret_cast<float *>(tile[buf] + S::kX) + tid * NG;
-        if constexpr (NG == 1) *s = to_f32(raw_scales);
+        if constexpr (NG == 1) *s = to_f32(raw_scales[set]);
         else if constexpr (NG == 2)
-            *reinterpret_cast<f32x2 *>(s) = f32x2{__uint_as_float(raw_scales << 16),
-                                                  __uint_as_float(raw_scales & 0xffff0000u)};
-        else *reinterpret_cast<f32x4 *>(s) = scales4(raw_scales);
+            *reinterpret_cast<f32x2 *>(s) = f32x2{__uint_as_float(raw_scales[set] << 16),
+                                                  __uint_as_float(raw_scales[set] & 0xffff0000u)};
+        else *reinterpret_cast<f32x4 *>(s) = scales4(raw_scales[set]);
         if constexpr (X == kQ8)
             *reinterpret_cast<float *>(tile[buf] + S::kX + S::kScales + 4 * (tid % S::kRows)) =
-                raw_xs;
+                raw_xs[set];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             char *dst = tile[buf] + (tid / 16 + 16 * i) * S::kLd;
@@ -367,17 +374,17 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             for (int h = 0; h < RAW; ++h)
 #pragma unroll
                 for (int e = 0; e < (X == kQ8 ? 2 : 4); ++e)
-                    raw[i][h][e] = ok ? raw[i][h][e] : 0u;
+                    mine[i][h][e] = ok ? mine[i][h][e] : 0u;
             if constexpr (X == kQ8) {
                 // the two pieces that an instruction's lane takes lie side by side
                 *reinterpret_cast<u32x2 *>(dst + 64 * (k8 / 8) + 16 * (k8 % 4) +
-                                           8 * (k8 / 4 % 2)) = raw[i][0];
+                                           8 * (k8 / 4 % 2)) = mine[i][0];
             } else if constexpr (X == kBf16) {
-                *reinterpret_cast<u32x4 *>(dst + 16 * k8) = raw[i][0];
+                *reinterpret_cast<u32x4 *>(dst + 16 * k8) = mine[i][0];
             } else {
                 float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(raw[i][e / 4][e % 4]);
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(mine[i][e / 4][e % 4]);
                 u32x4 t[3];
                 terms(v, t);
 #pragma unroll
@@ -396,7 +403,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     // A step's products, in units of two blocks by 16 rows whose sums are scaled and added
     // while the next unit's are multiplied: the scheduler, left to itself, starts them all
     // and runs out of registers.
-    auto multiply_whole = [&](int buf, auto &&next) {
+    auto multiply_whole = [&](auto set, int buf, auto &&next) {
         const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
         u32x4 x[2][2];
         auto read = [&](int i) {
@@ -413,7 +420,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const uint32_t w0 = words[j][2 * u], w1 = words[j][2 * u + 1];
+                const uint32_t w0 = words[set][j][2 * u], w1 = words[set][j][2 * u + 1];
                 a[j][u] = u32x4{(w0 << 4) & 0xf0f0f0f0u, w0 & 0xf0f0f0f0u, (w1 << 4) & 0xf0f0f0f0u,
                                 w1 & 0xf0f0f0f0u};
             }
@@ -478,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto multiply_float = [&](int buf, auto &&next) {
+    auto multiply_float = [&](auto set, int buf, auto &&next) {
         const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
         constexpr int KEEP = G == 128 ? 2 * MT : 2;  // sums alive: all rows' over two halves
         constexpr int UG = G == 32 ? 2 : 1;      // groups in a half
@@ -490,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t) a[j][t] = widen(words[j][2 * half + t]);
+                for (int t = 0; t < 2; ++t) a[j][t] = widen(words[set][j][2 * half + t]);
 #pragma unroll
                 for (int g = 0; g < UG; ++g)
                     s[j][g] = scales(buf, j, G == 128 ? 0 : half * UG + g);
@@ -596,16 +603,23 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     Tiles mine(p);
     int n, m, buf = 0;
     mine.place(p, mine.at, n, m);
-    load_x(m, 0);
-    load_w(n, m, 0);
-    stage(0, 0);
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, SETS - 1> second;
+    load_x(first, m, 0);
+    load_w(first, n, m, 0);
+    if constexpr (SETS == 2) {
+        load_x(second, m, 1);
+        load_w(second, n, m, 1);
+    }
+    stage(first, 0, 0);
     __syncthreads();
+    const int steps = round_up<SETS>(p.kb);
     for (;;) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < MT; ++i) total[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        // The next tile's first step is loaded with this one's last, so that memory is not
+        // The next tile's first steps are loaded with this one's last, so that memory is not
         // waited for between tiles.  (Behind the last tile: its own again.)
         const uint32_t after = mine.at + mine.step;
         const bool more = after < mine.count;
@@ -613,18 +627,27 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         mine.place(p, more ? after : mine.at, n1, m1);
         // One block of code: after a branch, the last step's sums would be scaled behind it,
         // all of them held until then.
-        for (int c = 0; c < p.kb; ++c) {
-            const bool within = c + 1 < p.kb;
-            const int c1 = within ? c + 1 : 0;
-            auto next = [&] {
-                load_w(within ? n : n1, within ? m : m1, c1);
-                load_x(within ? m : m1, c1);
+        for (int c = 0; c < steps; c += SETS) {
+            const bool within = c + SETS < steps;
+            const int n2 = within ? n : n1, m2 = within ? m : m1, c2 = within ? c + SETS : 0;
+            auto step = [&](auto set, auto other, int at, int staged) {
+                auto next = [&] {
+                    load_w(set, n2, m2, c2 + set);
+                    load_x(set, m2, c2 + set);
+                };
+                if constexpr (X == kQ8) multiply_whole(set, at, next);
+                else multiply_float(set, at, next);
+                stage(other, at ^ 1, staged);  // read a step ago, a barrier back
+                __syncthreads();
             };
-            if constexpr (X == kQ8) multiply_whole(buf, next);
-            else multiply_float(buf, next);
-            stage(buf ^ 1, c1);  // read a step ago, a barrier back
-            buf ^= 1;
-            __syncthreads();
+            if constexpr (SETS == 2) {
+                // an odd number of steps has one more, of rows of zeros
+                step(first, second, 0, c + 1);
+                step(second, first, 1, c2);
+            } else {
+                step(first, first, buf, c2);
+                buf ^= 1;
+            }
         }
         finish(n, m);
         if (!more) return;
