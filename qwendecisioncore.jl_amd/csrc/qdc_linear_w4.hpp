@@ -250,17 +250,18 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Product p, int32_t y_d
 }
 
 // --------------------------------------------------------------- many rows ---
-// A workgroup of 4 wavefronts takes tiles of 256 outputs (16 blocks) by 16 * MT rows, a
-// wavefront 64 outputs of them.  x and the scales go through LDS, a step of 128 inputs while
+// A workgroup of NW wavefronts takes tiles of NW * NJ blocks of outputs by 16 * MT rows, a
+// wavefront NJ blocks of them.  x and the scales go through LDS, a step of 128 inputs while
 // the step before is multiplied; the weights, each for one wavefront and in operand order
-// already, go to registers.  OUT8: the 256 outputs are gate and up of the 128 columns that
-// share a scale of an 8-bit row, whose maximum four wavefronts find together.
-template <int X, int G, int MT> struct Staged {
-    static constexpr int kRows = 16 * MT;
+// already, go to registers.  OUT8: the tile's 16 blocks are gate and up of the 128 columns
+// that share a scale of an 8-bit row, whose maximum the wavefronts find together.
+template <int X, int G, int MT, int NJ, int NW> struct Staged {
+    static constexpr int kRows = 16 * MT, kBlocks = NJ * NW, kThreads = NW * kWave;
+    static constexpr int kPass = kRows * 16 / kThreads;      // pieces of x a thread
     static constexpr int kTerms = Piece<X>::kTerms;
     static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
     static constexpr int kX = kRows * kLd * kTerms;          // x, then the weights' scales
-    static constexpr int kScales = 16 * (128 / G) * 64;      // (a block's groups, 16 fp32 each),
+    static constexpr int kScales = kBlocks * (128 / G) * 64;     // (a block's groups, 16 fp32 each),
     static constexpr int kBytes = kX + kScales + 4 * kRows;  // then those of 8-bit rows
 };
 
@@ -287,53 +288,57 @@ struct Tiles {
 
 template <int N> __device__ __forceinline__ int round_up(int v) { return (v + N - 1) / N * N; }
 
-template <int X, int G, int MT, bool GATED, bool OUT8>
-__global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype) {
-    typedef Staged<X, G, MT> S;
-    constexpr int NG = 128 / G;  // groups of a step
+template <int X, int G, int MT, int NJ, int NW, bool GATED, bool OUT8>
+__global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_dtype) {
+    typedef Staged<X, G, MT, NJ, NW> S;
+    constexpr int NG = 128 / G, PJ = NJ / 2;  // groups of a step, pairs of blocks
+    static_assert(NJ % 2 == 0 && S::kPass >= 1 && (!OUT8 || S::kBlocks == 16), "");
     __shared__ __align__(16) char tile[2][S::kBytes];
     const int tid = threadIdx.x, l = tid % kWave;
     // known to be one of a wavefront, so that its addresses are scalar
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int quarter = l / 16;
 
-    // this thread's pieces of 8 values: the same columns of MT rows.  Offsets are 32 bits from
+    // this thread's pieces of 8 values: the same columns of kPass rows.  Offsets are 32 bits from
     // the tile's first row; rows behind the last one are the last one, and not stored.
     const int k8 = tid % 16;
     const uint32_t row_bytes = (uint32_t)p.ld_x * kXBytes<X>;
-    uint32_t x_at[MT];
+    uint32_t x_at[S::kPass];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) x_at[i] = (uint32_t)(tid / 16 + 16 * i) * row_bytes;
+    for (int i = 0; i < S::kPass; ++i)
+        x_at[i] = (uint32_t)(tid / 16 + S::kThreads / 16 * i) * row_bytes;
     // and 1/16 of a block's scales (2, 4 or 8 bytes), and a row's
     const uint32_t block_bytes = (uint32_t)p.kb * (32 * NG), q8_bytes = 4 * (uint32_t)p.q8_groups;
-    const uint32_t scale_at = (uint32_t)(tid / 16) * block_bytes;
+    const int st = tid % (16 * S::kBlocks);  // (where there are more threads, again)
+    const uint32_t scale_at = (uint32_t)(st / 16) * block_bytes;
     const uint32_t xs_at = (uint32_t)(tid % S::kRows) * q8_bytes;
     typedef typename std::conditional<
         NG == 1, uint16_t, typename std::conditional<NG == 2, uint32_t, u32x2>::type>::type Scales;
     // The raw values of a step on their way, or of two where the registers have room: alone
     // on its unit a workgroup would wait for memory at every step.
     constexpr int RAW = X == kF32 ? 2 : 1;
-    constexpr int SETS = MT == 1 || (MT == 2 && !(X == kQ8 && G == 32)) ? 2 : 1;
+    constexpr int SETS = NJ * MT <= 4 || (NJ * MT <= 8 && !(X == kQ8 && G == 32)) ? 2 : 1;
     typedef typename std::conditional<X == kQ8, u32x2, u32x4>::type Raw;
-    Raw raw[SETS][MT][RAW];
+    Raw raw[SETS][S::kPass][RAW];
     Scales raw_scales[SETS];
     float raw_xs[SETS];
-    u32x4 words[SETS][4];
+    u32x4 words[SETS][NJ];
     const uint32_t word_at = 16 * l;
     auto load_w = [&](auto set, int n, int m, int c) {
         c = min(c, p.kb - 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NJ; ++j) {
             // behind the last block: loaded, not stored
-            const int64_t unit = (int64_t)min(16 * n + 4 * wave + j, p.nb - 1) * p.kb + c;
+            const int64_t unit = (int64_t)min(S::kBlocks * n + NJ * wave + j, p.nb - 1) * p.kb + c;
             words[set][j] =
                 load_raw(reinterpret_cast<const char *>(p.packed + unit * kWave) + word_at);
         }
         const char *base = reinterpret_cast<const char *>(p.scales) +
-                           ((int64_t)16 * n * p.kb + c) * (32 * NG);
-        const uint32_t most = (uint32_t)min(p.nb - 1 - 16 * n, 15) * block_bytes;
+                           ((int64_t)S::kBlocks * n * p.kb + c) * (32 * NG);
+        const uint32_t most =
+            (uint32_t)min(p.nb - 1 - S::kBlocks * n, S::kBlocks - 1) * block_bytes;
         raw_scales[set] = *reinterpret_cast<const Scales *>(
-            base + (min(scale_at, most) + (uint32_t)(tid % 16 * sizeof(Scales))));
+            base + (min(scale_at, most) + (uint32_t)(st % 16 * sizeof(Scales))));
         if constexpr (X == kQ8) {
             const int m0 = m * S::kRows;
             const char *from =
@@ -348,17 +353,17 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         const uint32_t most = (uint32_t)min(p.rows - 1 - m0, S::kRows - 1) * row_bytes;
         const uint32_t col = k < p.inner ? (uint32_t)k * kXBytes<X> : 0u;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < S::kPass; ++i)
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
                 raw[set][i][h] =
                     *reinterpret_cast<const Raw *>(base + (min(x_at[i], most) + col + 16 * h));
     };
     auto stage = [&](auto set, int buf, int c) {
-        Raw(&mine)[MT][RAW] = raw[set];
+        Raw(&mine)[S::kPass][RAW] = raw[set];
         // zeros behind the last input, where the weights are 0 but a float might be infinite
         const bool ok = (X == kQ8 && SETS == 1) || c * kW4Inputs + 8 * k8 < p.inner;
-        float *s = reinterpret_cast<float *>(tile[buf] + S::kX) + tid * NG;
+        float *s = reinterpret_cast<float *>(tile[buf] + S::kX) + st * NG;
         if constexpr (NG == 1) *s = to_f32(raw_scales[set]);
         else if constexpr (NG == 2)
             *reinterpret_cast<f32x2 *>(s) = f32x2{__uint_as_float(raw_scales[set] << 16),
@@ -368,8 +373,8 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             *reinterpret_cast<float *>(tile[buf] + S::kX + S::kScales + 4 * (tid % S::kRows)) =
                 raw_xs[set];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            char *dst = tile[buf] + (tid / 16 + 16 * i) * S::kLd;
+        for (int i = 0; i < S::kPass; ++i) {
+            char *dst = tile[buf] + (tid / 16 + S::kThreads / 16 * i) * S::kLd;
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
 #pragma unroll
@@ -396,10 +401,10 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     // the scales of 4 outputs of the wavefront's block j in group g of a step
     auto scales = [&](int buf, int j, int g) {
         return *reinterpret_cast<const f32x4 *>(tile[buf] + S::kX +
-                                                ((4 * wave + j) * NG + g) * 64 + 16 * quarter);
+                                                ((NJ * wave + j) * NG + g) * 64 + 16 * quarter);
     };
 
-    f32x4 total[4][MT];
+    f32x4 total[NJ][MT];
     // A step's products, in units of two blocks by 16 rows whose sums are scaled and added
     // while the next unit's are multiplied: the scheduler, left to itself, starts them all
     // and runs out of registers.
@@ -413,11 +418,11 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
                     *reinterpret_cast<const u32x4 *>(mine + 16 * i * S::kLd + 64 * u);
         };
         read(0);
-        u32x4 a[4][2];
-        f32x4 s[4][NG], bias[4];
+        u32x4 a[NJ][2];
+        f32x4 s[NJ][NG], bias[NJ];
         float own[MT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NJ; ++j) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const uint32_t w0 = words[set][j][2 * u], w1 = words[set][j][2 * u + 1];
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             own[i] = *reinterpret_cast<const float *>(tile[buf] + S::kX + S::kScales +
                                                       4 * (16 * i + l % 16));
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) bias[j][r] = s[j][0][r] * -__int_as_float(kWhole);
         next();
@@ -440,10 +445,10 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         i32x4 sum[2][2];
         f32x4 block[2];
 #pragma unroll
-        for (int n = 0; n <= MT * 2 * NG; ++n) {
-            if (n < MT * 2 * NG) {
-                const int i = n / (2 * NG), j0 = n / NG % 2 * 2, g = n % NG;
-                if (n % (2 * NG) == 0 && i + 1 < MT) read(i + 1);
+        for (int n = 0; n <= MT * PJ * NG; ++n) {
+            if (n < MT * PJ * NG) {
+                const int i = n / (PJ * NG), j0 = n / NG % PJ * 2, g = n % NG;
+                if (n % (PJ * NG) == 0 && i + 1 < MT) read(i + 1);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     i32x4 &to = sum[n % 2][j];
@@ -465,7 +470,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             }
             __builtin_amdgcn_sched_barrier(0);  // their results are a unit away
             if (n > 0) {
-                const int m = n - 1, i = m / (2 * NG), j0 = m / NG % 2 * 2, g = m % NG;
+                const int m = n - 1, i = m / (PJ * NG), j0 = m / NG % PJ * 2, g = m % NG;
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -487,15 +492,15 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     };
     auto multiply_float = [&](auto set, int buf, auto &&next) {
         const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
-        constexpr int KEEP = G == 128 ? 2 * MT : 2;  // sums alive: all rows' over two halves
+        constexpr int KEEP = G == 128 ? PJ * MT : 2;  // sums alive: all rows' over two halves
         constexpr int UG = G == 32 ? 2 : 1;      // groups in a half
         f32x4 sum[KEEP][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            bf16x8 a[4][2];
-            f32x4 s[4][UG];
+            bf16x8 a[NJ][2];
+            f32x4 s[NJ][UG];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < NJ; ++j) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) a[j][t] = widen(words[set][j][2 * half + t]);
 #pragma unroll
@@ -515,10 +520,10 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             };
             read(0);
 #pragma unroll
-            for (int n = 0; n <= MT * 2 * UG; ++n) {
-                if (n < MT * 2 * UG) {
-                    const int i = n / (2 * UG), j0 = n / UG % 2 * 2, g = n % UG;
-                    if (n % (2 * UG) == 0 && i + 1 < MT) read(i + 1);
+            for (int n = 0; n <= MT * PJ * UG; ++n) {
+                if (n < MT * PJ * UG) {
+                    const int i = n / (PJ * UG), j0 = n / UG % PJ * 2, g = n % UG;
+                    if (n % (PJ * UG) == 0 && i + 1 < MT) read(i + 1);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         f32x4 &to = sum[n % KEEP][j];
@@ -534,7 +539,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
                 }
                 __builtin_amdgcn_sched_barrier(0);  // their results are a unit away
                 if (n > 0 && (G != 128 || half == 1)) {
-                    const int m = n - 1, i = m / (2 * UG), j0 = m / UG % 2 * 2, g = m % UG;
+                    const int m = n - 1, i = m / (PJ * UG), j0 = m / UG % PJ * 2, g = m % UG;
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -547,16 +552,16 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
         }
     };
     constexpr int NB = GATED ? 2 : 1;
-    __shared__ uint32_t sizes[OUT8 ? 4 : 1][OUT8 ? S::kRows : 1];
+    __shared__ uint32_t sizes[OUT8 ? NW : 1][OUT8 ? S::kRows : 1];
     auto finish = [&](int n, int m) {
-        const int n0 = (16 * n + 4 * wave) / NB * kW4Outputs + 4 * quarter;
-        float act[MT][4 / NB][4];
+        const int n0 = (S::kBlocks * n + NJ * wave) / NB * kW4Outputs + 4 * quarter;
+        float act[MT][NJ / NB][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const int at = 16 * i + l % 16, row = m * S::kRows + at;
             uint32_t most = 0;
 #pragma unroll
-            for (int j = 0; j < 4 / NB; ++j)
+            for (int j = 0; j < NJ / NB; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float v = total[NB * j][i][r] * 0.0625f;
@@ -584,10 +589,12 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
             for (int i = 0; i < MT; ++i) {
                 const int at = 16 * i + l % 16, row = m * S::kRows + at;
                 if (row >= p.rows) continue;
-                const Q8Scale s(
-                    max(max(sizes[0][at], sizes[1][at]), max(sizes[2][at], sizes[3][at])));
+                uint32_t most = sizes[0][at];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int w = 1; w < NW; ++w) most = max(most, sizes[w][at]);
+                const Q8Scale s(most);
+#pragma unroll
+                for (int j = 0; j < NJ / 2; ++j) {
                     if (n0 + 16 * j >= p.cols) continue;
                     *reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.y) +
                                                   (int64_t)row * p.cols + n0 + 16 * j) =
@@ -616,7 +623,7 @@ __global__ __launch_bounds__(256, 2) void w4_tiles(W4Product p, int32_t y_dtype)
     const int steps = round_up<SETS>(p.kb);
     for (;;) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int i = 0; i < MT; ++i) total[j][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         // The next tile's first steps are loaded with this one's last, so that memory is not
@@ -666,41 +673,67 @@ int32_t launch_rows(const W4Product &p, int32_t y_dtype, hipStream_t s) {
                        y_dtype);
     return launch_status();
 }
-template <int X, int G, int MT, bool GATED, bool OUT8>
+template <int X, int G, int MT, int NJ, int NW, bool GATED, bool OUT8>
 int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     W4Product q = p;
-    const int64_t tiles_n = ceil_div((int64_t)p.nb, (int64_t)16);
+    const int64_t tiles_n = ceil_div((int64_t)p.nb, (int64_t)NJ * NW);
     q.tiles_m = (int)ceil_div((int64_t)p.rows, (int64_t)16 * MT);
     q.strip = make_fastdiv((uint32_t)(8 * tiles_n));
     const int64_t tiles = tiles_n * q.tiles_m;
     if (tiles >= (int64_t)1 << 30) return QDC_ERR_SHAPE;
     q.tiles = (uint32_t)tiles;
-    const uint32_t grid = tiles < 512 ? (uint32_t)tiles : 512;  // two a compute unit
-    hipLaunchKernelGGL((w4_tiles<X, G, MT, GATED, OUT8>), dim3(grid), dim3(256), 0, s, q, y_dtype);
+    const uint32_t most = 2048 / NW;  // two wavefronts a SIMD
+    const uint32_t grid = tiles < most ? (uint32_t)tiles : most;
+    hipLaunchKernelGGL((w4_tiles<X, G, MT, NJ, NW, GATED, OUT8>), dim3(grid), dim3(NW * kWave), 0,
+                       s, q, y_dtype);
     return launch_status();
 }
 
-// The kernel with the smallest tile of which the chip's 256 units take one each, the largest
-// where none is large enough.  us for 1024 -> 5120 of bf16 rows, groups of 64, tiles of 16 x
-// 16 / 16 x 32 / 32 x 32 / 32 x 64 / by tiles of 16, 32, 64 rows x 256 (workgroups in
-// brackets): 16 rows 4.7 (320) / 4.4 (160) / 4.5 / - / -, 32 rows 6.0 / 5.5 (320) / 5.2
-// (160) / 6.4 / -, 96 rows - / 8.1 / 7.4 (480) / 6.6 (240) / 10.6, 256 rows - / - / 14.7 /
-// 16.1 / 16.1 (320), 13.9 (160), 18, 512 rows: - / - / 26.5 / 27.1 / 23.3, 19.1 (320),
-// 18.8 (160).
+// The kernel with the smallest tile of which the chip's 256 units take one each at most; where
+// none is large enough the one that is fastest when they take many.  us for 1024 -> 5120,
+// groups of 64 (in brackets the workgroups, where they are more than 256):
+//   rows x outputs of a tile   16 x 16  16 x 32  32 x 32  32 x 64  32 x 128  32 x 256  64 x 256
+//   bf16   16 rows            4.7 (320)    4.4      4.5       -        -         -         -
+//          32                 6.0 (640) 5.5 (320)   5.2      6.4       -         -         -
+//          96                     -     8.1 (960) 7.4 (480)  6.6       -         -         -
+//         128                     -        -     9.4 (640) 11.3 (320) 8.9      11.1        -
+//         256                     -        -        -     16.1 (640) 11.8 (320) 11.9     14.9
+//         512                     -        -        -        -     16.6 (640) 20 (320)   15.9
+//   fp32  301                     -        -        -        -     24.6 (400)  19.9      30.0
+// and by tiles of 64 x 256 in 4 wavefronts, two workgroups a unit / 128 x 256 in 8 (fp32: 32 /
+// 64 rows), 2048 rows: 8-bit 30.8 / 37, bf16 37.1 / 42.2, fp32 73 / 82; 16384: 183 / 188, 234 /
+// 222, 575 / 532.
+template <int X, int G, bool GATED, bool OUT8>
+int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    auto tiles = [&](int rows, int blocks) {
+        return ceil_div((int64_t)p.rows, (int64_t)rows) * ceil_div((int64_t)p.nb, (int64_t)blocks);
+    };
+    if constexpr (X == kF32 || OUT8) {
+        if (tiles(16, 16) <= 256) return launch_tiles<X, G, 1, 4, 4, GATED, OUT8>(p, y_dtype, s);
+    } else {
+        if (tiles(32, 8) <= 256) return launch_tiles<X, G, 2, 2, 4, GATED, OUT8>(p, y_dtype, s);
+    }
+    if (tiles(32, 16) <= 256) return launch_tiles<X, G, 2, 2, 8, GATED, OUT8>(p, y_dtype, s);
+    // groups of 32 of 8-bit rows: more of them would not fit the registers
+    if (tiles(64, 16) <= 256 || (X == kF32 && tiles(64, 16) >= 768) || (X == kQ8 && G == 32))
+        return launch_tiles<X, G, 4, 2, 8, GATED, OUT8>(p, y_dtype, s);
+    if constexpr (X == kF32)  // three terms a row in LDS
+        return launch_tiles<X, G, 2, 4, 4, GATED, OUT8>(p, y_dtype, s);
+    if constexpr (X == kBf16)
+        if (tiles(128, 16) >= 768) return launch_tiles<X, G, 8, 2, 8, GATED, OUT8>(p, y_dtype, s);
+    if constexpr (X == kBf16 || (X == kQ8 && G != 32))
+        return launch_tiles<X, G, 4, 4, 4, GATED, OUT8>(p, y_dtype, s);
+    return QDC_ERR_SHAPE;  // not reached
+}
+
 template <int X, int G, bool GATED>
 int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    if constexpr (GATED)
+        if (y_dtype == QDC_Q8) return launch_many<X, G, true, true>(p, y_dtype, s);
     auto fits = [&](int rows, int blocks) {
         return ceil_div((int64_t)p.rows, (int64_t)rows) * ceil_div((int64_t)p.nb, (int64_t)blocks) <=
                256;
     };
-    // fp32: three terms a row in LDS; groups of 32: the scales fill the registers
-    constexpr int BIG = X == kF32 || (X == kQ8 && G == 32) ? 2 : 4;
-    if constexpr (GATED)
-        if (y_dtype == QDC_Q8) {  // 128 columns are a tile's
-            if (fits(16, 16)) return launch_tiles<X, G, 1, true, true>(p, y_dtype, s);
-            if (BIG == 2 || fits(32, 16)) return launch_tiles<X, G, 2, true, true>(p, y_dtype, s);
-            return launch_tiles<X, G, BIG, true, true>(p, y_dtype, s);
-        }
     if constexpr (!GATED)
         if (fits(16, 1)) {
             // a wavefront for each 128 inputs, up to 16: 3584 -> 1024, one row of bf16, 4.1
@@ -712,9 +745,7 @@ int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     if (fits(16, 2)) return launch_rows<X, G, 1, 2, GATED, 8>(p, y_dtype, s);
     if (fits(32, 2)) return launch_rows<X, G, 2, 2, GATED, 8>(p, y_dtype, s);
     if (fits(32, 4)) return launch_rows<X, G, 2, 4, GATED, 8>(p, y_dtype, s);
-    if (fits(16, 16)) return launch_tiles<X, G, 1, GATED, false>(p, y_dtype, s);
-    if (BIG == 2 || fits(32, 16)) return launch_tiles<X, G, 2, GATED, false>(p, y_dtype, s);
-    return launch_tiles<X, G, BIG, GATED, false>(p, y_dtype, s);
+    return launch_many<X, G, GATED, false>(p, y_dtype, s);
 }
 
 template <int X>
