@@ -31,15 +31,26 @@ __device__ __forceinline__ int64_t weight_row(const Pack &p, int b, int n) {
     return j < p.out ? (int64_t)j + (p.gated && (b & 1) ? p.out : 0) : -1;
 }
 
-// w / s to the nearest whole number, ties to even, exactly: the rounded quotient may reach
-// a half that the true one does not, but what it leaves, w - q s, is exact with FMA (q s
-// has 12 bits, and the rest at most the 24 from w's last to s's half), so its side is known.
-__device__ __forceinline__ int nearest(float w, float s) {
-    float q = __builtin_rintf(w / s);
-    const float d = 2.0f * __builtin_fmaf(-q, s, w);
-    if (d > s || (d == s && ((int)q & 1))) q += 1.0f;
-    if (d < -s || (d == -s && ((int)q & 1))) q -= 1.0f;
-    return (int)fminf(fmaxf(q, -7.0f), 7.0f);
+// The last 4 bits of w / s to the nearest whole number, ties to even, exactly.
+//
+// fp32: a product with the inverse may come to the other side of a half than the quotient, but
+// what it leaves, w - q s, is exact with FMA (q s has 12 bits, and the rest at most the 24 from
+// w's last to s's half), so its side is known: q goes on where more than half of s is left, or
+// half of it and q is odd.  1.5 * 2^23 + q has q in its last bits.
+__device__ __forceinline__ uint32_t nearest(float w, float s, float inverse, float) {
+    w = __builtin_amdgcn_fmed3f(w, -7.0f * s, 7.0f * s);
+    const float near = w * inverse + 12582912.0f;
+    const uint32_t q = __float_as_uint(near);
+    const float rest = __builtin_fmaf(12582912.0f - near, s, w);
+    const bool on = size_bits(rest) + (q & 1u) > __float_as_uint(0.5f * s);
+    return (on ? q + (rest < 0.0f ? ~0u : 1u) : q) & 15u;
+}
+// bf16: with 8 bits each, w / s is a half or 2^-9 from it at least, and the product with the
+// inverse within 2^-20 of it, so rounded to 2^-16 (the last bit of values from 128 on) it is
+// the half where the quotient is; the whole number is then in the last bits of 1.5 * 2^23 more.
+__device__ __forceinline__ uint32_t nearest(float w, float, float inverse, bf16_t) {
+    const float q = w * inverse + 192.0f - 192.0f;
+    return __float_as_uint(__builtin_amdgcn_fmed3f(q, -7.0f, 7.0f) + 12582912.0f) & 15u;
 }
 
 template <int G, typename T> __global__ __launch_bounds__(kBlock) void pack_w4(Pack p) {
@@ -75,14 +86,16 @@ template <int G, typename T> __global__ __launch_bounds__(kBlock) void pack_w4(P
         for (int i = 0; i < T32; ++i) m = max(m, most[t / T32 * T32 + i]);
         const bool finite = m < 0x7f800000u;
         const bf16_t held = finite ? from_f32<bf16_t>(__uint_as_float(m) / 7.0f) : (bf16_t)0x7fc0;
-        const float s = to_f32(held);
+        // the smallest scales have no inverse: those groups 2^64 times larger, which is exact
+        const float s = to_f32(held), up = s < 0x1p-64f ? 0x1p64f : 1.0f;
+        const float larger = s * up, inverse = 1.0f / larger;
         uint32_t word = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int q = finite && s > 0.0f ? nearest(v[t][i], s) : 0;
-            word |= (uint32_t)(q & 15) << (8 * (i % 4) + 4 * (i / 4));
+            const float w = v[t][i] * up;
+            word |= nearest(w, larger, inverse, T()) << (8 * (i % 4) + 4 * (i / 4));
         }
-        words[t] = word;
+        words[t] = finite && s > 0.0f ? word : 0u;
         if (t % T32 == 0 && quarter == 0)
             p.scales[((int64_t)unit * (4 / T32) + t / T32) * kW4Outputs + n] = held;
     }
