@@ -406,6 +406,65 @@ def test_gated(rows, inner, inter, group, kind):
         near_q8(qo.gated_w4(x, w, out_dtype=qo.Q8), want, tol)
 
 
+# Row and output counts at which the next larger tile is taken, the last two with several
+# tiles a workgroup; of 2 and 3 blocks of inputs, the last not whole.
+MANY = [(300, 2000, 272), (520, 2056, 144), (1030, 2056, 272), (2050, 2051, 144),
+        (4100, 2056, 272), (8200, 4104, 144)]
+
+
+def on_device(*tensors):
+    return [t.to(DEV) for t in tensors]
+
+
+def near_on_device(got, want, tol, dtype):
+    over = (got.double() - want).abs() - tol - HALF[dtype] * (want.abs() + tol)
+    assert got.shape == want.shape and not got.isnan().any() and float(over.max()) <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("rows,out,inner", MANY)
+def test_linear_many(rows, out, inner, group, kind):
+    g = torch.Generator().manual_seed(rows + out + group)
+    x, xv = rows_of(g, rows, inner, torch.bfloat16 if kind == "bf16" else torch.float32, kind)
+    w, wv = weight_of(g, out, inner, group)
+    want, tol = product(*on_device(xv, wv), group, kind == "q8")
+    for dtype in (torch.float32, torch.bfloat16):
+        near_on_device(qo.linear_w4(x, w, out_dtype=dtype), want, tol, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("rows,out,inner", MANY)
+def test_gated_many(rows, out, inner, group, kind):
+    inter = out // 2 if out % 2 else out // 2 // 16 * 16 - 16 * (rows % 3)
+    g = torch.Generator().manual_seed(rows + out + group + 1)
+    x, xv = rows_of(g, rows, inner, torch.bfloat16 if kind == "bf16" else torch.float32, kind)
+    w, wv = weight_of(g, 2 * inter, inner, group, gated=True)
+    want, tol = silu_product(*on_device(xv, wv), group, kind == "q8")
+    for dtype in (torch.float32, torch.bfloat16):
+        near_on_device(qo.gated_w4(x, w, out_dtype=dtype), want, tol, dtype)
+    if inter % 16 == 0:
+        near_q8(qo.gated_w4(x, w, out_dtype=qo.Q8), want.cpu(), tol.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,out", [(1, 768), (40, 4096), (300, 2000), (1030, 2056), (4100, 2056)])
+def test_nothing_behind_the_result(rows, out):
+    """Rows behind the last, and the gap behind the last output, are left as they were."""
+    g = torch.Generator().manual_seed(out)
+    w, _ = weight_of(g, out, 136, 64)
+    x = torch.randn(rows, 136, generator=g).bfloat16().to(DEV)
+    want = qo.linear_w4(x, w)
+    held = torch.full((rows + 70, out), 7.0, dtype=torch.bfloat16, device=DEV)
+    status = _lib.lib().qdc_linear_w4(
+        held.data_ptr(), None, BF16, x.data_ptr(), None, BF16, w.packed.data_ptr(),
+        w.scales.data_ptr(), rows, out, 136, 64, 136, 0, torch.cuda.current_stream().cuda_stream)
+    assert status == 0 and torch.equal(held[:rows], want) and (held[rows:] == 7).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("inner", [8, 24, 120, 136, 264])
 @pytest.mark.parametrize("rows", [2, 80])
@@ -420,13 +479,15 @@ def test_linear_short_inner(inner, rows):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [1, 20, 100, 600])
-def test_linear_values_at_the_edge(rows):
+@pytest.mark.parametrize("inner", [256, 200])
+@pytest.mark.parametrize("rows,out", [(1, 48), (20, 48), (100, 48), (600, 48), (300, 2000),
+                                      (2050, 2056)])
+def test_linear_values_at_the_edge(rows, out, inner):
     """fp32 rows keep all 24 bits; an infinity or NaN reaches its own row alone, a NaN scale
     its own output alone; large values stay finite."""
     g = torch.Generator().manual_seed(3)
-    w, wv = weight_of(g, 48, 256, 64)
-    x = torch.randn(rows, 256, generator=g) * torch.exp(torch.randn(rows, 256, generator=g) * 8)
+    w, wv = weight_of(g, out, inner, 64)
+    x = torch.randn(rows, inner, generator=g) * torch.exp(torch.randn(rows, inner, generator=g) * 8)
     want, tol = product(x.double(), wv, 64, False)
     near(qo.linear_w4(x.to(DEV), w), want, tol, torch.float32)
     big = x.clone()
@@ -455,7 +516,7 @@ def test_rows_do_not_depend_on_their_neighbours():
     """Within a call of one kernel a row's result is its own, whatever lies beside it."""
     g = torch.Generator().manual_seed(5)
     w, _ = weight_of(g, 64, 512, 64)
-    for n in (16, 64, 400, 1000):
+    for n in (16, 64, 400, 1000, 9000):
         x = torch.randn(n, 512, generator=g).to(DEV)
         y = qo.linear_w4(x, w)
         order = torch.randperm(n, generator=g).to(DEV)
