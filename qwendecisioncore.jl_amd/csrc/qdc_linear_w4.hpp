@@ -309,7 +309,8 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Rows p) {
 // that share a scale of an 8-bit row, whose maximum the wavefronts find together.
 template <int X, int G, int MT, int NJ, int NW> struct Staged {
     static constexpr int kRows = 16 * MT, kBlocks = NJ * NW, kThreads = NW * kWave;
-    static constexpr int kPass = kRows * 16 / kThreads;      // pieces of x a thread
+    static constexpr int kStep = kThreads / 16 < kRows ? kThreads / 16 : kRows;
+    static constexpr int kPass = kRows / kStep;              // pieces of x a thread
     static constexpr int kTerms = Piece<X>::kTerms;
     static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
     static constexpr int kX = kRows * kLd * kTerms;          // x, then the weights' scales
@@ -344,7 +345,7 @@ template <int X, int G, int MT, int NJ, int NW, bool GATED, bool OUT8>
 __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_dtype) {
     typedef Staged<X, G, MT, NJ, NW> S;
     constexpr int NG = 128 / G, PJ = NJ / 2;  // groups of a step, pairs of blocks
-    static_assert(NJ % 2 == 0 && S::kPass >= 1 && (!OUT8 || S::kBlocks == 16), "");
+    static_assert(NJ % 2 == 0 && (!OUT8 || S::kBlocks == 16), "");
     __shared__ __align__(16) char tile[2][S::kBytes];
     const int tid = threadIdx.x, l = tid % kWave;
     // known to be one of a wavefront, so that its addresses are scalar
@@ -353,15 +354,16 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
 
     // this thread's pieces of 8 values: the same columns of kPass rows.  Offsets are 32 bits from
     // the tile's first row; rows behind the last one are the last one, and not stored.
-    const int k8 = tid % 16;
+    // (Where there are more threads than pieces, and than 1/16 blocks below, they come again.)
+    const int k8 = tid % 16, x_row = tid / 16 % S::kStep;
     const uint32_t row_bytes = (uint32_t)p.ld_x * kXBytes<X>;
     uint32_t x_at[S::kPass];
 #pragma unroll
     for (int i = 0; i < S::kPass; ++i)
-        x_at[i] = (uint32_t)(tid / 16 + S::kThreads / 16 * i) * row_bytes;
+        x_at[i] = (uint32_t)(x_row + S::kStep * i) * row_bytes;
     // and 1/16 of a block's scales (2, 4 or 8 bytes), and a row's
     const uint32_t block_bytes = (uint32_t)p.kb * (32 * NG), q8_bytes = 4 * (uint32_t)p.q8_groups;
-    const int st = tid % (16 * S::kBlocks);  // (where there are more threads, again)
+    const int st = tid % (16 * S::kBlocks);
     const uint32_t scale_at = (uint32_t)(st / 16) * block_bytes;
     const uint32_t xs_at = (uint32_t)(tid % S::kRows) * q8_bytes;
     typedef typename std::conditional<
@@ -426,7 +428,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
                 raw_xs[set];
 #pragma unroll
         for (int i = 0; i < S::kPass; ++i) {
-            char *dst = tile[buf] + (tid / 16 + S::kThreads / 16 * i) * S::kLd;
+            char *dst = tile[buf] + (x_row + S::kStep * i) * S::kLd;
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
 #pragma unroll
@@ -769,8 +771,10 @@ int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     auto tiles = [&](int rows, int blocks) {
         return ceil_div((int64_t)p.rows, (int64_t)rows) * ceil_div((int64_t)p.nb, (int64_t)blocks);
     };
-    if constexpr (X == kF32 || OUT8) {
+    if constexpr (X == kF32) {
         if (tiles(16, 16) <= 256) return launch_tiles<X, G, 1, 4, 4, GATED, OUT8>(p, y_dtype, s);
+    } else if constexpr (OUT8) {
+        if (tiles(16, 16) <= 256) return launch_tiles<X, G, 1, 2, 8, GATED, OUT8>(p, y_dtype, s);
     } else {
         if (tiles(32, 8) <= 256) return launch_tiles<X, G, 2, 2, 4, GATED, OUT8>(p, y_dtype, s);
     }
