@@ -73,11 +73,17 @@ int32_t qdc_residual_rmsnorm_q8(float *residual, void *q, float *scales, const f
  * inner).  Sums are fp32 (whole numbers
  * within a group of 8-bit rows), the scale applied to each group's sum: q * x is summed
  * before it, so an fp32 or bf16 x beyond 2^116 may overflow where q * s * x would not.
- * x_scales and y_scales are ignored where they are not used. */
+ * x_scales and y_scales are ignored where they are not used.  workspace: device memory of
+ * qdc_linear_w4_workspace bytes (0 unless y is QDC_Q8, and its rows few: NULL then), 16-byte
+ * aligned, the call's alone until it is done. */
 int32_t qdc_linear_w4(void *y, float *y_scales, int32_t y_dtype, const void *x,
                       const float *x_scales, int32_t x_dtype, const void *packed,
                       const void *scales, int64_t rows, int64_t out, int64_t inner, int64_t group,
-                      int64_t ld_x, int32_t gated, hipStream_t stream);
+                      int64_t ld_x, int32_t gated, void *workspace, int64_t workspace_bytes,
+                      hipStream_t stream);
+/* -1 for sizes that it refuses. */
+int64_t qdc_linear_w4_workspace(int64_t rows, int64_t out, int64_t inner, int64_t group,
+                                int32_t gated, int32_t y_dtype);
 
 #ifdef __cplusplus
 }

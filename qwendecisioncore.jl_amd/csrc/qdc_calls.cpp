@@ -607,11 +607,15 @@ PyObject *linear_w4(Args a) {
     const at::Tensor y =
         fresh(call, {rows, cols}, out_code == QDC_Q8 ? at::kChar : type_of(out_code));
     const at::Tensor y_scales = out_code == QDC_Q8 ? q8_scales(call, rows, cols) : at::Tensor();
+    const int64_t need = out_code == QDC_Q8 ? qdc_linear_w4_workspace(rows, w.out, w.inner, w.group,
+                                                                      w.gated, out_code)
+                                            : 0;
+    const at::Tensor work = need > 0 ? fresh(call, {need}, at::kByte) : at::Tensor();
     call.run(w.gated ? "gated_w4" : "linear_w4", [&](hipStream_t stream) {
         return qdc_linear_w4(y.data_ptr(), out_code == QDC_Q8 ? data<float>(y_scales) : nullptr,
                              out_code, x0.data_ptr(), x_scales, code, w.packed.data_ptr(),
                              w.scales.data_ptr(), rows, w.out, w.inner, w.group, ld, w.gated,
-                             stream);
+                             need > 0 ? work.data_ptr() : nullptr, need > 0 ? need : 0, stream);
     });
     return out_code == QDC_Q8 ? pair(y, y_scales) : THPVariable_Wrap(y);
 }

@@ -151,35 +151,44 @@ template <int X> __device__ __forceinline__ Piece<X> load_piece(const void *row,
 }
 template <int X> constexpr int kXBytes = X == kF32 ? 4 : X == kBf16 ? 2 : 1;
 
-// 4 consecutive outputs from `at` on, of which `left` lie within the row.
-template <typename T>
-__device__ __forceinline__ void put4(T *at, int left, bool whole, const float (&v)[4]) {
-    if (whole) {  // uniform
-        // an ordinary store: the cache joins what the wavefront's next ones write of a line
-        if (left <= 0) return;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4 *>(at) = pack(v);
-        else *reinterpret_cast<u32x2 *>(at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-        return;
-    }
+// The first `left` of N outputs of T, held in words, from `at` on.  An ordinary store: the cache
+// joins what the wavefront's next ones write of a line; and one for all N whatever the
+// alignment, as rows of an odd number of outputs start anywhere (16235 x 64 ->
+// 1477, fp32 results, by elements 58 us, so 24).
+template <typename T, int N>
+__device__ __forceinline__ void put_piece(T *at, int left, const uint32_t (&v)[N * sizeof(T) / 4]) {
+    constexpr int W = N * (int)sizeof(T) / 4;
+    typedef uint32_t Words __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    if (left >= N) {
+        Words w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (j < left) at[j] = from_f32<T>(v[j]);
+        for (int i = 0; i < W; ++i) w[i] = v[i];
+        *reinterpret_cast<Words *>(at) = w;
+    } else if (left > 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < left) at[i] = sizeof(T) == 4 ? (T)v[i] : (T)(v[i / 2] >> (16 * (i % 2)));
+    }
 }
 // N pieces of 4 outputs of a row, 16 apart, n the first output.
 template <typename T, int N>
 __device__ __forceinline__ void put(void *y, int cols, int row, int n, const float (&v)[N][4]) {
-    T *at = reinterpret_cast<T *>(y) + (int64_t)row * cols + n;
+    typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type Bits;
+    Bits *at = reinterpret_cast<Bits *>(y) + (int64_t)row * cols + n;
 #pragma unroll
-    for (int j = 0; j < N; ++j) put4(at + 16 * j, cols - n - 16 * j, (cols & 3) == 0, v[j]);
+    for (int j = 0; j < N; ++j) {
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t w[4] = {__float_as_uint(v[j][0]), __float_as_uint(v[j][1]),
+                                   __float_as_uint(v[j][2]), __float_as_uint(v[j][3])};
+            put_piece<Bits, 4>(at + 16 * j, cols - n - 16 * j, w);
+        } else {
+            const uint32_t w[2] = {pack_bf16x2(v[j][0], v[j][1]), pack_bf16x2(v[j][2], v[j][3])};
+            put_piece<Bits, 4>(at + 16 * j, cols - n - 16 * j, w);
+        }
+    }
 }
 
-// ---------------------------------------------------------------- few rows ---
-// A workgroup per NB blocks of outputs (pairs of gate and up where gated) and 16 * MT rows,
-// whose wavefronts take the blocks of inputs in turn and add up at the end: bound by the
-// weights' way from memory and, for a row or two, by one trip there, so every load of a
-// wavefront's block leaves at once and x comes straight from the caches.
-// The same in bf16 for a wavefront's 2 or 4 pieces from output n on, a multiple of 8 in a row:
-// the lanes of a row first trade pieces, so that each has 8 or 16 outputs side by side and a
+// The same in bf16 for a wavefront's 2 or 4 pieces from output n on: the lanes of a row first trade pieces, so that each has 8 or 16 outputs side by side and a
 // line is written by two instructions in place of four (8-bit rows, 16384 x 1024 -> 8224, 265
 // -> 257 us).
 template <int N>
@@ -213,9 +222,10 @@ __device__ __forceinline__ void put_wide(void *y, int cols, int row, bool in, in
     bf16_t *at = reinterpret_cast<bf16_t *>(y) + (int64_t)row * cols + n;
 #pragma unroll
     for (int j = 0; j < N; j += 2)
-        if (in && n + 4 * j < cols)
-            *reinterpret_cast<u32x4 *>(at + 4 * j) =
-                u32x4{t[j][0], t[j][1], t[j + 1][0], t[j + 1][1]};
+        if (in) {
+            const uint32_t w[4] = {t[j][0], t[j][1], t[j + 1][0], t[j + 1][1]};
+            put_piece<bf16_t, 8>(at + 4 * j, cols - n - 4 * j, w);
+        }
 }
 
 // What they are given, in 64 bytes: a launch with 128 takes the host 0.3 us longer.
@@ -626,7 +636,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
             if constexpr (!OUT8) {
                 bool narrow = true;
                 if constexpr (NJ / NB > 1)
-                    if (y_dtype == QDC_BF16 && p.cols % 8 == 0) {  // uniform
+                    if (y_dtype == QDC_BF16) {  // uniform
                         put_wide(p.y, p.cols, row, row < p.rows, n0 - 4 * quarter, quarter,
                                  act[i]);
                         narrow = false;
@@ -771,6 +781,9 @@ int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     auto tiles = [&](int rows, int blocks) {
         return ceil_div((int64_t)p.rows, (int64_t)rows) * ceil_div((int64_t)p.nb, (int64_t)blocks);
     };
+    // 128 outputs or fewer take no tile of 256
+    if constexpr (!OUT8)
+        if (p.nb <= 8) return launch_tiles<X, G, 2, 2, 4, GATED, false>(p, y_dtype, s);
     if constexpr (X == kF32) {
         if (tiles(16, 16) <= 256) return launch_tiles<X, G, 1, 4, 4, GATED, OUT8>(p, y_dtype, s);
     } else if constexpr (OUT8) {
@@ -800,16 +813,20 @@ int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
                256;
     };
     if constexpr (!GATED)
-        if (fits(16, 1)) {
+        if (fits(16, 1) || p.nb == 1) {
             // a wavefront for each 128 inputs, up to 16: 3584 -> 1024, one row of bf16, 4.1
             // us, of fp32 8.7, with 8 wavefronts 4.3 and 10.4; 256 -> 768 with 4 2.3, 8 2.4
             if (p.kb <= 4) return launch_rows<X, G, 1, 1, false, 4>(p, y_dtype, s);
             if (p.kb < 16) return launch_rows<X, G, 1, 1, false, 8>(p, y_dtype, s);
             return launch_rows<X, G, 1, 1, false, 16>(p, y_dtype, s);
         }
-    if (fits(16, 2)) return launch_rows<X, G, 1, 2, GATED, 8>(p, y_dtype, s);
-    if (fits(32, 2)) return launch_rows<X, G, 2, 2, GATED, 8>(p, y_dtype, s);
-    if (fits(32, 4)) return launch_rows<X, G, 2, 4, GATED, 8>(p, y_dtype, s);
+    if (fits(16, 2)) {
+        if (p.kb >= 16) return launch_rows<X, G, 1, 2, GATED, 16>(p, y_dtype, s);
+        return launch_rows<X, G, 1, 2, GATED, 8>(p, y_dtype, s);
+    }
+    // (outputs of a tile or less: x is read once however many the rows are)
+    if (fits(32, 2) || p.nb <= 2) return launch_rows<X, G, 2, 2, GATED, 8>(p, y_dtype, s);
+    if (w4_few(p.rows, p.nb)) return launch_rows<X, G, 2, 4, GATED, 8>(p, y_dtype, s);
     return launch_many<X, G, GATED, false>(p, y_dtype, s);
 }
 

@@ -81,6 +81,18 @@ static inline int64_t w4_scale_bytes(int64_t out, int64_t inner, int64_t group, 
 }
 static inline int64_t q8_groups(int64_t width) { return ceil_div(width, (int64_t)kQ8Group); }
 
+// Whether the product of these rows and blocks of outputs is that of few rows: tiles of 32 rows
+// by 4 blocks are no more than the chip's 256 units, or the only ones.
+static inline bool w4_few(int64_t rows, int64_t nb) {
+    return ceil_div(rows, (int64_t)32) * ceil_div(nb, (int64_t)4) <= 256 || nb <= 4;
+}
+// Whether 8-bit results come by way of fp32 ones in a workspace: the kernel by tiles gives them
+// at once, but of few rows each of its steps of 128 inputs takes 0.9 us.  us for 1024 -> 3584
+// columns, 1 row 6.1 / 8.0, 32 rows 8.1 / 7.9; 4480 -> 4864, 9 rows 13 / 31.
+static inline bool w4_by_workspace(int64_t rows, int64_t nb, int64_t kb) {
+    return w4_few(rows, nb) && (rows <= 16 || kb > 8);
+}
+
 struct QuantRange {
     const void *p;
     int64_t bytes;

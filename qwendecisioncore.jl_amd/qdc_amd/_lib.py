@@ -114,7 +114,8 @@ QUANT_SIGNATURES = {
     "qdc_dequantize_q8": (_i32, [_vp] * 3 + [_i64] * 2 + [_i32, _vp]),
     "qdc_residual_rmsnorm_q8": (_i32, [_vp] * 7 + [_i64] * 2 + [_f32, _i32, _vp]),
     "qdc_linear_w4": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp] + [_i64] * 5
-                      + [_i32, _vp]),
+                      + [_i32, _vp, _i64, _vp]),
+    "qdc_linear_w4_workspace": (_i64, [_i64] * 4 + [_i32, _i32]),
 }
 
 _lib = None

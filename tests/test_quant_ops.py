@@ -87,9 +87,20 @@ def test_linear_validation():
     Y, YS, X, XS, P, S = (FAR + (i << 40) for i in range(6))
 
     def f(y=Y, ys=YS, x=X, xs=XS, p=P, s=S, yt=BF16, xt=BF16, rows=3, out=96, inner=256, group=64,
-          ld=256, gated=0):
-        return lib.qdc_linear_w4(y, ys, yt, x, xs, xt, p, s, rows, out, inner, group, ld, gated,
-                                 None)
+          ld=256, gated=0, ws=FAR + (6 << 40), nbytes=3 * 48 * 4):
+        return lib.qdc_linear_w4(y, ys, yt, x, xs, xt, p, s, rows, out, inner, group, ld, gated, ws,
+                                 nbytes, None)
+
+    size = lib.qdc_linear_w4_workspace
+    assert size(3, 96, 256, 64, 1, Q8) == 3 * 48 * 4
+    assert size(3, 96, 256, 64, 1, BF16) == 0 and size(3, 96, 256, 64, 0, F32) == 0
+    assert size(9000, 7168, 1024, 64, 1, Q8) == 0 and size(0, 96, 256, 64, 1, Q8) == 0
+    assert size(-1, 96, 256, 64, 1, Q8) == -1 and size(3, 80, 256, 64, 1, Q8) == -1
+    assert size(3, 96, 256, 64, 0, Q8) == -1 and size(3, 96, 252, 64, 1, Q8) == -1
+    for bad in (dict(nbytes=3 * 48 * 4 - 1), dict(ws=FAR + (6 << 40) + 8)):
+        assert f(yt=Q8, gated=1, **bad) == -2
+    assert f(yt=Q8, gated=1, ws=None) == -1 and f(yt=Q8, gated=1, ws=X) == -5
+    assert f(yt=Q8, gated=1, ws=Y + 64) == -5
 
     assert f(xt=X2) == -3 and f(yt=X2) == -3 and f(yt=Q8) == -3 and f(xt=7) == -3
     for bad in (dict(rows=-1), dict(rows=(1 << 20) - 15), dict(out=0), dict(inner=252),
@@ -394,7 +405,8 @@ def test_linear(rows, inner, out, group, kind):
 @pytest.mark.parametrize("group", GROUPS)
 @pytest.mark.parametrize("rows,inner,inter", [(1, 128, 16), (1, 1024, 304), (5, 272, 37),
                                               (16, 256, 128), (33, 512, 144), (70, 208, 1),
-                                              (150, 640, 272), (700, 144, 160)])
+                                              (150, 640, 272), (700, 144, 160), (40, 1200, 272),
+                                              (17, 128, 1040)])
 def test_gated(rows, inner, inter, group, kind):
     g = torch.Generator().manual_seed(rows + inner + inter + group)
     x, xv = rows_of(g, rows, inner, torch.bfloat16 if kind == "bf16" else torch.float32, kind)
@@ -451,6 +463,22 @@ def test_gated_many(rows, out, inner, group, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
+@pytest.mark.parametrize("rows,out,inner", [(9000, 1, 272), (9000, 30, 144), (4200, 60, 272),
+                                            (9000, 100, 144)])
+def test_few_outputs_of_many_rows(rows, out, inner, kind):
+    g = torch.Generator().manual_seed(out)
+    x, xv = rows_of(g, rows, inner, torch.bfloat16 if kind == "bf16" else torch.float32, kind)
+    w, wv = weight_of(g, out, inner, 64)
+    near_on_device(qo.linear_w4(x, w, out_dtype=torch.float32),
+                   *product(*on_device(xv, wv), 64, kind == "q8"), torch.float32)
+    if out > 1:
+        up, upv = weight_of(g, out, inner, 32, gated=True)
+        near_on_device(qo.gated_w4(x, up, out_dtype=torch.float32),
+                       *silu_product(*on_device(xv, upv), 32, kind == "q8"), torch.float32)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,out", [(1, 768), (40, 4096), (300, 2000), (1030, 2056), (4100, 2056)])
 def test_nothing_behind_the_result(rows, out):
     """Rows behind the last, and the gap behind the last output, are left as they were."""
@@ -461,7 +489,8 @@ def test_nothing_behind_the_result(rows, out):
     held = torch.full((rows + 70, out), 7.0, dtype=torch.bfloat16, device=DEV)
     status = _lib.lib().qdc_linear_w4(
         held.data_ptr(), None, BF16, x.data_ptr(), None, BF16, w.packed.data_ptr(),
-        w.scales.data_ptr(), rows, out, 136, 64, 136, 0, torch.cuda.current_stream().cuda_stream)
+        w.scales.data_ptr(), rows, out, 136, 64, 136, 0, None, 0,
+        torch.cuda.current_stream().cuda_stream)
     assert status == 0 and torch.equal(held[:rows], want) and (held[rows:] == 7).all()
 
 
