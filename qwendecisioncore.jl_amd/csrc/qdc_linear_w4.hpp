@@ -46,10 +46,9 @@ __device__ __forceinline__ void terms(const float (&v)[8], u32x4 (&r)[3]) {
     uint32_t h[8], m[8], l[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint32_t b = __float_as_uint(v[i]);
-        const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-        h[i] = b | (!finite && (b & 0xffffu) ? 0x400000u : 0u);  // a NaN stays one
-        const float rest = finite ? v[i] - __uint_as_float(b & 0xffff0000u) : 0.0f;
+        h[i] = __float_as_uint(__builtin_canonicalizef(v[i]));  // a NaN with its upper half set
+        const bool finite = !__builtin_amdgcn_classf(v[i], 0x207);
+        const float rest = finite ? v[i] - __uint_as_float(h[i] & 0xffff0000u) : 0.0f;
         m[i] = __float_as_uint(rest);
         l[i] = __float_as_uint(rest - __uint_as_float(m[i] & 0xffff0000u));
     }
