@@ -72,7 +72,8 @@ int32_t qdc_residual_rmsnorm_q8(float *residual, void *q, float *scales, const f
  * multiple of 8, at most 2^26 bytes) or QDC_Q8 (x_scales; inner a multiple of 16, ld_x =
  * inner).  Sums are fp32 (whole numbers
  * within a group of 8-bit rows), the scale applied to each group's sum: q * x is summed
- * before it, so an fp32 or bf16 x beyond 2^116 may overflow where q * s * x would not.
+ * before it and in steps of 1/16, so an fp32 or bf16 x beyond 2^113 and a result beyond 2^123
+ * may overflow where q * s * x would not; of an fp32 x what lies below 2^-133 is lost.
  * x_scales and y_scales are ignored where they are not used.  workspace: device memory of
  * qdc_linear_w4_workspace bytes (0 unless y is QDC_Q8, and its rows few: NULL then), 16-byte
  * aligned, the call's alone until it is done. */

@@ -772,9 +772,9 @@ int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
 //         256                     -        -        -     16.1 (640) 11.8 (320) 11.9     14.9
 //         512                     -        -        -        -     16.6 (640) 20 (320)   15.9
 //   fp32  301                     -        -        -        -     24.6 (400)  19.9      30.0
-// and by tiles of 64 x 256 in 4 wavefronts, two workgroups a unit / 128 x 256 in 8 (fp32: 32 /
-// 64 rows), 2048 rows: 8-bit 30.8 / 37, bf16 37.1 / 42.2, fp32 73 / 82; 16384: 183 / 188, 234 /
-// 222, 575 / 532.
+// and by tiles of 64 x 256 in 4 wavefronts, two workgroups a unit / 128 x 256 in 8 (fp32: 32 / 64
+// rows) 4096 rows: 8-bit 45 / 56, bf16 56 / 62, fp32 133 / 121; 16384: 185 / 189, 233 / 224, 517 /
+// 483; 2048 -> 6144 of 1024 rows: 34 / 36, 45 / 39, 79 / 88.
 template <int X, int G, bool GATED, bool OUT8>
 int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     auto tiles = [&](int rows, int blocks) {
@@ -792,7 +792,7 @@ int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     }
     if (tiles(32, 16) <= 256) return launch_tiles<X, G, 2, 2, 8, GATED, OUT8>(p, y_dtype, s);
     // groups of 32 of 8-bit rows: more of them would not fit the registers
-    if (tiles(64, 16) <= 256 || (X == kF32 && tiles(64, 16) >= 2048) || (X == kQ8 && G == 32))
+    if (tiles(64, 16) <= 256 || (X == kF32 && tiles(64, 16) >= 768) || (X == kQ8 && G == 32))
         return launch_tiles<X, G, 4, 2, 8, GATED, OUT8>(p, y_dtype, s);
     if constexpr (X == kF32)  // three terms a row in LDS
         return launch_tiles<X, G, 2, 4, 4, GATED, OUT8>(p, y_dtype, s);

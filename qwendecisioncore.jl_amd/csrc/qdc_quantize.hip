@@ -253,9 +253,11 @@ using namespace qdc;
 
 extern "C" const char *qdc_quant_version(void) { return QDC_HIP_QUANT_VERSION; }
 
+// A wavefront per 256 columns of a row, in workgroups of 4: fewer than 2^32 work-items.
 static bool quant_rows(int64_t rows, int64_t width) {
-    return rows >= 0 && rows < ((int64_t)1 << 26) && width > 0 && width < ((int64_t)1 << 24) &&
-           width % 16 == 0 && rows * ceil_div(width, (int64_t)256) < ((int64_t)1 << 26);
+    const int64_t lim = ((int64_t)1 << 26) - 3;
+    return rows >= 0 && rows < lim && width > 0 && width < ((int64_t)1 << 24) && width % 16 == 0 &&
+           rows * ceil_div(width, (int64_t)256) < lim;
 }
 
 extern "C" int32_t qdc_pack_w4(void *packed, void *scales, const void *w, int64_t out,
