@@ -812,7 +812,9 @@ int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
                256;
     };
     if constexpr (!GATED)
-        if (fits(16, 1) || p.nb == 1) {
+        // (of a row or four the rows cost nothing to read twice: 1024 -> 7168, one row of bf16,
+        // 448 workgroups 3.3 us, 224 of two blocks 3.8)
+        if (fits(16, 1) || p.nb == 1 || (X != kF32 && p.rows <= 4 && p.nb <= 512)) {
             // a wavefront for each 128 inputs, up to 16: 3584 -> 1024, one row of bf16, 4.1
             // us, of fp32 8.7, with 8 wavefronts 4.3 and 10.4; 256 -> 768 with 4 2.3, 8 2.4
             if (p.kb <= 4) return launch_rows<X, G, 1, 1, false, 4>(p, y_dtype, s);
@@ -820,7 +822,8 @@ int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
             return launch_rows<X, G, 1, 1, false, 16>(p, y_dtype, s);
         }
     if (fits(16, 2)) {
-        if (p.kb >= 16) return launch_rows<X, G, 1, 2, GATED, 16>(p, y_dtype, s);
+        if constexpr (X == kF32)  // 3584 -> 4096 of 8 rows 10.3 us, with 8 11.7; bf16 7.0, 7.1
+            if (p.kb >= 16) return launch_rows<X, G, 1, 2, GATED, 16>(p, y_dtype, s);
         return launch_rows<X, G, 1, 2, GATED, 8>(p, y_dtype, s);
     }
     // (outputs of a tile or less: x is read once however many the rows are)
