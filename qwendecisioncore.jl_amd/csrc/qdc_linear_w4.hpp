@@ -2,8 +2,8 @@
 //
 // y[m, n] = sum over groups g of s[n, g] * sum over k in g of q[n, k] x[m, k].  The whole
 // numbers enter the matrix instructions as they are (an 8-bit one holds 16 q, a bf16 one
-// 16 q exactly), so the only roundings are those of fp32 sums: a group's sum is scaled and
-// added in fp32, and the factor 16 taken out of the result.  fp32 rows enter as three bf16
+// q / 16 exactly), so the only roundings are those of fp32 sums: a group's sum is scaled and
+// added in fp32, and the factor taken out of the result.  fp32 rows enter as three bf16
 // terms that hold all 24 bits (8 each, by truncation); 8-bit rows as they are, with whole
 // sums, their own scale joining the weight's.
 //
@@ -24,15 +24,21 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 enum { kF32, kBf16, kQ8 };  // types of x
 
-// 8 bf16 values, of 4 + 4 signed bytes 16 q in the upper halves of a word's bytes.
+// A word's 8 whole numbers as bf16, q / 16: the conversion looks at the last 4 bits of a byte
+// alone and divides by 16 (from signed bytes 16 q, which take masks, 361 us in place of TODO for
+// 16384 x 1024 -> 8224 of bf16).
+constexpr float kBack(bool whole) { return whole ? 0.0625f : 16.0f; }
 __device__ __forceinline__ bf16x8 widen(uint32_t word) {
-    const uint32_t lo = (word << 4) & 0xf0f0f0f0u, hi = word & 0xf0f0f0f0u;
     u32x4 r;
+    uint32_t upper = word >> 4;
+    asm("" : "+v"(upper));  // a value of its own, whose bytes the conversions select themselves
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const uint32_t b = i ? hi : lo;
-        const float v0 = (float)(int8_t)b, v1 = (float)(int8_t)(b >> 8);
-        const float v2 = (float)(int8_t)(b >> 16), v3 = (float)(int8_t)(b >> 24);
+        const uint32_t b = i ? upper : word;
+        const float v0 = __builtin_amdgcn_cvt_off_f32_i4((int)(b & 0xffu));
+        const float v1 = __builtin_amdgcn_cvt_off_f32_i4((int)(b >> 8 & 0xffu));
+        const float v2 = __builtin_amdgcn_cvt_off_f32_i4((int)(b >> 16 & 0xffu));
+        const float v3 = __builtin_amdgcn_cvt_off_f32_i4((int)(b >> 24));
         // exact in bf16: the upper halves of the fp32 values
         r[2 * i] = __builtin_amdgcn_perm(__float_as_uint(v1), __float_as_uint(v0), 0x07060302u);
         r[2 * i + 1] = __builtin_amdgcn_perm(__float_as_uint(v3), __float_as_uint(v2), 0x07060302u);
@@ -302,8 +308,8 @@ __global__ __launch_bounds__(WAVES *kWave) void w4_rows(W4Rows p) {
     for (int b = 0; b < NB / PER; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            v[b][r] = sum[PER * b][r] * 0.0625f;
-            if constexpr (GATED) v[b][r] = silu(v[b][r]) * (sum[2 * b + 1][r] * 0.0625f);
+            v[b][r] = sum[PER * b][r] * kBack(X == kQ8);
+            if constexpr (GATED) v[b][r] = silu(v[b][r]) * (sum[2 * b + 1][r] * kBack(X == kQ8));
         }
     const int n = b0 / PER * kW4Outputs + 4 * quarter;
     if (p.y_dtype == QDC_F32) put<float>(p.y, p.cols, row, n, v);
@@ -627,8 +633,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
             for (int j = 0; j < NJ / NB; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float v = total[NB * j][i][r] * 0.0625f;
-                    if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * 0.0625f);
+                    float v = total[NB * j][i][r] * kBack(X == kQ8);
+                    if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * kBack(X == kQ8));
                     act[i][j][r] = v;
                     if (OUT8 && n0 + 16 * j < p.cols) most = max(most, size_bits(v));
                 }
