@@ -25,8 +25,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 enum { kF32, kBf16, kQ8 };  // types of x
 
 // A word's 8 whole numbers as bf16, q / 16: the conversion looks at the last 4 bits of a byte
-// alone and divides by 16 (from signed bytes 16 q, which take masks, 361 us in place of TODO for
-// 16384 x 1024 -> 8224 of bf16).
+// alone and divides by 16 (from signed bytes 16 q, which take masks, 16384 x 1024 -> 8224 of
+// bf16 took 361 us in place of 352, 301 x 2048 -> 6144 of fp32 32.9 in place of 30.0).
 constexpr float kBack(bool whole) { return whole ? 0.0625f : 16.0f; }
 __device__ __forceinline__ bf16x8 widen(uint32_t word) {
     u32x4 r;
