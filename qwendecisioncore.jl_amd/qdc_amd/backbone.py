@@ -144,8 +144,8 @@ class QwenBackbone:
             src = weights[name]
             w = dev(src)
             layer[key] = gemm_weight(w, split)
-            if dtype == torch.bfloat16 and not weight_format and ops.linear_parts_fits(w.shape[1], w.shape[0],
-                                                                 bool(split)):
+            if dtype == torch.bfloat16 and not weight_format and \
+                    ops.linear_parts_fits(w.shape[1], w.shape[0], bool(split)):
                 shared = isinstance(src, torch.Tensor) and w.data_ptr() == src.data_ptr()
                 layer[key + "_rows"] = w.clone() if shared else w
 
@@ -476,8 +476,11 @@ class QwenBackbone:
         w_kv = w.outputs(H * hd, (H + 2 * KV) * hd) if isinstance(w, W4) else \
             w[:, H * hd:(H + 2 * KV) * hd]
         kv = self._mm(x, w_kv)                               # [T, k | v] of every token
-        last = Q8(*(t.view(B, S, -1)[:, -1].contiguous() for t in x)) if isinstance(x, Q8) else \
-            x.view(B, S, -1)[:, -1].contiguous()
+        last_rows = lambda t: t.view(B, S, -1)[:, -1]  # noqa: E731
+        if isinstance(x, Q8):
+            last = Q8(*(last_rows(t).contiguous() for t in x))
+        else:  # 4-bit weights take rows no more than 2^26 bytes apart
+            last = last_rows(x).contiguous() if isinstance(w, W4) else last_rows(x)
         proj = self._mm(last, w)                             # [B, q | k | v | gate], last rows
         tables = self.rope_tables(S) if cfg.rotary_dim else None
         _, kt, v = ops.attention_prepare(None, kv[:, :KV * hd].view(T, KV, hd),
