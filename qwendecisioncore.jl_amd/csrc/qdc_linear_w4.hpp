@@ -789,12 +789,16 @@ int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     // 128 outputs or fewer take no tile of 256
     if constexpr (!OUT8)
         if (p.nb <= 8) return launch_tiles<X, G, 2, 2, 4, GATED, false>(p, y_dtype, s);
-    if constexpr (X == kF32) {
-        if (tiles(16, 16) <= 256) return launch_tiles<X, G, 1, 4, 4, GATED, OUT8>(p, y_dtype, s);
-    } else if constexpr (OUT8) {
+    if constexpr (X == kF32 || OUT8) {
         if (tiles(16, 16) <= 256) return launch_tiles<X, G, 1, 2, 8, GATED, OUT8>(p, y_dtype, s);
     } else {
-        if (tiles(32, 8) <= 256) return launch_tiles<X, G, 2, 2, 4, GATED, OUT8>(p, y_dtype, s);
+        // of 8-bit rows two of these to a unit are faster than one twice as large: us 128 rows
+        // 2048 -> 6144 11.5 / 12.2 / 14.7 of 16, 32 rows x 128, 32 x 256; 256 rows 17.7 / 14.7 /
+        // 15.3
+        constexpr int most = X == kQ8 ? 512 : 256;
+        if constexpr (X == kQ8)
+            if (tiles(16, 8) <= most) return launch_tiles<X, G, 1, 2, 4, GATED, false>(p, y_dtype, s);
+        if (tiles(32, 8) <= most) return launch_tiles<X, G, 2, 2, 4, GATED, false>(p, y_dtype, s);
     }
     if (tiles(32, 16) <= 256) return launch_tiles<X, G, 2, 2, 8, GATED, OUT8>(p, y_dtype, s);
     // groups of 32 of 8-bit rows: more of them would not fit the registers
@@ -832,9 +836,25 @@ int32_t launch(const W4Product &p, int32_t y_dtype, hipStream_t s) {
             if (p.kb >= 16) return launch_rows<X, G, 1, 2, GATED, 16>(p, y_dtype, s);
         return launch_rows<X, G, 1, 2, GATED, 8>(p, y_dtype, s);
     }
-    // (outputs of a tile or less: x is read once however many the rows are)
-    if (fits(32, 2) || p.nb <= 2) return launch_rows<X, G, 2, 2, GATED, 8>(p, y_dtype, s);
-    if (w4_few(p.rows, p.nb)) return launch_rows<X, G, 2, 4, GATED, 8>(p, y_dtype, s);
+    // Groups of 32 of 8-bit rows are nearer to bf16 than to larger ones: twice the sums to scale.
+    constexpr bool few_sums = X == kQ8 && G != 32;
+    // (outputs of a tile or less: x is read once however many the rows are.  Of 17 to 32 rows two
+    // sets of 16 share a weight's widening: 24 rows 1024 -> 7168 bf16 4.9 us, by 16 x 64 5.4)
+    if (p.nb <= 2 || (X != kF32 && !few_sums && p.rows <= 32 && fits(32, 2)))
+        return launch_rows<X, G, 2, 2, GATED, 8>(p, y_dtype, s);
+    // 64 rows 3584 -> 4096 fp32 16.7 us, bf16 10.3, 8-bit 9.7; by 32 x 32 20.5, 10.8, 11.3
+    if (fits(16, 4)) return launch_rows<X, G, 1, 4, GATED, 8>(p, y_dtype, s);
+    if (fits(32, 4)) {
+        // 32 x 64 with the inputs over 8 wavefronts, or 16 x 128 with the outputs over 4: us for
+        // 96 rows 512 -> 5120 of bf16 5.5 / 5.1, for 48 rows 2048 -> 6144 9.3 / 11.6, of fp32
+        // 16.2 / 17.3, of 8 bits 9.4 / 9.0 (groups of 32: 11.3 / 11.4; 3584 -> 4096 of 96 rows
+        // 16.5 / 18.0).  fp32 rows in groups of 32 would not fit the registers of the first:
+        // 25.8 / 17.5.
+        constexpr bool by_outputs = few_sums || (X == kF32 && G == 32);
+        if (p.nb > 4 && (by_outputs || p.kb <= (X == kQ8 ? 16 : 4)))
+            return launch_tiles<X, G, 1, 2, 4, GATED, false>(p, y_dtype, s);
+        if constexpr (!by_outputs) return launch_rows<X, G, 2, 4, GATED, 8>(p, y_dtype, s);
+    }
     return launch_many<X, G, GATED, false>(p, y_dtype, s);
 }
 

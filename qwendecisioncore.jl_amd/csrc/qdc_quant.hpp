@@ -81,8 +81,8 @@ static inline int64_t w4_scale_bytes(int64_t out, int64_t inner, int64_t group, 
 }
 static inline int64_t q8_groups(int64_t width) { return ceil_div(width, (int64_t)kQ8Group); }
 
-// Whether the product of these rows and blocks of outputs is that of few rows: tiles of 32 rows
-// by 4 blocks are no more than the chip's 256 units, or the only ones.
+// Whether the product of these rows and blocks of outputs is a small one: tiles of 32 rows by 4
+// blocks are no more than the chip's 256 units, or wider ones mostly empty.
 static inline bool w4_few(int64_t rows, int64_t nb) {
     return ceil_div(rows, (int64_t)32) * ceil_div(nb, (int64_t)4) <= 256 || nb <= 4;
 }

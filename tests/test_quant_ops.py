@@ -462,6 +462,28 @@ def test_gated_many(rows, out, inner, group, kind):
         near_q8(qo.gated_w4(x, w, out_dtype=qo.Q8), want.cpu(), tol.cpu())
 
 
+# Between few rows and many, on both sides of where the next kernel is taken: of 2 to 18 blocks
+# of inputs, with the last block of outputs and of inputs not whole.
+BETWEEN = [(24, 5098, 400), (48, 4090, 272), (48, 7030, 272), (47, 7030, 1040), (41, 7030, 2192),
+           (90, 2050, 2192), (128, 7190, 144), (200, 7190, 144), (33, 7190, 656)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("rows,out,inner", BETWEEN)
+def test_between_few_and_many(rows, out, inner, group, kind):
+    g = torch.Generator().manual_seed(rows + out + inner + group)
+    x, xv = rows_of(g, rows, inner, torch.bfloat16 if kind == "bf16" else torch.float32, kind)
+    w, wv = weight_of(g, out, inner, group)
+    want, tol = product(*on_device(xv, wv), group, kind == "q8")
+    gated, gv = weight_of(g, out, inner, group, gated=True)
+    both, both_tol = silu_product(*on_device(xv, gv), group, kind == "q8")
+    for dtype in (torch.float32, torch.bfloat16):
+        near_on_device(qo.linear_w4(x, w, out_dtype=dtype), want, tol, dtype)
+        near_on_device(qo.gated_w4(x, gated, out_dtype=dtype), both, both_tol, dtype)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
 @pytest.mark.parametrize("rows,out,inner", [(9000, 1, 272), (9000, 30, 144), (4200, 60, 272),
