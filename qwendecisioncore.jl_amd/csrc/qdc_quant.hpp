@@ -87,10 +87,12 @@ static inline bool w4_few(int64_t rows, int64_t nb) {
     return ceil_div(rows, (int64_t)32) * ceil_div(nb, (int64_t)4) <= 256 || nb <= 4;
 }
 // Whether 8-bit results come by way of fp32 ones in a workspace: the kernel by tiles gives them
-// at once, but of few rows each of its steps of 128 inputs takes 0.9 us.  us for 1024 -> 3584
-// columns, 1 row 6.1 / 8.0, 32 rows 8.1 / 7.9; 4480 -> 4864, 9 rows 13 / 31.
+// at once, but of few rows its steps of 128 inputs, 0.9 us each, are what it takes.  us by the
+// workspace / at once, of 8-bit and fp32 rows: 512 -> 1024 columns, 32 rows 5.3 / 5.7, 6.2 / 8.3,
+// 192 rows 6.4 / 5.7, 8.6 / 8.3; 1024 -> 3584, 32 rows 7.4 / 8.0, 9.1 / 12.9, 96 rows (more than
+// few) 9.4 / 8.1, 15.1 / 13.1; 2048 -> 2048, 128 rows 11.4 / 12.3, 18.0 / 22.4.
 static inline bool w4_by_workspace(int64_t rows, int64_t nb, int64_t kb) {
-    return w4_few(rows, nb) && (rows <= 16 || kb > 8);
+    return w4_few(rows, nb) && (rows <= 64 || kb > 4);
 }
 
 struct QuantRange {
