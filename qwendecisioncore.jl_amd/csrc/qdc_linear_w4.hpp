@@ -327,10 +327,24 @@ template <int X, int G, int MT, int NJ, int NW> struct Staged {
     static constexpr int kStep = kThreads / 16 < kRows ? kThreads / 16 : kRows;
     static constexpr int kPass = kRows / kStep;              // pieces of x a thread
     static constexpr int kTerms = Piece<X>::kTerms;
-    static constexpr int kLd = (X == kQ8 ? 128 : 256) + 16;  // bytes: 16 rows, all banks
+    static constexpr int kLd = X == kQ8 ? 144 : X == kBf16 ? 272 : 256;  // bytes of a row
     static constexpr int kX = kRows * kLd * kTerms;          // x, then the weights' scales
     static constexpr int kScales = kBlocks * (128 / G) * 64;     // (a block's groups, 16 fp32 each),
     static constexpr int kBytes = kX + kScales + 4 * kRows;  // then those of 8-bit rows
+
+    // Where 16 bytes of a row are.  The 16 lanes whose addresses LDS takes at once (0-3, 12-15
+    // and 20-27 of a read, and their like) are 16 rows in two quarters: the order of fp32 terms,
+    // another one in each row, puts them in all of its banks.  Rows 16 bytes longer than they
+    // need to be take 4 of 8 cycles of a read for conflicts, which three terms wait for and
+    // one does not.  us by order / longer rows: 301 rows 2048 -> 6144 fp32 29.2 / 31.0; 16384
+    // rows 1024 -> 8224 fp32 708 / 723, bf16 312 / 309, 8-bit 262 / 255.
+    __device__ static __forceinline__ uint32_t at(int row, int piece) {
+        return (uint32_t)(row * kLd + 16 * (X == kF32 ? piece ^ row % 16 : piece));
+    }
+    // 4 pieces a time further on
+    __device__ static __forceinline__ uint32_t along(uint32_t at, uint32_t times) {
+        return X == kF32 ? at ^ 64u * times : at + 64u * times;
+    }
 };
 
 // The tiles of a workgroup.  Workgroups go to the 8 dies in turn, each with a cache of its
@@ -443,7 +457,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
                 raw_xs[set];
 #pragma unroll
         for (int i = 0; i < S::kPass; ++i) {
-            char *dst = tile[buf] + (x_row + S::kStep * i) * S::kLd;
+            // (rows a multiple of 16 apart have one order)
+            char *dst = tile[buf] + S::kStep * i * S::kLd;
 #pragma unroll
             for (int h = 0; h < RAW; ++h)
 #pragma unroll
@@ -451,10 +466,10 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
                     mine[i][h][e] = ok ? mine[i][h][e] : 0u;
             if constexpr (X == kQ8) {
                 // the two pieces that an instruction's lane takes lie side by side
-                *reinterpret_cast<u32x2 *>(dst + 64 * (k8 / 8) + 16 * (k8 % 4) +
+                *reinterpret_cast<u32x2 *>(dst + S::at(x_row, 4 * (k8 / 8) + k8 % 4) +
                                            8 * (k8 / 4 % 2)) = mine[i][0];
             } else if constexpr (X == kBf16) {
-                *reinterpret_cast<u32x4 *>(dst + 16 * k8) = mine[i][0];
+                *reinterpret_cast<u32x4 *>(dst + S::at(x_row, k8)) = mine[i][0];
             } else {
                 float v[8];
 #pragma unroll
@@ -463,7 +478,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
                 terms(v, t);
 #pragma unroll
                 for (int n = 0; n < 3; ++n)
-                    *reinterpret_cast<u32x4 *>(dst + n * S::kRows * S::kLd + 16 * k8) = t[n];
+                    *reinterpret_cast<u32x4 *>(dst + n * S::kRows * S::kLd + S::at(x_row, k8)) = t[n];
             }
         }
     };
@@ -478,13 +493,13 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
     // while the next unit's are multiplied: the scheduler, left to itself, starts them all
     // and runs out of registers.
     auto multiply_whole = [&](auto set, int buf, auto &&next) {
-        const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
+        const uint32_t mine = S::at(l % 16, quarter);
         u32x4 x[2][2];
         auto read = [&](int i) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                x[i % 2][u] =
-                    *reinterpret_cast<const u32x4 *>(mine + 16 * i * S::kLd + 64 * u);
+                x[i % 2][u] = *reinterpret_cast<const u32x4 *>(tile[buf] + 16 * i * S::kLd +
+                                                               S::along(mine, u));
         };
         read(0);
         u32x4 a[NJ][2];
@@ -560,7 +575,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
         }
     };
     auto multiply_float = [&](auto set, int buf, auto &&next) {
-        const char *mine = tile[buf] + l % 16 * S::kLd + 16 * quarter;
+        const uint32_t mine = S::at(l % 16, quarter);
         constexpr int KEEP = G == 128 ? PJ * MT : 2;  // sums alive: all rows' over two halves
         constexpr int UG = G == 32 ? 2 : 1;      // groups in a half
         f32x4 sum[KEEP][2];
@@ -585,7 +600,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
 #pragma unroll
                     for (int n = 0; n < S::kTerms; ++n)
                         x[i % 2][t][n] = *reinterpret_cast<const u32x4 *>(
-                            mine + n * S::kRows * S::kLd + 16 * i * S::kLd + 64 * (2 * half + t));
+                            tile[buf] + n * S::kRows * S::kLd + 16 * i * S::kLd +
+                            S::along(mine, 2 * half + t));
             };
             read(0);
 #pragma unroll
