@@ -793,10 +793,10 @@ int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
 //         128                     -        -     9.4 (640) 11.3 (320) 8.9      11.1        -
 //         256                     -        -        -     16.1 (640) 11.8 (320) 11.9     14.9
 //         512                     -        -        -        -     16.6 (640) 20 (320)   15.9
-//   fp32  301                     -        -        -        -     24.6 (400)  19.9      30.0
+//   fp32  301                     -        -        -        -     19.2 (400)  15.4      23.4
 // and by tiles of 64 x 256 in 4 wavefronts, two workgroups a unit / 128 x 256 in 8 (fp32: 32 / 64
-// rows) 4096 rows: 8-bit 45 / 56, bf16 56 / 62, fp32 133 / 121; 16384: 185 / 189, 233 / 224, 517 /
-// 483; 2048 -> 6144 of 1024 rows: 34 / 36, 45 / 39, 79 / 88.
+// rows) 4096 rows: 8-bit 45 / 56, bf16 56 / 62, fp32 127 / 110; 16384: 185 / 189, 233 / 224, 466 /
+// 421; 2048 -> 6144 of 1024 rows: 34 / 36, 45 / 39, 71 / 81.
 template <int X, int G, bool GATED, bool OUT8>
 int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
     auto tiles = [&](int rows, int blocks) {
