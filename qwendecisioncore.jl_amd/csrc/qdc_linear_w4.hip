@@ -28,8 +28,7 @@ extern "C" int32_t qdc_linear_w4(void *y, float *y_scales, int32_t y_dtype, cons
     if (!product_shape(rows, out, inner, group, gated, y8)) return QDC_ERR_SHAPE;
     const int64_t cols = gated ? out / 2 : out;
     if (x8 ? inner % 16 != 0 || ld_x != inner : ld_x < inner || ld_x % 8) return QDC_ERR_SHAPE;
-    // offsets within 64 rows are 32 bits
-    if (ld_x > ((int64_t)1 << 26) / (x8 ? 1 : elem_size(x_dtype))) return QDC_ERR_SHAPE;
+    if (ld_x > kW4RowBytes / (x8 ? 1 : elem_size(x_dtype))) return QDC_ERR_SHAPE;
     if (rows == 0) return QDC_OK;
     const int64_t need = qdc_linear_w4_workspace(rows, out, inner, group, gated, y_dtype);
     if (!y || !x || !packed || !scales || (x8 && !x_scales) || (y8 && !y_scales) ||

@@ -331,6 +331,8 @@ template <int X, int G, int MT, int NJ, int NW> struct Staged {
     static constexpr int kX = kRows * kLd * kTerms;          // x, then the weights' scales
     static constexpr int kScales = kBlocks * (128 / G) * 64;     // (a block's groups, 16 fp32 each),
     static constexpr int kBytes = kX + kScales + 4 * kRows;  // then those of 8-bit rows
+    // The most bytes from a row of x to the next: offsets from a tile's first row are 32 bits.
+    static constexpr int64_t kFarthest = ((int64_t)1 << 32) / kRows;
 
     // Where 16 bytes of a row are.  The 16 lanes whose addresses LDS takes at once (0-3, 12-15
     // and 20-27 of a read, and their like) are 16 rows in two quarters: the order of fp32 terms,
@@ -769,6 +771,8 @@ int32_t launch_rows(const W4Product &p, int32_t y_dtype, hipStream_t s) {
 }
 template <int X, int G, int MT, int NJ, int NW, bool GATED, bool OUT8>
 int32_t launch_tiles(const W4Product &p, int32_t y_dtype, hipStream_t s) {
+    // (who launches a taller tile looks at the distance)
+    static_assert(MT == 8 || Staged<X, G, MT, NJ, NW>::kFarthest >= kW4RowBytes, "row offsets");
     W4Product q = p;
     const int64_t tiles_n = ceil_div((int64_t)p.nb, (int64_t)NJ * NW);
     q.tiles_m = (int)ceil_div((int64_t)p.rows, (int64_t)16 * MT);
@@ -822,8 +826,10 @@ int32_t launch_many(const W4Product &p, int32_t y_dtype, hipStream_t s) {
         return launch_tiles<X, G, 4, 2, 8, GATED, OUT8>(p, y_dtype, s);
     if constexpr (X == kF32)  // three terms a row in LDS
         return launch_tiles<X, G, 2, 4, 4, GATED, OUT8>(p, y_dtype, s);
+    // 128 rows of the greatest distance are more than a tile's offsets hold
     if constexpr (X == kBf16)
-        if (tiles(128, 16) >= 768) return launch_tiles<X, G, 8, 2, 8, GATED, OUT8>(p, y_dtype, s);
+        if (tiles(128, 16) >= 768 && p.ld_x * kXBytes<X> <= Staged<X, G, 8, 2, 8>::kFarthest)
+            return launch_tiles<X, G, 8, 2, 8, GATED, OUT8>(p, y_dtype, s);
     if constexpr (X == kBf16 || (X == kQ8 && G != 32))
         return launch_tiles<X, G, 4, 4, 4, GATED, OUT8>(p, y_dtype, s);
     return QDC_ERR_SHAPE;  // not reached

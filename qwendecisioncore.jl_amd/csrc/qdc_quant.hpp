@@ -10,6 +10,7 @@ constexpr int kQ8Group = 128;   // columns of an 8-bit row that share a scale
 constexpr int kW4Outputs = 16;  // of a block of 4-bit weights: a matrix instruction's rows,
 constexpr int kW4Inputs = 128;  // and as many inputs as make it 16 bytes a lane
 constexpr int kW4Words = 256;
+constexpr int64_t kW4RowBytes = (int64_t)1 << 26;  // of x, from a row to the next, at most
 
 // |v| as an integer that orders like it, NaN above infinity.
 __device__ __forceinline__ uint32_t size_bits(float v) {

@@ -1,0 +1,36 @@
+"""The operators on 4-bit weights and 8-bit rows at the ends of their documented ranges: rows
+far apart, the largest and smallest scales, quotients next to a half, tensors at any address."""
+import pytest
+import torch
+
+from qdc_amd import quant_ops as qo
+from test_quant_ops import DEV, near_on_device, product, silu_product
+
+
+def device_weight(seed, out, inner, group, gated=False, scale=0.1):
+    """A weight made on the device and the values that it stands for."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    w = qo.pack_w4(torch.randn(out, inner, generator=g, device=DEV) * scale, group, gated)
+    return w, qo.unpack_w4(w).double()
+
+
+# ------------------------------------------------------------ rows far apart --
+@pytest.mark.gpu
+@pytest.mark.parametrize("ld", [1 << 24, 17_000_000, 1 << 25])
+def test_rows_far_apart(ld):
+    """128 bf16 rows up to the documented 2^26 bytes apart, of as many outputs as take the
+    tallest tile: at 17e6 elements its last rows are more than 2^32 bytes from its first."""
+    rows, inner, out = 128, 64, 196608
+    held = torch.empty((rows - 1) * ld + inner, dtype=torch.bfloat16, device=DEV)
+    x = held.as_strided((rows, inner), (ld, 1))
+    x.copy_(torch.randn(rows, inner, generator=torch.Generator().manual_seed(ld)))
+    w, wv = device_weight(1, out, inner, 64)
+    near_on_device(qo.linear_w4(x, w), *product(x.double(), wv, 64, False), torch.bfloat16)
+    del w, wv
+    w, wv = device_weight(2, out, inner, 64, gated=True)
+    near_on_device(qo.gated_w4(x, w), *silu_product(x.double(), wv, 64, False), torch.bfloat16)
+    got = qo.gated_w4(x, w, out_dtype=qo.Q8)
+    want = qo.gated_w4(x.contiguous(), w, out_dtype=qo.Q8)
+    # another tile may add the same products in another order: a step of the scale
+    off = (qo.dequantize_q8(got) - qo.dequantize_q8(want)).abs()
+    assert (off <= 1.01 * want.scales.repeat_interleave(128, 1)).all()
