@@ -70,10 +70,12 @@ int32_t qdc_residual_rmsnorm_q8(float *residual, void *q, float *scales, const f
  * contiguous, fp32 or bf16, and of a gated product also QDC_Q8 (y_scales; out / 2 a multiple
  * of 16).  x [rows, inner], at most 2^20 - 16 rows, is fp32, bf16 (rows ld_x elements apart, a
  * multiple of 8, at most 2^26 bytes) or QDC_Q8 (x_scales; inner a multiple of 16, ld_x =
- * inner).  Sums are fp32 (whole numbers
- * within a group of 8-bit rows), the scale applied to each group's sum: q * x is summed
- * before it and in steps of 1/16, so an fp32 or bf16 x beyond 2^113 and a result beyond 2^123
- * may overflow where q * s * x would not; of an fp32 x what lies below 2^-133 is lost.
+ * inner).  Sums are fp32 (whole numbers within a group of 8-bit rows), the scale applied to
+ * each group's sum: q * x is summed before it and in steps of 1/16, so an fp32 or bf16 x
+ * beyond 2^113 and a result beyond 2^123 may overflow where q * s * x would not; of an fp32 x
+ * what lies below 2^-133 is lost.  Of 8-bit rows a weight's scale (2^127 / 3 at most, as those
+ * of finite weights are) below 2^-105, a result below 2^-109 and a product of both scales
+ * below 2^-126 lose bits, and such a product beyond 2^128 may overflow.
  * x_scales and y_scales are ignored where they are not used.  workspace: device memory of
  * qdc_linear_w4_workspace bytes (0 unless y is QDC_Q8, and its rows few: NULL then), 16-byte
  * aligned, the call's alone until it is done. */

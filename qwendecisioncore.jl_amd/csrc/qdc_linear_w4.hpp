@@ -76,8 +76,12 @@ __device__ __forceinline__ f32x4 scales4(u32x2 s) {
 // 1, and stay within the 2^22 to either side (128 products of 128 * 127 at most).  Four times
 // as fast as a conversion.
 constexpr int kWhole = 0x4b400000;
-__device__ __forceinline__ float whole(int sum) {
-    return __int_as_float(sum) - __int_as_float(kWhole);
+// The same in 2^-21: the bits of a float with an exponent lower by that.  1.5 * 2^23 times a
+// weight's scale, which the tiles take off as one product, is then within the range of fp32
+// for every scale that a finite weight has (up to 2^127 / 3).
+constexpr int kSmall = kWhole - (21 << 23);
+template <int START> __device__ __forceinline__ float whole(int sum) {
+    return __int_as_float(sum) - __int_as_float(START);
 }
 
 // The operand of x for 32 inputs of a block: raw words as they are loaded or staged.
@@ -116,7 +120,7 @@ __device__ __forceinline__ void block_product(f32x4 &total, u32x4 words, const u
             const f32x4 s = scales4(scales[g]);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                total[r] = __builtin_fmaf(whole(sum[r]), s[r] * x_scale, total[r]);
+                total[r] = __builtin_fmaf(whole<kWhole>(sum[r]), s[r] * x_scale, total[r]);
         }
     } else {
 #pragma unroll
@@ -525,7 +529,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) bias[j][r] = s[j][0][r] * -__int_as_float(kWhole);
+            for (int r = 0; r < 4; ++r) bias[j][r] = s[j][0][r] * -__int_as_float(kSmall);
         next();
         __builtin_amdgcn_sched_barrier(0);
         i32x4 sum[2][2];
@@ -538,7 +542,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     i32x4 &to = sum[n % 2][j];
-                    to = i32x4{kWhole, kWhole, kWhole, kWhole};
+                    to = i32x4{kSmall, kSmall, kSmall, kSmall};
                     if constexpr (G == 32) {
                         const u32x4 w = a[j0 + j][g / 2], v = x[i % 2][g / 2];
                         const int h = g % 2 * 2;
@@ -563,11 +567,11 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
                     for (int r = 0; r < 4; ++r) {
                         const float w = s[j0 + j][g][r];
                         const int v = sum[m % 2][j][r];
-                        // the first group's subtraction is part of its product: 3 * 2^22 of a
+                        // the first group's subtraction is part of its product: 1.5 * 2^2 of a
                         // scale's 8 bits is exact
                         block[j][r] =
                             g == 0 ? __builtin_fmaf(__int_as_float(v), w, bias[j0 + j][r])
-                                   : __builtin_fmaf(whole(v), w, block[j][r]);
+                                   : __builtin_fmaf(whole<kSmall>(v), w, block[j][r]);
                         if (g == NG - 1)
                             total[j0 + j][i][r] =
                                 __builtin_fmaf(block[j][r], own[i], total[j0 + j][i][r]);
@@ -639,6 +643,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
         }
     };
     constexpr int NB = GATED ? 2 : 1;
+    constexpr float back = X == kQ8 ? kBack(true) * 0x1p21f : kBack(false);
     __shared__ uint32_t sizes[OUT8 ? NW : 1][OUT8 ? S::kRows : 1];
     auto finish = [&](int n, int m) {
         const int n0 = (S::kBlocks * n + NJ * wave) / NB * kW4Outputs + 4 * quarter;
@@ -651,8 +656,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
             for (int j = 0; j < NJ / NB; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float v = total[NB * j][i][r] * kBack(X == kQ8);
-                    if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * kBack(X == kQ8));
+                    float v = total[NB * j][i][r] * back;
+                    if constexpr (GATED) v = silu(v) * (total[2 * j + 1][i][r] * back);
                     act[i][j][r] = v;
                     if (OUT8 && n0 + 16 * j < p.cols) most = max(most, size_bits(v));
                 }

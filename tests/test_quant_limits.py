@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from qdc_amd import quant_ops as qo
-from test_quant_ops import DEV, near_on_device, product, silu_product
+from test_quant_ops import DEV, GROUPS, near_on_device, near_q8, product, rows_of, silu_product
 
 
 def device_weight(seed, out, inner, group, gated=False, scale=0.1):
@@ -34,3 +34,28 @@ def test_rows_far_apart(ld):
     # another tile may add the same products in another order: a step of the scale
     off = (qo.dequantize_q8(got) - qo.dequantize_q8(want)).abs()
     assert (off <= 1.01 * want.scales.repeat_interleave(128, 1)).all()
+
+
+# ------------------------------------------------------------ extreme scales --
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("weights,scales", [(127, -116), (126, -115), (110, -100), (104, -100),
+                                            (-95, 90)])
+@pytest.mark.parametrize("rows,inner,out", [(3, 256, 64), (60, 1040, 512), (90, 272, 2080),
+                                            (300, 400, 2000), (600, 144, 272), (2100, 272, 2048)])
+def test_scales_of_8_bit_rows(rows, inner, out, weights, scales, group):
+    """Weights up to the largest that fp32 holds, and far below 1, beside rows that make up
+    for it: no kernel's way through the sums leaves the range of their result."""
+    g = torch.Generator().manual_seed(rows + weights)
+    q, _ = rows_of(g, rows, inner, torch.float32, "q8")
+    x = q._replace(scales=q.scales * 2.0 ** scales)
+    xv = qo.dequantize_q8(q).double() * 2.0 ** scales
+    w, wv = device_weight(out, out, inner, group, scale=0.25 * 2.0 ** weights)
+    assert wv.isfinite().all() and wv.abs().max() > 0.5 * 2.0 ** weights
+    want, tol = product(xv, wv, group, True)
+    near_on_device(qo.linear_w4(x, w, out_dtype=torch.float32), want, tol, torch.float32)
+    w, wv = device_weight(out + 1, 2 * out, inner, group, gated=True, scale=0.25 * 2.0 ** weights)
+    want, tol = silu_product(xv, wv, group, True)
+    near_on_device(qo.gated_w4(x, w, out_dtype=torch.float32), want, tol, torch.float32)
+    if out % 16 == 0:
+        near_q8(qo.gated_w4(x, w, out_dtype=qo.Q8), want.cpu(), tol.cpu())
