@@ -123,10 +123,13 @@ class QwenBackbone:
             t = x if isinstance(x, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(x))
             return t.to(self.device).to(dt or dtype).contiguous()
 
+        def aligned(t):  # as the operators on 4-bit weights take it; a view may begin anywhere
+            return t.clone() if weight_format and t.data_ptr() % 16 else t
+
         def gemm_weight(w, split, gated=False):
             # [out, in] -> [in, out] (input rows repeated when split), or in 4 bits
             if weight_format:
-                return quant_ops.pack_w4(w, weight_group, gated)
+                return quant_ops.pack_w4(aligned(w), weight_group, gated)
             w = w.t().contiguous()
             return ops.split_weight(w) if split else w
 
@@ -157,8 +160,8 @@ class QwenBackbone:
             p = f"layers.{i}."
             layer = {
                 "kind": kind,
-                "input_norm": dev(weights[p + "input_layernorm.weight"]),
-                "post_norm": dev(weights[p + "post_attention_layernorm.weight"]),
+                "input_norm": aligned(dev(weights[p + "input_layernorm.weight"])),
+                "post_norm": aligned(dev(weights[p + "post_attention_layernorm.weight"])),
                 "gate_up": lin(p + "mlp.gate_proj.weight", p + "mlp.up_proj.weight", mlp=True),
             }
             residual_stream("down", p + "mlp.down_proj.weight", self.mlp_in)

@@ -1,9 +1,12 @@
 """The operators on 4-bit weights and 8-bit rows at the ends of their documented ranges: rows
 far apart, the largest and smallest scales, quotients next to a half, tensors at any address."""
+import numpy as np
 import pytest
 import torch
 
-from qdc_amd import quant_ops as qo
+from conftest import normwise
+from qdc_amd import backbone, quant_ops as qo
+from test_quant_backbone import BARS, inputs, weights_of
 from test_quant_ops import DEV, GROUPS, near_on_device, near_q8, product, rows_of, silu_product
 
 
@@ -59,3 +62,30 @@ def test_scales_of_8_bit_rows(rows, inner, out, weights, scales, group):
     near_on_device(qo.gated_w4(x, w, out_dtype=torch.float32), want, tol, torch.float32)
     if out % 16 == 0:
         near_q8(qo.gated_w4(x, w, out_dtype=qo.Q8), want.cpu(), tol.cpu())
+
+
+# ------------------------------------------------------------- any address --
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fmt", [None, "w4", "w4a8"])
+def test_checkpoint_tensors_at_any_address(fmt, dtype):
+    """A model of device tensors that begin anywhere is the model of aligned ones."""
+    cfg, weights = weights_of("synthetic")
+    held = {k: torch.from_numpy(np.ascontiguousarray(w)).to(DEV, dtype) for k, w in weights.items()}
+
+    def shifted(t):
+        wide = torch.empty(t.numel() + 1, dtype=t.dtype, device=DEV)
+        wide[1:] = t.flatten()
+        return wide[1:].view(t.shape)
+
+    at_odd = {k: shifted(t) for k, t in held.items()}
+    assert all(t.data_ptr() % 16 for t in at_odd.values())
+    models = [backbone.QwenBackbone.from_weights(w, cfg, DEV, dtype, weight_format=fmt)
+              for w in (held, at_odd)]
+    for B, S in ((1, 1), (2, 40)):
+        ids, mask = inputs(models[0], B, S, seed=S)
+        want, got = (backbone.batch_backbone_states(m, ids, mask) for m in models)
+        # where a table or norm is not aligned another kernel takes it, whose sums have
+        # another order: as far apart as two paths of a model of the same values
+        bar = BARS[fmt, dtype] if fmt else BARS["w4", dtype]
+        assert normwise(got.cpu().numpy(), want.cpu().numpy()) <= bar
