@@ -49,7 +49,7 @@ int32_t qdc_unpack_w4(void *w, const void *packed, const void *scales, int64_t o
                       int64_t group, int32_t gated, int32_t dtype, hipStream_t stream);
 
 /* Rows x [rows, width] (fp32 or bf16, ld elements apart, a multiple of 8) in 8 bits: a = max
- * |x| / 127 of each group, i = x / a rounded to nearest. */
+ * |x| / 127 of each group, in fp32, i = x / a rounded to nearest even, within -127..127. */
 int32_t qdc_quantize_q8(void *q, float *scales, const void *x, int64_t rows, int64_t width,
                         int64_t ld, int32_t dtype, hipStream_t stream);
 

@@ -698,8 +698,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void w4_tiles(W4Product p, int32_t y_
                     if (n0 + 16 * j >= p.cols) continue;
                     *reinterpret_cast<uint32_t *>(reinterpret_cast<char *>(p.y) +
                                                   (int64_t)row * p.cols + n0 + 16 * j) =
-                        pack_bytes(s.value(act[i][j][0]), s.value(act[i][j][1]),
-                                   s.value(act[i][j][2]), s.value(act[i][j][3]));
+                        s.word(act[i][j]);
                 }
                 if (wave == 0 && quarter == 0)
                     p.y_scales[(int64_t)row * groups + n] = s.scale;

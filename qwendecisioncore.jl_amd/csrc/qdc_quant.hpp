@@ -36,10 +36,18 @@ template <int N> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
     return v;
 }
 
-// The scale of a group of 8-bit values whose largest size is `most`, and values under it.
+__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
+    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 |
+           (uint32_t)d << 24;
+}
+
+// The scale of a group of 8-bit values whose largest size is `most`, and values under it: the
+// nearest whole numbers of v / scale, of two the even one.  Of bf16 values one in 400 is
+// a half (127 times a quotient of 8 bits), of fp32 ones one in 14000 next to it: looked at they
+// take rows of 16384 x 1024 from 12.6 to 14.0 us, and none (14.3 to 14.1; the norm 33.8 both).
 struct Q8Scale {
     float scale, inverse;
-    bool plain;  // whether a product with the inverse will do
+    bool plain;  // whether there is an inverse
 
     __device__ explicit Q8Scale(uint32_t most) {
         scale = __uint_as_float(most) / 127.0f;
@@ -47,18 +55,38 @@ struct Q8Scale {
         plain = most >= 0x0d800000u && most < 0x7f800000u;
         inverse = plain ? 1.0f / scale : 0.0f;
     }
-    // within -127..127: |v| <= most, and the product is off by 2 roundings at most
-    __device__ __forceinline__ int value(float v) const {
-        if (plain) return (int)__builtin_rintf(v * inverse);
+    // The nearest to v / s, which `near` is or the one beside it: what is left, v - near s, is
+    // exact with FMA (24 bits from the last of v or of half of s), so its side of a half is
+    // known.  q goes on where more than half of s is left, or half of it and q is odd.
+    static __device__ __forceinline__ int settle(float near, float v, float s) {
+        const float rest = __builtin_fmaf(-near, s, v);
+        const int q = (int)near;
+        const bool on = size_bits(rest + rest) + (uint32_t)(q & 1) > __float_as_uint(s);
+        return q + (on ? (rest < 0.0f ? -1 : 1) : 0);
+    }
+    // Of a scale without an inverse: 2^64 times both, which is exact, as is half of such a scale.
+    __device__ __forceinline__ int small(float v) const {
         if (!(scale > 0.0f && scale < __builtin_inff())) return 0;
-        return (int)fminf(fmaxf(__builtin_rintf(v / scale), -127.0f), 127.0f);
+        const float s = scale * 0x1p64f, w = v * 0x1p64f;
+        // (one of few bits may be less than 1/127 of the largest value)
+        return min(max(settle(__builtin_rintf(w / s), w, s), -127), 127);
+    }
+    // 4 values.  A product with the inverse is within 2^-16 of the quotient (127, twice rounded),
+    // so only next to a half is there more to do.
+    __device__ __forceinline__ uint32_t word(const float (&v)[4]) const {
+        if (!plain) return pack_bytes(small(v[0]), small(v[1]), small(v[2]), small(v[3]));
+        float q[4], off = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float near = v[i] * inverse;
+            q[i] = __builtin_rintf(near);
+            off = fmaxf(off, __builtin_fabsf(near - q[i]));
+        }
+        if (off < 0.5f - 0x1p-15f) return pack_bytes((int)q[0], (int)q[1], (int)q[2], (int)q[3]);
+        return pack_bytes(settle(q[0], v[0], scale), settle(q[1], v[1], scale),
+                          settle(q[2], v[2], scale), settle(q[3], v[3], scale));
     }
 };
-
-__device__ __forceinline__ uint32_t pack_bytes(int a, int b, int c, int d) {
-    return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 |
-           (uint32_t)d << 24;
-}
 
 static inline bool w4_group(int64_t group) { return group == 32 || group == 64 || group == 128; }
 // Blocks of outputs and of inputs.

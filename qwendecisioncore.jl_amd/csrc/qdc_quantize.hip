@@ -148,8 +148,7 @@ template <typename T> __global__ __launch_bounds__(kBlock) void quantize_q8(Rows
     for (int i = 0; i < 4; ++i) m = max(m, size_bits(v[i]));
     const Q8Scale s(group_max<32>(m));
     if (!in) return;
-    p.q[((int64_t)row * p.width + col) / 4] =
-        pack_bytes(s.value(v[0]), s.value(v[1]), s.value(v[2]), s.value(v[3]));
+    p.q[((int64_t)row * p.width + col) / 4] = s.word(v);
     if (l % 32 == 0) p.scales[(int64_t)row * p.groups + col / kQ8Group] = s.scale;
 }
 
@@ -240,8 +239,7 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * kWave : kBlock) void residual_r
         const Q8Scale q(group_max<32>(m));
         if (col >= p.width) continue;
         if (p.add) store_frag<4>(p.residual + base + col, r);
-        p.q[(base + col) / 4] =
-            pack_bytes(q.value(y[0]), q.value(y[1]), q.value(y[2]), q.value(y[3]));
+        p.q[(base + col) / 4] = q.word(y);
         if (l % 32 == 0) p.scales[(int64_t)row * p.groups + col / kQ8Group] = q.scale;
     }
 }

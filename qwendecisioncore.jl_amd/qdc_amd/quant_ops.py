@@ -78,7 +78,8 @@ def unpack_w4(w: W4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
 
 def quantize_q8(x: torch.Tensor) -> Q8:
     """Rows ``x [rows, width]`` (float32 or bfloat16, contiguous rows a multiple of 8
-    elements apart) in 8 bits: the scale of 128 columns is ``max |x| / 127``."""
+    elements apart) in 8 bits: the scale of 128 columns is ``max |x| / 127``, a value the
+    nearest whole number of it (ties to even)."""
     return Q8(*calls().quantize_q8(x))
 
 

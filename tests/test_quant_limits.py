@@ -89,3 +89,58 @@ def test_checkpoint_tensors_at_any_address(fmt, dtype):
         # another order: as far apart as two paths of a model of the same values
         bar = BARS[fmt, dtype] if fmt else BARS["w4", dtype]
         assert normwise(got.cpu().numpy(), want.cpu().numpy()) <= bar
+
+
+# --------------------------------------------------- quotients next to a half --
+def nearest_of(v, scale):
+    """The nearest whole numbers of ``v / scale`` (fp32), ties to the even one, within -127..127:
+    in 64 bits the product of a whole number and a half with a scale is exact, and so is what
+    lies between it and v."""
+    v, scale = v.double(), scale.double()
+    q = (v / scale).round()
+    for _ in range(2):
+        left = 2 * (v - q * scale)
+        over = (left.abs() > scale) | ((left.abs() == scale) & (q % 2 != 0))
+        q = torch.where(over, q + left.sign(), q)
+    return q.clamp(-127, 127)
+
+
+def test_nearest_of():
+    """The oracle itself, against fractions."""
+    from fractions import Fraction
+    g = torch.Generator().manual_seed(0)
+    scale = torch.rand(40, generator=g) + 0.5
+    half = torch.randint(-126, 126, (40,), generator=g) + 0.5
+    exact = (half * scale).float()
+    for v in (exact, torch.nextafter(exact, torch.tensor(9e9)), torch.nextafter(exact, torch.tensor(-9e9)),
+              half * 0.5):
+        s = torch.full((40,), 0.5) if v.equal(half * 0.5) else scale
+        for a, b, q in zip(v.tolist(), s.tolist(), nearest_of(v, s).tolist()):
+            assert q == round(Fraction(a) / Fraction(b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [0, -40, 110, -98, -110, -125, -135])
+def test_8_bit_values_next_to_a_half(power):
+    """Values on a half of their scale and as near to it as fp32 goes: the documented nearest
+    whole number, of two the even one, for scales down to those that fp32 holds a few bits of."""
+    rows = 600
+    g = torch.Generator().manual_seed(power + 1000)
+    most = (torch.rand(rows, generator=g) + 1) * 2.0 ** power
+    most[:40] = 127 * 2.0 ** power           # scales of one bit: halves are exact
+    scale = most / 127
+    x = torch.zeros(rows, 256)
+    half = torch.arange(126) + 0.5
+    x[:, :126] = (half * scale[:, None].double()).float()
+    x[:, 128:254] = torch.nextafter(x[:, :126], torch.tensor(float("inf")))
+    x[rows // 2:, :126] = torch.nextafter(x[rows // 2:, :126], torch.tensor(0.0))
+    x[:, 1:254:3] *= -1
+    x[:, 126], x[:, 254] = most, -most
+    x[:, :128] = torch.where(x[:, :128].abs() > most[:, None], 0.0, x[:, :128])
+    x[:, 128:] = torch.where(x[:, 128:].abs() > most[:, None], 0.0, x[:, 128:])
+    q = qo.quantize_q8(x.to(DEV))
+    scales = q.scales.cpu()
+    assert torch.equal(scales, scale[:, None].expand(rows, 2))
+    wide = scales.repeat_interleave(128, 1)
+    want = torch.where(wide > 0, nearest_of(x, wide), 0.0)
+    assert torch.equal(q.values.cpu().double(), want)
