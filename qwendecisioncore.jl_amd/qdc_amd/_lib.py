@@ -159,8 +159,9 @@ def calls():
         module = importlib.util.module_from_spec(
             importlib.util.spec_from_file_location("qdc_calls", CALLS_PATH, loader=loader))
         loader.exec_module(module)
-        for built, name in ((module.version, "qdc_cache_version"),
-                            (module.quant_version, "qdc_quant_version")):
+        for attribute, name in (("version", "qdc_cache_version"),
+                                ("quant_version", "qdc_quant_version")):
+            built = getattr(module, attribute, None)   # an earlier build lacks the later ones
             version = getattr(lib(), name)().decode()
             if built != version:   # the arguments may be others
                 raise RuntimeError(f"{CALLS_PATH} was built for {built!r}, the library is "

@@ -1,11 +1,14 @@
 """The operators on 4-bit weights and 8-bit rows at the ends of their documented ranges: rows
 far apart, the largest and smallest scales, quotients next to a half, tensors at any address."""
+import importlib.machinery
+import types
+
 import numpy as np
 import pytest
 import torch
 
 from conftest import normwise
-from qdc_amd import backbone, quant_ops as qo
+from qdc_amd import _lib, backbone, quant_ops as qo
 from test_quant_backbone import BARS, inputs, weights_of
 from test_quant_ops import DEV, GROUPS, near_on_device, near_q8, product, rows_of, silu_product
 
@@ -144,3 +147,21 @@ def test_8_bit_values_next_to_a_half(power):
     wide = scales.repeat_interleave(128, 1)
     want = torch.where(wide > 0, nearest_of(x, wide), 0.0)
     assert torch.equal(q.values.cpu().double(), want)
+
+
+# ----------------------------------------------------------- an earlier build --
+def test_calls_of_an_earlier_build(monkeypatch):
+    """A module built before the header existed has no version of it: refused with what to run."""
+    class Earlier(importlib.machinery.ExtensionFileLoader):
+        def create_module(self, spec):
+            module = types.ModuleType("qdc_calls")
+            module.version = _lib.lib().qdc_cache_version().decode()
+            return module
+
+        def exec_module(self, module):
+            pass
+
+    monkeypatch.setattr(importlib.machinery, "ExtensionFileLoader", Earlier)
+    monkeypatch.setattr(_lib, "_calls", None)
+    with pytest.raises(RuntimeError, match="csrc python"):
+        _lib.calls()
