@@ -36,6 +36,11 @@ float real(PyObject *o) {
     if (v == -1.0 && PyErr_Occurred()) throw python_error();
     return (float)v;
 }
+bool truth(PyObject *o) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) throw python_error();
+    return v == 1;
+}
 template <typename T> T *data(const at::Tensor &t) { return static_cast<T *>(t.data_ptr()); }
 
 // What a call's tensors have in common: the device of the first one.
@@ -452,7 +457,7 @@ struct Weight4 {
 
     Weight4(const Call &call, Args a)
         : packed(tensor(a[0], "packed")), scales(tensor(a[1], "scales")), out(integer(a[2])),
-          inner(integer(a[3])), group(integer(a[4])), gated(PyObject_IsTrue(a[5]) == 1) {
+          inner(integer(a[3])), group(integer(a[4])), gated(truth(a[5])) {
         TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128,
                           "group must be 32, 64 or 128");
         TORCH_CHECK_VALUE(out > 0 && inner > 0 && (!gated || out % 2 == 0),
@@ -490,7 +495,7 @@ PyObject *pack_w4(Args a) {
     const Matrix w(call, a[0], "w");
     const int32_t code = dtype_code(w.t);
     const int64_t group = integer(a[1]);
-    const bool gated = PyObject_IsTrue(a[2]) == 1;
+    const bool gated = truth(a[2]);
     TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, "group must be 32, 64 or 128");
     TORCH_CHECK_VALUE(w.rows > 0 && w.width > 0 && w.width % 8 == 0 && (!gated || w.rows % 2 == 0),
                       "w must be [out, inner] with inner a multiple of 8, a gated one's out even");

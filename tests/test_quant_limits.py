@@ -165,3 +165,15 @@ def test_calls_of_an_earlier_build(monkeypatch):
     monkeypatch.setattr(_lib, "_calls", None)
     with pytest.raises(RuntimeError, match="csrc python"):
         _lib.calls()
+
+
+# -------------------------------------------------------------------- refusals --
+@pytest.mark.gpu
+def test_a_flag_without_a_truth_value():
+    """What is neither true nor false is refused with its own error, not with the call's end."""
+    w = torch.zeros(32, 64, device=DEV)
+    packed = qo.pack_w4(w)
+    with pytest.raises(ValueError, match="truth value"):
+        qo.pack_w4(w, gated=np.zeros(2))
+    with pytest.raises(ValueError, match="truth value"):
+        qo.unpack_w4(packed._replace(gated=np.zeros(2)))
