@@ -111,10 +111,11 @@ def linear_w4(x, w: W4, out_dtype: torch.dtype | None = None) -> torch.Tensor:
 
 
 def gated_w4(x, w: W4, out_dtype=None):
-    """``silu(x @ gate.T) * (x @ up.T) [rows, out / 2]`` in one kernel, for ``w`` packed with
-    ``gated=True`` and ``x`` as in :func:`linear_w4`: :func:`ops.native_mlp_gate` of both
-    projections, kept in float32 in between.  ``out_dtype`` may also be :class:`Q8` (out /
-    2 a multiple of 16), for the next product."""
+    """``silu(x @ gate.T) * (x @ up.T) [rows, out / 2]``, for ``w`` packed with ``gated=True`` and
+    ``x`` as in :func:`linear_w4`: :func:`ops.native_mlp_gate` of both projections, kept in
+    float32 in between.  ``out_dtype`` may also be :class:`Q8` (out / 2 a multiple of 16), for
+    the next product.  One kernel; for 8-bit results of few rows two, with the float32 ones
+    between them in a scratch tensor of the call's stream."""
     if not w.gated:
         raise ValueError("gated_w4 takes a weight packed with gated=True")
     if out_dtype is Q8:

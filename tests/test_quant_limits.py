@@ -10,7 +10,8 @@ import torch
 from conftest import normwise
 from qdc_amd import _lib, backbone, quant_ops as qo
 from test_quant_backbone import BARS, inputs, weights_of
-from test_quant_ops import DEV, GROUPS, near_on_device, near_q8, product, rows_of, silu_product
+from test_quant_ops import (DEV, GROUPS, feed_forward, near_on_device, near_q8, product, rows_of,
+                            silu_product)
 
 
 def device_weight(seed, out, inner, group, gated=False, scale=0.1):
@@ -177,3 +178,46 @@ def test_a_flag_without_a_truth_value():
         qo.pack_w4(w, gated=np.zeros(2))
     with pytest.raises(ValueError, match="truth value"):
         qo.unpack_w4(packed._replace(gated=np.zeros(2)))
+
+
+# ------------------------------------------------------------ at the same time --
+@pytest.mark.gpu
+def test_graphs_side_by_side():
+    """Two captured blocks and an eager one on three streams with nothing between them to wait
+    for, all with 8-bit results that go through a workspace: every result is its own inputs'."""
+    g = torch.Generator().manual_seed(11)
+    up = qo.pack_w4((torch.randn(2 * 2048, 1024, generator=g) * 0.1).to(DEV), 64, gated=True)
+    down = qo.pack_w4((torch.randn(1024, 2048, generator=g) * 0.1).to(DEV), 64)
+    norm = torch.zeros(1024, device=DEV)
+    sizes = (24, 40, 33)
+    assert all(_lib.lib().qdc_linear_w4_workspace(n, 4096, 1024, 64, 1, _lib.QDC_Q8) > 0
+               for n in sizes)
+    streams = [torch.cuda.Stream() for _ in sizes]
+    inputs_, outputs, replays = [], [], []
+    for n, stream in zip(sizes, streams):
+        x, a = (torch.randn(n, 1024, generator=g).to(DEV) for _ in range(2))
+        inputs_.append((x, a))
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            feed_forward(x, a, norm, up, down)
+        stream.synchronize()
+        if len(replays) < 2:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outputs.append(feed_forward(x, a, norm, up, down))
+            replays.append(graph)
+    for turn in range(4):
+        for x, _ in inputs_:
+            x.copy_(torch.randn(x.shape, generator=g))
+        want = [[t.clone() for t in feed_forward(x, a, norm, up, down)] for x, a in inputs_]
+        torch.cuda.synchronize()
+        eager = []
+        for _ in range(10):
+            for graph, stream in zip(replays, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            with torch.cuda.stream(streams[2]):
+                eager.append(feed_forward(*inputs_[2], norm, up, down))
+        torch.cuda.synchronize()
+        for got, right in [(outputs[0], want[0]), (outputs[1], want[1])] + [(e, want[2]) for e in eager]:
+            assert torch.equal(got[0], right[0]) and torch.equal(got[1], right[1]), turn
