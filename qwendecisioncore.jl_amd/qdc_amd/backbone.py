@@ -77,8 +77,9 @@ class QwenBackbone:
         ``weight_format`` (None, ``"w4"`` or ``"w4a8"``, without split inputs): the
         projections in 4 bits with a scale for each ``weight_group`` inputs (32, 64 or
         128), as the module docstring says; inner widths are multiples of 8, and with
-        ``"w4a8"`` hidden and intermediate of 16.  ``dtype`` is then that of the
-        activations, the embedding and the norms."""
+        ``"w4a8"`` hidden and intermediate of 16; a call takes up to 2^20 - 16 tokens.
+        ``dtype`` is then that of the activations, the embedding and the norms, and a weight
+        is rounded to it before it is packed."""
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be float32 or bfloat16")
         modes = {False: None, None: None, "none": None, True: "all", "all": "all", "mlp": "mlp"}

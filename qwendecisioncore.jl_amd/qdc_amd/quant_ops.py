@@ -4,7 +4,8 @@ The reference keeps every weight in fp32 or bf16 and has none of these.  They fo
 :mod:`qdc_amd.ops`: each call enqueues kernels of ``libqdc_hip.so`` on the tensor
 device's current PyTorch stream, torch supplies memory and stream only, and argument
 errors raise ``ValueError`` before anything is enqueued.  Nothing is kept between calls,
-and every call can be captured into a HIP graph.
+and every call can be captured into a HIP graph.  Tensors begin at 16-byte addresses (the
+scales of 8-bit rows at 4-byte ones).
 
 A :class:`W4` is a projection ``[out, inner]`` whose weights are whole numbers of -8..7
 times a bfloat16 scale for each output and ``group`` inputs, laid out once by
@@ -101,7 +102,7 @@ def residual_rms_q8(x: torch.Tensor, add: torch.Tensor | None, weight: torch.Ten
 
 def linear_w4(x, w: W4, out_dtype: torch.dtype | None = None) -> torch.Tensor:
     """``x @ W.T [rows, out]`` for ``x [rows, inner]``: float32 or bfloat16 (contiguous rows
-    a multiple of 8 elements apart) or :class:`Q8`.  Sums are float32, of whole numbers
+    a multiple of 8 elements and at most 2^26 bytes apart) or :class:`Q8`.  Sums are float32, of whole numbers
     times ``x`` within a group and scaled after, and rounded once to ``out_dtype`` (float32
     or bfloat16; default ``x``'s, bfloat16 for Q8 rows).  float32 rows keep all their bits.
     Up to 2^20 - 16 rows."""

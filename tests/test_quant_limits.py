@@ -116,8 +116,8 @@ def test_nearest_of():
     scale = torch.rand(40, generator=g) + 0.5
     half = torch.randint(-126, 126, (40,), generator=g) + 0.5
     exact = (half * scale).float()
-    for v in (exact, torch.nextafter(exact, torch.tensor(9e9)), torch.nextafter(exact, torch.tensor(-9e9)),
-              half * 0.5):
+    for v in (exact, torch.nextafter(exact, torch.tensor(9e9)),
+              torch.nextafter(exact, torch.tensor(-9e9)), half * 0.5):
         s = torch.full((40,), 0.5) if v.equal(half * 0.5) else scale
         for a, b, q in zip(v.tolist(), s.tolist(), nearest_of(v, s).tolist()):
             assert q == round(Fraction(a) / Fraction(b))
@@ -219,5 +219,6 @@ def test_graphs_side_by_side():
             with torch.cuda.stream(streams[2]):
                 eager.append(feed_forward(*inputs_[2], norm, up, down))
         torch.cuda.synchronize()
-        for got, right in [(outputs[0], want[0]), (outputs[1], want[1])] + [(e, want[2]) for e in eager]:
+        pairs = list(zip(outputs, want)) + [(e, want[2]) for e in eager]
+        for got, right in pairs:
             assert torch.equal(got[0], right[0]) and torch.equal(got[1], right[1]), turn
