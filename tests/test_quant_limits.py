@@ -10,8 +10,8 @@ import torch
 from conftest import normwise
 from qdc_amd import _lib, backbone, quant_ops as qo
 from test_quant_backbone import BARS, inputs, weights_of
-from test_quant_ops import (DEV, GROUPS, feed_forward, near_on_device, near_q8, product, rows_of,
-                            silu_product)
+from test_quant_ops import (DEV, GROUPS, blocks, feed_forward, near_on_device, near_q8,
+                            plain_values, product, rows_of, silu_product)
 
 
 def device_weight(seed, out, inner, group, gated=False, scale=0.1):
@@ -66,6 +66,32 @@ def test_scales_of_8_bit_rows(rows, inner, out, weights, scales, group):
     near_on_device(qo.gated_w4(x, w, out_dtype=torch.float32), want, tol, torch.float32)
     if out % 16 == 0:
         near_q8(qo.gated_w4(x, w, out_dtype=qo.Q8), want.cpu(), tol.cpu())
+
+
+# --------------------------------------------------- a program's own weights --
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
+@pytest.mark.parametrize("group", GROUPS)
+@pytest.mark.parametrize("rows", [1, 40, 90, 300, 2100])
+def test_weights_of_all_16_values(rows, group, kind):
+    """A weight that a program has laid out itself, of -8 too, which packing never gives; its
+    first outputs and rows are of the largest sums there are."""
+    out, inner = 528, 272
+    g = torch.Generator().manual_seed(rows + group)
+    q = torch.randint(-8, 8, (out, inner), generator=g)
+    q[:20] = -8
+    s = (torch.rand(out, -(-inner // group), generator=g) * 0.02 + 0.01).bfloat16()
+    packed, scales = (t.to(DEV) for t in blocks(q, s, group))
+    w, wv = qo.W4(packed, scales, out, inner, group), plain_values(q, s, group).to(DEV)
+    assert torch.equal(qo.unpack_w4(w).double(), wv)
+    x, xv = rows_of(g, rows, inner, torch.bfloat16 if kind == "bf16" else torch.float32, kind)
+    if kind == "q8":
+        x.values[::3] = 127
+        x.values[1::3, ::2] = -127
+        xv = qo.dequantize_q8(x).double()
+    want, tol = product(xv.to(DEV), wv, group, kind == "q8")
+    for dtype in (torch.float32, torch.bfloat16):
+        near_on_device(qo.linear_w4(x, w, out_dtype=dtype), want, tol, dtype)
 
 
 # ------------------------------------------------------------- any address --
